@@ -2,10 +2,10 @@
  * nt.h -- C ABI of libnt, the MI355X (gfx950) compute library behind the
  * nanotorch_amd Tensor/autograd API.
  *
- * Every entry point replaces one binding of the reference's pybind11 module
- * `nanotorch._C` (src/cpp/_C.cpp:12-24, typed in src/nanotorch/_C.pyi).  The
- * citation above each declaration names the reference interface it stands in
- * for.  Conventions:
+ * Every entry point but those of the token operators replaces one binding of
+ * the reference's pybind11 module `nanotorch._C` (src/cpp/_C.cpp:12-24, typed
+ * in src/nanotorch/_C.pyi).  The citation above each declaration names the
+ * reference interface it stands in for.  Conventions:
  *
  *  - All tensors are described by `nt_view`: a base pointer to device memory,
  *    an element offset, a dtype and up to NT_MAX_DIMS (shape, element-stride)
@@ -342,6 +342,63 @@ int nt_scatter_axes(const nt_view *src, const nt_view *out, int32_t nfancy,
                     const nt_view *index_arrays,
                     const int32_t *out_axis_is_fancy,
                     const int32_t *out_axis_target, const nt_view *keep);
+
+/* -------------------------------------------------------- token operators */
+
+/* No counterpart in the reference: what a model over token numbers needs
+ * around its matrix products.  Tokens are int32 or int64, 1-D, any stride.  A
+ * token outside its range is treated as left out (a zero row, no gradient,
+ * no alternatives), and the next nt_sync() or nt_memcpy_d2h() returns
+ * NT_ERR_INDEX. */
+
+/* out[i, :] = scale * table[t_i, :], one rounding; a zero row where t_i is
+ * `padding` (-1: none is).  table is [V, D] with any strides, float32 or
+ * float64; out is contiguous [N, D]. */
+int nt_embedding(const nt_view *table, const nt_view *tokens, double scale,
+                 int64_t padding, const nt_view *out);
+
+/* The gradient of the table: dtable[v, :] = scale * the sum of g[i, :] over
+ * the i with t_i = v.  Every row is written, rows that no token names with
+ * zeros; with accumulate != 0 the sums are added to dtable and the other rows
+ * stay as they are.  The order of the additions is fixed by the tokens and
+ * the shapes alone.  g is contiguous [N, D]; dtable is [V, D] with adjacent
+ * elements in each row.  N is below 2^31. */
+int nt_embedding_bwd(const nt_view *g, const nt_view *tokens, double scale,
+                     int64_t padding, const nt_view *dtable, int32_t accumulate);
+
+/* y_i = x_i / (1 - p) where word i mod 4 of Philox4x32-10 (key seed, counter
+ * (i div 4, offset)) is at least round(p * 2^32), else 0; i is the row-major
+ * index, so any view of the same values loses the same elements.  Its
+ * gradient is the same call on the upstream gradient.  With accumulate != 0
+ * the result is added to y.  x and y share one shape and float dtype, any
+ * strides; 0 <= p <= 1. */
+int nt_dropout(const nt_view *x, double p, uint64_t seed, uint64_t offset,
+               const nt_view *y, int32_t accumulate);
+
+/* For each row z of logits [rows, V] (adjacent elements in a row, any row
+ * stride, float32 or float64; 1 <= V <= 2^31 - 2^20):
+ *   logprob       log p_t of the row's given token, p = exp(z) / sum exp(z)
+ *   entropy       -sum p log p
+ *   top_logprobs, top_tokens   [rows, k], 1 <= k <= 64: the k largest log p
+ *                 and their tokens (int64), ties to the lowest token, NaN
+ *                 above every number
+ *   stats         [3, rows]: what nt_token_logprobs_bwd needs
+ * each NULL where it is not wanted (top_logprobs and top_tokens together);
+ * all contiguous.  tokens may be NULL when logprob is.  A row whose token is
+ * `ignore` is left out: 0, 0, -inf and -1, and no gradient.  A row of nothing
+ * but -inf has log probability -inf and entropy 0. */
+int nt_token_logprobs(const nt_view *logits, const nt_view *tokens,
+                      int64_t ignore, const nt_view *logprob,
+                      const nt_view *entropy, const nt_view *stats,
+                      const nt_view *top_logprobs, const nt_view *top_tokens);
+
+/* dlogits (accumulate != 0: +)= a ([j = t] - p_j) - b p_j (log p_j + H) with
+ * a = g_logprob and b = g_entropy of the row (1-D, any stride; NULL: zero).
+ * dlogits has the logits' shape and adjacent elements in a row. */
+int nt_token_logprobs_bwd(const nt_view *logits, const nt_view *tokens,
+                          int64_t ignore, const nt_view *stats,
+                          const nt_view *g_logprob, const nt_view *g_entropy,
+                          const nt_view *dlogits, int32_t accumulate);
 
 /* ------------------------------------------------------------- host utils */
 

@@ -32,11 +32,14 @@ from .core import Tensor, TensorLike
 from .cuda import Device, is_available, sync
 from .factories import arange, eye, full, manual_seed, ones, rand, randint, tensor, zeros
 from .ops import (
+    TokenLogProbs,
     add,
     argmax,
     argmin,
     clone,
     divide,
+    dropout,
+    embedding,
     eq,
     equal_op_,
     equals,
@@ -61,6 +64,7 @@ from .ops import (
     subtract,
     sum,
     tanh,
+    token_logprobs,
     transpose,
 )
 
@@ -69,6 +73,7 @@ __all__ = [
     "Dtype",
     "Tensor",
     "TensorLike",
+    "TokenLogProbs",
     "add",
     "arange",
     "argmax",
@@ -76,6 +81,8 @@ __all__ = [
     "bool_",
     "clone",
     "divide",
+    "dropout",
+    "embedding",
     "eq",
     "equals",
     "exp",
@@ -111,6 +118,7 @@ __all__ = [
     "sync",
     "tanh",
     "tensor",
+    "token_logprobs",
     "transpose",
     "zeros",
 ]

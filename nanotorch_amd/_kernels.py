@@ -342,6 +342,97 @@ def matmul_into(x1, x2, target, accumulate: bool) -> None:
     target._storage.bump_version()
 
 
+# --------------------------------------------------------- token operators
+
+
+def embedding(table, tokens, scale: float, padding: int) -> Storage:
+    """Rows of a [V, D] table for 1-D tokens, times scale."""
+    require_device(table, tokens)
+    shape = (tokens._shape[0], table._shape[1])
+    out = Storage.allocate(shape[0] * shape[1], table._storage._dtype, Device.Cuda)
+    _lib.call_packed("nt_embedding", _packed(table), _packed(tokens), scale, padding,
+                     _packed_flat(out, shape))
+    return out
+
+
+def embedding_bwd(g, tokens, scale: float, padding: int, shape, target) -> "Storage | None":
+    """The table's gradient from a contiguous [N, D] g; added to `target`
+    (adjacent elements in each row) when given, else a new storage."""
+    require_device(g, tokens)
+    if target is None:
+        out = Storage.allocate(shape[0] * shape[1], g._storage._dtype, Device.Cuda)
+        _lib.call_packed("nt_embedding_bwd", _packed(g), _packed(tokens), scale, padding,
+                         _packed_flat(out, shape), 0)
+        return out
+    _lib.call_packed("nt_embedding_bwd", _packed(g), _packed(tokens), scale, padding,
+                     _packed(target), 1)
+    target._storage.bump_version()
+    return None
+
+
+def dropout(x, p: float, seed: int, offset: int, target=None) -> "Storage | None":
+    """Dropout of x (or of a gradient); added to `target` when given, else a
+    new storage."""
+    require_device(x)
+    if target is None:
+        out = Storage.allocate(_numel(x._shape), x._storage._dtype, Device.Cuda)
+        _lib.call_packed("nt_dropout", _packed(x), p, seed, offset,
+                         _packed_flat(out, x._shape), 0)
+        return out
+    _lib.call_packed("nt_dropout", _packed(x), p, seed, offset, _packed(target), 1)
+    target._storage.bump_version()
+    return None
+
+
+def token_logprobs(z, tokens, ignore: int, entropy: bool, top: int, stats: bool):
+    """(results, stats, top_logprobs, top_tokens) of [rows, V] logits: results
+    holds the log probabilities (if tokens are given), then the entropies (if
+    wanted), rows of each; what is not wanted is None."""
+    require_device(z) if tokens is None else require_device(z, tokens)
+    rows, dtype = z._shape[0], z._storage._dtype
+    given = tokens is not None
+    out = st = value = token = None
+    v_lp = v_h = v_st = v_value = v_token = None
+    if given or entropy:
+        out = Storage.allocate(rows * (given + entropy), dtype, Device.Cuda)
+        if given:
+            v_lp = _lib.pack_view(out._ptr, 0, dtype, (rows,), (1,))
+        if entropy:
+            v_h = _lib.pack_view(out._ptr, rows * given, dtype, (rows,), (1,))
+    if stats:
+        st = Storage.allocate(3 * rows, dtype, Device.Cuda)
+        v_st = _lib.pack_view(st._ptr, 0, dtype, (3, rows), (rows, 1))
+    if top:
+        value = Storage.allocate(rows * top, dtype, Device.Cuda)
+        token = Storage.allocate(rows * top, Dtype.Int64, Device.Cuda)
+        v_value = _packed_flat(value, (rows, top))
+        v_token = _packed_flat(token, (rows, top))
+    _lib.call_packed("nt_token_logprobs", _packed(z), _packed(tokens) if given else None,
+                     ignore, v_lp, v_h, v_st, v_value, v_token)
+    return out, st, value, token
+
+
+def token_logprobs_bwd(z, tokens, ignore: int, stats: Storage, ga, gb,
+                       target) -> "Storage | None":
+    """The gradient of [rows, V] logits from 1-D gradients ga of the log
+    probabilities and gb of the entropies (None: zero); added to `target`
+    (adjacent elements in each row) when given, else a new storage."""
+    rows = z._shape[0]
+    if target is None:
+        out = Storage.allocate(_numel(z._shape), z._storage._dtype, Device.Cuda)
+        v_out = _packed_flat(out, z._shape)
+    else:
+        out, v_out = None, _packed(target)
+    _lib.call_packed("nt_token_logprobs_bwd", _packed(z),
+                     _packed(tokens) if tokens is not None else None, ignore,
+                     _lib.pack_view(stats._ptr, 0, stats._dtype, (3, rows), (rows, 1)),
+                     _packed(ga) if ga is not None else None,
+                     _packed(gb) if gb is not None else None, v_out, int(target is not None))
+    if target is not None:
+        target._storage.bump_version()
+    return out
+
+
 # ------------------------------------------------------------- host helpers
 
 

@@ -6,6 +6,7 @@ from .grad_mode import is_grad_enabled, no_grad
 from .ops_binary import AddOp, MatmulOp, MulOp, SubOp, TrueDivOp
 from .ops_reduction import MaxOp, MeanOp, MinOp, SumOp
 from .ops_special import ExpandOp, ReshapeOp, TOp, TransposeOp
+from .ops_token import DropoutOp, EmbeddingOp, TokenLogProbOp
 from .ops_unary import ExpOp, LogOp, NegOp, PowOp, ReluOp, SigmoidOp, SqrtOp, TanhOp
 
 ALL_OPS_ = [
@@ -34,6 +35,8 @@ ALL_OPS_ = [
 
 __all__ = [
     "AddOp",
+    "DropoutOp",
+    "EmbeddingOp",
     "ExpandOp",
     "ExpOp",
     "Function",
@@ -53,6 +56,7 @@ __all__ = [
     "SumOp",
     "TanhOp",
     "TOp",
+    "TokenLogProbOp",
     "TransposeOp",
     "TrueDivOp",
     "is_grad_enabled",

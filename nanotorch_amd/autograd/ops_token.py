@@ -1,0 +1,257 @@
+"""Differentiable ops of a model over token numbers: the embedding lookup,
+dropout, and the log probabilities of given tokens with the rows' entropies.
+The reference has none of them.
+
+Each backward is one fused pass that writes a new gradient or adds into an
+existing one (``_backward_into``); token numbers have no gradient.
+"""
+
+from __future__ import annotations
+
+import math
+
+from .. import _kernels as K
+from .. import _lib
+from .._data_type import is_float, is_int, sizeof
+from .._indexing import row_major_strides
+from ..core import Tensor, reshape_view
+from .function import Function
+from .grad_mode import is_grad_enabled
+
+
+def _check_tokens(tokens: Tensor) -> None:
+    if not is_int(tokens.dtype):
+        raise ValueError(f"Tokens must be int32 or int64, got {tokens.dtype.name}.")
+
+
+def _vector(x: Tensor) -> Tensor:
+    """x as a 1-D view, copied only where it is neither 1-D nor contiguous."""
+    return x if len(x._shape) == 1 else reshape_view(x, (x.numel,))
+
+
+def _rows_in_place(x: Tensor) -> Tensor | None:
+    """x [..., n] as a [rows, n] view of adjacent elements; None if its
+    strides do not allow one."""
+    shape, st = x._shape, x._strides
+    if shape[-1] > 1 and st[-1] != 1:
+        return None
+    rows, step = 1, 0  # the leading axes merged so far, innermost first
+    for s, t in zip(reversed(shape[:-1]), reversed(st[:-1])):
+        if s == 1:
+            continue
+        if rows == 1:
+            step = t
+        elif t != step * rows:
+            return None
+        rows *= s
+    if rows == 1:
+        rows, step = math.prod(shape[:-1]), shape[-1]
+    return Tensor._unchecked_view(x._storage, (rows, shape[-1]), (step, 1), x._offset)
+
+
+def _as_rows(x: Tensor) -> Tensor:
+    v = _rows_in_place(x)
+    return v if v is not None else _rows_in_place(x._to_contiguous(force=True))
+
+
+def _added(target: Tensor, storage, shape) -> Tensor:
+    """Adds a new gradient's storage into `target` of any strides."""
+    K.inplace(_lib.ADD, target, Tensor._new_contiguous(storage, shape))
+    return target
+
+
+class EmbeddingOp(Function):
+    """scale * table[tokens]; zero rows where a token is padding_idx."""
+
+    def forward(self, table: Tensor, tokens: Tensor, scale: float = 1.0,
+                padding_idx: int | None = None) -> Tensor:
+        shape = table._shape
+        if len(shape) != 2 or not is_float(table.dtype):
+            raise ValueError(
+                f"An embedding table is 2-D and float, got {table.dtype.name} {shape}.")
+        _check_tokens(tokens)
+        if padding_idx is None:
+            padding_idx = -1
+        elif not 0 <= padding_idx < shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} is no row of a table of {shape[0]}.")
+        self.save_for_backward(tokens)
+        self._scale, self._padding, self._shape = float(scale), padding_idx, shape
+        self._flat = _vector(tokens)
+        st = K.embedding(table, self._flat, self._scale, padding_idx)
+        return Tensor._unchecked_view(
+            st, tokens._shape + shape[1:], row_major_strides(tokens._shape + shape[1:]), 0)
+
+    def backward(self, grad_out: Tensor) -> tuple:
+        return (self._grad(grad_out, None), None)
+
+    def fused_ok(self) -> bool:
+        return True
+
+    def _backward_into(self, g: Tensor, needs, targets):
+        return [self._grad(g, targets[0]) if needs[0] else None, None]
+
+    def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
+        self.saved_tensors  # raises if the tokens were modified in place
+        shape = self._shape
+        g = reshape_view(g, (self._flat._shape[0], shape[1]))._to_contiguous()
+        into = target
+        if target is not None and shape[1] > 1 and target._strides[1] != 1:
+            into = None
+        st = K.embedding_bwd(g, self._flat, self._scale, self._padding, shape, into)
+        if into is not None:
+            return target
+        if target is not None:
+            return _added(target, st, shape)
+        return Tensor._unchecked_view(st, shape, (shape[1], 1), 0)
+
+    @classmethod
+    def flops(cls, table: Tensor, tokens: Tensor, *args) -> int:
+        return tokens.numel * table.shape[1]
+
+    @classmethod
+    def mem_bytes(cls, table: Tensor, tokens: Tensor, *args) -> int:
+        return (tokens.numel * sizeof(tokens.dtype)
+                + 2 * tokens.numel * table.shape[1] * sizeof(table.dtype))
+
+
+class DropoutOp(Function):
+    """x / (1 - p) where word i mod 4 of Philox4x32-10 (key seed, counter
+    (i div 4, offset)) is at least round(p * 2^32), else 0, for the row-major
+    index i.  The mask is drawn again in the backward pass, never stored."""
+
+    def forward(self, x: Tensor, p: float, seed: int, offset: int) -> Tensor:
+        if not is_float(x.dtype):
+            raise ValueError(f"dropout() needs a float tensor, got {x.dtype.name}.")
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout() needs 0 <= p <= 1, got {p}.")
+        K.require_device(x)
+        self._args = (float(p), seed, offset)
+        if p == 0.0:
+            return x
+        return Tensor._unchecked_view(
+            K.dropout(x, *self._args), x._shape, row_major_strides(x._shape), 0)
+
+    def backward(self, grad_out: Tensor) -> tuple:
+        return (self._grad(grad_out, None),)
+
+    def fused_ok(self) -> bool:
+        return True
+
+    def _backward_into(self, g: Tensor, needs, targets):
+        return [self._grad(g, targets[0]) if needs[0] else None]
+
+    def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
+        if self._args[0] == 0.0:
+            if target is None:
+                return g
+            K.inplace(_lib.ADD, target, g)
+            return target
+        st = K.dropout(g, *self._args, target)
+        if target is not None:
+            return target
+        return Tensor._unchecked_view(st, g._shape, row_major_strides(g._shape), 0)
+
+    @classmethod
+    def flops(cls, x: Tensor, *args) -> int:
+        return x.numel
+
+    @classmethod
+    def mem_bytes(cls, x: Tensor, *args) -> int:
+        return 2 * x.numel * sizeof(x.dtype)
+
+
+class TokenLogProbOp(Function):
+    """Log probabilities of given tokens and entropies of rows of logits.
+
+    Returns the one that is wanted, or both as [2, ...] (log probabilities
+    first), so that one pass computes the logits' gradient of both.  The top
+    alternatives go into `extras`; they have no gradient."""
+
+    def forward(self, logits: Tensor, tokens: Tensor | None, ignore_index: int,
+                entropy: bool, top: int, extras: list) -> Tensor:
+        lead = logits._shape[:-1]
+        z = _as_rows(logits)
+        flat = None if tokens is None else _vector(tokens)
+        keep = is_grad_enabled() and logits.requires_grad
+        out, self._stats, value, token = K.token_logprobs(
+            z, flat, ignore_index, entropy, top, keep)
+        if top:
+            extras.append(Tensor._new_contiguous(value, lead + (top,)))
+            extras.append(Tensor._new_contiguous(token, lead + (top,)))
+        self._both = entropy and tokens is not None
+        if keep:
+            self.save_for_backward(*((logits,) if tokens is None else (logits, tokens)))
+            self._call = (z, flat, ignore_index)
+            self._shape = logits._shape
+        shape = (2,) + lead if self._both else lead
+        return Tensor._unchecked_view(out, shape, row_major_strides(shape), 0)
+
+    def backward(self, grad_out: Tensor) -> tuple:
+        return (self._grad(grad_out, None), None)
+
+    def fused_ok(self) -> bool:
+        return True
+
+    def _backward_into(self, g: Tensor, needs, targets):
+        none = [None] * (len(needs) - 1)
+        return [self._grad(g, targets[0]) if needs[0] else None] + none
+
+    def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
+        self.saved_tensors  # raises if logits or tokens were modified in place
+        z, flat, ignore = self._call
+        rows = z._shape[0]
+        if g.dtype != z.dtype:
+            g = g.to(z.dtype)
+        if self._both:
+            g = reshape_view(g, (2, rows))._to_contiguous()
+            ga, gb = _row_of(g, 0), _row_of(g, 1)
+        else:
+            g = _vector(g)
+            ga, gb = (None, g) if flat is None else (g, None)
+        into = None if target is None else _rows_in_place(target)
+        st = K.token_logprobs_bwd(z, flat, ignore, self._stats, ga, gb, into)
+        if into is not None:
+            return target
+        if target is not None:
+            return _added(target, st, self._shape)
+        return Tensor._unchecked_view(st, self._shape, row_major_strides(self._shape), 0)
+
+    @classmethod
+    def flops(cls, logits: Tensor, *args) -> int:
+        return 5 * logits.numel
+
+    @classmethod
+    def mem_bytes(cls, logits: Tensor, *args) -> int:
+        return logits.numel * sizeof(logits.dtype)
+
+
+class RowOp(Function):
+    """x[i] of x [2, ...], with a gradient: the upstream one in row i, zeros
+    in the other."""
+
+    def forward(self, x: Tensor, i: int) -> Tensor:
+        self._i, self._shape = i, x._shape
+        return _row_of(x, i)
+
+    def backward(self, grad_out: Tensor) -> tuple:
+        return (self._backward_into(grad_out, [True], [None])[0],)
+
+    def fused_ok(self) -> bool:
+        return True
+
+    def _backward_into(self, g: Tensor, needs, targets):
+        if not needs[0]:
+            return [None]
+        if targets[0] is not None:
+            K.inplace(_lib.ADD, _row_of(targets[0], self._i), g)
+            return [targets[0]]
+        full = Tensor._new_contiguous(
+            K.fill(math.prod(self._shape), 0, g.dtype, g.device), self._shape)
+        K.copy_view(g, _row_of(full, self._i))
+        return [full]
+
+
+def _row_of(x: Tensor, i: int) -> Tensor:
+    return Tensor._unchecked_view(
+        x._storage, x._shape[1:], x._strides[1:], x._offset + i * x._strides[0])
+

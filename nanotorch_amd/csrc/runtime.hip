@@ -260,8 +260,9 @@ void raise_deferred_error() {
     return;
   const int code = *w;
   *w = NT_OK;
-  fail(code, "an earlier gather/scatter call met an index outside its axis "
-             "(found by the device-side check; those elements were skipped)");
+  fail(code, "an earlier gather/scatter call met an index, or a token operator "
+             "a token, outside its axis (found by the device-side check; those "
+             "elements were skipped)");
 }
 int device_cu_count() { return rt().cu_count; }
 void *device_alloc(size_t nbytes) { return allocator().alloc(nbytes); }

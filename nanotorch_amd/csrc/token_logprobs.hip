@@ -1,0 +1,718 @@
+// Log probabilities of given tokens from rows of logits, the entropy of each
+// row, its top alternatives, and the gradient of the logits.
+//
+// One pass over a row keeps, per lane, the running maximum m and the sums
+//   s = sum exp(z_j - m),   u = sum exp(z_j - m) (z_j - m),
+// from which
+//   log p_t = (z_t - m) - log s,
+//   H       = -sum p log p = log s - u / s.
+// Two such states join by moving both to the larger maximum: with d = m - m'
+//   s' = exp(d) s,   u' = exp(d) (u + d s).
+// The gradient for upstream a (of log p_t) and b (of H) is
+//   dz_j = a [j = t] - p_j (a + b (log p_j + H)),   p_j = exp(z_j - m) / s,
+// one pass that reads z and writes dz.
+//
+// Logits of -inf are tokens without probability and count for nothing; a row
+// that holds nothing else has log probability -inf, entropy 0 and no
+// gradient.  A NaN or +inf makes the row's results NaN.  A row whose token
+// is `ignore` is not read: results 0, alternatives -inf and -1, gradient 0.
+// One whose token lies outside the row is treated so too and reported at the
+// next synchronisation (the library's deferred error).
+//
+// The alternatives are the k largest logits, ties to the lowest token, NaN
+// above every number.  Each wave keeps its own k best, the i-th in lane i;
+// a chunk's elements are looked at one by one only where some lane's maximum
+// (which the pass computes anyway) exceeds the k-th best so far: about
+// k ln(n / k) times in n elements of random order.
+#include "tokens.h"
+
+#include <algorithm>
+#include <limits>
+
+namespace nt {
+
+constexpr int LP_THREADS = 256;
+constexpr int LP_WAVES = LP_THREADS / WAVE;
+constexpr int LP_UNROLL = 4;  // vectors in flight per lane
+constexpr int LP_TOP_MAX = WAVE;
+
+// exp of d <= 0.  exp2's argument d log2 e is taken in two parts, so that its
+// rounding (2^-24 of |d| log2 e) is not multiplied up by large |d|.
+__device__ __forceinline__ float exp_of(float d) {
+  constexpr float L = 1.44269504f;          // log2 e, rounded
+  constexpr float L_LOW = 1.92596303e-8f;   // log2 e - L
+  constexpr float LN2 = 0.693147181f;
+  const float h = d * L;
+  const float l = __builtin_fmaf(d, L_LOW, __builtin_fmaf(d, L, -h));
+  const float e = __builtin_amdgcn_exp2f(h);
+  return __builtin_fmaf(e, l * LN2, e);
+}
+__device__ __forceinline__ double exp_of(double d) { return exp(d); }
+
+// Past this distance from the maximum exp() is 0 in T.
+template <class T> constexpr T LP_CUT = sizeof(T) == 4 ? T(-200) : T(-800);
+
+template <class T> __device__ __forceinline__ T not_below_cut(T d) {
+  return d < LP_CUT<T> ? LP_CUT<T> : d; // NaN stays
+}
+
+// The larger one; NaN if either is.
+template <class T> __device__ __forceinline__ T max_nan(T a, T b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
+template <class T> struct RowState {
+  T m = -std::numeric_limits<T>::infinity(), s = T(0), u = T(0);
+
+  __device__ __forceinline__ void move_to(T to) {
+    if (s != T(0) && m != to) {
+      const T d = not_below_cut(m - to), c = exp_of(d);
+      u = c * (u + d * s);
+      s = c * s;
+    }
+    m = to;
+  }
+  __device__ __forceinline__ void join(RowState o) {
+    const T to = max_nan(m, o.m);
+    move_to(to);
+    o.move_to(to);
+    s += o.s;
+    u += o.u;
+  }
+  // A lane's N values; -inf where there is none.
+  template <int N> __device__ __forceinline__ void add(const T (&z)[N], T top) {
+    if (!(top <= m))
+      move_to(max_nan(m, top));
+    const T ref = m == -std::numeric_limits<T>::infinity() ? T(0) : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const T d = not_below_cut(z[i] - ref), e = exp_of(d);
+      s += e;
+      u = __builtin_fma(e, d, u);
+    }
+  }
+  // Every lane gets the wave's state.
+  __device__ __forceinline__ void join_lanes() {
+    for (int k = 1; k < WAVE; k <<= 1) {
+      RowState o;
+      o.m = __shfl_xor(m, k);
+      o.s = __shfl_xor(s, k);
+      o.u = __shfl_xor(u, k);
+      join(o);
+    }
+    m = __shfl(m, 0);
+    s = __shfl(s, 0);
+    u = __shfl(u, 0);
+  }
+};
+
+// ------------------------------------------------------------ alternatives
+
+// Keys order as the logits do, as unsigned integers: 0 is no entry, NaN is
+// the largest, -0 equals 0.
+template <class T> struct Key;
+template <> struct Key<float> {
+  using K = uint32_t;
+  static __device__ __forceinline__ K of(float v) {
+    if (v != v)
+      return ~K(0);
+    const K b = __builtin_bit_cast(K, v + 0.0f);
+    return b >> 31 ? ~b : b | K(1) << 31;
+  }
+  static __device__ __forceinline__ float value(K k) {
+    if (k == ~K(0))
+      return std::numeric_limits<float>::quiet_NaN();
+    return __builtin_bit_cast(float, k >> 31 ? k ^ K(1) << 31 : ~k);
+  }
+};
+template <> struct Key<double> {
+  using K = uint64_t;
+  static __device__ __forceinline__ K of(double v) {
+    if (v != v)
+      return ~K(0);
+    const K b = __builtin_bit_cast(K, v + 0.0);
+    return b >> 63 ? ~b : b | K(1) << 63;
+  }
+  static __device__ __forceinline__ double value(K k) {
+    if (k == ~K(0))
+      return std::numeric_limits<double>::quiet_NaN();
+    return __builtin_bit_cast(double, k >> 63 ? k ^ K(1) << 63 : ~k);
+  }
+};
+
+__device__ __forceinline__ uint32_t read_lane(uint32_t v, int l) {
+  return __builtin_amdgcn_readlane(v, l);
+}
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int l) {
+  return uint64_t(__builtin_amdgcn_readlane(uint32_t(v >> 32), l)) << 32 |
+         uint32_t(__builtin_amdgcn_readlane(uint32_t(v), l));
+}
+
+// A wave's best `k` entries in falling order, the i-th in lane i.
+template <class T> struct TopList {
+  using K = typename Key<T>::K;
+  K key = 0;
+  int32_t token = -1;
+  K least = 0; // the k-th key: what an entry has to exceed
+
+  __device__ __forceinline__ void insert(K v, int32_t t, int k) {
+    const int lane = threadIdx.x & 63;
+    const int pos = __popcll(__ballot(key >= v));
+    const K up = __shfl_up(key, 1);
+    const int32_t up_t = __shfl_up(token, 1);
+    if (lane == pos) {
+      key = v;
+      token = t;
+    } else if (lane > pos && lane < k) {
+      key = up;
+      token = up_t;
+    }
+    least = read_lane(key, k - 1);
+  }
+  // One entry per lane, in rising order of their tokens among equal keys.
+  __device__ __forceinline__ void insert_lanes(K v, int32_t t, int k) {
+    uint64_t m = __ballot(v > least);
+    while (m) {
+      const int l = __ffsll((unsigned long long)m) - 1;
+      m &= m - 1;
+      const K c = read_lane(v, l);
+      if (c > least)
+        insert(c, int32_t(read_lane(uint32_t(t), l)), k);
+    }
+  }
+};
+
+// ---------------------------------------------------------------- forward
+
+template <class T> struct LpForward {
+  const T *z;
+  int64_t row_stride;
+  int64_t rows;
+  int32_t V;
+  Tokens tok; // p null: no given tokens
+  int64_t ignore;
+  T *logprob, *entropy, *stats, *top_value; // null: not wanted
+  int64_t *top_token;
+  int k;
+  int splits;    // workgroups per row
+  int32_t part;  // elements per wave
+  // partial states of split rows: [rows][splits] each
+  T *pm, *ps, *pu;
+  typename Key<T>::K *pkey; // [rows][splits][k]
+  int32_t *ptoken;
+  int *err;
+};
+
+template <class T>
+__device__ __forceinline__ void write_left_out(const LpForward<T> &a, int64_t row) {
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
+    if (a.logprob)
+      a.logprob[row] = T(0);
+    if (a.entropy)
+      a.entropy[row] = T(0);
+    if (a.stats) {
+      a.stats[row] = T(0);
+      a.stats[a.rows + row] = T(0);
+      a.stats[2 * a.rows + row] = T(0);
+    }
+  }
+  if (lane < a.k) {
+    a.top_value[row * a.k + lane] = -std::numeric_limits<T>::infinity();
+    a.top_token[row * a.k + lane] = -1;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void write_row(const LpForward<T> &a, int64_t row, int64_t t,
+                                          const RowState<T> &r, const TopList<T> &top) {
+  const int lane = threadIdx.x & 63;
+  const bool none = r.s == T(0);
+  const T log_s = log(r.s), low = -std::numeric_limits<T>::infinity();
+  if (lane == 0) {
+    if (a.logprob)
+      a.logprob[row] = none ? low : (a.z[row * a.row_stride + t] - r.m) - log_s;
+    if (a.entropy)
+      a.entropy[row] = none ? T(0) : log_s - r.u / r.s;
+    if (a.stats) {
+      a.stats[row] = r.m;
+      a.stats[a.rows + row] = r.s;
+      a.stats[2 * a.rows + row] = r.u;
+    }
+  }
+  if (lane < a.k) {
+    a.top_value[row * a.k + lane] =
+        none ? low : (Key<T>::value(top.key) - r.m) - log_s;
+    a.top_token[row * a.k + lane] = top.token;
+  }
+}
+
+// The row's token, and whether the row is left out.
+template <class T>
+__device__ __forceinline__ bool row_left_out(const LpForward<T> &a, int64_t row,
+                                             int64_t &t) {
+  t = 0;
+  if (a.tok.p == nullptr)
+    return false;
+  t = a.tok[row];
+  if (t == a.ignore)
+    return true;
+  if (t < 0 || t >= a.V) {
+    *a.err = NT_ERR_INDEX;
+    return true;
+  }
+  return false;
+}
+
+// Elements beg .. end - 1 of a row into the wave's state and list.
+template <class T, bool TOP>
+__device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k,
+                                     RowState<T> &r, TopList<T> &top) {
+  using RV = RowVec<T>;
+  constexpr int N = RV::N, CHUNK = WAVE * N * LP_UNROLL;
+  const int lane = threadIdx.x & 63;
+  const T none = -std::numeric_limits<T>::infinity();
+  for (int64_t b = beg; b < end; b += CHUNK) {
+    T v[LP_UNROLL * N];
+#pragma unroll
+    for (int c = 0; c < LP_UNROLL; ++c) {
+      const int64_t i = b + (c * WAVE + lane) * N;
+      if (i + N <= end) {
+        const typename RV::V w = RV::load(z + i);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          v[c * N + j] = w[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          v[c * N + j] = i + j < end ? z[i + j] : none;
+      }
+    }
+    T most = v[0];
+#pragma unroll
+    for (int j = 1; j < LP_UNROLL * N; ++j)
+      most = max_nan(most, v[j]);
+    if constexpr (TOP) {
+      const T least = Key<T>::value(top.least); // NaN while there are fewer than k
+      if (__ballot(!(most <= least))) {
+#pragma unroll
+        for (int c = 0; c < LP_UNROLL; ++c) {
+          const int64_t i = b + (c * WAVE + lane) * N;
+          typename Key<T>::K key[N];
+          bool any = false;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            key[j] = i + j < end ? Key<T>::of(v[c * N + j]) : 0;
+            any |= key[j] > top.least;
+          }
+          uint64_t m = __ballot(any);
+          while (m) {
+            const int l = __ffsll((unsigned long long)m) - 1;
+            m &= m - 1;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const typename Key<T>::K x = read_lane(key[j], l);
+              if (x > top.least)
+                top.insert(x, int32_t(b + (c * WAVE + l) * N + j), k);
+            }
+          }
+        }
+      }
+    }
+    r.add(v, most);
+  }
+}
+
+// A wave per row.
+template <class T, bool TOP>
+__global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a,
+                                                                  int64_t row0) {
+  const int64_t row = row0 + int64_t(blockIdx.x) * LP_WAVES + (threadIdx.x >> 6);
+  if (row >= a.rows)
+    return;
+  int64_t t;
+  if (row_left_out(a, row, t))
+    return write_left_out(a, row);
+  RowState<T> r;
+  TopList<T> top;
+  walk<T, TOP>(a.z + row * a.row_stride, 0, a.V, a.k, r, top);
+  r.join_lanes();
+  write_row(a, row, t, r, top);
+}
+
+// `splits` workgroups per row, each wave a part of `part` elements.
+template <class T, bool TOP>
+__global__ __launch_bounds__(LP_THREADS) void logprob_group_kernel(LpForward<T> a,
+                                                                   int64_t row0) {
+  __shared__ T sm[3][LP_WAVES];
+  __shared__ typename Key<T>::K skey[LP_WAVES][LP_TOP_MAX];
+  __shared__ int32_t stoken[LP_WAVES][LP_TOP_MAX];
+  const int64_t row = row0 + blockIdx.x / a.splits;
+  const int split = blockIdx.x % a.splits;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t t;
+  if (row_left_out(a, row, t)) {
+    if (wave == 0 && a.splits == 1)
+      write_left_out(a, row);
+    return;
+  }
+  RowState<T> r;
+  TopList<T> top;
+  const int64_t beg = int64_t(split * LP_WAVES + wave) * a.part;
+  if (beg < a.V)
+    walk<T, TOP>(a.z + row * a.row_stride, int32_t(beg),
+                 int32_t(std::min<int64_t>(a.V, beg + a.part)), a.k, r, top);
+  r.join_lanes();
+  if (lane == 0) {
+    sm[0][wave] = r.m;
+    sm[1][wave] = r.s;
+    sm[2][wave] = r.u;
+  }
+  if (TOP && lane < a.k) {
+    skey[wave][lane] = top.key;
+    stoken[wave][lane] = top.token;
+  }
+  __syncthreads();
+  if (wave != 0)
+    return;
+  for (int w = 1; w < LP_WAVES; ++w) {
+    RowState<T> o;
+    o.m = sm[0][w];
+    o.s = sm[1][w];
+    o.u = sm[2][w];
+    r.join(o);
+    if constexpr (TOP)
+      top.insert_lanes(lane < a.k ? skey[w][lane] : 0, lane < a.k ? stoken[w][lane] : -1,
+                       a.k);
+  }
+  if (a.splits == 1)
+    return write_row(a, row, t, r, top);
+  const int64_t at = row * a.splits + split;
+  if (lane == 0) {
+    a.pm[at] = r.m;
+    a.ps[at] = r.s;
+    a.pu[at] = r.u;
+  }
+  if (TOP && lane < a.k) {
+    a.pkey[at * a.k + lane] = top.key;
+    a.ptoken[at * a.k + lane] = top.token;
+  }
+}
+
+// Joins the splits of a row; a wave per row.
+template <class T, bool TOP>
+__global__ __launch_bounds__(WAVE) void logprob_join_kernel(LpForward<T> a,
+                                                            int64_t row0) {
+  const int64_t row = row0 + blockIdx.x;
+  const int lane = threadIdx.x;
+  int64_t t;
+  if (row_left_out(a, row, t))
+    return write_left_out(a, row);
+  RowState<T> r;
+  TopList<T> top;
+  for (int b = lane; b < a.splits; b += WAVE) {
+    RowState<T> o;
+    o.m = a.pm[row * a.splits + b];
+    o.s = a.ps[row * a.splits + b];
+    o.u = a.pu[row * a.splits + b];
+    r.join(o);
+  }
+  r.join_lanes();
+  if constexpr (TOP) {
+    const int64_t n = int64_t(a.splits) * a.k, base = row * n;
+    for (int64_t b = 0; b < n; b += WAVE) {
+      const bool in = b + lane < n;
+      top.insert_lanes(in ? a.pkey[base + b + lane] : 0, in ? a.ptoken[base + b + lane] : -1,
+                       a.k);
+    }
+  }
+  write_row(a, row, t, r, top);
+}
+
+// --------------------------------------------------------------- backward
+
+template <class T> struct LpBackward {
+  const T *z;
+  int64_t row_stride;
+  int64_t rows;
+  int32_t V;
+  Tokens tok;
+  int64_t ignore;
+  const T *stats;
+  const T *ga, *gb; // null: zero
+  int64_t sa, sb;   // their strides
+  T *dz;
+  int64_t dz_stride;
+};
+
+// A workgroup of W waves per row, or (W = 1) four rows per workgroup, each
+// lane LP_UNROLL vectors.
+template <class T, int W, bool ACC>
+__global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a,
+                                                                 int64_t row0, int chunks) {
+  using RV = RowVec<T>;
+  constexpr int N = RV::N;
+  int64_t row;
+  int32_t first;
+  if constexpr (W == 1) {
+    row = row0 + int64_t(blockIdx.x) * LP_WAVES + (threadIdx.x >> 6);
+    if (row >= a.rows)
+      return;
+    first = (threadIdx.x & 63) * N;
+  } else {
+    row = row0 + blockIdx.x / chunks;
+    first = (blockIdx.x % chunks) * (LP_THREADS * N * LP_UNROLL) + threadIdx.x * N;
+  }
+  constexpr int STEP = W * WAVE * N;
+  const int64_t t = a.tok.p ? a.tok[row] : 0;
+  const T m = a.stats[row], s = a.stats[a.rows + row], u = a.stats[2 * a.rows + row];
+  const bool none = s == T(0) || (a.tok.p && (t == a.ignore || t < 0 || t >= a.V));
+  T *dz = a.dz + row * a.dz_stride;
+  if (none) {
+    if (!ACC)
+      for (int c = 0; c < LP_UNROLL; ++c)
+        for (int j = 0; j < N; ++j) {
+          const int64_t i = int64_t(first) + c * STEP + j;
+          if (i < a.V)
+            dz[i] = T(0);
+        }
+    return;
+  }
+  const T log_s = log(s), H = log_s - u / s, inv = T(1) / s;
+  const T ga = a.ga ? a.ga[row * a.sa] : T(0), gb = a.gb ? a.gb[row * a.sb] : T(0);
+  // dz = p (c0 + c1 d), d = z - m, + ga at the token
+  const T c0 = -ga - gb * (H - log_s), c1 = -gb;
+  const T *z = a.z + row * a.row_stride;
+#pragma unroll
+  for (int c = 0; c < LP_UNROLL; ++c) {
+    const int64_t i = int64_t(first) + c * STEP;
+    if (i >= a.V)
+      break;
+    const bool whole = i + N <= a.V;
+    typename RV::V w, old = {};
+    if (whole) {
+      w = RV::load(z + i);
+      if (ACC)
+        old = RV::load(dz + i);
+    } else {
+      for (int j = 0; j < N; ++j) {
+        w[j] = i + j < a.V ? z[i + j] : T(0);
+        if (ACC)
+          old[j] = i + j < a.V ? dz[i + j] : T(0);
+      }
+    }
+    typename RV::V o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const T d = not_below_cut(w[j] - m);
+      T v = exp_of(d) * inv * __builtin_fma(c1, d, c0);
+      if (a.ga && i + j == t)
+        v += ga;
+      o[j] = ACC ? old[j] + v : v;
+    }
+    if (whole) {
+      RV::store(dz + i, o);
+    } else {
+      for (int j = 0; j < N; ++j)
+        if (i + j < a.V)
+          dz[i + j] = o[j];
+    }
+  }
+}
+
+namespace {
+
+// Rows of a [rows, V] view as (pointer, row stride): rows in place, elements
+// of a row next to each other.
+template <class T> T *row_view(const nt_view *v, int64_t &stride, const char *fname) {
+  if (v->ndim != 2 || (v->shape[1] > 1 && v->strides[1] != 1))
+    fail(NT_ERR_RUNTIME, std::string(fname) + ": expected rows of adjacent elements");
+  stride = v->strides[0];
+  return typed_ptr<T>(v);
+}
+
+template <class T>
+T *out_vector(const nt_view *v, int64_t n, int dtype, const char *what) {
+  if (v == nullptr)
+    return nullptr;
+  check_view(v, "token_logprobs");
+  if (v->dtype != dtype || numel(v) != n || !is_contiguous(v))
+    fail(NT_ERR_RUNTIME, std::string("token_logprobs: bad ") + what);
+  return typed_ptr<T>(v);
+}
+
+template <class T> void run_forward(LpForward<T> a) {
+  constexpr int CHUNK = WAVE * RowVec<T>::N * LP_UNROLL;
+  const auto launch = [&](auto kernel, int threads, int64_t rows_per_block,
+                          int64_t blocks_per_row) {
+    const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / blocks_per_row);
+    for (int64_t r = 0; r < a.rows; r += most * rows_per_block) {
+      const int64_t rows = std::min(a.rows - r, most * rows_per_block);
+      const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block * blocks_per_row;
+      kernel<<<dim3(unsigned(blocks)), threads, 0, stream()>>>(a, r);
+      NT_LAUNCH_CHECK();
+    }
+  };
+  if (a.V <= 2 * CHUNK) {
+    if (a.k)
+      launch(logprob_wave_kernel<T, true>, LP_THREADS, LP_WAVES, 1);
+    else
+      launch(logprob_wave_kernel<T, false>, LP_THREADS, LP_WAVES, 1);
+    return;
+  }
+  const int64_t chunks = (a.V + CHUNK - 1) / CHUNK;
+  const int64_t want = std::max<int64_t>(1, 4 * device_cu_count() / a.rows);
+  a.splits = int(std::min<int64_t>(want, (chunks + LP_WAVES - 1) / LP_WAVES));
+  const int64_t parts = int64_t(a.splits) * LP_WAVES;
+  a.part = int32_t((chunks + parts - 1) / parts * CHUNK);
+  const int64_t n = a.splits > 1 ? a.rows * a.splits : 0;
+  DeviceScratch sums(size_t(3 * n) * sizeof(T));
+  DeviceScratch keys(size_t(n * a.k) * sizeof(typename Key<T>::K));
+  DeviceScratch toks(size_t(n * a.k) * sizeof(int32_t));
+  a.pm = sums.get<T>();
+  a.ps = a.pm + n;
+  a.pu = a.ps + n;
+  a.pkey = keys.get<typename Key<T>::K>();
+  a.ptoken = toks.get<int32_t>();
+  if (a.k)
+    launch(logprob_group_kernel<T, true>, LP_THREADS, 1, a.splits);
+  else
+    launch(logprob_group_kernel<T, false>, LP_THREADS, 1, a.splits);
+  if (a.splits == 1)
+    return;
+  if (a.k)
+    launch(logprob_join_kernel<T, true>, WAVE, 1, 1);
+  else
+    launch(logprob_join_kernel<T, false>, WAVE, 1, 1);
+}
+
+template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
+  constexpr int SPAN = LP_THREADS * RowVec<T>::N * LP_UNROLL; // of a workgroup
+  const bool small = a.V <= SPAN / LP_WAVES;
+  const int64_t chunks = small ? 1 : (a.V + SPAN - 1) / SPAN;
+  const int64_t per = small ? LP_WAVES : 1;
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / chunks) * per;
+  for (int64_t r = 0; r < a.rows; r += most) {
+    const int64_t rows = std::min(a.rows - r, most);
+    const dim3 grid{unsigned((rows + per - 1) / per * chunks)};
+    if (small)
+      logprob_bwd_kernel<T, 1, ACC><<<grid, LP_THREADS, 0, stream()>>>(a, r, 1);
+    else
+      logprob_bwd_kernel<T, LP_WAVES, ACC>
+          <<<grid, LP_THREADS, 0, stream()>>>(a, r, int(chunks));
+    NT_LAUNCH_CHECK();
+  }
+}
+
+void check_logits(const nt_view *z, const nt_view *tokens, const char *fname) {
+  check_view(z, fname);
+  if (z->ndim != 2)
+    fail(NT_ERR_RUNTIME, std::string(fname) + ": logits must be [rows, V]");
+  if (z->shape[1] < 1 || z->shape[1] > std::numeric_limits<int32_t>::max() - (1 << 20))
+    fail(NT_ERR_VALUE, std::string(fname) + ": a row must hold 1 to 2^31 - 2^20 logits");
+  if (tokens && tokens->ndim == 1 && tokens->shape[0] != z->shape[0])
+    fail(NT_ERR_RUNTIME, std::string(fname) + ": one token per row");
+}
+
+} // namespace
+} // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+int nt_token_logprobs(const nt_view *logits, const nt_view *tokens, int64_t ignore,
+                      const nt_view *logprob, const nt_view *entropy,
+                      const nt_view *stats, const nt_view *top_logprobs,
+                      const nt_view *top_tokens) {
+  return guard([&] {
+    check_logits(logits, tokens, "token_logprobs");
+    const int64_t rows = logits->shape[0];
+    int64_t k = 0;
+    if (top_logprobs || top_tokens) {
+      check_view(top_logprobs, "token_logprobs");
+      check_view(top_tokens, "token_logprobs");
+      if (top_logprobs->ndim != 2 || top_tokens->ndim != 2 ||
+          top_logprobs->shape[1] != top_tokens->shape[1])
+        fail(NT_ERR_RUNTIME, "token_logprobs: alternatives must be [rows, k]");
+      k = top_logprobs->shape[1];
+      if (k < 1 || k > LP_TOP_MAX || k > logits->shape[1])
+        fail(NT_ERR_VALUE, "token_logprobs: 1 to 64 alternatives, at most V");
+    }
+    if (logprob && !tokens)
+      fail(NT_ERR_RUNTIME, "token_logprobs: a log probability needs given tokens");
+    dispatch_float(logits->dtype, [&]<class T>() {
+      LpForward<T> a{};
+      a.z = row_view<const T>(logits, a.row_stride, "token_logprobs");
+      a.rows = rows;
+      a.V = int32_t(logits->shape[1]);
+      if (tokens)
+        a.tok = token_view(tokens, "token_logprobs");
+      a.ignore = ignore;
+      const int dt = logits->dtype;
+      a.logprob = out_vector<T>(logprob, rows, dt, "logprob");
+      a.entropy = out_vector<T>(entropy, rows, dt, "entropy");
+      a.stats = out_vector<T>(stats, 3 * rows, dt, "stats");
+      a.top_value = out_vector<T>(k ? top_logprobs : nullptr, rows * k, dt, "top_logprobs");
+      a.top_token =
+          out_vector<int64_t>(k ? top_tokens : nullptr, rows * k, NT_INT64, "top_tokens");
+      a.k = int(k);
+      a.splits = 1;
+      a.err = deferred_error_word();
+      if (rows)
+        run_forward(a);
+    });
+  });
+}
+
+int nt_token_logprobs_bwd(const nt_view *logits, const nt_view *tokens, int64_t ignore,
+                          const nt_view *stats, const nt_view *g_logprob,
+                          const nt_view *g_entropy, const nt_view *dlogits,
+                          int32_t accumulate) {
+  return guard([&] {
+    check_logits(logits, tokens, "token_logprobs_bwd");
+    check_view(dlogits, "token_logprobs_bwd");
+    require_same_shape(logits, dlogits, "token_logprobs_bwd");
+    require_same_dtype(logits, dlogits, "token_logprobs_bwd");
+    const int64_t rows = logits->shape[0];
+    for (const nt_view *g : {g_logprob, g_entropy}) {
+      if (g == nullptr)
+        continue;
+      check_view(g, "token_logprobs_bwd");
+      require_same_dtype(g, logits, "token_logprobs_bwd");
+      if (g->ndim != 1 || g->shape[0] != rows)
+        fail(NT_ERR_RUNTIME, "token_logprobs_bwd: one gradient per row");
+    }
+    if (g_logprob && !tokens)
+      fail(NT_ERR_RUNTIME, "token_logprobs_bwd: a log probability needs given tokens");
+    dispatch_float(logits->dtype, [&]<class T>() {
+      LpBackward<T> a{};
+      a.z = row_view<const T>(logits, a.row_stride, "token_logprobs_bwd");
+      a.dz = row_view<T>(dlogits, a.dz_stride, "token_logprobs_bwd");
+      a.rows = rows;
+      a.V = int32_t(logits->shape[1]);
+      if (tokens)
+        a.tok = token_view(tokens, "token_logprobs_bwd");
+      a.ignore = ignore;
+      a.stats = out_vector<const T>(stats, 3 * rows, logits->dtype, "stats");
+      if (a.stats == nullptr)
+        fail(NT_ERR_RUNTIME, "token_logprobs_bwd: stats missing");
+      if (g_logprob) {
+        a.ga = typed_ptr<const T>(g_logprob);
+        a.sa = g_logprob->strides[0];
+      }
+      if (g_entropy) {
+        a.gb = typed_ptr<const T>(g_entropy);
+        a.sb = g_entropy->strides[0];
+      }
+      if (rows == 0)
+        return;
+      if (accumulate)
+        run_backward<T, true>(a);
+      else
+        run_backward<T, false>(a);
+    });
+  });
+}
+
+} // extern "C"

@@ -3,7 +3,9 @@
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
+import os
 
 from . import _kernels as K
 from . import _lib
@@ -60,10 +62,23 @@ def arange(n: int, start: int = 0, step: int = 1, dtype: Dtype = dt.int64,
     return _factory((n,), st, requires_grad)
 
 
+# Dropout's generator: the key and the next call's offset.  Apart from the
+# stream of rand / randint, which dropout leaves as it is.
+_dropout_seed = int.from_bytes(os.urandom(8), "little")
+_dropout_calls = itertools.count()
+
+
 def manual_seed(seed: int) -> None:
     """Seeds the one generator behind rand / randint (host and device draws
-    continue the same stream)."""
+    continue the same stream), and dropout's."""
+    global _dropout_seed, _dropout_calls
     _lib.call("nt_manual_seed", int(seed) & (2**64 - 1))
+    _dropout_seed, _dropout_calls = int(seed) & (2**64 - 1), itertools.count()
+
+
+def next_dropout_counter() -> tuple[int, int]:
+    """(seed, offset) of the next dropout call without a seed of its own."""
+    return _dropout_seed, next(_dropout_calls)
 
 
 def _uniform(n: int, dtype: Dtype, device: Device) -> Storage:

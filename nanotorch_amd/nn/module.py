@@ -7,6 +7,8 @@ start on ``device`` (default "cuda").  ``Sigmoid`` is added next to ReLU and
 Tanh (the reference exposes sigmoid only as a function).  ``Linear.forward``
 on float32 device tensors runs the product and the bias add as one kernel
 (``LinearOp``): same values and gradients as the reference's two ops.
+``Embedding`` and ``Dropout`` are additions too, and with ``Dropout`` the
+modules' ``train`` / ``eval`` switch.
 """
 
 from __future__ import annotations
@@ -14,11 +16,12 @@ from __future__ import annotations
 import math
 from typing import Any, Sequence
 
-from ..autograd import ReluOp, SigmoidOp, TanhOp
+from ..autograd import EmbeddingOp, ReluOp, SigmoidOp, TanhOp
 from ..autograd.ops_binary import LinearOp
 from ..core import Tensor
 from ..cuda import Device
 from ..factories import rand, zeros
+from ..ops import dropout
 
 
 class Module:
@@ -30,6 +33,13 @@ class Module:
 
     def to(self, device: Device | str) -> "Module":
         return self
+
+    def train(self, mode: bool = True) -> "Module":
+        """Training (True) or answering (False): only Dropout differs."""
+        return self
+
+    def eval(self) -> "Module":
+        return self.train(False)
 
     def forward(self, *args: Any, **kwargs: Any) -> Any:
         raise NotImplementedError
@@ -67,6 +77,53 @@ class Linear(Module):
         return z
 
 
+class Embedding(Module):
+    """scale * W[tokens] with W [num_tokens, dim] drawn uniformly with unit
+    variance; a token equal to padding_idx gives zeros and trains nothing."""
+
+    def __init__(self, num_tokens: int, dim: int, scale: float = 1.0, *,
+                 padding_idx: int | None = None, device: Device | str = "cuda") -> None:
+        if num_tokens <= 0 or dim <= 0:
+            raise ValueError(
+                f"Cannot initialize Embedding with {num_tokens=}, {dim=} (non-positive)."
+            )
+        if padding_idx is not None and not 0 <= padding_idx < num_tokens:
+            raise ValueError(f"padding_idx {padding_idx} is no row of a table of {num_tokens}.")
+        z = math.sqrt(3.0)
+        w = 2 * rand(num_tokens, dim, device="cuda") * z - z
+        self._W = w.to(device)
+        self._W.enable_grad()
+        self._scale, self._padding_idx = scale, padding_idx
+
+    def parameters(self) -> Sequence[Tensor]:
+        return [self._W]
+
+    def to(self, device: Device | str) -> "Embedding":
+        self._W = self._W.to(device)
+        return self
+
+    def forward(self, tokens: Tensor) -> Tensor:
+        return EmbeddingOp.apply(self._W, tokens, self._scale, self._padding_idx)
+
+
+class Dropout(Module):
+    """Drops each element with probability p while training and scales the
+    others by 1 / (1 - p); passes its input on otherwise."""
+
+    def __init__(self, p: float = 0.5) -> None:
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"Dropout needs 0 <= p <= 1, got {p}.")
+        self._p = p
+        self._training = True
+
+    def train(self, mode: bool = True) -> "Dropout":
+        self._training = mode
+        return self
+
+    def forward(self, x: Tensor) -> Tensor:
+        return dropout(x, self._p) if self._training else x
+
+
 class ReLU(Module):
     def forward(self, x: Tensor) -> Tensor:
         return ReluOp.apply(x)
@@ -94,6 +151,11 @@ class Sequential(Module):
 
     def to(self, device: Device | str) -> "Sequential":
         self._modules = [m.to(device) for m in self._modules]
+        return self
+
+    def train(self, mode: bool = True) -> "Sequential":
+        for m in self._modules:
+            m.train(mode)
         return self
 
     def forward(self, *args: Any, **kwargs: Any) -> Any:

@@ -3,13 +3,16 @@
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 from . import _kernels as K
 from . import _lib
 from . import autograd
-from ._data_type import Dtype, promote_dtypes
+from ._data_type import Dtype, is_float, promote_dtypes
 from ._indexing import broadcast_shapes
+from .autograd.ops_token import RowOp, _as_rows, _check_tokens
 from .core import Tensor
+from .factories import next_dropout_counter
 
 
 def clone(x: Tensor) -> Tensor:
@@ -110,6 +113,87 @@ def sqrt(x: Tensor) -> Tensor:
 
 def sigmoid(x: Tensor) -> Tensor:
     return autograd.SigmoidOp.apply(x)
+
+
+def embedding(table: Tensor, tokens: Tensor, scale: float = 1.0, *,
+              padding_idx: int | None = None) -> Tensor:
+    """scale * table[tokens]: the rows of a [V, D] float table that int32 or
+    int64 tokens of any shape name, [*tokens.shape, D].
+
+    A token equal to ``padding_idx`` gives a zero row and no gradient.  Tokens
+    are checked on the device: one outside the table gives a zero row, and the
+    next synchronisation (``sync``, ``cpu``) raises IndexError.  The table's
+    gradient sums each row's terms in the order of the tokens, so it comes out
+    the same every time."""
+    return autograd.EmbeddingOp.apply(table, tokens, scale, padding_idx)
+
+
+def dropout(x: Tensor, p: float = 0.5, *, seed: int | None = None, offset: int = 0) -> Tensor:
+    """x / (1 - p) with each element kept with probability 1 - p, else 0.
+
+    Element i (row-major) is kept where word i mod 4 of Philox4x32-10 under the
+    64-bit key ``seed`` at the counter (i div 4, ``offset``) is at least
+    round(p * 2^32): one seed and offset give one mask, whatever x's strides,
+    and the backward pass draws it again.  Without a seed every call takes the
+    next offset of the generator that ``manual_seed`` sets."""
+    if seed is None:
+        seed, offset = next_dropout_counter()
+    return autograd.DropoutOp.apply(x, p, int(seed) & (2**64 - 1), int(offset) & (2**64 - 1))
+
+
+class TokenLogProbs(NamedTuple):
+    """What token_logprobs returns; None for what was not asked for."""
+
+    logprob: Tensor | None
+    entropy: Tensor | None
+    top_logprobs: Tensor | None
+    top_tokens: Tensor | None
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: bool = False,
+                   top: int = 0, ignore_index: int = -100) -> TokenLogProbs:
+    """Log probabilities under softmax over the last axis of float logits
+    [..., V], in one pass over them.
+
+    * ``logprob`` [...]: of the given int32 or int64 tokens [...];
+    * ``entropy`` [...]: -sum p log p of each row, if asked for;
+    * ``top_logprobs`` and ``top_tokens`` [..., top]: the most likely tokens,
+      0 <= top <= min(V, 64), ties to the lowest token; without a gradient.
+
+    ``logprob`` and ``entropy`` are differentiable, together in one pass.  A
+    row whose token is ``ignore_index`` is left out: logprob and entropy 0, no
+    gradient, alternatives -inf and -1.  Logits of -inf are tokens that cannot
+    occur; a row of nothing else has logprob -inf, entropy 0 and no gradient.
+    Tokens are checked on the device: one outside [0, V) leaves its row out,
+    and the next synchronisation (``sync``, ``cpu``) raises IndexError."""
+    shape = logits.shape
+    if not shape or not is_float(logits.dtype):
+        raise ValueError(f"Logits are float with an axis of tokens, got {logits.dtype.name} "
+                         f"{shape}.")
+    if not 0 <= top <= min(shape[-1], 64):
+        raise ValueError(f"top must lie in [0, min(V, 64)], got {top} with V = {shape[-1]}.")
+    if tokens is None:
+        if not entropy and not top:
+            raise ValueError("token_logprobs() needs tokens, entropy=True or top > 0.")
+    else:
+        _check_tokens(tokens)
+        if tokens.shape != shape[:-1]:
+            raise ValueError(f"One token for each row of {shape[:-1]}, got {tokens.shape}.")
+    extras = [] if top else [None, None]
+    logprob = ent = None
+    if tokens is None and not entropy:
+        _, _, value, token = K.token_logprobs(_as_rows(logits), None, ignore_index, False, top,
+                                              False)
+        extras = [Tensor._new_contiguous(s, shape[:-1] + (top,)) for s in (value, token)]
+    else:
+        out = autograd.TokenLogProbOp.apply(logits, tokens, ignore_index, entropy, top, extras)
+        if tokens is None:
+            ent = out
+        elif not entropy:
+            logprob = out
+        else:
+            logprob, ent = RowOp.apply(out, 0), RowOp.apply(out, 1)
+    return TokenLogProbs(logprob, ent, *extras)
 
 
 def _arg_reduce(op: int, name: str, x: Tensor, axis, keepdim: bool) -> Tensor:
