@@ -362,7 +362,7 @@ int nt_embedding(const nt_view *table, const nt_view *tokens, double scale,
  * zeros; with accumulate != 0 the sums are added to dtable and the other rows
  * stay as they are.  The order of the additions is fixed by the tokens and
  * the shapes alone.  g is contiguous [N, D]; dtable is [V, D] with adjacent
- * elements in each row.  N is below 2^31. */
+ * elements in each row.  N, V and D are below 2^30, here and in the lookup. */
 int nt_embedding_bwd(const nt_view *g, const nt_view *tokens, double scale,
                      int64_t padding, const nt_view *dtable, int32_t accumulate);
 
