@@ -33,19 +33,20 @@ template <class T, bool EVEN> struct RowPart {
       width = min(RV::N, D - col);
     }
   }
+  template <bool STREAM = false>
   __device__ __forceinline__ typename RV::V load(const T *row) const {
     if (EVEN || width == RV::N)
-      return RV::load(row + col);
+      return RV::template load<STREAM>(row + col);
     typename RV::V v = {};
     for (int j = 0; j < width; ++j)
       v[j] = row[col + j];
     return v;
   }
-  template <bool ACC>
+  template <bool ACC, bool STREAM = true>
   __device__ __forceinline__ void store(T *row, typename RV::V v) const {
     T *to = row + col;
     if (EVEN || (width == RV::N && skip == 0)) {
-      RV::store(to, ACC ? RV::load(to) + v : v);
+      RV::template store<STREAM>(to, ACC ? RV::load(to) + v : v);
     } else {
 #pragma unroll
       for (int j = 0; j < RV::N; ++j)
@@ -85,6 +86,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_kernel(
   typename RV::V v[EMB_LOOKUP];
   uint32_t row[EMB_LOOKUP];
   int64_t t[EMB_LOOKUP];
+  bool has[EMB_LOOKUP];
 #pragma unroll
   for (int k = 0; k < EMB_LOOKUP; ++k) {
     row[k] = vectors.div(min(first + k * EMB_THREADS, items - 1));
@@ -93,16 +95,17 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_kernel(
 #pragma unroll
   for (int k = 0; k < EMB_LOOKUP; ++k) {
     const uint32_t item = min(first + k * EMB_THREADS, items - 1);
-    v[k] = typename RV::V{};
-    if (rows.has(t[k]))
-      v[k] = RowPart<T, EVEN>(item - row[k] * vectors.d, D).load(table + t[k] * rs);
+    has[k] = rows.has(t[k]);
+    // row 0 in place of none, so that the loads need no branches
+    v[k] = RowPart<T, EVEN>(item - row[k] * vectors.d, D).load(table + (has[k] ? t[k] : 0) * rs);
   }
 #pragma unroll
   for (int k = 0; k < EMB_LOOKUP; ++k) {
     const uint32_t item = first + k * EMB_THREADS;
     if (item < items)
       RowPart<T, EVEN>(item - row[k] * vectors.d, D)
-          .template store<false>(out + (i0 + row[k]) * D, v[k] * scale);
+          .template store<false>(out + (i0 + row[k]) * D,
+                                 has[k] ? v[k] * scale : typename RV::V{});
   }
 }
 
@@ -230,6 +233,11 @@ struct SortPlan {
   Pairs side[2];    // pass k writes side[k & 1]
 };
 
+__device__ __forceinline__ uint32_t key_of(const SortPlan &p, uint32_t i) {
+  const int64_t t = p.tok[i];
+  return p.rows.has(t) ? uint32_t(t) : uint32_t(p.rows.V);
+}
+
 // A workgroup's pairs, in registers: each wave takes a contiguous part,
 // 64 adjacent pairs a round.
 struct SortRegs {
@@ -250,8 +258,7 @@ struct SortRegs {
       key[r] = pos[r] = 0;
       if (i < end) {
         if (pass == 0) {
-          const int64_t t = p.tok[i];
-          key[r] = p.rows.has(t) ? uint32_t(t) : uint32_t(p.rows.V);
+          key[r] = key_of(p, i);
           pos[r] = i;
         } else {
           key[r] = p.side[(pass - 1) & 1].key[i];
@@ -291,10 +298,8 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t (&sums)[SORT
 // goes through its rounds once: lanes of equal digit find each other by a
 // ballot per bit, take their places in lane order behind the rounds before
 // (`count`, per wave and digit), and the last of them moves the count on.
-// The counts then become the places where each wave's pairs of a digit start.
-// ALONE: the workgroup has all pairs; else `table` has every workgroup's
-// counts, and s.out comes from them.
-template <bool ALONE>
+// The counts then become the places where each wave's pairs of a digit start;
+// s.out comes from `table`, which has every workgroup's counts.
 __device__ __forceinline__ void sort_pass(const SortPlan &p, int pass, const SortRegs &x,
                                           SortShared &s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -330,7 +335,7 @@ __device__ __forceinline__ void sort_pass(const SortPlan &p, int pass, const Sor
   }
   // all workgroups' pairs of a digit, a digit per thread of the first EMB_BINS
   uint32_t total = 0, before = 0;
-  if (!ALONE && tid < EMB_BINS) {
+  if (tid < EMB_BINS) {
 #pragma unroll 8
     for (int b = 0; b < p.groups; ++b) {
       const uint32_t c = p.table[b * EMB_BINS + tid];
@@ -346,8 +351,7 @@ __device__ __forceinline__ void sort_pass(const SortPlan &p, int pass, const Sor
       own += s.count[w][tid];
   }
   const uint32_t first = sum_before(own, s.sums);
-  if (!ALONE)
-    before += sum_before(total, s.sums);
+  before += sum_before(total, s.sums);
   if (tid < EMB_BINS) {
     uint32_t at = first;
 #pragma unroll
@@ -356,7 +360,7 @@ __device__ __forceinline__ void sort_pass(const SortPlan &p, int pass, const Sor
       s.count[w][tid] = at;
       at += c;
     }
-    s.out[tid] = ALONE ? 0 : before - first;
+    s.out[tid] = before - first;
   }
   __syncthreads();
 #pragma unroll
@@ -397,27 +401,6 @@ __device__ __forceinline__ void set_present(const SortPlan &p, const SortRegs &x
         p.present[x.key[r]] = 1;
 }
 
-// All passes in one workgroup: n <= SORT_MOST.
-__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_kernel(SortPlan p) {
-  __shared__ SortShared s;
-  clear_present(p);
-  SortRegs x;
-  x.load(p, 0);
-  for (int pass = 0; pass < p.passes; ++pass) {
-    if (pass > 0)
-#pragma unroll
-      for (int r = 0; r < SORT_ROUNDS; ++r)
-        if (x.in(r)) {
-          const uint64_t v = s.pair[x.beg + r * WAVE + (threadIdx.x & 63)];
-          x.key[r] = uint32_t(v >> 32);
-          x.pos[r] = uint32_t(v);
-        }
-    sort_pass<true>(p, pass, x, s);
-  }
-  set_present(p, x); // cleared before sort_pass's barriers
-  sort_out(p, p.passes - 1, s);
-}
-
 // One pass over many workgroups: the counts, then the places.
 __global__ __launch_bounds__(SORT_THREADS) void embedding_count_kernel(SortPlan p, int pass) {
   __shared__ uint32_t bin[EMB_BINS];
@@ -443,7 +426,7 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_place_kernel(SortPlan 
   x.load(p, pass);
   if (pass == 0)
     set_present(p, x);
-  sort_pass<false>(p, pass, x, s);
+  sort_pass(p, pass, x, s);
   sort_out(p, pass, s);
 }
 
@@ -491,7 +474,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_sum_kernel(
     }
 #pragma unroll
     for (int j = 0; j < EMB_FLIGHT; ++j)
-      v[j] = part_of.load(g + int64_t(pos[j]) * p.D);
+      v[j] = part_of.template load<true>(g + int64_t(pos[j]) * p.D);
 #pragma unroll
     for (int j = 0; j < EMB_FLIGHT; ++j) {
       if (b + j >= end)
@@ -533,7 +516,80 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_fill_kernel(
     const uint32_t row = p.vectors.div(item);
     if (!present[row0 + row])
       RowPart<T, EVEN>(item - row * p.vectors.d, p.D)
-          .template store<false>(dw + (row0 + row) * p.rs, typename RowVec<T>::V{});
+          .template store<false, false>(dw + (row0 + row) * p.rs, typename RowVec<T>::V{});
+  }
+}
+
+// Up to RANK_MOST tokens are sorted in one launch: a workgroup takes 64 of
+// them, one per lane, and each of its waves counts, in its part of all
+// tokens, those that come before (smaller ones, and equal ones of smaller i).
+// The further workgroups write the zero rows meanwhile: each looks which of
+// its rows the tokens name.
+constexpr int RANK_MOST = 16384;
+constexpr int RANK_ROWS = 1024; // rows of a filling workgroup, at most
+
+template <class T, bool EVEN>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_rank_kernel(
+    SortPlan p, uint32_t ranking, uint32_t R, FastDivU32 vectors, int D, int64_t rs,
+    T *__restrict__ dw) {
+  __shared__ __align__(16) uint32_t key[RANK_MOST];
+  __shared__ uint32_t part[SORT_WAVES][WAVE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (blockIdx.x >= ranking) {
+    const uint32_t v0 = (blockIdx.x - ranking) * R, rows = min(R, uint32_t(p.rows.V) - v0);
+    for (uint32_t v = tid; v < rows; v += SORT_THREADS)
+      key[v] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < p.n; i += SORT_THREADS) {
+      const int64_t t = p.tok[i];
+      if (t >= v0 && t < int64_t(v0) + rows && t != p.rows.padding)
+        key[t - v0] = 1;
+    }
+    __syncthreads();
+    const uint32_t items = rows * vectors.d;
+#pragma unroll 4
+    for (uint32_t e = tid; e < items; e += SORT_THREADS) {
+      const uint32_t row = vectors.div(e);
+      if (!key[row])
+        RowPart<T, EVEN>(e - row * vectors.d, D)
+            .template store<false, false>(dw + (v0 + row) * rs, typename RowVec<T>::V{});
+    }
+    return;
+  }
+  const uint32_t padded = (p.n + 63) / 64 * 64;
+  for (uint32_t i = tid; i < padded; i += SORT_THREADS)
+    key[i] = i < p.n ? key_of(p, i) : ~0u; // past the end: before nothing
+  __syncthreads();
+  const uint32_t i0 = blockIdx.x * WAVE, i = i0 + lane;
+  const uint32_t mine = key[i];
+  const uint32_t per = (padded / WAVE + SORT_WAVES - 1) / SORT_WAVES * WAVE;
+  const uint32_t beg = min(padded, wave * per), end = min(padded, beg + per);
+  uint32_t n = 0;
+  const auto count = [&](uint32_t from, uint32_t to, uint32_t below) {
+    for (uint32_t j = from; j < to; j += 16) {
+      uint4 k[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        k[q] = reinterpret_cast<const uint4 *>(key + j)[q];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        n += (k[q].x < below) + (k[q].y < below) + (k[q].z < below) + (k[q].w < below);
+    }
+  };
+  count(beg, min(end, i0), mine + 1);
+  if (i0 >= beg && i0 < end)
+    for (int j = 0; j < WAVE; ++j)
+      n += key[i0 + j] < mine + (j < lane);
+  count(max(beg, i0 + WAVE), end, mine);
+  part[wave][lane] = n;
+  __syncthreads();
+  if (wave == 0 && i < p.n) {
+    uint32_t at = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w)
+      at += part[w][lane];
+    p.side[0].key[at] = mine;
+    p.side[0].pos[at] = i;
   }
 }
 
@@ -603,7 +659,7 @@ void run_embedding(const nt_view *table, const Tokens &tok, int64_t N,
   const Rows rows{V, padding, deferred_error_word()};
   const T *from = typed_ptr<const T>(table);
   T *to = typed_ptr<T>(out);
-  if (D > 1 && table->strides[1] != 1) {
+  if (V == 0 || (D > 1 && table->strides[1] != 1)) {
     const int64_t blocks = std::min<int64_t>((N * D + EMB_THREADS - 1) / EMB_THREADS,
                                              int64_t(1) << 22);
     embedding_strided_kernel<T><<<dim3(unsigned(blocks)), EMB_THREADS, 0, stream()>>>(
@@ -655,19 +711,31 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
   p.n = uint32_t(N);
   p.passes = (bits + EMB_DIGIT - 1) / EMB_DIGIT;
   p.digit = (bits + p.passes - 1) / p.passes;
-  // up to 64 workgroups of at least 2048 pairs; more once those are full
-  const int64_t per = std::clamp<int64_t>((N + 63) / 64, 2048, SORT_MOST);
-  p.per = N <= SORT_MOST ? SORT_MOST : uint32_t((per + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS);
-  p.groups = int((N + p.per - 1) / p.per);
-  DeviceScratch table(size_t(p.groups) * EMB_BINS * 4), pairs(size_t(N) * 16),
-      present(ACC ? 0 : size_t(V));
-  p.table = table.get<uint32_t>();
-  p.present = present.get<uint8_t>();
+  const uint32_t vectors = row_vectors<T>(D);
+  T *const to = typed_ptr<T>(dw);
+  // a filling workgroup's rows: about 2^15 vectors, which take longer to
+  // write than the tokens to read, and fewer than 2^32 in any case
+  const uint32_t R = std::clamp<uint32_t>((1u << 15) / vectors, 1, RANK_ROWS);
+  const bool ranked = N <= RANK_MOST && (ACC || (V + R - 1) / R < int64_t(1) << 20);
+  DeviceScratch pairs(size_t(N) * (ranked ? 8 : 16));
   uint32_t *const base = pairs.get<uint32_t>();
   p.side[0] = {base, base + N};
-  p.side[1] = {base + 2 * N, base + 3 * N};
-  if (p.groups == 1) {
-    embedding_sort_kernel<<<dim3(1), SORT_THREADS, 0, s>>>(p);
+  if (!ranked)
+    p.side[1] = {base + 2 * N, base + 3 * N};
+  // up to 64 workgroups of at least 2048 pairs; more once those are full
+  const int64_t per = std::clamp<int64_t>((N + 63) / 64, 2048, SORT_MOST);
+  p.per = uint32_t((per + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS);
+  p.groups = int((N + p.per - 1) / p.per);
+  DeviceScratch table(ranked ? 0 : size_t(p.groups) * EMB_BINS * 4),
+      present(ACC || ranked ? 0 : size_t(V));
+  p.table = table.get<uint32_t>();
+  p.present = present.get<uint8_t>();
+  if (ranked) {
+    p.passes = 1;
+    const uint32_t ranking = uint32_t((N + WAVE - 1) / WAVE);
+    const uint32_t filling = ACC ? 0 : uint32_t((V + R - 1) / R);
+    embedding_rank_kernel<T, EVEN><<<dim3(ranking + filling), SORT_THREADS, 0, s>>>(
+        p, ranking, R, FastDivU32(vectors), int(D), dw->strides[0], to);
     NT_LAUNCH_CHECK();
   } else {
     for (int k = 0; k < p.passes; ++k) {
@@ -677,13 +745,11 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
       NT_LAUNCH_CHECK();
     }
   }
-  const uint32_t vectors = row_vectors<T>(D);
   const Pairs &sorted = p.side[(p.passes - 1) & 1];
   const SumPlan q{sorted.key, sorted.pos, p.n, uint32_t(V), FastDivU32(vectors), int(D),
                   dw->strides[0]};
   const int64_t tiles = (N + EMB_TILE - 1) / EMB_TILE;
   DeviceScratch part(size_t(2 * tiles * vectors) * 16);
-  T *const to = typed_ptr<T>(dw);
   in_launches(tiles, vectors, [&](int64_t t0, int64_t n) {
     embedding_sum_kernel<T, ACC, EVEN>
         <<<dim3(blocks_for(n * vectors, EMB_THREADS)), EMB_THREADS, 0, s>>>(
@@ -697,7 +763,7 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
             q, scale, to, part.get<T>(), uint32_t(t0), uint32_t(n * vectors));
     NT_LAUNCH_CHECK();
   });
-  if (!ACC)
+  if (!ACC && !ranked)
     in_launches(V, vectors, [&](int64_t r0, int64_t n) {
       embedding_fill_kernel<T, EVEN>
           <<<dim3(blocks_for(n * vectors, EMB_THREADS * EMB_FILL)), EMB_THREADS, 0, s>>>(
