@@ -385,23 +385,25 @@ def dropout(x, p: float, seed: int, offset: int, target=None) -> "Storage | None
 
 
 def token_logprobs(z, tokens, ignore: int, entropy: bool, top: int, stats: bool):
-    """(results, stats, top_logprobs, top_tokens) of [rows, V] logits: results
-    holds the log probabilities (if tokens are given), then the entropies (if
-    wanted), rows of each; what is not wanted is None."""
+    """(results, top_logprobs, top_tokens) of [rows, V] logits.  results holds
+    rows of each of: the log probabilities (if tokens are given), the entropies
+    (if wanted), and last the three statistics that the backward pass needs (if
+    wanted): one buffer, since each allocation costs the host a microsecond.
+    What is not wanted is None."""
     require_device(z) if tokens is None else require_device(z, tokens)
     rows, dtype = z._shape[0], z._storage._dtype
     given = tokens is not None
-    out = st = value = token = None
-    v_lp = v_h = v_st = v_value = v_token = None
-    if given or entropy:
-        out = Storage.allocate(rows * (given + entropy), dtype, Device.Cuda)
+    n = given + entropy
+    out = value = token = v_lp = v_h = v_st = v_value = v_token = None
+    if n or stats:
+        out = Storage.allocate(rows * (n + 3 * stats), dtype, Device.Cuda)
+        ptr = out._ptr
         if given:
-            v_lp = _lib.pack_view(out._ptr, 0, dtype, (rows,), (1,))
+            v_lp = _lib.pack_view(ptr, 0, dtype, (rows,), (1,))
         if entropy:
-            v_h = _lib.pack_view(out._ptr, rows * given, dtype, (rows,), (1,))
-    if stats:
-        st = Storage.allocate(3 * rows, dtype, Device.Cuda)
-        v_st = _lib.pack_view(st._ptr, 0, dtype, (3, rows), (rows, 1))
+            v_h = _lib.pack_view(ptr, rows * given, dtype, (rows,), (1,))
+        if stats:
+            v_st = _lib.pack_view(ptr, rows * n, dtype, (3, rows), (rows, 1))
     if top:
         value = Storage.allocate(rows * top, dtype, Device.Cuda)
         token = Storage.allocate(rows * top, Dtype.Int64, Device.Cuda)
@@ -409,14 +411,15 @@ def token_logprobs(z, tokens, ignore: int, entropy: bool, top: int, stats: bool)
         v_token = _packed_flat(token, (rows, top))
     _lib.call_packed("nt_token_logprobs", _packed(z), _packed(tokens) if given else None,
                      ignore, v_lp, v_h, v_st, v_value, v_token)
-    return out, st, value, token
+    return out, value, token
 
 
-def token_logprobs_bwd(z, tokens, ignore: int, stats: Storage, ga, gb,
+def token_logprobs_bwd(z, tokens, ignore: int, results: Storage, ga, gb,
                        target) -> "Storage | None":
     """The gradient of [rows, V] logits from 1-D gradients ga of the log
     probabilities and gb of the entropies (None: zero); added to `target`
-    (adjacent elements in each row) when given, else a new storage."""
+    (adjacent elements in each row) when given, else a new storage.  `results`
+    is token_logprobs's buffer, the statistics at its end."""
     rows = z._shape[0]
     if target is None:
         out = Storage.allocate(_numel(z._shape), z._storage._dtype, Device.Cuda)
@@ -425,7 +428,8 @@ def token_logprobs_bwd(z, tokens, ignore: int, stats: Storage, ga, gb,
         out, v_out = None, _packed(target)
     _lib.call_packed("nt_token_logprobs_bwd", _packed(z),
                      _packed(tokens) if tokens is not None else None, ignore,
-                     _lib.pack_view(stats._ptr, 0, stats._dtype, (3, rows), (rows, 1)),
+                     _lib.pack_view(results._ptr, results._size - 3 * rows, results._dtype,
+                                    (3, rows), (rows, 1)),
                      _packed(ga) if ga is not None else None,
                      _packed(gb) if gb is not None else None, v_out, int(target is not None))
     if target is not None:

@@ -20,7 +20,7 @@ from .grad_mode import is_grad_enabled
 
 
 def _check_tokens(tokens: Tensor) -> None:
-    if not is_int(tokens.dtype):
+    if not is_int(tokens._storage._dtype):
         raise ValueError(f"Tokens must be int32 or int64, got {tokens.dtype.name}.")
 
 
@@ -66,7 +66,7 @@ class EmbeddingOp(Function):
     def forward(self, table: Tensor, tokens: Tensor, scale: float = 1.0,
                 padding_idx: int | None = None) -> Tensor:
         shape = table._shape
-        if len(shape) != 2 or not is_float(table.dtype):
+        if len(shape) != 2 or not is_float(table._storage._dtype):
             raise ValueError(
                 f"An embedding table is 2-D and float, got {table.dtype.name} {shape}.")
         _check_tokens(tokens)
@@ -120,7 +120,7 @@ class DropoutOp(Function):
     index i.  The mask is drawn again in the backward pass, never stored."""
 
     def forward(self, x: Tensor, p: float, seed: int, offset: int) -> Tensor:
-        if not is_float(x.dtype):
+        if not is_float(x._storage._dtype):
             raise ValueError(f"dropout() needs a float tensor, got {x.dtype.name}.")
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout() needs 0 <= p <= 1, got {p}.")
@@ -173,15 +173,14 @@ class TokenLogProbOp(Function):
         z = _as_rows(logits)
         flat = None if tokens is None else _vector(tokens)
         keep = is_grad_enabled() and logits.requires_grad
-        out, self._stats, value, token = K.token_logprobs(
-            z, flat, ignore_index, entropy, top, keep)
+        out, value, token = K.token_logprobs(z, flat, ignore_index, entropy, top, keep)
         if top:
             extras.append(Tensor._new_contiguous(value, lead + (top,)))
             extras.append(Tensor._new_contiguous(token, lead + (top,)))
         self._both = entropy and tokens is not None
         if keep:
             self.save_for_backward(*((logits,) if tokens is None else (logits, tokens)))
-            self._call = (z, flat, ignore_index)
+            self._call = (z, flat, ignore_index, out)
             self._shape = logits._shape
         shape = (2,) + lead if self._both else lead
         return Tensor._unchecked_view(out, shape, row_major_strides(shape), 0)
@@ -198,7 +197,7 @@ class TokenLogProbOp(Function):
 
     def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
         self.saved_tensors  # raises if logits or tokens were modified in place
-        z, flat, ignore = self._call
+        z, flat, ignore, results = self._call
         rows = z._shape[0]
         if g.dtype != z.dtype:
             g = g.to(z.dtype)
@@ -209,7 +208,7 @@ class TokenLogProbOp(Function):
             g = _vector(g)
             ga, gb = (None, g) if flat is None else (g, None)
         into = None if target is None else _rows_in_place(target)
-        st = K.token_logprobs_bwd(z, flat, ignore, self._stats, ga, gb, into)
+        st = K.token_logprobs_bwd(z, flat, ignore, results, ga, gb, into)
         if into is not None:
             return target
         if target is not None:

@@ -22,8 +22,10 @@
 // The alternatives are the k largest logits, ties to the lowest token, NaN
 // above every number.  Each wave keeps its own k best, the i-th in lane i;
 // a chunk's elements are looked at one by one only where some lane's maximum
-// (which the pass computes anyway) exceeds the k-th best so far: about
-// k ln(n / k) times in n elements of random order.
+// (which the pass computes anyway) exceeds the k-th best so far, and the first
+// chunk's only where they reach the k-th largest of the maxima of all lanes
+// that share the row: in n elements of random order about k (1 + ln(n / c))
+// of them, c being a chunk.
 #include "tokens.h"
 
 #include <algorithm>
@@ -31,6 +33,9 @@
 
 namespace nt {
 
+#ifndef XB
+#define XB 2
+#endif
 constexpr int LP_THREADS = 256;
 constexpr int LP_WAVES = LP_THREADS / WAVE;
 constexpr int LP_UNROLL = 4;  // vectors in flight per lane
@@ -59,6 +64,44 @@ template <class T> __device__ __forceinline__ T not_below_cut(T d) {
 // The larger one; NaN if either is.
 template <class T> __device__ __forceinline__ T max_nan(T a, T b) {
   return __builtin_elementwise_maximum(a, b);
+}
+
+// A lane's value from the lane that the data-parallel control CTRL names;
+// `none` where there is no such lane or ROWS leaves the lane's row out.
+template <int CTRL, int ROWS, class T> __device__ __forceinline__ T from_lane(T v, T none) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(
+        T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none),
+                                       __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else {
+    const uint64_t a = __builtin_bit_cast(uint64_t, none), b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(int(a), int(b), CTRL, ROWS, 0xf, false);
+    const uint32_t hi =
+        __builtin_amdgcn_update_dpp(int(a >> 32), int(b >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(T, uint64_t(hi) << 32 | lo);
+  }
+}
+constexpr int DPP_ROW_SHR = 0x110, DPP_WAVE_SHR1 = 0x138, DPP_BCAST15 = 0x142,
+              DPP_BCAST31 = 0x143;
+
+__device__ __forceinline__ uint32_t read_lane(uint32_t v, int l) {
+  return __builtin_amdgcn_readlane(v, l);
+}
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int l) {
+  return uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(v >> 32), l))) << 32 |
+         uint32_t(__builtin_amdgcn_readlane(uint32_t(v), l));
+}
+
+// f over the wave's values, in every lane; `none` is f's neutral value.
+template <class T, class F> __device__ __forceinline__ T over_wave(T v, T none, F f) {
+  v = f(v, from_lane<DPP_ROW_SHR + 1, 0xf>(v, none));
+  v = f(v, from_lane<DPP_ROW_SHR + 2, 0xf>(v, none));
+  v = f(v, from_lane<DPP_ROW_SHR + 4, 0xf>(v, none));
+  v = f(v, from_lane<DPP_ROW_SHR + 8, 0xf>(v, none));
+  v = f(v, from_lane<DPP_BCAST15, 0xa>(v, none));
+  v = f(v, from_lane<DPP_BCAST31, 0xc>(v, none));
+  using I = std::conditional_t<sizeof(T) == 4, uint32_t, uint64_t>;
+  return __builtin_bit_cast(T, read_lane(__builtin_bit_cast(I, v), WAVE - 1));
 }
 
 template <class T> struct RowState {
@@ -93,16 +136,11 @@ template <class T> struct RowState {
   }
   // Every lane gets the wave's state.
   __device__ __forceinline__ void join_lanes() {
-    for (int k = 1; k < WAVE; k <<= 1) {
-      RowState o;
-      o.m = __shfl_xor(m, k);
-      o.s = __shfl_xor(s, k);
-      o.u = __shfl_xor(u, k);
-      join(o);
-    }
-    m = __shfl(m, 0);
-    s = __shfl(s, 0);
-    u = __shfl(u, 0);
+    move_to(over_wave(m, -std::numeric_limits<T>::infinity(),
+                      [](T a, T b) { return max_nan(a, b); }));
+    const auto add = [](T a, T b) { return a + b; };
+    s = over_wave(s, T(0), add);
+    u = over_wave(u, T(0), add);
   }
 };
 
@@ -140,34 +178,24 @@ template <> struct Key<double> {
   }
 };
 
-__device__ __forceinline__ uint32_t read_lane(uint32_t v, int l) {
-  return __builtin_amdgcn_readlane(v, l);
-}
-__device__ __forceinline__ uint64_t read_lane(uint64_t v, int l) {
-  return uint64_t(__builtin_amdgcn_readlane(uint32_t(v >> 32), l)) << 32 |
-         uint32_t(__builtin_amdgcn_readlane(uint32_t(v), l));
-}
+constexpr int RAISE_BITS = 20; // sign, exponent and 11 (of a double, 8) bits more
 
-// A wave's best `k` entries in falling order, the i-th in lane i.
+// A wave's best entries in falling order, the i-th in lane i.
 template <class T> struct TopList {
   using K = typename Key<T>::K;
   K key = 0;
   int32_t token = -1;
-  K least = 0; // the k-th key: what an entry has to exceed
+  K least = 0; // what an entry has to exceed to be among the k best
 
   __device__ __forceinline__ void insert(K v, int32_t t, int k) {
-    const int lane = threadIdx.x & 63;
-    const int pos = __popcll(__ballot(key >= v));
-    const K up = __shfl_up(key, 1);
-    const int32_t up_t = __shfl_up(token, 1);
-    if (lane == pos) {
-      key = v;
-      token = t;
-    } else if (lane > pos && lane < k) {
-      key = up;
-      token = up_t;
-    }
-    least = read_lane(key, k - 1);
+    // Lanes of smaller keys move on by one: each key becomes the middle one
+    // of itself, its neighbour's (no smaller) and v.
+    const K up = from_lane<DPP_WAVE_SHR1, 0xf>(key, ~K(0));
+    const int32_t up_t = from_lane<DPP_WAVE_SHR1, 0xf>(token, 0);
+    const bool stays = key >= v, here = up >= v;
+    token = stays ? token : here ? t : up_t;
+    key = stays ? key : here ? v : up;
+    least = max(least, read_lane(key, k - 1));
   }
   // One entry per lane, in rising order of their tokens among equal keys.
   __device__ __forceinline__ void insert_lanes(K v, int32_t t, int k) {
@@ -179,6 +207,24 @@ template <class T> struct TopList {
       if (c > least)
         insert(c, int32_t(read_lane(uint32_t(t), l)), k);
     }
+  }
+  // Of the lanes' keys x, N each, the k-th largest is found bit by bit, its
+  // leading RAISE_BITS; nothing below it is among the k best of anything that
+  // holds those keys.
+  template <int N> __device__ __forceinline__ void raise(const K (&x)[N], int k) {
+    K at = 0;
+#pragma unroll
+    for (int b = 0; b < RAISE_BITS; ++b) {
+      const K up = at | K(1) << (8 * sizeof(K) - 1 - b);
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        n += __popcll(__ballot(x[j] >= up));
+      at = n >= k ? up : at;
+    }
+    // just below it; no logit has the key below 0's (that of -0)
+    if (at)
+      least = max(least, at - (at == Key<T>::of(T(0)) ? 2 : 1));
   }
 };
 
@@ -264,10 +310,11 @@ __device__ __forceinline__ bool row_left_out(const LpForward<T> &a, int64_t row,
   return false;
 }
 
-// Elements beg .. end - 1 of a row into the wave's state and list.
-template <class T, bool TOP>
+// Elements beg .. end - 1 of a row into the wave's state and list; `first`
+// gets each lane's largest key of the first chunk.
+template <class T, bool TOP, bool STREAM, class F>
 __device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k,
-                                     RowState<T> &r, TopList<T> &top) {
+                                     RowState<T> &r, TopList<T> &top, F &&first) {
   using RV = RowVec<T>;
   constexpr int N = RV::N, CHUNK = WAVE * N * LP_UNROLL;
   const int lane = threadIdx.x & 63;
@@ -278,7 +325,7 @@ __device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k
     for (int c = 0; c < LP_UNROLL; ++c) {
       const int64_t i = b + (c * WAVE + lane) * N;
       if (i + N <= end) {
-        const typename RV::V w = RV::load(z + i);
+        const typename RV::V w = RV::template load<STREAM>(z + i);
 #pragma unroll
         for (int j = 0; j < N; ++j)
           v[c * N + j] = w[j];
@@ -293,28 +340,32 @@ __device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k
     for (int j = 1; j < LP_UNROLL * N; ++j)
       most = max_nan(most, v[j]);
     if constexpr (TOP) {
-      const T least = Key<T>::value(top.least); // NaN while there are fewer than k
+      if (b == beg)
+        first(Key<T>::of(most));
+      // NaN, which nothing is below, while there is no such bound
+      const T least = Key<T>::value(top.least);
       if (__ballot(!(most <= least))) {
 #pragma unroll
         for (int c = 0; c < LP_UNROLL; ++c) {
           const int64_t i = b + (c * WAVE + lane) * N;
-          typename Key<T>::K key[N];
-          bool any = false;
+          uint32_t hits = 0; // a bit per element
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            key[j] = i + j < end ? Key<T>::of(v[c * N + j]) : 0;
-            any |= key[j] > top.least;
-          }
-          uint64_t m = __ballot(any);
-          while (m) {
+          for (int j = 0; j < N; ++j)
+            hits |= uint32_t(!(v[c * N + j] <= least) && i + j < end) << j;
+          uint64_t m = __ballot(hits != 0);
+          while (m) { // lane by lane, element by element: in rising order
             const int l = __ffsll((unsigned long long)m) - 1;
             m &= m - 1;
+            const uint32_t h = read_lane(hits, l);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-              const typename Key<T>::K x = read_lane(key[j], l);
-              if (x > top.least)
-                top.insert(x, int32_t(b + (c * WAVE + l) * N + j), k);
-            }
+            for (int j = 0; j < N; ++j)
+              if (h >> j & 1) {
+                using K = typename Key<T>::K;
+                const K x = Key<T>::of(__builtin_bit_cast(
+                    T, read_lane(__builtin_bit_cast(K, v[c * N + j]), l)));
+                if (x > top.least)
+                  top.insert(x, int32_t(b) + (c * WAVE + l) * N + j, k);
+              }
           }
         }
       }
@@ -335,13 +386,17 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a
     return write_left_out(a, row);
   RowState<T> r;
   TopList<T> top;
-  walk<T, TOP>(a.z + row * a.row_stride, 0, a.V, a.k, r, top);
+  walk<T, TOP, false>(a.z + row * a.row_stride, 0, a.V, a.k, r, top,
+                      [&](typename Key<T>::K x) {
+                        const typename Key<T>::K one[1] = {x};
+                        top.raise(one, a.k);
+                      });
   r.join_lanes();
   write_row(a, row, t, r, top);
 }
 
 // `splits` workgroups per row, each wave a part of `part` elements.
-template <class T, bool TOP>
+template <class T, bool TOP, bool STREAM>
 __global__ __launch_bounds__(LP_THREADS) void logprob_group_kernel(LpForward<T> a,
                                                                    int64_t row0) {
   __shared__ T sm[3][LP_WAVES];
@@ -359,9 +414,21 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_group_kernel(LpForward<T> 
   RowState<T> r;
   TopList<T> top;
   const int64_t beg = int64_t(split * LP_WAVES + wave) * a.part;
+  const auto first = [&](typename Key<T>::K x) { // by all waves together
+    __shared__ typename Key<T>::K most[LP_WAVES][WAVE];
+    most[wave][lane] = x;
+    __syncthreads();
+    typename Key<T>::K all[LP_WAVES];
+#pragma unroll
+    for (int w = 0; w < LP_WAVES; ++w)
+      all[w] = most[w][lane];
+    top.raise(all, a.k);
+  };
   if (beg < a.V)
-    walk<T, TOP>(a.z + row * a.row_stride, int32_t(beg),
-                 int32_t(std::min<int64_t>(a.V, beg + a.part)), a.k, r, top);
+    walk<T, TOP, STREAM>(a.z + row * a.row_stride, int32_t(beg),
+                         int32_t(std::min<int64_t>(a.V, beg + a.part)), a.k, r, top, first);
+  else if (TOP)
+    first(0);
   r.join_lanes();
   if (lane == 0) {
     sm[0][wave] = r.m;
@@ -446,8 +513,8 @@ template <class T> struct LpBackward {
 };
 
 // A workgroup of W waves per row, or (W = 1) four rows per workgroup, each
-// lane LP_UNROLL vectors.
-template <class T, int W, bool ACC>
+// lane UNROLL vectors.
+template <class T, int W, int UNROLL, bool ACC>
 __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a,
                                                                  int64_t row0, int chunks) {
   using RV = RowVec<T>;
@@ -461,7 +528,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a
     first = (threadIdx.x & 63) * N;
   } else {
     row = row0 + blockIdx.x / chunks;
-    first = (blockIdx.x % chunks) * (LP_THREADS * N * LP_UNROLL) + threadIdx.x * N;
+    first = (blockIdx.x % chunks) * (LP_THREADS * N * UNROLL) + threadIdx.x * N;
   }
   constexpr int STEP = W * WAVE * N;
   const int64_t t = a.tok.p ? a.tok[row] : 0;
@@ -470,7 +537,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a
   T *dz = a.dz + row * a.dz_stride;
   if (none) {
     if (!ACC)
-      for (int c = 0; c < LP_UNROLL; ++c)
+      for (int c = 0; c < UNROLL; ++c)
         for (int j = 0; j < N; ++j) {
           const int64_t i = int64_t(first) + c * STEP + j;
           if (i < a.V)
@@ -484,7 +551,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a
   const T c0 = -ga - gb * (H - log_s), c1 = -gb;
   const T *z = a.z + row * a.row_stride;
 #pragma unroll
-  for (int c = 0; c < LP_UNROLL; ++c) {
+  for (int c = 0; c < UNROLL; ++c) {
     const int64_t i = int64_t(first) + c * STEP;
     if (i >= a.V)
       break;
@@ -574,10 +641,17 @@ template <class T> void run_forward(LpForward<T> a) {
   a.pu = a.ps + n;
   a.pkey = keys.get<typename Key<T>::K>();
   a.ptoken = toks.get<int32_t>();
+  // logits that outgrow the 256 MB Infinity Cache are streamed past it
+  const bool stream_in = a.rows * int64_t(a.V) * int64_t(sizeof(T)) > int64_t(256) << 20;
+  const auto group = [&](auto top, auto streams) {
+    launch(logprob_group_kernel<T, top.value, streams.value>, LP_THREADS, 1, a.splits);
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
   if (a.k)
-    launch(logprob_group_kernel<T, true>, LP_THREADS, 1, a.splits);
+    stream_in ? group(Yes{}, Yes{}) : group(Yes{}, No{});
   else
-    launch(logprob_group_kernel<T, false>, LP_THREADS, 1, a.splits);
+    stream_in ? group(No{}, Yes{}) : group(No{}, No{});
   if (a.splits == 1)
     return;
   if (a.k)
@@ -587,8 +661,10 @@ template <class T> void run_forward(LpForward<T> a) {
 }
 
 template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
-  constexpr int SPAN = LP_THREADS * RowVec<T>::N * LP_UNROLL; // of a workgroup
-  const bool small = a.V <= SPAN / LP_WAVES;
+  constexpr int ONE = LP_UNROLL, MANY = XB; // vectors per lane
+  constexpr int WAVE_SPAN = WAVE * RowVec<T>::N * ONE;
+  constexpr int SPAN = LP_THREADS * RowVec<T>::N * MANY; // of a workgroup
+  const bool small = a.V <= WAVE_SPAN;
   const int64_t chunks = small ? 1 : (a.V + SPAN - 1) / SPAN;
   const int64_t per = small ? LP_WAVES : 1;
   const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / chunks) * per;
@@ -596,9 +672,9 @@ template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
     const int64_t rows = std::min(a.rows - r, most);
     const dim3 grid{unsigned((rows + per - 1) / per * chunks)};
     if (small)
-      logprob_bwd_kernel<T, 1, ACC><<<grid, LP_THREADS, 0, stream()>>>(a, r, 1);
+      logprob_bwd_kernel<T, 1, ONE, ACC><<<grid, LP_THREADS, 0, stream()>>>(a, r, 1);
     else
-      logprob_bwd_kernel<T, LP_WAVES, ACC>
+      logprob_bwd_kernel<T, LP_WAVES, MANY, ACC>
           <<<grid, LP_THREADS, 0, stream()>>>(a, r, int(chunks));
     NT_LAUNCH_CHECK();
   }

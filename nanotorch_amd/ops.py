@@ -166,8 +166,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
     occur; a row of nothing else has logprob -inf, entropy 0 and no gradient.
     Tokens are checked on the device: one outside [0, V) leaves its row out,
     and the next synchronisation (``sync``, ``cpu``) raises IndexError."""
-    shape = logits.shape
-    if not shape or not is_float(logits.dtype):
+    shape = logits._shape
+    if not shape or not is_float(logits._storage._dtype):
         raise ValueError(f"Logits are float with an axis of tokens, got {logits.dtype.name} "
                          f"{shape}.")
     if not 0 <= top <= min(shape[-1], 64):
@@ -177,12 +177,12 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
             raise ValueError("token_logprobs() needs tokens, entropy=True or top > 0.")
     else:
         _check_tokens(tokens)
-        if tokens.shape != shape[:-1]:
+        if tokens._shape != shape[:-1]:
             raise ValueError(f"One token for each row of {shape[:-1]}, got {tokens.shape}.")
     extras = [] if top else [None, None]
     logprob = ent = None
     if tokens is None and not entropy:
-        _, _, value, token = K.token_logprobs(_as_rows(logits), None, ignore_index, False, top,
+        _, value, token = K.token_logprobs(_as_rows(logits), None, ignore_index, False, top,
                                               False)
         extras = [Tensor._new_contiguous(s, shape[:-1] + (top,)) for s in (value, token)]
     else:
