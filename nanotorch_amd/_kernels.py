@@ -385,33 +385,29 @@ def dropout(x, p: float, seed: int, offset: int, target=None) -> "Storage | None
 
 
 def token_logprobs(z, tokens, ignore: int, entropy: bool, top: int, stats: bool):
-    """(results, top_logprobs, top_tokens) of [rows, V] logits.  results holds
+    """(results, tokens of the alternatives) of [rows, V] logits.  results holds
     rows of each of: the log probabilities (if tokens are given), the entropies
-    (if wanted), and last the three statistics that the backward pass needs (if
-    wanted): one buffer, since each allocation costs the host a microsecond.
-    What is not wanted is None."""
+    (if wanted), the alternatives' log probabilities [rows, top], and last the
+    three statistics that the backward pass needs (if wanted).  One buffer,
+    since each allocation costs the host a microsecond or two."""
     require_device(z) if tokens is None else require_device(z, tokens)
     rows, dtype = z._shape[0], z._storage._dtype
     given = tokens is not None
     n = given + entropy
-    out = value = token = v_lp = v_h = v_st = v_value = v_token = None
-    if n or stats:
-        out = Storage.allocate(rows * (n + 3 * stats), dtype, Device.Cuda)
-        ptr = out._ptr
-        if given:
-            v_lp = _lib.pack_view(ptr, 0, dtype, (rows,), (1,))
-        if entropy:
-            v_h = _lib.pack_view(ptr, rows * given, dtype, (rows,), (1,))
-        if stats:
-            v_st = _lib.pack_view(ptr, rows * n, dtype, (3, rows), (rows, 1))
+    out = Storage.allocate(rows * (n + top + 3 * stats), dtype, Device.Cuda)
+    ptr, pack = out._ptr, _lib.pack_view
+    token = v_value = v_token = None
     if top:
-        value = Storage.allocate(rows * top, dtype, Device.Cuda)
         token = Storage.allocate(rows * top, Dtype.Int64, Device.Cuda)
-        v_value = _packed_flat(value, (rows, top))
+        v_value = pack(ptr, rows * n, dtype, (rows, top), (top, 1))
         v_token = _packed_flat(token, (rows, top))
-    _lib.call_packed("nt_token_logprobs", _packed(z), _packed(tokens) if given else None,
-                     ignore, v_lp, v_h, v_st, v_value, v_token)
-    return out, value, token
+    _lib.call_packed(
+        "nt_token_logprobs", _packed(z), _packed(tokens) if given else None, ignore,
+        pack(ptr, 0, dtype, (rows,), (1,)) if given else None,
+        pack(ptr, rows * given, dtype, (rows,), (1,)) if entropy else None,
+        pack(ptr, rows * (n + top), dtype, (3, rows), (rows, 1)) if stats else None,
+        v_value, v_token)
+    return out, token
 
 
 def token_logprobs_bwd(z, tokens, ignore: int, results: Storage, ga, gb,

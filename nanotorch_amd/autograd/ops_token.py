@@ -173,10 +173,10 @@ class TokenLogProbOp(Function):
         z = _as_rows(logits)
         flat = None if tokens is None else _vector(tokens)
         keep = is_grad_enabled() and logits.requires_grad
-        out, value, token = K.token_logprobs(z, flat, ignore_index, entropy, top, keep)
+        out, token = K.token_logprobs(z, flat, ignore_index, entropy, top, keep)
         if top:
-            extras.append(Tensor._new_contiguous(value, lead + (top,)))
-            extras.append(Tensor._new_contiguous(token, lead + (top,)))
+            n = entropy + (tokens is not None)
+            extras.extend(top_views(out, n * z._shape[0], token, lead + (top,)))
         self._both = entropy and tokens is not None
         if keep:
             self.save_for_backward(*((logits,) if tokens is None else (logits, tokens)))
@@ -222,6 +222,14 @@ class TokenLogProbOp(Function):
     @classmethod
     def mem_bytes(cls, logits: Tensor, *args) -> int:
         return logits.numel * sizeof(logits.dtype)
+
+
+def top_views(out, offset: int, token, shape) -> tuple[Tensor, Tensor]:
+    """The alternatives' log probabilities, in `out` from `offset` on, and
+    their tokens."""
+    strides = row_major_strides(shape)
+    return (Tensor._unchecked_view(out, shape, strides, offset),
+            Tensor._unchecked_view(token, shape, strides, 0))
 
 
 class RowOp(Function):

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_strided_kernel(
 
 // ------------------------------------------------- gradient, few tokens
 
-constexpr int EMB_SCAN = 2048;          // tokens that one scan holds
+constexpr int EMB_SCAN = 256;           // tokens that one scan holds
 constexpr int EMB_SEG = EMB_SCAN / 4;   // of them per wave
 constexpr int EMB_FLIGHT = 8;           // rows of g in flight per wave
 
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
     T *__restrict__ dw, int64_t rs, int64_t V, int D, int R, int chunks,
     int *err) {
   using RV = RowVec<T>;
-  __shared__ uint32_t list[4][EMB_SEG]; // row in the tile << 11 | token
+  __shared__ uint32_t list[4][EMB_SEG]; // row in the tile << 8 | token
   __shared__ int count[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t v0 = int64_t(blockIdx.x / chunks) * R;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
       const uint64_t m = __ballot(mine);
       if (mine)
         list[wave][have + __popcll(m & ((uint64_t(1) << lane) - 1))] =
-            uint32_t(t - v0) << 11 | uint32_t(i);
+            uint32_t(t - v0) << 8 | uint32_t(i);
       have += __popcll(m);
     }
     if (lane == 0)
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
       const int have = count[s];
       for (int b = 0; b < have; b += 64) {
         const uint32_t e = b + lane < have ? list[s][b + lane] : ~0u;
-        uint64_t m = __ballot(e != ~0u && int(e >> 11) == r);
+        uint64_t m = __ballot(e != ~0u && int(e >> 8) == r);
         any |= m != 0;
         while (m) {
           typename RV::V v[EMB_FLIGHT];
@@ -546,8 +546,15 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_rank_kernel(
         key[t - v0] = 1;
     }
     __syncthreads();
+    if (vectors.d >= WAVE) { // a row per wave
+      for (uint32_t row = wave; row < rows; row += SORT_WAVES)
+        if (!key[row])
+          for (uint32_t c = lane; c < vectors.d; c += WAVE)
+            RowPart<T, EVEN>(c, D).template store<false, false>(dw + (v0 + row) * rs,
+                                                                typename RowVec<T>::V{});
+      return;
+    }
     const uint32_t items = rows * vectors.d;
-#pragma unroll 4
     for (uint32_t e = tid; e < items; e += SORT_THREADS) {
       const uint32_t row = vectors.div(e);
       if (!key[row])
@@ -593,45 +600,93 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_rank_kernel(
   }
 }
 
-// Runs over several tiles, by the tile that they begin in.  The keys and the
-// sums of the next EMB_JOIN tiles are loaded together; those past the run's
-// end are in bounds and not used.
+// Runs over several tiles, by the tile that they begin in.  A run of up to
+// EMB_JOIN tiles more is joined by one work-item per vector of columns.  The
+// further workgroups take the longer ones: each looks through 64 tiles, and
+// its waves add every fourth group of EMB_JOIN tiles of a run and then each
+// other's sums, in their order.
 constexpr int EMB_JOIN = 16;
+constexpr uint32_t EMB_GROUP = EMB_JOIN * EMB_TILE; // tokens of a group
+
+// Whether a run begins in the tile and goes on; its key.
+__device__ __forceinline__ bool run_begins(const SumPlan &p, uint32_t tile, uint32_t &key) {
+  const uint32_t beg = tile * EMB_TILE, end = beg + EMB_TILE;
+  if (end >= p.n)
+    return false;
+  key = p.key[end - 1];
+  return key < p.V && p.key[end] == key && !(beg > 0 && p.key[beg - 1] == key);
+}
+
+// Adds the sums that the tiles from token b on carry of the key's run.
+template <class T>
+__device__ __forceinline__ typename RowVec<T>::V
+add_group(const SumPlan &p, T *part, uint32_t b, uint32_t key, uint32_t c,
+          typename RowVec<T>::V acc) {
+  using RV = RowVec<T>;
+  typename RV::V v[EMB_JOIN];
+  bool same[EMB_JOIN];
+#pragma unroll
+  for (int j = 0; j < EMB_JOIN; ++j)
+    same[j] = (b + j * EMB_TILE < p.n) & (p.key[min(b + j * EMB_TILE, p.n - 1)] == key);
+#pragma unroll
+  for (int j = 0; j < EMB_JOIN; ++j)
+    if (same[j])
+      v[j] = RV::load(partial(p, part, b / EMB_TILE + j, 0, c));
+#pragma unroll
+  for (int j = 0; j < EMB_JOIN; ++j)
+    acc = same[j] ? acc + v[j] : acc;
+  return acc;
+}
 
 template <class T, bool ACC, bool EVEN>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(
-    SumPlan p, T scale, T *__restrict__ dw, T *part, uint32_t tile0, uint32_t items) {
+    SumPlan p, T scale, T *__restrict__ dw, T *part, uint32_t tile0, uint32_t tiles,
+    uint32_t joining, uint32_t chunks) {
   using RV = RowVec<T>;
-  const uint32_t item = blockIdx.x * EMB_THREADS + threadIdx.x;
-  if (item >= items)
+  if (blockIdx.x < joining) {
+    const uint32_t item = blockIdx.x * EMB_THREADS + threadIdx.x;
+    const uint32_t tile = p.vectors.div(item), c = item - tile * p.vectors.d;
+    uint32_t key;
+    if (tile >= tiles || !run_begins(p, tile0 + tile, key))
+      return;
+    const uint32_t b = (tile0 + tile + 1) * EMB_TILE;
+    if (b + EMB_GROUP < p.n && p.key[b + EMB_GROUP] == key)
+      return; // a longer one
+    const typename RV::V acc = RV::load(partial(p, part, tile0 + tile, 1, c));
+    RowPart<T, EVEN>(c, p.D).template store<ACC>(dw + key * p.rs,
+                                                 add_group(p, part, b, key, c, acc) * scale);
     return;
-  uint32_t tile = p.vectors.div(item);
-  const uint32_t c = item - tile * p.vectors.d;
-  tile += tile0;
-  const uint32_t beg = tile * EMB_TILE, end = beg + EMB_TILE;
-  if (end >= p.n)
-    return;
-  const uint32_t key = p.key[end - 1];
-  if (key >= p.V || p.key[end] != key || (beg > 0 && p.key[beg - 1] == key))
-    return;
-  typename RV::V acc = RV::load(partial(p, part, tile, 1, c));
-  bool more = true;
-  for (uint32_t b = end; more && b < p.n; b += EMB_JOIN * EMB_TILE) {
-    typename RV::V v[EMB_JOIN];
-    bool same[EMB_JOIN];
+  }
+  constexpr int WAVES = EMB_THREADS / WAVE;
+  __shared__ typename RV::V sums[WAVES][WAVE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t block = blockIdx.x - joining, t64 = block / chunks * WAVE;
+  const uint32_t c = block % chunks * WAVE + lane, at_c = min(c, p.vectors.d - 1);
+  uint32_t mine = 0;
+  const uint32_t next = (tile0 + t64 + lane + 1) * EMB_TILE;
+  const bool longer = t64 + lane < tiles && run_begins(p, tile0 + t64 + lane, mine) &&
+                      next + EMB_GROUP < p.n && p.key[next + EMB_GROUP] == mine;
+  uint64_t m = __ballot(longer); // the same in every wave
+  while (m) {
+    const int l = __ffsll((unsigned long long)m) - 1;
+    m &= m - 1;
+    const uint32_t tile = tile0 + t64 + l, key = __builtin_amdgcn_readlane(mine, l);
+    typename RV::V acc = {};
+    if (wave == 0)
+      acc = RV::load(partial(p, part, tile, 1, at_c));
+    for (uint32_t b = (tile + 1) * EMB_TILE + wave * EMB_GROUP; b < p.n && p.key[b] == key;
+         b += WAVES * EMB_GROUP)
+      acc = add_group(p, part, b, key, at_c, acc);
+    __syncthreads(); // the sums of the run before have been read
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && c < p.vectors.d) {
 #pragma unroll
-    for (int j = 0; j < EMB_JOIN; ++j) {
-      const uint32_t at = min(b + j * EMB_TILE, p.n - 1);
-      same[j] = (b + j * EMB_TILE < p.n) & (p.key[at] == key);
-      v[j] = RV::load(partial(p, part, at / EMB_TILE, 0, c));
-    }
-#pragma unroll
-    for (int j = 0; j < EMB_JOIN; ++j) {
-      more = more & same[j];
-      acc = more ? acc + v[j] : acc;
+      for (int w = 1; w < WAVES; ++w)
+        acc += sums[w][lane];
+      RowPart<T, EVEN>(c, p.D).template store<ACC>(dw + key * p.rs, acc * scale);
     }
   }
-  RowPart<T, EVEN>(c, p.D).template store<ACC>(dw + key * p.rs, acc * scale);
 }
 
 namespace {
@@ -715,7 +770,7 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
   T *const to = typed_ptr<T>(dw);
   // a filling workgroup's rows: about 2^15 vectors, which take longer to
   // write than the tokens to read, and fewer than 2^32 in any case
-  const uint32_t R = std::clamp<uint32_t>((1u << 15) / vectors, 1, RANK_ROWS);
+    const uint32_t R = std::clamp<uint32_t>((1u << 15) / vectors, 1, RANK_ROWS);
   const bool ranked = N <= RANK_MOST && (ACC || (V + R - 1) / R < int64_t(1) << 20);
   DeviceScratch pairs(size_t(N) * (ranked ? 8 : 16));
   uint32_t *const base = pairs.get<uint32_t>();
@@ -757,10 +812,12 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
             uint32_t(n * vectors));
     NT_LAUNCH_CHECK();
   });
+  const uint32_t chunks = (vectors + WAVE - 1) / WAVE;
   in_launches(tiles, vectors, [&](int64_t t0, int64_t n) {
-    embedding_join_kernel<T, ACC, EVEN>
-        <<<dim3(blocks_for(n * vectors, EMB_THREADS)), EMB_THREADS, 0, s>>>(
-            q, scale, to, part.get<T>(), uint32_t(t0), uint32_t(n * vectors));
+    const unsigned joining = blocks_for(n * vectors, EMB_THREADS);
+    const unsigned longer = unsigned((n + WAVE - 1) / WAVE * chunks);
+    embedding_join_kernel<T, ACC, EVEN><<<dim3(joining + longer), EMB_THREADS, 0, s>>>(
+        q, scale, to, part.get<T>(), uint32_t(t0), uint32_t(n), joining, chunks);
     NT_LAUNCH_CHECK();
   });
   if (!ACC && !ranked)

@@ -397,7 +397,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a
 
 // `splits` workgroups per row, each wave a part of `part` elements.
 template <class T, bool TOP, bool STREAM>
-__global__ __launch_bounds__(LP_THREADS) void logprob_group_kernel(LpForward<T> a,
+__global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_group_kernel(LpForward<T> a,
                                                                    int64_t row0) {
   __shared__ T sm[3][LP_WAVES];
   __shared__ typename Key<T>::K skey[LP_WAVES][LP_TOP_MAX];

@@ -10,7 +10,7 @@ from . import _lib
 from . import autograd
 from ._data_type import Dtype, is_float, promote_dtypes
 from ._indexing import broadcast_shapes
-from .autograd.ops_token import RowOp, _as_rows, _check_tokens
+from .autograd.ops_token import RowOp, _as_rows, _check_tokens, top_views
 from .core import Tensor
 from .factories import next_dropout_counter
 
@@ -182,9 +182,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
     extras = [] if top else [None, None]
     logprob = ent = None
     if tokens is None and not entropy:
-        _, value, token = K.token_logprobs(_as_rows(logits), None, ignore_index, False, top,
-                                              False)
-        extras = [Tensor._new_contiguous(s, shape[:-1] + (top,)) for s in (value, token)]
+        out, token = K.token_logprobs(_as_rows(logits), None, ignore_index, False, top, False)
+        extras = top_views(out, 0, token, shape[:-1] + (top,))
     else:
         out = autograd.TokenLogProbOp.apply(logits, tokens, ignore_index, entropy, top, extras)
         if tokens is None:
