@@ -199,14 +199,14 @@ class TokenLogProbOp(Function):
         self.saved_tensors  # raises if logits or tokens were modified in place
         z, flat, ignore, results = self._call
         rows = z._shape[0]
-        if g.dtype != z.dtype:
-            g = g.to(z.dtype)
-        if self._both:
+        if not self._both:
+            ga, gb = (None, g) if flat is None else (g, None)
+        elif hasattr(g, "_parts"):
+            ga, gb = g._parts.get(0), g._parts.get(1)
+        else:
             g = reshape_view(g, (2, rows))._to_contiguous()
             ga, gb = _row_of(g, 0), _row_of(g, 1)
-        else:
-            g = _vector(g)
-            ga, gb = (None, g) if flat is None else (g, None)
+        ga, gb = (None if x is None else _vector(x.to(z.dtype)) for x in (ga, gb))
         into = None if target is None else _rows_in_place(target)
         st = K.token_logprobs_bwd(z, flat, ignore, results, ga, gb, into)
         if into is not None:
@@ -233,15 +233,22 @@ def top_views(out, offset: int, token, shape) -> tuple[Tensor, Tensor]:
 
 
 class RowOp(Function):
-    """x[i] of x [2, ...], with a gradient: the upstream one in row i, zeros
-    in the other."""
+    """x[i] of TokenLogProbOp's x [2, ...].
+
+    In the engine's pass the rows' gradients reach TokenLogProbOp side by
+    side, in a stand-in for the gradient of x that carries them (``_parts``),
+    without being copied into one tensor: on few rows three launches are most
+    of what the backward pass costs.  ``backward`` returns that tensor."""
 
     def forward(self, x: Tensor, i: int) -> Tensor:
-        self._i, self._shape = i, x._shape
+        self._i, self._x = i, x
         return _row_of(x, i)
 
     def backward(self, grad_out: Tensor) -> tuple:
-        return (self._backward_into(grad_out, [True], [None])[0],)
+        full = Tensor._new_contiguous(
+            K.fill(self._x.numel, 0, grad_out.dtype, grad_out.device), self._x._shape)
+        K.copy_view(grad_out, _row_of(full, self._i))
+        return (full,)
 
     def fused_ok(self) -> bool:
         return True
@@ -249,13 +256,15 @@ class RowOp(Function):
     def _backward_into(self, g: Tensor, needs, targets):
         if not needs[0]:
             return [None]
-        if targets[0] is not None:
-            K.inplace(_lib.ADD, _row_of(targets[0], self._i), g)
-            return [targets[0]]
-        full = Tensor._new_contiguous(
-            K.fill(math.prod(self._shape), 0, g.dtype, g.device), self._shape)
-        K.copy_view(g, _row_of(full, self._i))
-        return [full]
+        into = targets[0]
+        if into is None:
+            into = self._x._alias()
+            into._parts = {}
+        elif not hasattr(into, "_parts"):
+            K.inplace(_lib.ADD, _row_of(into, self._i), g)
+            return [into]
+        into._parts[self._i] = g
+        return [into]
 
 
 def _row_of(x: Tensor, i: int) -> Tensor:

@@ -768,9 +768,10 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
   p.digit = (bits + p.passes - 1) / p.passes;
   const uint32_t vectors = row_vectors<T>(D);
   T *const to = typed_ptr<T>(dw);
-  // a filling workgroup's rows: about 2^15 vectors, which take longer to
-  // write than the tokens to read, and fewer than 2^32 in any case
-    const uint32_t R = std::clamp<uint32_t>((1u << 15) / vectors, 1, RANK_ROWS);
+  // a filling workgroup's rows: 512 workgroups, but 2^12 to 2^15 vectors each,
+  // which take longer to write than the tokens to read
+  const int64_t fill = std::clamp<int64_t>((V * vectors + 511) / 512, 1 << 12, 1 << 15);
+  const uint32_t R = uint32_t(std::clamp<int64_t>(fill / vectors, 1, RANK_ROWS));
   const bool ranked = N <= RANK_MOST && (ACC || (V + R - 1) / R < int64_t(1) << 20);
   DeviceScratch pairs(size_t(N) * (ranked ? 8 : 16));
   uint32_t *const base = pairs.get<uint32_t>();
