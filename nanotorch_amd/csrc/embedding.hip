@@ -74,7 +74,10 @@ struct Rows {
 
 // A workgroup writes EMB_THREADS * EMB_LOOKUP adjacent vectors of the output,
 // each work-item every EMB_THREADS-th of them, so that as many loads are in
-// flight.  Rows of adjacent elements.
+// flight.  Rows of adjacent elements.  65536 rows of 2048 float32 (0.54 GB
+// written, about 0.13 GB of different rows read) take 131 us alone and 157
+// behind a gradient whose zero rows are still on their way to memory; with a
+// branch around each load 181, with stores that stay in the cache 144.
 constexpr int EMB_LOOKUP = 4;
 
 template <class T, bool EVEN>
@@ -131,7 +134,10 @@ constexpr int EMB_FLIGHT = 8;           // rows of g in flight per wave
 // N <= EMB_SCAN tokens, one launch.  A workgroup owns R rows of dW and 64
 // vectors of columns.  Each wave lists the tokens of its quarter that name
 // one of the rows, in order; then each wave sums and writes the rows
-// wave, wave + 4, ...
+// wave, wave + 4, ...  Against the sorted form below (us, 1000 x 64, Zipf-like
+// tokens): N = 64 7 and 13, N = 256 7.5 and 13.6, N = 1024 12 and 15; but one
+// token throughout, which a single wave then sums: N = 256 18 and 12,
+// N = 1024 67 and 13.
 template <class T, bool ACC, bool EVEN>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
     const T *__restrict__ g, Tokens tok, int n, int64_t padding, T scale,
@@ -203,15 +209,18 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
 
 // ------------------------------------------------ gradient, many tokens
 //
-// The tokens are sorted (stably, so a row's terms stay in rising i) by a
-// radix sort of (key, i) pairs, the key being the token, or V where there is
-// no gradient.  The sorted pairs are cut into tiles of EMB_TILE.  A work-item
+// The tokens are sorted (stably, so a row's terms stay in rising i): up to
+// RANK_MOST by counting, more by a radix sort of (key, i) pairs, the key being
+// the token, or V where there is no gradient.  The sorted pairs are cut into tiles of 8 or 32.  A work-item
 // sums one vector of columns over one tile, run by run.  A run within a tile
 // is written to dW; a run that goes on into the next tile leaves one partial
 // sum per tile, which a last kernel joins in tile order.  So a token that
 // fills a tenth of the batch is spread over the chip like any other.
+//
+// 65536 tokens into 128000 x 2048 float32: sort 27 us, sums 137 (0.54 GB read,
+// 0.13 GB written), joins 15, zero rows 129 (0.92 GB, 7.1 TB/s).  8192 into
+// 32000 x 1024: sort and zero rows 20 us, sums 13, joins 4.
 
-constexpr int EMB_TILE = 32;
 constexpr int EMB_DIGIT = 9; // bits of a pass, at most
 constexpr int EMB_BINS = 1 << EMB_DIGIT;
 constexpr int SORT_THREADS = 1024;
@@ -436,6 +445,7 @@ struct SumPlan {
   FastDivU32 vectors; // columns in vectors
   int D;
   int64_t rs; // of dW
+  uint32_t tile; // pairs of a tile
 };
 
 // Partial sums: two vectors for each tile and vector of columns, the first
@@ -459,7 +469,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_sum_kernel(
   uint32_t tile = p.vectors.div(item);
   const uint32_t c = item - tile * p.vectors.d;
   tile += tile0;
-  const uint32_t beg = tile * EMB_TILE, end = min(p.n, beg + EMB_TILE);
+  const uint32_t beg = tile * p.tile, end = min(p.n, beg + p.tile);
   const RowPart<T, EVEN> part_of(c, p.D);
   uint32_t key = p.key[beg];
   bool carried = beg > 0 && p.key[beg - 1] == key;
@@ -524,7 +534,9 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_fill_kernel(
 // them, one per lane, and each of its waves counts, in its part of all
 // tokens, those that come before (smaller ones, and equal ones of smaller i).
 // The further workgroups write the zero rows meanwhile: each looks which of
-// its rows the tokens name.
+// its rows the tokens name.  n^2 comparisons over the chip: 9000 tokens into
+// 1000 x 64 take 27 us in all, by the radix sort 36; at 16384 both take 39 and
+// 37, into 32000 x 1024 both 65.
 constexpr int RANK_MOST = 16384;
 constexpr int RANK_ROWS = 1024; // rows of a filling workgroup, at most
 
@@ -606,32 +618,33 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_rank_kernel(
 // its waves add every fourth group of EMB_JOIN tiles of a run and then each
 // other's sums, in their order.
 constexpr int EMB_JOIN = 16;
-constexpr uint32_t EMB_GROUP = EMB_JOIN * EMB_TILE; // tokens of a group
 
 // Whether a run begins in the tile and goes on; its key.
 __device__ __forceinline__ bool run_begins(const SumPlan &p, uint32_t tile, uint32_t &key) {
-  const uint32_t beg = tile * EMB_TILE, end = beg + EMB_TILE;
+  const uint32_t beg = tile * p.tile, end = beg + p.tile;
   if (end >= p.n)
     return false;
   key = p.key[end - 1];
   return key < p.V && p.key[end] == key && !(beg > 0 && p.key[beg - 1] == key);
 }
 
-// Adds the sums that the tiles from token b on carry of the key's run.
+// Adds the sums that the EMB_JOIN tiles from `tile` on carry of the key's run.
 template <class T>
 __device__ __forceinline__ typename RowVec<T>::V
-add_group(const SumPlan &p, T *part, uint32_t b, uint32_t key, uint32_t c,
+add_group(const SumPlan &p, T *part, uint32_t tile, uint32_t key, uint32_t c,
           typename RowVec<T>::V acc) {
   using RV = RowVec<T>;
   typename RV::V v[EMB_JOIN];
   bool same[EMB_JOIN];
 #pragma unroll
-  for (int j = 0; j < EMB_JOIN; ++j)
-    same[j] = (b + j * EMB_TILE < p.n) & (p.key[min(b + j * EMB_TILE, p.n - 1)] == key);
+  for (int j = 0; j < EMB_JOIN; ++j) {
+    const uint32_t b = (tile + j) * p.tile;
+    same[j] = (b < p.n) & (p.key[min(b, p.n - 1)] == key);
+  }
 #pragma unroll
   for (int j = 0; j < EMB_JOIN; ++j)
     if (same[j])
-      v[j] = RV::load(partial(p, part, b / EMB_TILE + j, 0, c));
+      v[j] = RV::load(partial(p, part, tile + j, 0, c));
 #pragma unroll
   for (int j = 0; j < EMB_JOIN; ++j)
     acc = same[j] ? acc + v[j] : acc;
@@ -649,12 +662,12 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(
     uint32_t key;
     if (tile >= tiles || !run_begins(p, tile0 + tile, key))
       return;
-    const uint32_t b = (tile0 + tile + 1) * EMB_TILE;
-    if (b + EMB_GROUP < p.n && p.key[b + EMB_GROUP] == key)
+    const uint32_t b = (tile0 + tile + 1) * p.tile;
+    if (b + EMB_JOIN * p.tile < p.n && p.key[b + EMB_JOIN * p.tile] == key)
       return; // a longer one
     const typename RV::V acc = RV::load(partial(p, part, tile0 + tile, 1, c));
-    RowPart<T, EVEN>(c, p.D).template store<ACC>(dw + key * p.rs,
-                                                 add_group(p, part, b, key, c, acc) * scale);
+    RowPart<T, EVEN>(c, p.D).template store<ACC>(
+        dw + key * p.rs, add_group(p, part, tile0 + tile + 1, key, c, acc) * scale);
     return;
   }
   constexpr int WAVES = EMB_THREADS / WAVE;
@@ -663,9 +676,9 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(
   const uint32_t block = blockIdx.x - joining, t64 = block / chunks * WAVE;
   const uint32_t c = block % chunks * WAVE + lane, at_c = min(c, p.vectors.d - 1);
   uint32_t mine = 0;
-  const uint32_t next = (tile0 + t64 + lane + 1) * EMB_TILE;
+  const uint32_t next = (tile0 + t64 + lane + 1) * p.tile;
   const bool longer = t64 + lane < tiles && run_begins(p, tile0 + t64 + lane, mine) &&
-                      next + EMB_GROUP < p.n && p.key[next + EMB_GROUP] == mine;
+                      next + EMB_JOIN * p.tile < p.n && p.key[next + EMB_JOIN * p.tile] == mine;
   uint64_t m = __ballot(longer); // the same in every wave
   while (m) {
     const int l = __ffsll((unsigned long long)m) - 1;
@@ -674,9 +687,9 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(
     typename RV::V acc = {};
     if (wave == 0)
       acc = RV::load(partial(p, part, tile, 1, at_c));
-    for (uint32_t b = (tile + 1) * EMB_TILE + wave * EMB_GROUP; b < p.n && p.key[b] == key;
-         b += WAVES * EMB_GROUP)
-      acc = add_group(p, part, b, key, at_c, acc);
+    for (uint32_t t = tile + 1 + wave * EMB_JOIN; t * p.tile < p.n && p.key[t * p.tile] == key;
+         t += WAVES * EMB_JOIN)
+      acc = add_group(p, part, t, key, at_c, acc);
     __syncthreads(); // the sums of the run before have been read
     sums[wave][lane] = acc;
     __syncthreads();
@@ -801,10 +814,16 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
       NT_LAUNCH_CHECK();
     }
   }
+  // Few tokens: small tiles, since the chip is not full and a tile's loads
+  // follow each other (us for 8 and 32 a tile, Zipf-like tokens: 50000 x 129,
+  // N = 1500 16 and 25, N = 4000 22 and 28; 1000 x 64, N = 4000 18.5 and
+  // 18.7, N = 8192 27 and 25).  One token throughout, whose sums the join
+  // adds up, takes longer (N = 4000 28 and 19; N = 16384 91 and 47).
+  const uint32_t tile = N <= 4096 ? 8 : 32;
+  const int64_t tiles = (N + tile - 1) / tile;
   const Pairs &sorted = p.side[(p.passes - 1) & 1];
   const SumPlan q{sorted.key, sorted.pos, p.n, uint32_t(V), FastDivU32(vectors), int(D),
-                  dw->strides[0]};
-  const int64_t tiles = (N + EMB_TILE - 1) / EMB_TILE;
+                  dw->strides[0], tile};
   DeviceScratch part(size_t(2 * tiles * vectors) * 16);
   in_launches(tiles, vectors, [&](int64_t t0, int64_t n) {
     embedding_sum_kernel<T, ACC, EVEN>
