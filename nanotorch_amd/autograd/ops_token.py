@@ -124,10 +124,7 @@ class DropoutOp(Function):
             raise ValueError(f"dropout() needs a float tensor, got {x.dtype.name}.")
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout() needs 0 <= p <= 1, got {p}.")
-        K.require_device(x)
         self._args = (float(p), seed, offset)
-        if p == 0.0:
-            return x
         return Tensor._unchecked_view(
             K.dropout(x, *self._args), x._shape, row_major_strides(x._shape), 0)
 
@@ -141,11 +138,6 @@ class DropoutOp(Function):
         return [self._grad(g, targets[0]) if needs[0] else None]
 
     def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
-        if self._args[0] == 0.0:
-            if target is None:
-                return g
-            K.inplace(_lib.ADD, target, g)
-            return target
         st = K.dropout(g, *self._args, target)
         if target is not None:
             return target

@@ -75,7 +75,7 @@ struct Rows {
 // A workgroup writes EMB_THREADS * EMB_LOOKUP adjacent vectors of the output,
 // each work-item every EMB_THREADS-th of them, so that as many loads are in
 // flight.  Rows of adjacent elements.  65536 rows of 2048 float32 (0.54 GB
-// written, about 0.13 GB of different rows read) take 131 us alone and 157
+// written, 0.16 GB of different rows read) take 131 us alone and 157
 // behind a gradient whose zero rows are still on their way to memory; with a
 // branch around each load 181, with stores that stay in the cache 144.
 constexpr int EMB_LOOKUP = 4;
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
 // fills a tenth of the batch is spread over the chip like any other.
 //
 // 65536 tokens into 128000 x 2048 float32: sort 27 us, sums 137 (0.54 GB read,
-// 0.13 GB written), joins 15, zero rows 129 (0.92 GB, 7.1 TB/s).  8192 into
+// 0.17 GB written), joins 15, zero rows 129 (0.89 GB, 6.9 TB/s).  8192 into
 // 32000 x 1024: sort and zero rows 20 us, sums 13, joins 4.
 
 constexpr int EMB_DIGIT = 9; // bits of a pass, at most

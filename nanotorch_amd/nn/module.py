@@ -121,7 +121,7 @@ class Dropout(Module):
         return self
 
     def forward(self, x: Tensor) -> Tensor:
-        return dropout(x, self._p) if self._training else x
+        return dropout(x, self._p) if self._training and self._p > 0.0 else x
 
 
 class ReLU(Module):
@@ -155,7 +155,8 @@ class Sequential(Module):
 
     def train(self, mode: bool = True) -> "Sequential":
         for m in self._modules:
-            m.train(mode)
+            if isinstance(m, Module):  # a plain function has no mode
+                m.train(mode)
         return self
 
     def forward(self, *args: Any, **kwargs: Any) -> Any:

@@ -81,6 +81,8 @@ def check_table_grad(got, g, t, V, scale, dtype, padding=None, parts=1):
     (300, 257, 2048, "zipf"), (300, 260, 2049, "zipf"), (4000, 33, 9000, "zipf"),
     (70000, 20, 17000, "any"), (129, 512, 5000, "one"), (5, 1023, 4097, "few"),
     (131072, 8, 40000, "zipf"), (300000, 4, 20001, "any"), (2, 16, 70001, "any"),
+    (3, 300, 4000, "one"), (511, 8, 17000, "any"), (512, 8, 17000, "any"),
+    (600, 3, 1100000, "zipf"),
 ])
 def test_embedding(gpu, dtype, V, D, N, kind):
     r = rng(seed_of(dtype.__name__, V, D, N))
@@ -252,7 +254,10 @@ def test_embedding_refusals(gpu):
 
 def words(n, seed, offset):
     """The first n words of Philox4x32-10 over the counters (i, offset)."""
-    i = np.arange((n + 3) // 4, dtype=np.uint64)
+    return words_of(np.arange((n + 3) // 4, dtype=np.uint64), seed, offset)[:n]
+
+
+def words_of(i, seed, offset):
     low, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)
     c = [i & low, i >> s32, np.full_like(i, offset & 0xFFFFFFFF), np.full_like(i, offset >> 32)]
     k = [seed & 0xFFFFFFFF, seed >> 32]
@@ -261,7 +266,7 @@ def words(n, seed, offset):
         c = [(b >> s32) ^ c[1] ^ np.uint64(k[0]), b & low,
              (a >> s32) ^ c[3] ^ np.uint64(k[1]), a & low]
         k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
-    return np.stack(c, 1).reshape(-1)[:n]
+    return np.stack(c, 1).reshape(-1)
 
 
 def dropped(x, p, seed, offset):
@@ -700,7 +705,35 @@ def test_logprob_refusals(gpu):
         lp.sum().backward()
 
 
+def test_operators_between_elementwise_ops(gpu):
+    """Kernels that may overlap (launched without the stream's barrier) and
+    those that may not, each reading what the one before has written."""
+    r = rng(61)
+    x = r.standard_normal((300, 70)).astype(np.float32)
+    t = r.integers(0, 300, 300)
+    y, want = dev(x), x
+    for k in range(12):
+        y = nt.dropout(y, 0.25, seed=k) * 2.0
+        want = dropped(want, 0.25, k, 0) * np.float32(2)
+        if k % 4 == 3:
+            y = nt.embedding(y, dev(t)) * 0.125
+            want = want[t] * np.float32(0.125)
+    assert_bitexact(host(y), want)
+
+
 # -------------------------------------------------------------- large tensors
+
+
+def test_dropout_past_32_bits(gpu):
+    n = (1 << 32) + 13
+    x = nt.ones(n, device="cuda")
+    y = nt.dropout(x, 0.5, seed=3, offset=4)
+    for at in (0, (1 << 32) - 8, n - 13):
+        part = host(y[at:at + 13])
+        i = np.arange(at // 4, at // 4 + 5, dtype=np.uint64)
+        w = words_of(i, 3, 4)[at % 4:at % 4 + 13]
+        assert_bitexact(part, np.where(w >= np.uint64(1 << 31), np.float32(2), np.float32(0)))
+
 
 
 def test_offsets_past_32_bits(gpu):
