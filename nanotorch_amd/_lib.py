@@ -183,8 +183,9 @@ def call_packed(name: str, *args) -> None:
         check(rc)
 
 
-_pack = struct.Struct("=Qqii16q").pack
-_PAD = [(0,) * (NT_MAX_DIMS - n) for n in range(NT_MAX_DIMS + 1)]
+# One packer per number of dimensions, the unused ones as zero bytes.
+_pack = [struct.Struct(f"=Qqii{n}q{8 * (NT_MAX_DIMS - n)}x{n}q{8 * (NT_MAX_DIMS - n)}x").pack
+         for n in range(NT_MAX_DIMS + 1)]
 
 
 def pack_view(data: int, offset: int, dtype: int, shape, strides) -> bytes:
@@ -192,8 +193,7 @@ def pack_view(data: int, offset: int, dtype: int, shape, strides) -> bytes:
     nd = len(shape)
     if nd > NT_MAX_DIMS:
         raise RuntimeError(f"Tensors are limited to {NT_MAX_DIMS} dims on device.")
-    pad = _PAD[nd]
-    return _pack(data, offset, dtype, nd, *shape, *pad, *strides, *pad)
+    return _pack[nd](data, offset, dtype, nd, *shape, *strides)
 
 
 def is_available() -> bool:

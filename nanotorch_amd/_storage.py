@@ -12,7 +12,7 @@ from __future__ import annotations
 import ctypes
 
 from . import _lib
-from ._data_type import Dtype, ctype_of, sizeof
+from ._data_type import _SIZES, Dtype, ctype_of, sizeof
 from .cuda import Device
 
 
@@ -43,7 +43,19 @@ class Storage:
     @classmethod
     def allocate(cls, size: int, dtype: Dtype, device: Device) -> "Storage":
         """Uninitialised (device) or zeroed (host) buffer."""
-        return cls(size, dtype, device, _zero=False)
+        if device is not Device.Cuda or type(dtype) is not Dtype:
+            return cls(size, dtype, device, _zero=False)
+        # an op's output: __init__ without its conversions and choices
+        self = cls.__new__(cls)
+        self._dtype, self._device, self._size = dtype, device, size
+        self.version = 0
+        self._ptr = self._host = None
+        p = ctypes.c_void_p()
+        rc = (_lib._lib or _lib.load()).nt_malloc(ctypes.byref(p), (size or 1) * _SIZES[dtype])
+        if rc:
+            _lib.check(rc)
+        self._ptr = p.value
+        return self
 
     @classmethod
     def from_iterable(cls, values, dtype: Dtype, device: Device) -> "Storage":
