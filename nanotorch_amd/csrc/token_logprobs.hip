@@ -15,8 +15,11 @@
 // Bound by memory where rows are many: 8192 x 32000 float32 (a tenth of the
 // rows left out) reads 0.94 GB in 156 us (6.0 TB/s), and its gradient moves
 // 2.0 GB in 328 us (6.1 TB/s).  2000 x 50001 takes 68 us, with 5 alternatives
-// 74, with 20 84, with 64 140.  Few rows are split over several workgroups,
-// the last of which joins their parts.
+// 74, with 20 84, with 64 140.  Few rows are split over several workgroups
+// and joined by a second kernel: 8 x 128000 with 8 alternatives 7 + 8 us,
+// 64 x 128000 10 us in all without alternatives.  Joined by each row's last
+// workgroup instead, one launch less, those take 20 and 50: every part's
+// release to the other XCDs writes back an L2.
 //
 // Logits of -inf are tokens without probability and count for nothing; a row
 // that holds nothing else has log probability -inf, entropy 0 and no
@@ -398,37 +401,6 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a
   write_row(a, row, t, r, top);
 }
 
-// Workgroups of a split row that are done; all 0 between launches, of which
-// the stream runs one at a time.  Rows are split while they are fewer than the
-// workgroups that fill the chip, and LP_SPLIT_ROWS at most.
-constexpr int LP_SPLIT_ROWS = 1024;
-__device__ uint32_t arrivals[LP_SPLIT_ROWS];
-
-// Joins the parts of a split row, in their order; by one wave.
-template <class T, bool TOP>
-__device__ __forceinline__ void join_parts(const LpForward<T> &a, int64_t row, int64_t t) {
-  const int lane = threadIdx.x & 63;
-  RowState<T> r;
-  TopList<T> top;
-  for (int b = lane; b < a.splits; b += WAVE) {
-    RowState<T> o;
-    o.m = a.pm[row * a.splits + b];
-    o.s = a.ps[row * a.splits + b];
-    o.u = a.pu[row * a.splits + b];
-    r.join(o);
-  }
-  r.join_lanes();
-  if constexpr (TOP) {
-    const int64_t n = int64_t(a.splits) * a.k, base = row * n;
-    for (int64_t b = 0; b < n; b += WAVE) {
-      const bool in = b + lane < n;
-      top.insert_lanes(in ? a.pkey[base + b + lane] : 0, in ? a.ptoken[base + b + lane] : -1,
-                       a.k);
-    }
-  }
-  write_row(a, row, t, r, top);
-}
-
 // `splits` workgroups per row, each wave a part of `part` elements.  Eight waves per SIMD (at most 64 registers) hold 2000 rows at once.
 template <class T, bool TOP, bool STREAM>
 __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_group_kernel(LpForward<T> a,
@@ -441,7 +413,7 @@ __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_gr
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t t;
   if (row_left_out(a, row, t)) {
-    if (wave == 0 && split == 0)
+    if (wave == 0 && a.splits == 1)
       write_left_out(a, row);
     return;
   }
@@ -498,19 +470,36 @@ __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_gr
     a.pkey[at * a.k + lane] = top.key;
     a.ptoken[at * a.k + lane] = top.token;
   }
-  // The row's last workgroup joins the parts: what it reads was written before
-  // its writers' fences and their arrivals, and is read after its own.
-  __threadfence();
-  uint32_t before = 0;
-  if (lane == 0)
-    before = __hip_atomic_fetch_add(&arrivals[row], 1u, __ATOMIC_RELAXED,
-                                    __HIP_MEMORY_SCOPE_AGENT);
-  if (read_lane(before, 0) != uint32_t(a.splits - 1))
-    return;
-  __threadfence();
-  if (lane == 0) // for the next launch
-    __hip_atomic_store(&arrivals[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  join_parts<T, TOP>(a, row, t);
+}
+
+// Joins the splits of a row; a wave per row.
+template <class T, bool TOP>
+__global__ __launch_bounds__(WAVE) void logprob_join_kernel(LpForward<T> a,
+                                                            int64_t row0) {
+  const int64_t row = row0 + blockIdx.x;
+  const int lane = threadIdx.x;
+  int64_t t;
+  if (row_left_out(a, row, t))
+    return write_left_out(a, row);
+  RowState<T> r;
+  TopList<T> top;
+  for (int b = lane; b < a.splits; b += WAVE) {
+    RowState<T> o;
+    o.m = a.pm[row * a.splits + b];
+    o.s = a.ps[row * a.splits + b];
+    o.u = a.pu[row * a.splits + b];
+    r.join(o);
+  }
+  r.join_lanes();
+  if constexpr (TOP) {
+    const int64_t n = int64_t(a.splits) * a.k, base = row * n;
+    for (int64_t b = 0; b < n; b += WAVE) {
+      const bool in = b + lane < n;
+      top.insert_lanes(in ? a.pkey[base + b + lane] : 0, in ? a.ptoken[base + b + lane] : -1,
+                       a.k);
+    }
+  }
+  write_row(a, row, t, r, top);
 }
 
 // --------------------------------------------------------------- backward
@@ -646,9 +635,7 @@ template <class T> void run_forward(LpForward<T> a) {
   }
   const int64_t chunks = (a.V + CHUNK - 1) / CHUNK;
   const int64_t want = std::max<int64_t>(1, 4 * device_cu_count() / a.rows);
-  a.splits = a.rows > LP_SPLIT_ROWS
-                 ? 1
-                 : int(std::min<int64_t>(want, (chunks + LP_WAVES - 1) / LP_WAVES));
+  a.splits = int(std::min<int64_t>(want, (chunks + LP_WAVES - 1) / LP_WAVES));
   const int64_t parts = int64_t(a.splits) * LP_WAVES;
   a.part = int32_t((chunks + parts - 1) / parts * CHUNK);
   const int64_t n = a.splits > 1 ? a.rows * a.splits : 0;
@@ -672,6 +659,12 @@ template <class T> void run_forward(LpForward<T> a) {
     stream_in ? group(Yes{}, Yes{}) : group(Yes{}, No{});
   else
     stream_in ? group(No{}, Yes{}) : group(No{}, No{});
+  if (a.splits == 1)
+    return;
+  if (a.k)
+    launch(logprob_join_kernel<T, true>, WAVE, 1, 1);
+  else
+    launch(logprob_join_kernel<T, false>, WAVE, 1, 1);
 }
 
 template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
