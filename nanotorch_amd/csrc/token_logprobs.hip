@@ -110,6 +110,19 @@ template <class T, class F> __device__ __forceinline__ T over_wave(T v, T none, 
   return __builtin_bit_cast(T, read_lane(__builtin_bit_cast(I, v), WAVE - 1));
 }
 
+// f over each group of G adjacent lanes (4 or 16), in every lane of it; f is
+// commutative.
+template <int G, class T, class F> __device__ __forceinline__ T over_lanes(T v, F f) {
+  static_assert(G == 4 || G == 16);
+  v = f(v, from_lane<0xB1, 0xf>(v, v)); // lane i: i ^ 1
+  v = f(v, from_lane<0x4E, 0xf>(v, v)); // i ^ 2
+  if constexpr (G == 16) {
+    v = f(v, from_lane<0x141, 0xf>(v, v)); // the other end of eight
+    v = f(v, from_lane<0x140, 0xf>(v, v)); // of sixteen
+  }
+  return v;
+}
+
 template <class T> struct RowState {
   T m = -std::numeric_limits<T>::infinity(), s = T(0), u = T(0);
 
@@ -140,13 +153,19 @@ template <class T> struct RowState {
       u = __builtin_elementwise_fma(e, d, u);
     }
   }
-  // Every lane gets the wave's state.
-  __device__ __forceinline__ void join_lanes() {
-    move_to(over_wave(m, -std::numeric_limits<T>::infinity(),
-                      [](T a, T b) { return max_nan(a, b); }));
+  // Every lane gets the state of its group of G lanes.
+  template <int G = WAVE> __device__ __forceinline__ void join_lanes() {
+    const auto larger = [](T a, T b) { return max_nan(a, b); };
     const auto add = [](T a, T b) { return a + b; };
-    s = over_wave(s, T(0), add);
-    u = over_wave(u, T(0), add);
+    if constexpr (G == WAVE) {
+      move_to(over_wave(m, -std::numeric_limits<T>::infinity(), larger));
+      s = over_wave(s, T(0), add);
+      u = over_wave(u, T(0), add);
+    } else {
+      move_to(over_lanes<G>(m, larger));
+      s = over_lanes<G>(s, add);
+      u = over_lanes<G>(u, add);
+    }
   }
 };
 
@@ -255,9 +274,9 @@ template <class T> struct LpForward {
   int *err;
 };
 
-template <class T>
+template <class T, int G = WAVE>
 __device__ __forceinline__ void write_left_out(const LpForward<T> &a, int64_t row) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x % G;
   if (lane == 0) {
     if (a.logprob)
       a.logprob[row] = T(0);
@@ -275,10 +294,10 @@ __device__ __forceinline__ void write_left_out(const LpForward<T> &a, int64_t ro
   }
 }
 
-template <class T>
+template <class T, int G = WAVE>
 __device__ __forceinline__ void write_row(const LpForward<T> &a, int64_t row, int64_t t,
                                           const RowState<T> &r, const TopList<T> &top) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x % G;
   const bool none = r.s == T(0);
   const T log_s = log(r.s), low = -std::numeric_limits<T>::infinity();
   if (lane == 0) {
@@ -380,6 +399,48 @@ __device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k
   }
 }
 
+// G lanes per row, for short rows without alternatives: 1000000 x 10 float32
+// takes 21 us and 22 for its gradient, 100000 x 100 12 and 16 (with a wave per
+// row 660 and 71 for both).
+template <class T, int G>
+__global__ __launch_bounds__(LP_THREADS) void logprob_lanes_kernel(LpForward<T> a,
+                                                                   int64_t row0) {
+  using RV = RowVec<T>;
+  constexpr int N = RV::N;
+  const int64_t row = row0 + (int64_t(blockIdx.x) * LP_THREADS + threadIdx.x) / G;
+  if (row >= a.rows)
+    return;
+  int64_t t;
+  if (row_left_out(a, row, t))
+    return write_left_out<T, G>(a, row);
+  const T *z = a.z + row * a.row_stride;
+  RowState<T> r;
+#pragma unroll
+  for (int c = 0; c < LP_UNROLL; ++c) {
+    const int i = (c * G + int(threadIdx.x % G)) * N;
+    if (c * G * N >= a.V)
+      break;
+    T v[N];
+    if (i + N <= a.V) {
+      const typename RV::V w = RV::load(z + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        v[j] = w[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        v[j] = i + j < a.V ? z[i + j] : -std::numeric_limits<T>::infinity();
+    }
+    T most = v[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j)
+      most = max_nan(most, v[j]);
+    r.add(v, most);
+  }
+  r.template join_lanes<G>();
+  write_row<T, G>(a, row, t, r, TopList<T>());
+}
+
 // A wave per row.
 template <class T, bool TOP>
 __global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a,
@@ -401,10 +462,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a
   write_row(a, row, t, r, top);
 }
 
-// `splits` workgroups per row, each wave a part of `part` elements.  Eight waves per SIMD (at most 64 registers) hold 2000 rows at once.
+// `splits` workgroups per row, each wave a part of `part` elements.  Eight
+// waves per SIMD (at most 64 registers) hold 2000 rows at once.
 template <class T, bool TOP, bool STREAM>
-__global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_group_kernel(LpForward<T> a,
-                                                                   int64_t row0) {
+__global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_group_kernel(
+    LpForward<T> a, int64_t row0) {
   __shared__ T sm[3][LP_WAVES];
   __shared__ typename Key<T>::K skey[LP_WAVES][LP_TOP_MAX];
   __shared__ int32_t stoken[LP_WAVES][LP_TOP_MAX];
@@ -518,25 +580,23 @@ template <class T> struct LpBackward {
   int64_t dz_stride;
 };
 
-// A workgroup of W waves per row, or (W = 1) four rows per workgroup, each
-// lane UNROLL vectors.
-template <class T, int W, int UNROLL, bool ACC>
+// G lanes per row, each UNROLL vectors; a whole workgroup (G = LP_THREADS)
+// takes one of the row's `chunks`.
+template <class T, int G, int UNROLL, bool ACC>
 __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a,
                                                                  int64_t row0, int chunks) {
   using RV = RowVec<T>;
-  constexpr int N = RV::N;
+  constexpr int N = RV::N, STEP = G * N;
   int64_t row;
-  int32_t first;
-  if constexpr (W == 1) {
-    row = row0 + int64_t(blockIdx.x) * LP_WAVES + (threadIdx.x >> 6);
+  int32_t first = (threadIdx.x % G) * N;
+  if constexpr (G < LP_THREADS) {
+    row = row0 + (int64_t(blockIdx.x) * LP_THREADS + threadIdx.x) / G;
     if (row >= a.rows)
       return;
-    first = (threadIdx.x & 63) * N;
   } else {
     row = row0 + blockIdx.x / chunks;
-    first = (blockIdx.x % chunks) * (LP_THREADS * N * UNROLL) + threadIdx.x * N;
+    first += (blockIdx.x % chunks) * (STEP * UNROLL);
   }
-  constexpr int STEP = W * WAVE * N;
   const int64_t t = a.tok.p ? a.tok[row] : 0;
   const T m = a.stats[row], s = a.stats[a.rows + row], u = a.stats[2 * a.rows + row];
   const bool none = s == T(0) || (a.tok.p && (t == a.ignore || t < 0 || t >= a.V));
@@ -626,7 +686,15 @@ template <class T> void run_forward(LpForward<T> a) {
       NT_LAUNCH_CHECK();
     }
   };
-  if (a.V <= 2 * CHUNK) {
+  constexpr int SPAN = RowVec<T>::N * LP_UNROLL; // of a lane
+  if (a.k == 0 && a.V <= 4 * SPAN)
+    return launch(logprob_lanes_kernel<T, 4>, LP_THREADS, LP_THREADS / 4, 1);
+  if (a.k == 0 && a.V <= 16 * SPAN)
+    return launch(logprob_lanes_kernel<T, 16>, LP_THREADS, LP_THREADS / 16, 1);
+  // A wave per row where that gives every SIMD four of them (float32, us for a
+  // wave and a workgroup per row: 16384 x 3001 34 and 37, with 5 alternatives
+  // 43 and 60; 8192 x 8000 43 and 41.5, 51.5 and 51), else up to two chunks.
+  if (a.V <= (a.rows >= 16 * device_cu_count() ? 4 : 2) * CHUNK) {
     if (a.k)
       launch(logprob_wave_kernel<T, true>, LP_THREADS, LP_WAVES, 1);
     else
@@ -667,26 +735,29 @@ template <class T> void run_forward(LpForward<T> a) {
     launch(logprob_join_kernel<T, false>, WAVE, 1, 1);
 }
 
-template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
-  // Vectors per lane: with a workgroup per row two (8192 x 32000 float32 takes
-  // 328 us, with one 361, with four 347); rows that fit a wave need four.
-  constexpr int ONE = LP_UNROLL, MANY = 2;
-  constexpr int WAVE_SPAN = WAVE * RowVec<T>::N * ONE;
-  constexpr int SPAN = LP_THREADS * RowVec<T>::N * MANY; // of a workgroup
-  const bool small = a.V <= WAVE_SPAN;
-  const int64_t chunks = small ? 1 : (a.V + SPAN - 1) / SPAN;
-  const int64_t per = small ? LP_WAVES : 1;
-  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / chunks) * per;
+template <class T, bool ACC, int G, int UNROLL> void launch_backward(const LpBackward<T> &a) {
+  constexpr int SPAN = G * RowVec<T>::N * UNROLL, PER = LP_THREADS / G; // rows at once
+  const int64_t chunks = PER > 1 ? 1 : (a.V + SPAN - 1) / SPAN;
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / chunks) * PER;
   for (int64_t r = 0; r < a.rows; r += most) {
     const int64_t rows = std::min(a.rows - r, most);
-    const dim3 grid{unsigned((rows + per - 1) / per * chunks)};
-    if (small)
-      logprob_bwd_kernel<T, 1, ONE, ACC><<<grid, LP_THREADS, 0, stream()>>>(a, r, 1);
-    else
-      logprob_bwd_kernel<T, LP_WAVES, MANY, ACC>
-          <<<grid, LP_THREADS, 0, stream()>>>(a, r, int(chunks));
+    logprob_bwd_kernel<T, G, UNROLL, ACC>
+        <<<dim3(unsigned((rows + PER - 1) / PER * chunks)), LP_THREADS, 0, stream()>>>(
+            a, r, int(chunks));
     NT_LAUNCH_CHECK();
   }
+}
+
+template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
+  constexpr int SPAN = RowVec<T>::N * LP_UNROLL; // of a lane
+  if (a.V <= 4 * SPAN)
+    launch_backward<T, ACC, 4, LP_UNROLL>(a);
+  else if (a.V <= 16 * SPAN)
+    launch_backward<T, ACC, 16, LP_UNROLL>(a);
+  else if (a.V <= WAVE * SPAN)
+    launch_backward<T, ACC, WAVE, LP_UNROLL>(a);
+  else // 8192 x 32000 float32 takes 328 us, with one vector per lane 361, with four 347
+    launch_backward<T, ACC, LP_THREADS, 2>(a);
 }
 
 void check_logits(const nt_view *z, const nt_view *tokens, const char *fname) {

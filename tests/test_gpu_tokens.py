@@ -476,7 +476,8 @@ def draw_rows(r, rows, V, dtype, masked=0.0):
 @pytest.mark.parametrize("rows,V", [(1, 1), (2, 2), (3, 10), (65, 63), (5, 64), (3, 257),
                                     (9, 1000), (4, 1024), (4, 1025), (2, 2048), (3, 2049),
                                     (7, 4097), (2, 9000), (1, 50001), (300, 5003),
-                                    (1030, 4100), (1, 131072)])
+                                    (1030, 4100), (1, 131072), (70, 17), (3, 33), (1001, 65),
+                                    (17, 129), (9, 256), (4100, 2100)])
 def test_token_logprobs(gpu, dtype, rows, V):
     r = rng(seed_of("lp", dtype.__name__, rows, V))
     z, t = draw_rows(r, rows, V, dtype, 0.1 if V > 200 else 0.0)
@@ -521,7 +522,7 @@ LOW = {np.float32: np.finfo(np.float32).min, np.float64: np.finfo(np.float64).mi
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("V", [5, 300, 3001, 20000])
+@pytest.mark.parametrize("V", [5, 100, 300, 3001, 20000])
 def test_masked_rows(gpu, dtype, V):
     """Rows that a mask empties, leaves one token of, or fills with the type's
     lowest value; scores far apart; infinities and NaN."""
@@ -548,6 +549,7 @@ def test_masked_rows(gpu, dtype, V):
     t[9] = 1
     ref = Rows(z, dtype)
     Z = dev(z, True)
+    ref.check(nt.token_logprobs(Z, dev(t), entropy=True), t, True)
     out = nt.token_logprobs(Z, dev(t), entropy=True, top=3)
     ref.check(out, t, True, 3)
     a, b = r.standard_normal(10).astype(dtype), r.standard_normal(10).astype(dtype)
@@ -557,7 +559,7 @@ def test_masked_rows(gpu, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("rows,V", [(12, 30), (40, 3000), (3, 30000), (2000, 2500)])
+@pytest.mark.parametrize("rows,V", [(12, 30), (50, 200), (40, 3000), (3, 30000), (2000, 2500)])
 def test_rows_left_out(gpu, dtype, rows, V):
     r = rng(seed_of("ignored", rows, V))
     z, t = draw_rows(r, rows, V, dtype)
@@ -572,6 +574,7 @@ def test_rows_left_out(gpu, dtype, rows, V):
     ref.tol_lp[0] = 0
     ref.d[0] = 0
     Z = dev(z, True)
+    ref.check(nt.token_logprobs(Z, dev(t), entropy=True, ignore_index=-7), t, True)
     out = nt.token_logprobs(Z, dev(t), entropy=True, top=2, ignore_index=-7)
     ref.check(out, t, True, 2)
     a, b = r.standard_normal(rows).astype(dtype), r.standard_normal(rows).astype(dtype)
