@@ -1,0 +1,63 @@
+"""The token operators' argument checks and switches that need no device."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import nanotorch_amd as nt
+from nanotorch_amd import nn
+from nanotorch_amd.autograd import ops_token
+from nanotorch_amd.factories import next_dropout_counter
+
+
+def test_arguments_are_checked_before_the_device():
+    w, t = nt.ones(4, 3), nt.zeros(2, dtype=nt.int64)
+    for bad in (lambda: nt.embedding(nt.ones(4), t), lambda: nt.embedding(w, w),
+                lambda: nt.embedding(w, t, padding_idx=9), lambda: nt.dropout(w, 2.0),
+                lambda: nt.dropout(t, 0.5), lambda: nt.token_logprobs(w),
+                lambda: nt.token_logprobs(w, t), lambda: nt.token_logprobs(w, entropy=True, top=4),
+                lambda: nt.token_logprobs(t, t), lambda: nn.Dropout(-1.0),
+                lambda: nn.Embedding(3, 0)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_host_tensors_are_refused():
+    w, t = nt.ones(4, 3), nt.zeros(4, dtype=nt.int64)
+    for call in (lambda: nt.embedding(w, t), lambda: nt.dropout(w), lambda: nt.dropout(w, 0.0),
+                 lambda: nt.token_logprobs(w, t), lambda: nt.token_logprobs(w, top=2)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_dropout_counter():
+    nt.manual_seed(5)
+    assert [next_dropout_counter() for _ in range(3)] == [(5, 0), (5, 1), (5, 2)]
+    nt.manual_seed(-1)
+    assert next_dropout_counter() == (2 ** 64 - 1, 0)
+
+
+def test_train_and_eval_reach_nested_modules():
+    a, b = nn.Dropout(0.5), nn.Dropout(0.5)
+    net = nn.Sequential(a, nn.Sequential(nn.Tanh(), b), lambda x: x)
+    x = nt.ones(3)
+    assert net.eval() is net
+    assert a(x) is x and b(x) is x
+    net.train()
+    with pytest.raises(RuntimeError):  # drops again: needs the device
+        b(x)
+
+
+@pytest.mark.parametrize("make,in_place", [
+    (lambda a: a, True), (lambda a: a[1], True), (lambda a: a[:, :, 2:7], True),
+    (lambda a: a[0, 0], True), (lambda a: a[:, 1:], False), (lambda a: a[:, :, ::2], False),
+    (lambda a: a.transpose(0, 1), False), (lambda a: a[:, ::2, 1:2], False)])
+def test_rows_in_place(make, in_place):
+    """A view of rows where the strides allow one, else a copy; the same values."""
+    x = make(nt.Tensor(np.arange(2 * 3 * 20, dtype=np.float32).reshape(2, 3, 20)))
+    assert (ops_token._rows_in_place(x) is not None) == in_place
+    rows = ops_token._as_rows(x)
+    assert (rows.storage is x.storage) == in_place
+    want = x.numpy().reshape(-1, x.shape[-1])
+    assert rows.shape == want.shape and (rows.numpy() == want).all()
