@@ -66,40 +66,53 @@ template <class T> struct Four {
   }
 };
 
-// Contiguous operands: a counter per work-item; the last, partial one is
-// taken element by element.  Bound by memory: 8192 x 4096 float32 takes 42 us
-// (6.3 TB/s), with two or four counters per work-item no less.
+// Contiguous operands: 16 bytes per work-item (two work-items share a counter
+// in float64, each drawing it); the last, partial vector is taken element by
+// element.  Bound by memory: 8192 x 4096 float32 takes 42 us (6.4 TB/s), with
+// two or four vectors per work-item no less.
 template <class T, bool ACC>
 __global__ __launch_bounds__(DROP_THREADS) void dropout_flat_kernel(
-    const T *__restrict__ x, T *__restrict__ y, int64_t n, int64_t group0, DropoutPlan p) {
-  const int64_t g = group0 + int64_t(blockIdx.x) * DROP_THREADS + threadIdx.x, i = 4 * g;
-  const bool whole = i + 4 <= n;
-  Four<T> v, old;
+    const T *__restrict__ x, T *__restrict__ y, int64_t n, int64_t vec0, DropoutPlan p) {
+  using RV = RowVec<T>;
+  constexpr int N = RV::N;
+  const int64_t vec = vec0 + int64_t(blockIdx.x) * DROP_THREADS + threadIdx.x, i = N * vec;
+  if (i >= n)
+    return;
+  const bool whole = i + N <= n;
+  typename RV::V v = {}, old = {};
   if (whole) {
-    v.template load<true>(x + i);
+    v = RV::template load<true>(x + i);
     if (ACC)
-      old.template load<true>(y + i);
+      old = RV::template load<true>(y + i);
   } else {
-    for (int j = 0; j < 4; ++j) {
-      v.set(j, i + j < n ? x[i + j] : T(0));
+#pragma unroll
+    for (int j = 0; j < N - 1; ++j) {
+      const int64_t at = min(i + j, n - 1);
+      v[j] = x[at];
       if (ACC)
-        old.set(j, i + j < n ? y[i + j] : T(0));
+        old[j] = y[at];
     }
   }
   uint32_t w[4];
-  philox(uint64_t(g), p, w);
+  philox(uint64_t(i) >> 2, p, w);
+  if constexpr (N == 2) { // of an odd vector, the counter's words 2 and 3
+    w[0] = vec & 1 ? w[2] : w[0];
+    w[1] = vec & 1 ? w[3] : w[1];
+  }
   const T scale = T(p.scale);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const T r = p.keeps(w[j]) ? v.get(j) * scale : T(0);
-    v.set(j, ACC ? old.get(j) + r : r);
+  for (int j = 0; j < N; ++j) {
+    const T r = p.keeps(w[j]) ? v[j] * scale : T(0);
+    v[j] = ACC ? old[j] + r : r;
   }
-  if (whole)
-    v.template store<true>(y + i);
-  else
-    for (int j = 0; j < 4; ++j)
+  if (whole) {
+    RV::template store<true>(y + i, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N - 1; ++j)
       if (i + j < n)
-        y[i + j] = v.get(j);
+        y[i + j] = v[j];
+  }
 }
 
 // x [R, C] stored by columns (adjacent elements along R), y by rows: tiles
@@ -204,11 +217,12 @@ void run_dropout(const nt_view *x, const nt_view *y, const DropoutPlan &p) {
   const bool flat = L.ndim == 0 ||
                     (L.ndim == 1 && L.strides[0][0] == 1 && L.strides[1][0] == 1);
   if (flat) {
-    const int64_t groups = (n + 3) / 4, most = int64_t(DROP_THREADS) << 22;
-    for (int64_t g = 0; g < groups; g += most) {
-      const dim3 grid{unsigned((std::min(most, groups - g) + DROP_THREADS - 1) / DROP_THREADS)};
+    const int64_t vecs = (n + RowVec<T>::N - 1) / RowVec<T>::N;
+    const int64_t most = int64_t(DROP_THREADS) << 22;
+    for (int64_t v = 0; v < vecs; v += most) {
+      const dim3 grid{unsigned((std::min(most, vecs - v) + DROP_THREADS - 1) / DROP_THREADS)};
       ew_launch(dropout_flat_kernel<T, ACC>, grid, DROP_THREADS, stream(), flags, px, py, n,
-                g, p);
+                v, p);
     }
     return;
   }
