@@ -9,7 +9,6 @@
 // nothing: the lookup reads N rows and writes N rows, the gradient reads N
 // rows and writes every row of dW once, zeros included (accumulating, it
 // reads and writes only the rows that a token names).
-#include "ew_engine.h"
 #include "tokens.h"
 
 #include <algorithm>
@@ -76,7 +75,7 @@ struct Rows {
 // A workgroup writes EMB_THREADS * EMB_LOOKUP adjacent vectors of the output,
 // each work-item every EMB_THREADS-th of them, so that as many loads are in
 // flight.  Rows of adjacent elements.  65536 rows of 2048 float32 (0.54 GB
-// written, 0.16 GB of different rows read) take 131 us alone and 147
+// written, 0.16 GB of different rows read) take 131 us alone and 157
 // behind a gradient that is still on its way to memory; with a branch around
 // each load 181, with stores that stay in the cache 144.
 constexpr int EMB_LOOKUP = 4;
@@ -218,8 +217,8 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_scan_kernel(
 // sum per tile, which a last kernel joins in tile order.  So a token that
 // fills a tenth of the batch is spread over the chip like any other.
 //
-// 65536 tokens into 128000 x 2048 float32: sort 27 us, sums 134 (0.54 GB read,
-// 0.17 GB written), joins 15, zero rows 127 (0.89 GB, 7.0 TB/s).  8192 into
+// 65536 tokens into 128000 x 2048 float32: sort 27 us, sums 137 (0.54 GB read,
+// 0.17 GB written), joins 15, zero rows 129 (0.89 GB, 6.9 TB/s).  8192 into
 // 32000 x 1024: sort and zero rows 20 us, sums 13, joins 4.
 
 constexpr int EMB_DIGIT = 9; // bits of a pass, at most
@@ -825,15 +824,12 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
   const Pairs &sorted = p.side[(p.passes - 1) & 1];
   const SumPlan q{sorted.key, sorted.pos, p.n, uint32_t(V), FastDivU32(vectors), int(D),
                   dw->strides[0], tile};
-  // The zero rows need the first pass's flags alone, so they are written
-  // beside the last pass (65536 tokens, 128000 x 2048: both passes through the
-  // table 440 us; behind the sums 462).
   if (!ACC && !ranked)
     in_launches(V, vectors, [&](int64_t r0, int64_t n) {
-      const uint32_t flags = p.passes > 1 && r0 == 0 ? beside_launch_flag() : 0;
-      ew_launch(embedding_fill_kernel<T, EVEN>,
-                dim3(blocks_for(n * vectors, EMB_THREADS * EMB_FILL)), EMB_THREADS, s, flags,
-                q, to, p.present, uint32_t(r0), uint32_t(n * vectors));
+      embedding_fill_kernel<T, EVEN>
+          <<<dim3(blocks_for(n * vectors, EMB_THREADS * EMB_FILL)), EMB_THREADS, 0, s>>>(
+              q, to, p.present, uint32_t(r0), uint32_t(n * vectors));
+      NT_LAUNCH_CHECK();
     });
   DeviceScratch part(size_t(2 * tiles * vectors) * 16);
   in_launches(tiles, vectors, [&](int64_t t0, int64_t n) {

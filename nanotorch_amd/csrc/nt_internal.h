@@ -94,10 +94,6 @@ std::recursive_mutex &api_mutex();
 // the overlap off.
 uint32_t ew_launch_flags(const ByteRange *reads, int nr,
                          const ByteRange *writes, int nw);
-// hipExtAnyOrderLaunch, or 0 with NT_OVERLAP=0: for an entry point that lets
-// one of its own kernels start beside the one queued just before it (which
-// took the barrier, so everything earlier has finished).
-uint32_t beside_launch_flag();
 // Closes the launch window: when a kernel of it went without the barrier,
 // queues an empty barrier kernel, so that whatever is queued next (a copy,
 // an event, a synchronisation, any other kernel) starts after every earlier

@@ -184,10 +184,6 @@ uint32_t ew_launch_flags(const ByteRange *reads, int nr,
   return 0u;
 }
 
-uint32_t beside_launch_flag() {
-  return overlap_enabled() ? uint32_t(hipExtAnyOrderLaunch) : 0u;
-}
-
 void stream_fence() {
   Runtime &r = rt();
   if (r.window.close()) {
