@@ -14,7 +14,7 @@
 //
 // Bound by memory where rows are many: 8192 x 32000 float32 (a tenth of the
 // rows left out) reads 0.94 GB in 156 us (6.0 TB/s), and its gradient moves
-// 2.0 GB in 328 us (6.1 TB/s).  2000 x 50001 takes 68 us, with 5 alternatives
+// 2.0 GB in 328 us (6.1 TB/s; with half of the rows left out 268, with all 182).  2000 x 50001 takes 68 us, with 5 alternatives
 // 74, with 20 84, with 64 140.  Few rows are split over several workgroups
 // and joined by a second kernel: 8 x 128000 with 8 alternatives 7 + 8 us,
 // 64 x 128000 10 us in all without alternatives.  Joined by each row's last
@@ -602,13 +602,17 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a
   const bool none = s == T(0) || (a.tok.p && (t == a.ignore || t < 0 || t >= a.V));
   T *dz = a.dz + row * a.dz_stride;
   if (none) {
-    if (!ACC)
-      for (int c = 0; c < UNROLL; ++c)
-        for (int j = 0; j < N; ++j) {
-          const int64_t i = int64_t(first) + c * STEP + j;
-          if (i < a.V)
-            dz[i] = T(0);
-        }
+    if (!ACC) {
+#pragma unroll
+      for (int c = 0; c < UNROLL; ++c) {
+        const int64_t i = int64_t(first) + c * STEP;
+        if (i + N <= a.V)
+          RV::store(dz + i, typename RV::V{});
+        else
+          for (int64_t j = i; j < a.V; ++j)
+            dz[j] = T(0);
+      }
+    }
     return;
   }
   const T log_s = log(s), H = log_s - u / s, inv = T(1) / s;
