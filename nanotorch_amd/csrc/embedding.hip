@@ -1,7 +1,7 @@
 // Rows of a table looked up by token, and the table's gradient:
 //
 //   y[i, :]  = scale * W[t_i, :]
-//   dW[v, :] = scale * sum over the i with t_i = v, in rising i, of g[i, :]
+//   dW[v, :] = scale * sum over the i with t_i = v of g[i, :]
 //
 // A token equal to `padding` gives a zero row and no gradient; one outside
 // the table does too, and is reported at the next synchronisation (the
@@ -238,6 +238,7 @@ struct SortPlan {
   uint32_t n, per; // pairs; of them per workgroup, at most SORT_MOST
   int groups, digit, passes;
   uint32_t *table;  // [groups][EMB_BINS] counts
+  uint32_t *total;  // [EMB_BINS], or null: then table holds the counts of the groups before
   uint8_t *present; // [V], or null: 1 where a row has a gradient
   Pairs side[2];    // pass k writes side[k & 1]
 };
@@ -345,11 +346,16 @@ __device__ __forceinline__ void sort_pass(const SortPlan &p, int pass, const Sor
   // all workgroups' pairs of a digit, a digit per thread of the first EMB_BINS
   uint32_t total = 0, before = 0;
   if (tid < EMB_BINS) {
+    if (p.total) {
+      before = p.table[blockIdx.x * EMB_BINS + tid];
+      total = p.total[tid];
+    } else {
 #pragma unroll 8
-    for (int b = 0; b < p.groups; ++b) {
-      const uint32_t c = p.table[b * EMB_BINS + tid];
-      before += b < int(blockIdx.x) ? c : 0;
-      total += c;
+      for (int b = 0; b < p.groups; ++b) {
+        const uint32_t c = p.table[b * EMB_BINS + tid];
+        before += b < int(blockIdx.x) ? c : 0;
+        total += c;
+      }
     }
   }
   __syncthreads();
@@ -427,6 +433,39 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_count_kernel(SortPlan 
   __syncthreads();
   for (int d = threadIdx.x; d < EMB_BINS; d += SORT_THREADS)
     p.table[blockIdx.x * EMB_BINS + d] = bin[d];
+}
+
+// Where the groups are many, each count becomes the sum of those of the groups
+// before.  A workgroup takes 64 digits, a wave of it a part of the groups.  By
+// this and by each workgroup of the places adding up all counts (us, 1000 x
+// 16): 1048576 tokens (128 groups) 90 and 84, 4194304 242 and 304, 16777216
+// 935 and 2304.
+constexpr int SORT_ADDED = 256; // groups up to which they are added up
+
+__global__ __launch_bounds__(SORT_THREADS) void embedding_offsets_kernel(SortPlan p) {
+  __shared__ uint32_t sums[SORT_WAVES][WAVE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int digit = blockIdx.x * WAVE + lane;
+  const int per = (p.groups + SORT_WAVES - 1) / SORT_WAVES;
+  const int beg = min(p.groups, wave * per), end = min(p.groups, beg + per);
+  uint32_t *const at = p.table + digit;
+  uint32_t sum = 0;
+#pragma unroll 16
+  for (int b = beg; b < end; ++b)
+    sum += at[int64_t(b) * EMB_BINS];
+  sums[wave][lane] = sum;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w)
+    before += sums[w][lane];
+  if (wave == SORT_WAVES - 1)
+    p.total[digit] = before + sum;
+#pragma unroll 16
+  for (int b = beg; b < end; ++b) {
+    const uint32_t c = at[int64_t(b) * EMB_BINS];
+    at[int64_t(b) * EMB_BINS] = before;
+    before += c;
+  }
 }
 
 __global__ __launch_bounds__(SORT_THREADS) void embedding_place_kernel(SortPlan p, int pass) {
@@ -795,9 +834,11 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
   const int64_t per = std::clamp<int64_t>((N + 63) / 64, 2048, SORT_MOST);
   p.per = uint32_t((per + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS);
   p.groups = int((N + p.per - 1) / p.per);
-  DeviceScratch table(ranked ? 0 : size_t(p.groups) * EMB_BINS * 4),
+  const bool added = p.groups <= SORT_ADDED;
+  DeviceScratch table(ranked ? 0 : size_t(p.groups + !added) * EMB_BINS * 4),
       present(ACC || ranked ? 0 : size_t(V));
   p.table = table.get<uint32_t>();
+  p.total = added ? nullptr : p.table + int64_t(p.groups) * EMB_BINS;
   p.present = present.get<uint8_t>();
   if (ranked) {
     p.passes = 1;
@@ -810,6 +851,10 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
     for (int k = 0; k < p.passes; ++k) {
       embedding_count_kernel<<<dim3(unsigned(p.groups)), SORT_THREADS, 0, s>>>(p, k);
       NT_LAUNCH_CHECK();
+      if (!added) {
+        embedding_offsets_kernel<<<dim3(EMB_BINS / WAVE), SORT_THREADS, 0, s>>>(p);
+        NT_LAUNCH_CHECK();
+      }
       embedding_place_kernel<<<dim3(unsigned(p.groups)), SORT_THREADS, 0, s>>>(p, k);
       NT_LAUNCH_CHECK();
     }

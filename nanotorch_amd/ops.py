@@ -123,8 +123,8 @@ def embedding(table: Tensor, tokens: Tensor, scale: float = 1.0, *,
     A token equal to ``padding_idx`` gives a zero row and no gradient.  Tokens
     are checked on the device: one outside the table gives a zero row, and the
     next synchronisation (``sync``, ``cpu``) raises IndexError.  The table's
-    gradient sums each row's terms in the order of the tokens, so it comes out
-    the same every time."""
+    gradient sums each row's terms in an order that the tokens alone fix, so it
+    comes out the same every time."""
     return autograd.EmbeddingOp.apply(table, tokens, scale, padding_idx)
 
 
