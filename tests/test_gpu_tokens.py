@@ -103,6 +103,19 @@ def test_embedding(gpu, dtype, V, D, N, kind):
         assert_bitexact(host(again), host(dw), "a second run")
 
 
+@pytest.mark.parametrize("V", [700, 100000])
+def test_embedding_gradient_of_very_many_tokens(gpu, V):
+    """Sorted by more workgroups than add up each other's counts.  Small
+    integers, whose sums are exact in any order."""
+    N, D = (1 << 21) + 5001, 5
+    r = rng(seed_of("many", V))
+    t = np.where(r.random(N) < 0.2, 3, r.integers(0, V, N))
+    g = r.integers(-8, 9, (N, D)).astype(np.float32)
+    y = nt.embedding(dev(np.zeros((V, D), np.float32), True), dev(t))
+    want = np.stack([np.bincount(t, g[:, c], V) for c in range(D)], 1)
+    assert_bitexact(host(y.grad_fn.backward(dev(g))[0]), want.astype(np.float32))
+
+
 @pytest.mark.parametrize("shape", [(), (0,), (4, 0), (3, 1, 5), (2, 3, 4, 5)])
 def test_embedding_token_shapes(gpu, shape):
     r = rng(seed_of(shape))
@@ -323,6 +336,45 @@ def test_dropout_transposed(gpu, dtype, shape):
     g = rng(1).standard_normal(shape[::-1]).astype(dtype)
     assert_bitexact(host(y.grad_fn.backward(dev(np.ascontiguousarray(g.T)).T)[0]),
                     dropped(g, 0.25, 4, 6))
+
+
+@pytest.mark.parametrize("shape", [(3, 5, 1), (2, 3, 3), (5, 4, 4), (9, 17, 31), (40, 33, 64)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_dropout_rows_of_views(gpu, dtype, shape):
+    """Rows of adjacent elements, of lengths below and beside a counter's
+    four, in views of two to four dimensions; planes of columns; both passes,
+    new and added."""
+    a = rng(seed_of("rows", shape)).standard_normal((2,) + shape[:2] + (shape[2] + 3,))
+    a = a.astype(dtype)
+    swapped = (0, 2, 1, 3), (0, 1, 3, 2), (3, 1, 2, 0), (2, 3, 0, 1)
+    for cut in (lambda x: x[..., 1:shape[2] + 1], lambda x: x[0, :, ::2, :shape[2]],
+                lambda x: x[1, 1, :, :shape[2]], lambda x: x[..., ::2]):
+        v, V = cut(a), cut(dev(a))
+        orders = swapped if v.ndim == 4 else [tuple(range(v.ndim)), tuple(range(v.ndim))[::-1]]
+        for order in orders:
+            w, W = v.transpose(order), V
+            left = list(range(v.ndim))
+            for k, o in enumerate(order):  # one exchange of axes at a time
+                j = left.index(o)
+                if j != k:
+                    W = W.transpose(k, j)
+                    left[k], left[j] = left[j], left[k]
+            assert W.shape == w.shape
+            assert_bitexact(host(nt.dropout(W, 0.4, seed=8, offset=3)), dropped(w, 0.4, 8, 3))
+            x = dev(np.ascontiguousarray(w), True)
+            y = nt.dropout(x, 0.4, seed=8, offset=3)
+            target = dev(a.copy())
+            into = cut(target)
+            left = list(range(v.ndim))
+            for k, o in enumerate(order):
+                j = left.index(o)
+                if j != k:
+                    into = into.transpose(k, j)
+                    left[k], left[j] = left[j], left[k]
+            y.grad_fn._backward_into(W, [True], [into])
+            want = a.copy()
+            cut(want).transpose(order)[...] += dropped(w, 0.4, 8, 3)
+            assert_bitexact(host(target), want)
 
 
 @pytest.mark.parametrize("strided", [False, True])
@@ -737,6 +789,16 @@ def test_dropout_past_32_bits(gpu):
         w = words_of(i, 3, 4)[at % 4:at % 4 + 13]
         assert_bitexact(part, np.where(w >= np.uint64(1 << 31), np.float32(2), np.float32(0)))
 
+
+def test_dropout_of_a_view_past_32_bits(gpu):
+    m = (1 << 16) + 1
+    x = nt.ones(m, m + 63, device="cuda")[:, 5:m + 5]
+    y = nt.dropout(x, 0.5, seed=3, offset=4)
+    for row in (0, 1, 40000, m - 1):
+        i = np.arange(row * m // 4, (row + 1) * m // 4 + 1, dtype=np.uint64)
+        w = words_of(i, 3, 4)[row * m % 4:][:m]
+        assert_bitexact(host(y[row]), np.where(w >= np.uint64(1 << 31), np.float32(2),
+                                               np.float32(0)))
 
 
 def test_offsets_past_32_bits(gpu):
