@@ -58,13 +58,36 @@ __device__ __forceinline__ float exp_of(float d) {
   const float e = __builtin_amdgcn_exp2f(h);
   return __builtin_fmaf(e, l * LN2, e);
 }
-__device__ __forceinline__ double exp_of(double d) { return exp(d); }
+// 2^k exp(r) with |r| <= ln 2 / 2, where exp(r) is 1 + r + r^2 q(r); q
+// interpolates at the Chebyshev nodes of that interval (error 0.15 2^-53).
+// 8192 x 16000 takes 207 us and 383 for its gradient, with the general exp()
+// 236 and 389.
+__device__ __forceinline__ double exp_of(double d) {
+  const double k = __builtin_rint(d * 1.4426950408889634);
+  const double r = __builtin_fma(k, -2.3190468138462996e-17,
+                                 __builtin_fma(k, -0.6931471805599453, d));
+  double q = 2.510038549551032e-08;
+  q = __builtin_fma(q, r, 2.7620088445409746e-07);
+  q = __builtin_fma(q, r, 2.7557268459997064e-06);
+  q = __builtin_fma(q, r, 2.4801521295954376e-05);
+  q = __builtin_fma(q, r, 0.00019841269863053618);
+  q = __builtin_fma(q, r, 0.0013888888917213717);
+  q = __builtin_fma(q, r, 0.008333333333330062);
+  q = __builtin_fma(q, r, 0.04166666666662413);
+  q = __builtin_fma(q, r, 0.16666666666666669);
+  q = __builtin_fma(q, r, 0.5000000000000001);
+  q = __builtin_fma(q * r, r, r);
+  return __builtin_amdgcn_ldexp(1.0 + q, int(k));
+}
 
 // Past this distance from the maximum exp() is 0 in T.
 template <class T> constexpr T LP_CUT = sizeof(T) == 4 ? T(-200) : T(-800);
 
 template <class T> __device__ __forceinline__ T not_below_cut(T d) {
-  return __builtin_elementwise_maximum(d, T(LP_CUT<T>)); // NaN stays
+  if constexpr (sizeof(T) == 4)
+    return __builtin_elementwise_maximum(d, LP_CUT<T>); // NaN stays
+  else // float64 has no such instruction
+    return d < LP_CUT<T> ? LP_CUT<T> : d;
 }
 
 // The larger one; NaN if either is.
