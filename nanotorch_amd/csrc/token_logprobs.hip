@@ -14,7 +14,7 @@
 //
 // Bound by memory where rows are many: 8192 x 32000 float32 (a tenth of the
 // rows left out) reads 0.94 GB in 156 us (6.0 TB/s), and its gradient moves
-// 2.0 GB in 328 us (6.1 TB/s; with half of the rows left out 268, with all 182).  2000 x 50001 takes 68 us, with 5 alternatives
+// 2.0 GB in 328 us (6.1 TB/s; with half of the rows left out 268, with all 183).  2000 x 50001 takes 68 us, with 5 alternatives
 // 74, with 20 84, with 64 140.  Few rows are split over several workgroups
 // and joined by a second kernel: 8 x 128000 with 8 alternatives 7 + 8 us,
 // 64 x 128000 10 us in all without alternatives.  Joined by each row's last
