@@ -601,6 +601,7 @@ template <class T> struct LpBackward {
   int64_t sa, sb;   // their strides
   T *dz;
   int64_t dz_stride;
+  int last_first; // the last rows first
 };
 
 // G lanes per row, each UNROLL vectors; a whole workgroup (G = LP_THREADS)
@@ -620,6 +621,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a
     row = row0 + blockIdx.x / chunks;
     first += (blockIdx.x % chunks) * (STEP * UNROLL);
   }
+  if (G != WAVE && a.last_first)
+    row = a.rows - 1 - row;
   const int64_t t = a.tok.p ? a.tok[row] : 0;
   const T m = a.stats[row], s = a.stats[a.rows + row], u = a.stats[2 * a.rows + row];
   const bool none = s == T(0) || (a.tok.p && (t == a.ignore || t < 0 || t >= a.V));
@@ -701,6 +704,11 @@ T *out_vector(const nt_view *v, int64_t n, int dtype, const char *what) {
   return typed_ptr<T>(v);
 }
 
+// Whether logits are larger than the 256 MB of the Infinity Cache.
+template <class T> bool outgrow_cache(int64_t rows, int64_t V) {
+  return rows * V * int64_t(sizeof(T)) > int64_t(256) << 20;
+}
+
 template <class T> void run_forward(LpForward<T> a) {
   constexpr int CHUNK = WAVE * RowVec<T>::N * LP_UNROLL;
   const auto launch = [&](auto kernel, int threads, int64_t rows_per_block,
@@ -741,10 +749,10 @@ template <class T> void run_forward(LpForward<T> a) {
   a.pu = a.ps + n;
   a.pkey = reinterpret_cast<K *>(a.pu + n);
   a.ptoken = reinterpret_cast<int32_t *>(a.pkey + n * a.k);
-  // Logits that outgrow the 256 MB Infinity Cache are streamed past it (8192 x
-  // 32000 float32: 214 us without, 160 with); smaller ones stay there for the
+  // Logits that outgrow the Infinity Cache are streamed past it (8192 x 32000
+  // float32: 214 us without, 160 with); smaller ones stay there for the
   // backward pass (8192 x 1000: both passes 24 us, streamed 26).
-  const bool stream_in = a.rows * int64_t(a.V) * int64_t(sizeof(T)) > int64_t(256) << 20;
+  const bool stream_in = outgrow_cache<T>(a.rows, a.V);
   const auto group = [&](auto top, auto streams) {
     launch(logprob_group_kernel<T, top.value, streams.value>, LP_THREADS, 1, a.splits);
   };
@@ -775,7 +783,14 @@ template <class T, bool ACC, int G, int UNROLL> void launch_backward(const LpBac
   }
 }
 
-template <class T, bool ACC> void run_backward(const LpBackward<T> &a) {
+template <class T, bool ACC> void run_backward(LpBackward<T> a) {
+  // Of logits that outgrow the Infinity Cache, what the forward pass read last
+  // is still there: the backward pass begins with it, unless a wave takes a
+  // row (both passes, us, rows in order and last rows first: 8192 x 32000
+  // float32 with the entropy 509 and 492, 1000000 x 100 265 and 252, but 200000 x
+  // 1000 476 and 487).  Smaller ones lie in the L2 of the XCD that takes the
+  // same row again (8192 x 1000 18.9 and 20.4).
+  a.last_first = outgrow_cache<T>(a.rows, a.V);
   constexpr int SPAN = RowVec<T>::N * LP_UNROLL; // of a lane
   if (a.V <= 4 * SPAN)
     launch_backward<T, ACC, 4, LP_UNROLL>(a);
