@@ -14,12 +14,14 @@
 //
 // Bound by memory where rows are many: 8192 x 32000 float32 (a tenth of the
 // rows left out) reads 0.94 GB in 156 us (6.0 TB/s), and its gradient moves
-// 2.0 GB in 328 us (6.1 TB/s; with half of the rows left out 268, with all 183).  2000 x 50001 takes 68 us, with 5 alternatives
-// 74, with 20 84, with 64 140.  Few rows are split over several workgroups
-// and joined by a second kernel: 8 x 128000 with 8 alternatives 7 + 8 us,
-// 64 x 128000 10 us in all without alternatives.  Joined by each row's last
-// workgroup instead, one launch less, those take 20 and 50: every part's
-// release to the other XCDs writes back an L2.
+// 2.0 GB in 328 us (6.1 TB/s; with half of the rows left out 268, with all
+// 183).  2000 x 50001 takes 68 us, with 5 alternatives 74, with 20 79, with 64
+// 115.  Few rows are split over several workgroups and joined by a second
+// kernel: 8 x 128000 with 8 alternatives 7.5 + 5.5 us, with 50 14 + 5.5;
+// 64 x 128000 10 us in all without alternatives, with 50 25.  Joined by each
+// row's last workgroup instead, one launch less, 64 x 128000 without
+// alternatives takes 50: every part's release to the other XCDs writes back an
+// L2.
 //
 // Logits of -inf are tokens without probability and count for nothing; a row
 // that holds nothing else has log probability -inf, entropy 0 and no
@@ -34,7 +36,10 @@
 // (which the pass computes anyway) exceeds the k-th best so far, and the first
 // chunk's only where they reach the k-th largest of the maxima of all lanes
 // that share the row: in n elements of random order about k (1 + ln(n / c))
-// of them, c being a chunk.
+// of them, c being a chunk.  The lists of waves and workgroups are merged by a
+// bitonic network over the lanes (K. Batcher, "Sorting networks and their
+// applications", AFIPS 1968), about a hundred instructions a list; entry by
+// entry, 8 x 128000 with 50 alternatives took 18 + 28 us.
 #include "tokens.h"
 
 #include <algorithm>
@@ -146,6 +151,30 @@ template <int G, class T, class F> __device__ __forceinline__ T over_lanes(T v, 
   return v;
 }
 
+// A word from lane i ^ S.
+template <int S> __device__ __forceinline__ uint32_t from_xor(uint32_t v) {
+  if constexpr (S == 1)
+    return from_lane<0xB1, 0xf>(v, v);
+  else if constexpr (S == 2)
+    return from_lane<0x4E, 0xf>(v, v);
+  else if constexpr (S == 4) { // four lanes up in every other four, down in the rest
+    const int up = __builtin_amdgcn_update_dpp(int(v), int(v), 0x104, 0xf, 0x5, false);
+    return __builtin_amdgcn_update_dpp(up, int(v), 0x114, 0xf, 0xa, false);
+  } else if constexpr (S == 8)
+    return from_lane<0x128, 0xf>(v, v);
+  else if constexpr (S == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    static_assert(S == 32);
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int S> __device__ __forceinline__ uint64_t from_xor(uint64_t v) {
+  return uint64_t(from_xor<S>(uint32_t(v >> 32))) << 32 | from_xor<S>(uint32_t(v));
+}
+
 template <class T> struct RowState {
   T m = -std::numeric_limits<T>::infinity(), s = T(0), u = T(0);
 
@@ -228,6 +257,8 @@ template <> struct Key<double> {
 
 constexpr int RAISE_BITS = 20; // sign, exponent and 11 (of a double, 8) bits more
 
+constexpr int TOP_ALONE = WAVE / 2;
+
 // A wave's best entries in falling order, the i-th in lane i.
 template <class T> struct TopList {
   using K = typename Key<T>::K;
@@ -245,16 +276,38 @@ template <class T> struct TopList {
     key = stays ? key : here ? v : up;
     least = max(least, read_lane(key, k - 1));
   }
-  // One entry per lane, in rising order of their tokens among equal keys.
-  __device__ __forceinline__ void insert_lanes(K v, int32_t t, int k) {
-    uint64_t m = __ballot(v > least);
-    while (m) {
-      const int l = __ffsll((unsigned long long)m) - 1;
-      m &= m - 1;
-      const K c = read_lane(v, l);
-      if (c > least)
-        insert(c, int32_t(read_lane(uint32_t(t), l)), k);
+  // Lists of up to 16 entries are joined within 16 lanes.
+  static __device__ __forceinline__ int width(int k) { return k <= 16 ? 16 : WAVE; }
+  // The entry that a lane brings to merge(); its list has it if it is below k.
+  static __device__ __forceinline__ uint32_t brings(int lane, int k) {
+    return uint32_t(width(k) - 1 - lane);
+  }
+  // Another list, from its end.  The better one of each lane's two entries is
+  // among the best of both lists, and these rise and then fall along the
+  // lanes: exchanges at halving distances sort them.
+  __device__ __forceinline__ void merge(K v, int32_t t, int k) {
+    if (read_lane(v, width(k) - 1) < least)
+      return;
+    const bool take = v > key || (v == key && t < token);
+    key = take ? v : key;
+    token = take ? t : token;
+    if (k > 16) {
+      exchange<32>();
+      exchange<16>();
     }
+    exchange<8>();
+    exchange<4>();
+    exchange<2>();
+    exchange<1>();
+    least = max(least, read_lane(key, k - 1));
+  }
+  template <int S> __device__ __forceinline__ void exchange() {
+    const K v = from_xor<S>(key);
+    const int32_t t = int32_t(from_xor<S>(uint32_t(token)));
+    const bool better = v > key || (v == key && t < token);
+    const bool take = better == ((threadIdx.x & S) == 0);
+    key = take ? v : key;
+    token = take ? t : token;
   }
   // Of the lanes' keys x, N each, the k-th largest is found bit by bit, its
   // leading RAISE_BITS; nothing below it is among the k best of anything that
@@ -273,6 +326,26 @@ template <class T> struct TopList {
     // just below it; no logit has the key below 0's (that of -0)
     if (at)
       least = max(least, at - (at == Key<T>::of(T(0)) ? 2 : 1));
+  }
+  // From a wave's first chunk alone.  Beyond TOP_ALONE alternatives the 64
+  // maxima bound little: then a lane gives the maximum of each of its vectors
+  // (8192 x 1000, k = 50 and 64, us: 33 and 39, by 64 maxima 46 and 100).
+  template <int N> __device__ __forceinline__ void raise_alone(const T (&v)[N], T most, int k) {
+    if (k <= TOP_ALONE) {
+      const K one[1] = {Key<T>::of(most)};
+      return raise(one, k);
+    }
+    constexpr int PER = N / LP_UNROLL;
+    K each[LP_UNROLL];
+#pragma unroll
+    for (int c = 0; c < LP_UNROLL; ++c) {
+      T x = v[c * PER];
+#pragma unroll
+      for (int j = 1; j < PER; ++j)
+        x = max_nan(x, v[c * PER + j]);
+      each[c] = Key<T>::of(x);
+    }
+    raise(each, k);
   }
 };
 
@@ -359,7 +432,7 @@ __device__ __forceinline__ bool row_left_out(const LpForward<T> &a, int64_t row,
 }
 
 // Elements beg .. end - 1 of a row into the wave's state and list; `first`
-// gets each lane's largest key of the first chunk.
+// gets each lane's values of the first chunk and their maximum.
 template <class T, bool TOP, bool STREAM, class F>
 __device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k,
                                      RowState<T> &r, TopList<T> &top, F &&first) {
@@ -389,7 +462,7 @@ __device__ __forceinline__ void walk(const T *z, int32_t beg, int32_t end, int k
       most = max_nan(most, v[j]);
     if constexpr (TOP) {
       if (b == beg)
-        first(Key<T>::of(most));
+        first(v, most);
       // NaN, which nothing is below, while there is no such bound
       const T least = Key<T>::value(top.least);
       if (__ballot(!(most <= least))) {
@@ -477,10 +550,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_wave_kernel(LpForward<T> a
   RowState<T> r;
   TopList<T> top;
   walk<T, TOP, false>(a.z + row * a.row_stride, 0, a.V, a.k, r, top,
-                      [&](typename Key<T>::K x) {
-                        const typename Key<T>::K one[1] = {x};
-                        top.raise(one, a.k);
-                      });
+                      [&](const auto &v, T most) { top.raise_alone(v, most, a.k); });
   r.join_lanes();
   write_row(a, row, t, r, top);
 }
@@ -504,8 +574,11 @@ __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_gr
   }
   RowState<T> r;
   TopList<T> top;
-  const int64_t beg = int64_t(split * LP_WAVES + wave) * a.part;
-  const auto first = [&](typename Key<T>::K x) { // by all waves together
+  const int64_t row_part = int64_t(split) * LP_WAVES * a.part; // of the workgroup
+  const int64_t beg = row_part + wave * int64_t(a.part);
+  // the bound by all waves together, unless most of them have nothing
+  const bool alone = a.k > TOP_ALONE && row_part + a.part >= a.V;
+  const auto share = [&](typename Key<T>::K x) {
     __shared__ typename Key<T>::K most[LP_WAVES][WAVE];
     most[wave][lane] = x;
     __syncthreads();
@@ -517,9 +590,15 @@ __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_gr
   };
   if (beg < a.V)
     walk<T, TOP, STREAM>(a.z + row * a.row_stride, int32_t(beg),
-                         int32_t(std::min<int64_t>(a.V, beg + a.part)), a.k, r, top, first);
-  else if (TOP)
-    first(0);
+                         int32_t(std::min<int64_t>(a.V, beg + a.part)), a.k, r, top,
+                         [&](const auto &v, T most) {
+                           if (alone)
+                             top.raise_alone(v, most, a.k);
+                           else
+                             share(Key<T>::of(most));
+                         });
+  else if (TOP && !alone)
+    share(0);
   r.join_lanes();
   if (lane == 0) {
     sm[0][wave] = r.m;
@@ -539,9 +618,10 @@ __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_gr
     o.s = sm[1][w];
     o.u = sm[2][w];
     r.join(o);
-    if constexpr (TOP)
-      top.insert_lanes(lane < a.k ? skey[w][lane] : 0, lane < a.k ? stoken[w][lane] : -1,
-                       a.k);
+    if constexpr (TOP) {
+      const uint32_t e = top.brings(lane, a.k);
+      top.merge(e < uint32_t(a.k) ? skey[w][e] : 0, e < uint32_t(a.k) ? stoken[w][e] : -1, a.k);
+    }
   }
   if (a.splits == 1)
     return write_row(a, row, t, r, top);
@@ -557,31 +637,61 @@ __global__ __launch_bounds__(LP_THREADS, sizeof(T) == 4 ? 8 : 4) void logprob_gr
   }
 }
 
-// Joins the splits of a row; a wave per row.
+// Joins the splits of a row: a wave the states, four waves the alternatives.
 template <class T, bool TOP>
-__global__ __launch_bounds__(WAVE) void logprob_join_kernel(LpForward<T> a,
-                                                            int64_t row0) {
+__global__ __launch_bounds__(TOP ? LP_THREADS : WAVE) void logprob_join_kernel(LpForward<T> a,
+                                                                               int64_t row0) {
+  using K = typename Key<T>::K;
   const int64_t row = row0 + blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t t;
-  if (row_left_out(a, row, t))
-    return write_left_out(a, row);
+  if (row_left_out(a, row, t)) {
+    if (wave == 0)
+      write_left_out(a, row);
+    return;
+  }
   RowState<T> r;
   TopList<T> top;
-  for (int b = lane; b < a.splits; b += WAVE) {
-    RowState<T> o;
-    o.m = a.pm[row * a.splits + b];
-    o.s = a.ps[row * a.splits + b];
-    o.u = a.pu[row * a.splits + b];
-    r.join(o);
+  if (wave == 0) {
+    for (int b = lane; b < a.splits; b += WAVE) {
+      RowState<T> o;
+      o.m = a.pm[row * a.splits + b];
+      o.s = a.ps[row * a.splits + b];
+      o.u = a.pu[row * a.splits + b];
+      r.join(o);
+    }
+    r.join_lanes();
   }
-  r.join_lanes();
   if constexpr (TOP) {
-    const int64_t n = int64_t(a.splits) * a.k, base = row * n;
-    for (int64_t b = 0; b < n; b += WAVE) {
-      const bool in = b + lane < n;
-      top.insert_lanes(in ? a.pkey[base + b + lane] : 0, in ? a.ptoken[base + b + lane] : -1,
-                       a.k);
+    __shared__ K skey[LP_WAVES][WAVE];
+    __shared__ int32_t stoken[LP_WAVES][WAVE];
+    constexpr int AHEAD = 8; // lists on their way
+    const uint32_t e = top.brings(lane, a.k);
+    for (int b = wave; b < a.splits; b += LP_WAVES * AHEAD) {
+      K key[AHEAD];
+      int32_t token[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int at = b + j * LP_WAVES;
+        const bool in = at < a.splits && e < uint32_t(a.k);
+        key[j] = in ? a.pkey[(row * a.splits + at) * a.k + e] : 0;
+        token[j] = in ? a.ptoken[(row * a.splits + at) * a.k + e] : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (b + j * LP_WAVES < a.splits)
+          top.merge(key[j], token[j], a.k);
+    }
+    if (lane < a.k) {
+      skey[wave][lane] = top.key;
+      stoken[wave][lane] = top.token;
+    }
+    __syncthreads();
+    if (wave != 0)
+      return;
+    for (int w = 1; w < LP_WAVES; ++w) {
+      const bool in = e < uint32_t(a.k);
+      top.merge(in ? skey[w][e] : 0, in ? stoken[w][e] : -1, a.k);
     }
   }
   write_row(a, row, t, r, top);
@@ -765,7 +875,7 @@ template <class T> void run_forward(LpForward<T> a) {
   if (a.splits == 1)
     return;
   if (a.k)
-    launch(logprob_join_kernel<T, true>, WAVE, 1, 1);
+    launch(logprob_join_kernel<T, true>, LP_THREADS, 1, 1);
   else
     launch(logprob_join_kernel<T, false>, WAVE, 1, 1);
 }

@@ -570,6 +570,30 @@ def test_top_alternatives(gpu, dtype, rows, V, top, kind):
     Rows(z, dtype).check(nt.token_logprobs(dev(z), entropy=True, top=top), None, True, top)
 
 
+@pytest.mark.parametrize("kind", ["random", "tied", "rising"])
+@pytest.mark.parametrize("top", [1, 15, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("rows,V", [(1, 131073), (3, 66000), (40, 20000), (1100, 4500)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_top_alternatives_of_split_rows(gpu, dtype, rows, V, top, kind):
+    """Lists joined by waves and by workgroups, in 16 lanes and in 64; equal
+    logits in different parts; parts of a few elements; the largest last."""
+    r = rng(seed_of("split", rows, V, kind))
+    z = r.standard_normal((rows, V)).astype(dtype)
+    if kind == "tied":
+        z = np.round(z)
+    elif kind == "rising":
+        z.sort(1)
+    out = nt.token_logprobs(dev(z), top=top)
+    # the largest first, equal ones by their tokens
+    found = np.argpartition(-z, top - 1, 1)[:, top - 1:top]
+    least = np.take_along_axis(z, found, 1)
+    want = []
+    for row, low in zip(z, least):
+        at = np.flatnonzero(row >= low)
+        want.append(at[np.argsort(-row[at], kind="stable")][:top])
+    assert_bitexact(host(out.top_tokens), np.array(want))
+
+
 LOW = {np.float32: np.finfo(np.float32).min, np.float64: np.finfo(np.float64).min}
 
 
