@@ -76,6 +76,7 @@ class EmbeddingOp(Function):
             raise ValueError(f"padding_idx {padding_idx} is no row of a table of {shape[0]}.")
         self.save_for_backward(tokens)
         self._scale, self._padding, self._shape = float(scale), padding_idx, shape
+        self._dtype = table._storage._dtype
         self._flat = _vector(tokens)
         st = K.embedding(table, self._flat, self._scale, padding_idx)
         return Tensor._unchecked_view(
@@ -93,7 +94,7 @@ class EmbeddingOp(Function):
     def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
         self.saved_tensors  # raises if the tokens were modified in place
         shape = self._shape
-        g = reshape_view(g, (self._flat._shape[0], shape[1]))._to_contiguous()
+        g = reshape_view(g.to(self._dtype), (self._flat._shape[0], shape[1]))._to_contiguous()
         into = target
         if target is not None and shape[1] > 1 and target._strides[1] != 1:
             into = None
@@ -125,6 +126,7 @@ class DropoutOp(Function):
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout() needs 0 <= p <= 1, got {p}.")
         self._args = (float(p), seed, offset)
+        self._dtype = x._storage._dtype
         return Tensor._unchecked_view(
             K.dropout(x, *self._args), x._shape, row_major_strides(x._shape), 0)
 
@@ -138,6 +140,7 @@ class DropoutOp(Function):
         return [self._grad(g, targets[0]) if needs[0] else None]
 
     def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
+        g = g.to(self._dtype)
         st = K.dropout(g, *self._args, target)
         if target is not None:
             return target

@@ -784,6 +784,32 @@ def test_logprob_refusals(gpu):
         lp.sum().backward()
 
 
+@pytest.mark.parametrize("op", ["embedding", "dropout", "logprob"])
+@pytest.mark.parametrize("N", [20, 700])
+def test_gradient_of_another_type(gpu, op, N):
+    """Float32 operators under float64 weights: the gradient that arrives is
+    float64, what they give is float32, new and added.  The weights are small
+    integers, so the cast is exact and the results are those of float32 ones."""
+    r = rng(seed_of("type", op, N))
+    x = r.standard_normal((N, 12)).astype(np.float32)
+    t = r.integers(0, 12, N)
+    shape = (N,) if op == "logprob" else (N, 12)
+    a = r.integers(-4, 5, shape).astype(np.float32)
+    f = {"embedding": lambda X: nt.embedding(X, dev(t)),
+         "dropout": lambda X: nt.dropout(X, 0.5, seed=3),
+         "logprob": lambda X: nt.token_logprobs(X, dev(t)).logprob}[op]
+    grads = []
+    for weights in (a, a.astype(np.float64)):
+        X = dev(x, True)
+        (f(X) * dev(weights)).sum().backward()
+        once = host(X.grad).copy()
+        (f(X) * dev(weights)).sum().backward()
+        grads.append((once, host(X.grad)))
+    for got, want in zip(grads[1], grads[0]):
+        assert got.dtype == np.float32
+        assert_bitexact(got, want)
+
+
 def test_operators_between_elementwise_ops(gpu):
     """Kernels that may overlap (launched without the stream's barrier) and
     those that may not, each reading what the one before has written."""
