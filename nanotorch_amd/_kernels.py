@@ -348,7 +348,7 @@ def matmul_into(x1, x2, target, accumulate: bool) -> None:
 def embedding(table, tokens, scale: float, padding: int) -> Storage:
     """Rows of a [V, D] table for 1-D tokens, times scale."""
     require_device(table, tokens)
-    shape = (tokens._shape[0], table._shape[1])
+    shape = (int(tokens._shape[0]), int(table._shape[1]))
     out = Storage.allocate(shape[0] * shape[1], table._storage._dtype, Device.Cuda)
     _lib.call_packed("nt_embedding", _packed(table), _packed(tokens), scale, padding,
                      _packed_flat(out, shape))
@@ -360,7 +360,7 @@ def embedding_bwd(g, tokens, scale: float, padding: int, shape, target) -> "Stor
     (adjacent elements in each row) when given, else a new storage."""
     require_device(g, tokens)
     if target is None:
-        out = Storage.allocate(shape[0] * shape[1], g._storage._dtype, Device.Cuda)
+        out = Storage.allocate(int(shape[0]) * int(shape[1]), g._storage._dtype, Device.Cuda)
         _lib.call_packed("nt_embedding_bwd", _packed(g), _packed(tokens), scale, padding,
                          _packed_flat(out, shape), 0)
         return out
@@ -391,7 +391,7 @@ def token_logprobs(z, tokens, ignore: int, entropy: bool, top: int, stats: bool)
     three statistics that the backward pass needs (if wanted).  One buffer,
     since each allocation costs the host a microsecond or two."""
     require_device(z) if tokens is None else require_device(z, tokens)
-    rows, dtype = z._shape[0], z._storage._dtype
+    rows, dtype = int(z._shape[0]), z._storage._dtype
     given = tokens is not None
     n = given + entropy
     out = Storage.allocate(rows * (n + top + 3 * stats), dtype, Device.Cuda)
@@ -416,9 +416,9 @@ def token_logprobs_bwd(z, tokens, ignore: int, results: Storage, ga, gb,
     probabilities and gb of the entropies (None: zero); added to `target`
     (adjacent elements in each row) when given, else a new storage.  `results`
     is token_logprobs's buffer, the statistics at its end."""
-    rows = z._shape[0]
+    rows = int(z._shape[0])
     if target is None:
-        out = Storage.allocate(_numel(z._shape), z._storage._dtype, Device.Cuda)
+        out = Storage.allocate(rows * int(z._shape[1]), z._storage._dtype, Device.Cuda)
         v_out = _packed_flat(out, z._shape)
     else:
         out, v_out = None, _packed(target)

@@ -45,7 +45,8 @@ class Storage:
         """Uninitialised (device) or zeroed (host) buffer."""
         if device is not Device.Cuda or type(dtype) is not Dtype:
             return cls(size, dtype, device, _zero=False)
-        # an op's output: __init__ without its conversions and choices
+        # an op's output: __init__ without its choices
+        size = int(size)  # a product of numpy's small integers wraps round
         self = cls.__new__(cls)
         self._dtype, self._device, self._size = dtype, device, size
         self.version = 0

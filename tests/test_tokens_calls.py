@@ -1,0 +1,110 @@
+"""What the token operators hand to the library, recorded in place of it: the
+memory that views cover, and the gradients that reach the backward pass.  No
+device is needed."""
+
+from __future__ import annotations
+
+import collections
+import math
+import struct
+
+import numpy as np
+import pytest
+
+from nanotorch_amd import _kernels as K
+from nanotorch_amd import _lib
+from nanotorch_amd._data_type import Dtype, sizeof
+from nanotorch_amd._storage import Storage
+from nanotorch_amd.core import Tensor
+from nanotorch_amd.cuda import Device
+
+View = collections.namedtuple("View", "ptr offset dtype shape strides")
+
+
+def parse(view: bytes) -> View:
+    f = struct.unpack("=Qqii16q", view)
+    return View(f[0], f[1], Dtype(f[2]), f[4:4 + f[3]], f[12:12 + f[3]])
+
+
+class Recorder:
+    """Stands in for the library: addresses that no memory is behind, calls
+    that do nothing but are kept."""
+
+    def __init__(self) -> None:
+        self.sizes: dict[int, int] = {}  # bytes of each allocation
+        self.freed: list[int] = []
+        self.calls: list[tuple[str, tuple]] = []
+
+    def nt_malloc(self, p, nbytes) -> int:
+        p._obj.value = (1 << 40) * (len(self.sizes) + 1)
+        self.sizes[p._obj.value] = int(nbytes)
+        return 0
+
+    def nt_free(self, ptr) -> int:
+        self.freed.append(ptr)
+        return 0
+
+    def __getattr__(self, name):
+        def call(*args) -> int:
+            self.calls.append((name, args))
+            return 0
+        return call
+
+    __getitem__ = __getattr__
+
+    def args(self, name: str) -> tuple:
+        """Of the last such call, views parsed."""
+        found = [a for n, a in self.calls if n == name][-1]
+        return tuple(parse(a) if isinstance(a, bytes) else a for a in found)
+
+    def within(self, v: View) -> range:
+        """The bytes of a contiguous view, which its allocation has to hold."""
+        item, n = sizeof(v.dtype), math.prod(v.shape)
+        base = v.ptr // (1 << 40) * (1 << 40)
+        beg = v.ptr - base + v.offset * item
+        assert 0 <= beg and beg + n * item <= self.sizes[base], v
+        return range(base + beg, base + beg + n * item)
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    r = Recorder()
+    monkeypatch.setattr(_lib, "_lib", r)
+    monkeypatch.setattr(_lib, "_packed", r)
+    return r
+
+
+def tensor(*shape, dtype=Dtype.Float32, requires_grad=False) -> Tensor:
+    shape = tuple(int(n) for n in shape)
+    t = Tensor._new_contiguous(Storage.allocate(math.prod(shape), dtype, Device.Cuda), shape)
+    t._requires_grad = requires_grad
+    return t
+
+
+@pytest.mark.parametrize("size", [7, np.int64(7), np.uint8(200), np.int32(600_000_000),
+                                  np.int32(1_200_000_000), True])
+def test_an_allocation_holds_its_elements(lib, size):
+    """Sizes of numpy's small integers, whose products with an element's size
+    do not fit them."""
+    st = Storage.allocate(size, Dtype.Float64, Device.Cuda)
+    assert lib.sizes[st.data_ptr()] == int(size) * 8
+    assert type(st.size) is int and st.nbytes == int(size) * 8
+
+
+@pytest.mark.parametrize("rows,V", [(np.uint8(200), 64), (np.int32(3_000_000), 1000)])
+def test_outputs_of_small_integer_shapes(lib, rows, V):
+    """Shapes hold what they were given, numpy's small integers too."""
+    z, w = tensor(rows, V), tensor(50, V)
+    z._shape = (rows, V)  # as reshape keeps it
+    t = tensor(rows, dtype=Dtype.Int64)
+    t._shape = (rows,)
+    lib.calls.clear()
+    K.embedding(w, t, 1.0, -1)
+    lib.within(lib.args("nt_embedding")[4])
+    K.embedding_bwd(z, t, 1.0, -1, (rows, V), None)
+    assert len(lib.within(lib.args("nt_embedding_bwd")[4])) == int(rows) * V * 4
+    out, _ = K.token_logprobs(z, t, -100, True, 2, True)
+    for v in lib.args("nt_token_logprobs")[3:]:
+        lib.within(v)
+    K.token_logprobs_bwd(z, t, -100, out, None, None, None)
+    assert len(lib.within(lib.args("nt_token_logprobs_bwd")[6])) == int(rows) * V * 4
