@@ -166,7 +166,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
     occur; a row of nothing else has logprob -inf, entropy 0 and no gradient.
     Tokens are checked on the device: one outside [0, V) leaves its row out,
     and the next synchronisation (``sync``, ``cpu``) raises IndexError."""
-    shape = logits._shape
+    shape, entropy = logits._shape, bool(entropy)
     if not shape or not is_float(logits._storage._dtype):
         raise ValueError(f"Logits are float with an axis of tokens, got {logits.dtype.name} "
                          f"{shape}.")

@@ -11,6 +11,7 @@ import struct
 import numpy as np
 import pytest
 
+import nanotorch_amd as nt
 from nanotorch_amd import _kernels as K
 from nanotorch_amd import _lib
 from nanotorch_amd._data_type import Dtype, sizeof
@@ -108,3 +109,20 @@ def test_outputs_of_small_integer_shapes(lib, rows, V):
         lib.within(v)
     K.token_logprobs_bwd(z, t, -100, out, None, None, None)
     assert len(lib.within(lib.args("nt_token_logprobs_bwd")[6])) == int(rows) * V * 4
+
+
+@pytest.mark.parametrize("entropy", [np.True_, np.False_, 1, 2, "yes", "", None])
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("grad", [False, True])
+def test_entropy_is_a_truth_value(lib, entropy, top, grad):
+    """The results lie side by side in their allocation, whatever the truth
+    value's type: True + numpy's True is one result, not two."""
+    z, t = tensor(700, 20, requires_grad=grad), tensor(700, dtype=Dtype.Int64)
+    out = nt.token_logprobs(z, t, entropy=entropy, top=top)
+    assert (out.entropy is not None) == bool(entropy)
+    _, _, _, logprob, ent, stats, value, token = lib.args("nt_token_logprobs")
+    assert (ent is None, stats is None, value is None) == (not entropy, not grad, not top)
+    used = [lib.within(v) for v in (logprob, ent, stats, value, token) if v is not None]
+    for i, a in enumerate(used):
+        for b in used[:i]:
+            assert a.stop <= b.start or b.stop <= a.start
