@@ -167,7 +167,7 @@ class TokenLogProbOp(Function):
         lead = logits._shape[:-1]
         z = _as_rows(logits)
         flat = None if tokens is None else _vector(tokens)
-        keep = is_grad_enabled() and logits.requires_grad
+        keep = bool(is_grad_enabled() and logits.requires_grad)
         out, token = K.token_logprobs(z, flat, ignore_index, entropy, top, keep)
         if top:
             n = entropy + (tokens is not None)

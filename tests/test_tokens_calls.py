@@ -126,3 +126,15 @@ def test_entropy_is_a_truth_value(lib, entropy, top, grad):
     for i, a in enumerate(used):
         for b in used[:i]:
             assert a.stop <= b.start or b.stop <= a.start
+
+
+@pytest.mark.parametrize("flag", [True, 1, 2, "yes"])
+@pytest.mark.parametrize("entropy,top", [(False, 0), (True, 2)])
+def test_the_backward_pass_reads_the_statistics_written(lib, flag, entropy, top):
+    """requires_grad is taken by its truth; the constructor keeps what it was
+    given."""
+    z, t = tensor(30, 20, requires_grad=flag), tensor(30, dtype=Dtype.Int64)
+    out = nt.token_logprobs(z, t, entropy=entropy, top=top)
+    written = lib.args("nt_token_logprobs")[5]
+    out.logprob.sum().backward()
+    assert lib.within(lib.args("nt_token_logprobs_bwd")[3]) == lib.within(written)
