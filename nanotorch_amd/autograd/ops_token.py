@@ -12,9 +12,11 @@ import math
 
 from .. import _kernels as K
 from .. import _lib
-from .._data_type import is_float, is_int, sizeof
+from .._data_type import Dtype, is_float, is_int, sizeof
 from .._indexing import row_major_strides
+from .._storage import Storage
 from ..core import Tensor, reshape_view
+from ..cuda import Device
 from .function import Function
 from .grad_mode import is_grad_enabled
 
@@ -196,8 +198,8 @@ class TokenLogProbOp(Function):
         rows = z._shape[0]
         if not self._both:
             ga, gb = (None, g) if flat is None else (g, None)
-        elif hasattr(g, "_parts"):
-            ga, gb = g._parts.get(0), g._parts.get(1)
+        elif isinstance(g, _RowGradients):
+            ga, gb = g.rows.get(0), g.rows.get(1)
         else:
             g = reshape_view(g, (2, rows))._to_contiguous()
             ga, gb = _row_of(g, 0), _row_of(g, 1)
@@ -227,13 +229,29 @@ def top_views(out, offset: int, token, shape) -> tuple[Tensor, Tensor]:
             Tensor._unchecked_view(token, shape, strides, 0))
 
 
-class RowOp(Function):
-    """x[i] of TokenLogProbOp's x [2, ...].
+class _RowGradients(Tensor):
+    """The gradient of TokenLogProbOp's x [2, ...] while the engine carries it:
+    the gradients of its rows as they arrived, not copied into one tensor, as
+    on few rows three launches are most of what the backward pass costs.
 
-    In the engine's pass the rows' gradients reach TokenLogProbOp side by
-    side, in a stand-in for the gradient of x that carries them (``_parts``),
-    without being copied into one tensor: on few rows three launches are most
-    of what the backward pass costs.  ``backward`` returns that tensor."""
+    It has no memory, so nothing but TokenLogProbOp can take it for values; a
+    copy of it, which the engine makes of gradients that may be shared, is the
+    same object."""
+
+    _NONE = Storage(0, Dtype.Float32, Device.Cpu)
+
+    @classmethod
+    def of(cls, x: Tensor) -> "_RowGradients":
+        new = cls._unchecked_view(cls._NONE, x._shape, x._strides, 0)
+        new.rows = {}
+        return new
+
+    def _to_contiguous(self, force: bool = False) -> Tensor:
+        return self
+
+
+class RowOp(Function):
+    """x[i] of TokenLogProbOp's x [2, ...]."""
 
     def forward(self, x: Tensor, i: int) -> Tensor:
         self._i, self._x = i, x
@@ -253,12 +271,11 @@ class RowOp(Function):
             return [None]
         into = targets[0]
         if into is None:
-            into = self._x._alias()
-            into._parts = {}
-        elif not hasattr(into, "_parts"):
+            into = _RowGradients.of(self._x)
+        elif not isinstance(into, _RowGradients):
             K.inplace(_lib.ADD, _row_of(into, self._i), g)
             return [into]
-        into._parts[self._i] = g
+        into.rows[self._i] = g
         return [into]
 
 

@@ -10,12 +10,58 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from helpers import dev, host, rng
-from test_gpu_tokens import Rows, draw_rows
+from helpers import assert_bitexact, dev, host, rng, seed_of
+from test_gpu_tokens import FLOATS, Rows, draw_rows
 
 import nanotorch_amd as nt
+from nanotorch_amd.autograd.function import Function
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------- gradients that share memory
+
+
+class HandsOn(Function):
+    """sum(x * y), whose backward hands its saved tensors on as they are."""
+
+    def forward(self, x, y):
+        self.save_for_backward(x, y)
+        with nt.no_grad():
+            return (x * y).sum()
+
+    def backward(self, grad_out):
+        x, y = self.saved_tensors
+        return y, x
+
+
+@pytest.mark.parametrize("swapped", [False, True])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,V", [(1, 5), (7, 40), (3, 9000)])
+def test_results_as_gradients(gpu, dtype, rows, V, swapped):
+    """The gradient of logprob is the entropy's own tensor and the other way
+    round: sum(logprob * entropy)."""
+    z, t = draw_rows(rng(seed_of("hands", rows, V)), rows, V, dtype)
+    Z = dev(z, True)
+    out = nt.token_logprobs(Z, dev(t), entropy=True)
+    a, b = host(out.entropy), host(out.logprob)
+    pair = (out.entropy, out.logprob) if swapped else (out.logprob, out.entropy)
+    HandsOn.apply(*pair).backward()
+    Rows(z, dtype).check_grad(host(Z.grad), t, a, b)
+    assert_bitexact(host(out.entropy), a)
+    assert_bitexact(host(out.logprob), b)
+
+
+@pytest.mark.parametrize("wanted", ["logprob", "entropy"])
+@pytest.mark.parametrize("rows,V", [(1, 1), (9, 100), (3, 9000)])
+def test_one_result_of_two_in_the_loss(gpu, rows, V, wanted):
+    z, t = draw_rows(rng(seed_of("one", rows, V)), rows, V, np.float32)
+    w = rng(1).standard_normal(rows).astype(np.float32)
+    Z = dev(z, True)
+    for times in (1, 2):  # a new gradient, then added to it
+        (getattr(nt.token_logprobs(Z, dev(t), entropy=True), wanted) * dev(w)).sum().backward()
+        a, b = (times * w, None) if wanted == "logprob" else (None, times * w)
+        Rows(z, np.float32).check_grad(host(Z.grad), t, a, b)
 
 
 # ------------------------------------------------------------------- types

@@ -16,6 +16,7 @@ from nanotorch_amd import _kernels as K
 from nanotorch_amd import _lib
 from nanotorch_amd._data_type import Dtype, sizeof
 from nanotorch_amd._storage import Storage
+from nanotorch_amd.autograd.function import Function
 from nanotorch_amd.core import Tensor
 from nanotorch_amd.cuda import Device
 
@@ -138,3 +139,51 @@ def test_the_backward_pass_reads_the_statistics_written(lib, flag, entropy, top)
     written = lib.args("nt_token_logprobs")[5]
     out.logprob.sum().backward()
     assert lib.within(lib.args("nt_token_logprobs_bwd")[3]) == lib.within(written)
+
+
+class Hands(Function):
+    """Over (logprob, entropy), with the backward pass's results given."""
+
+    def forward(self, x, y, grads):
+        self._grads = grads
+        return tensor()
+
+    def backward(self, grad_out):
+        return self._grads(*self.inputs[:2])
+
+
+@pytest.mark.parametrize("order", [(0, 1), (1, 0)])
+@pytest.mark.parametrize("which", ["itself", "other", "upstream", "new"])
+@pytest.mark.parametrize("rows", [4, 0])
+def test_row_gradients_reach_the_backward_pass(lib, rows, which, order):
+    """Gradients that are the results' own tensors, one tensor for both, or
+    new ones: the backward pass reads each as it is, and nothing else runs."""
+    z, t = tensor(rows, 20, requires_grad=True), tensor(rows, dtype=Dtype.Int64)
+    out = nt.token_logprobs(z, t, entropy=True)
+    one = tensor(rows)
+    grads = {"itself": lambda x, y: (x, y), "other": lambda x, y: (y, x),
+             "upstream": lambda x, y: (one, one),
+             "new": lambda x, y: (tensor(rows), tensor(rows))}[which]
+    given = {}
+
+    def record(x, y):
+        given["all"] = grads(x, y)
+        return given["all"]
+
+    pair = [out.logprob, out.entropy]
+    loss = Hands.apply(pair[order[0]], pair[order[1]], record)
+    lib.calls.clear()
+    loss.backward()
+    assert [n for n, _ in lib.calls if n != "nt_fill"] == ["nt_token_logprobs_bwd"]
+    got = lib.args("nt_token_logprobs_bwd")[4:6]
+    for k, g in zip(order, given["all"]):
+        assert got[k][:4] == (g.storage.data_ptr(), g.strides[1], g.dtype, (rows,))
+
+
+@pytest.mark.parametrize("i", [0, 1])
+def test_one_row_gradient_reaches_the_backward_pass(lib, i):
+    z, t = tensor(4, 20, requires_grad=True), tensor(4, dtype=Dtype.Int64)
+    out = nt.token_logprobs(z, t, entropy=True)
+    out[i].sum().backward()
+    got = lib.args("nt_token_logprobs_bwd")[4:6]
+    assert got[i] is not None and got[1 - i] is None
