@@ -10,7 +10,10 @@
 //   s' = exp(d) s,   u' = exp(d) (u + d s).
 // The gradient for upstream a (of log p_t) and b (of H) is
 //   dz_j = a [j = t] - p_j (a + b (log p_j + H)),   p_j = exp(z_j - m) / s,
-// one pass that reads z and writes dz.
+// one pass that reads z and writes dz.  There log p_j + H = (z_j - m) - u / s:
+// log s drops out, whose rounding would be all of that difference where a row
+// is nearly uniform, as a model's are at its start (64 x 32000 float32 of
+// deviation 2^-13: off by 3.0e-7 of its norm, by way of H by 2.5e-3).
 //
 // Bound by memory where rows are many: 8192 x 32000 float32 (a tenth of the
 // rows left out) reads 0.94 GB in 156 us (6.0 TB/s), and its gradient moves
@@ -751,10 +754,10 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_bwd_kernel(LpBackward<T> a
     }
     return;
   }
-  const T log_s = log(s), H = log_s - u / s, inv = T(1) / s;
+  const T inv = T(1) / s;
   const T ga = a.ga ? a.ga[row * a.sa] : T(0), gb = a.gb ? a.gb[row * a.sb] : T(0);
   // dz = p (c0 + c1 d), d = z - m, + ga at the token
-  const T c0 = -ga - gb * (H - log_s), c1 = -gb;
+  const T c0 = __builtin_elementwise_fma(gb, u / s, -ga), c1 = -gb;
   const T *z = a.z + row * a.row_stride;
 #pragma unroll
   for (int c = 0; c < UNROLL; ++c) {

@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 from helpers import assert_bitexact, dev, host, rng, seed_of
-from test_gpu_tokens import FLOATS, Rows, draw_rows
+from test_gpu_tokens import FLOATS, U, Rows, draw_rows, within
 
 import nanotorch_amd as nt
 from nanotorch_amd.autograd.function import Function
@@ -62,6 +62,37 @@ def test_one_result_of_two_in_the_loss(gpu, rows, V, wanted):
         (getattr(nt.token_logprobs(Z, dev(t), entropy=True), wanted) * dev(w)).sum().backward()
         a, b = (times * w, None) if wanted == "logprob" else (None, times * w)
         Rows(z, np.float32).check_grad(host(Z.grad), t, a, b)
+
+
+# ------------------------------------------------------ nearly uniform rows
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("base", [0.0, 1.0])
+@pytest.mark.parametrize("rows,V", [(5, 10), (4, 200), (6, 1000), (4, 3001), (2, 32000)])
+def test_entropy_gradient_of_nearly_uniform_rows(gpu, dtype, rows, V, base):
+    """-p_j (log p_j + H) = p_j (E d - d_j), d = z - max z: it vanishes with
+    the logits' spread, and so does its bound, which holds no log s (u the unit
+    roundoff, r a sum's relative error as in test_gpu_tokens): p_j is off by
+    r + u (8 + |d_j|) of itself, E d = u / s by 2 r + 2u, d_j by u."""
+    u = U[dtype]
+    r = rng(seed_of("uniform", rows, V))
+    z = (base + r.standard_normal((rows, V)) * 2.0 ** -13).astype(dtype)
+    b = r.standard_normal(rows).astype(dtype)
+    Z = dev(z, True)
+    (nt.token_logprobs(Z, entropy=True).entropy * dev(b)).sum().backward()
+    z = z.astype(np.longdouble)
+    d = z - z.max(1, keepdims=True)
+    e = np.exp(d)
+    p = e / e.sum(1, keepdims=True)
+    ed = (p * d).sum(1, keepdims=True)
+    b = b[:, None].astype(np.longdouble)
+    want = b * p * (ed - d)
+    rel = u * (8 + np.abs(ed) + V / 64 + 32)
+    size = np.abs(b) * p
+    tol = (size * (np.abs(ed) + np.abs(d)) * (rel + u * (16 + np.abs(d)))
+           + size * ((2 * rel + 2 * u) * np.abs(ed) + u * np.abs(d)) + 2 * u * np.abs(want))
+    within(host(Z.grad), want, tol, "dz")
 
 
 # ------------------------------------------------------------------- types
