@@ -147,11 +147,27 @@ class Storage:
                 ctypes.memmove(out._host, self._host, self.nbytes)
         return out
 
+    def part(self, offset: int, size: int) -> "Storage":
+        """Some of a device buffer's elements as a storage of their own: the
+        same memory, which stays until both are gone, another version."""
+        new = _Part.__new__(_Part)
+        new._whole, new._dtype, new._device = self, self._dtype, self._device
+        new._size, new.version, new._host = int(size), 0, None
+        new._ptr = self._ptr + int(offset) * _SIZES[self._dtype]
+        return new
+
     def __del__(self) -> None:
         ptr = getattr(self, "_ptr", None)
         if ptr is not None and _lib._lib is not None:
             _lib._lib.nt_free(ptr)
             self._ptr = None
+
+
+class _Part(Storage):
+    __slots__ = ("_whole",)
+
+    def __del__(self) -> None:  # the memory is the whole's
+        pass
 
 
 def _convert(v, dtype: Dtype):

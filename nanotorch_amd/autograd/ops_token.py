@@ -222,10 +222,12 @@ class TokenLogProbOp(Function):
 
 
 def top_views(out, offset: int, token, shape) -> tuple[Tensor, Tensor]:
-    """The alternatives' log probabilities, in `out` from `offset` on, and
-    their tokens."""
+    """The alternatives' log probabilities, in `out` from `offset` on with a
+    version of their own, and their tokens."""
     strides = row_major_strides(shape)
-    return (Tensor._unchecked_view(out, shape, strides, offset),
+    if offset:
+        out = out.part(offset, token._size)
+    return (Tensor._unchecked_view(out, shape, strides, 0),
             Tensor._unchecked_view(token, shape, strides, 0))
 
 
@@ -250,12 +252,22 @@ class _RowGradients(Tensor):
         return self
 
 
+def result_row(x: Tensor, i: int) -> Tensor:
+    """x[i] of TokenLogProbOp's x [2, ...], with a version of its own: a change
+    of one row in place leaves a graph that needs the other."""
+    shape = x._shape[1:]
+    if i == 0:  # x itself is no one's result
+        return Tensor._unchecked_view(x._storage, shape, x._strides[1:], 0)
+    n = math.prod(shape)
+    return Tensor._unchecked_view(x._storage.part(n, n), shape, x._strides[1:], 0)
+
+
 class RowOp(Function):
-    """x[i] of TokenLogProbOp's x [2, ...]."""
+    """result_row, differentiable."""
 
     def forward(self, x: Tensor, i: int) -> Tensor:
         self._i, self._x = i, x
-        return _row_of(x, i)
+        return result_row(x, i)
 
     def backward(self, grad_out: Tensor) -> tuple:
         full = Tensor._new_contiguous(

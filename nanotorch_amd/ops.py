@@ -10,7 +10,7 @@ from . import _lib
 from . import autograd
 from ._data_type import Dtype, is_float, promote_dtypes
 from ._indexing import broadcast_shapes
-from .autograd.ops_token import RowOp, _as_rows, _check_tokens, top_views
+from .autograd.ops_token import RowOp, _as_rows, _check_tokens, result_row, top_views
 from .core import Tensor
 from .factories import next_dropout_counter
 
@@ -185,13 +185,16 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
         out, token = K.token_logprobs(_as_rows(logits), None, ignore_index, False, top, False)
         extras = top_views(out, 0, token, shape[:-1] + (top,))
     else:
-        out = autograd.TokenLogProbOp.apply(logits, tokens, ignore_index, entropy, top, extras)
+        op, tracked = autograd.TokenLogProbOp, logits.requires_grad and autograd.is_grad_enabled()
+        call = op.apply if tracked else op().forward  # a serving call has no node to attach
+        out = call(logits, tokens, ignore_index, entropy, top, extras)
         if tokens is None:
             ent = out
         elif not entropy:
             logprob = out
         else:
-            logprob, ent = RowOp.apply(out, 0), RowOp.apply(out, 1)
+            row = RowOp.apply if tracked else result_row
+            logprob, ent = row(out, 0), row(out, 1)
     return TokenLogProbs(logprob, ent, *extras)
 
 

@@ -95,6 +95,56 @@ def test_entropy_gradient_of_nearly_uniform_rows(gpu, dtype, rows, V, base):
     within(host(Z.grad), want, tol, "dz")
 
 
+# ------------------------------------------------- results changed in place
+
+
+@pytest.mark.parametrize("saved,changed", [
+    ("entropy", "logprob"), ("logprob", "entropy"), ("logprob", "top_logprobs"),
+    ("entropy", "top_logprobs"), ("logprob", "top_tokens")])
+def test_a_result_changed_in_place_leaves_the_others(gpu, saved, changed):
+    z, t = draw_rows(rng(3), 6, 30, np.float32)
+    w = dev(rng(4).standard_normal(6).astype(np.float32), True)
+    Z = dev(z, True)
+    out = nt.token_logprobs(Z, dev(t), entropy=True, top=4)
+    before = host(getattr(out, saved))
+    loss = (getattr(out, saved) * w).sum()  # keeps the result for w's gradient
+    with nt.no_grad():
+        other = getattr(out, changed)
+        other += 1
+    loss.backward()
+    assert_bitexact(host(w.grad), before)
+    a, b = (host(w), None) if saved == "logprob" else (None, host(w))
+    Rows(z, np.float32).check_grad(host(Z.grad), t, a, b)
+
+
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("name", ["logprob", "entropy"])
+def test_a_saved_result_changed_in_place_is_refused(gpu, name, top):
+    z, t = draw_rows(rng(5), 6, 30, np.float32)
+    w = dev(np.ones(6, np.float32), True)
+    out = nt.token_logprobs(dev(z, True), dev(t), entropy=True, top=top)
+    loss = (getattr(out, name) * w).sum()
+    with nt.no_grad():
+        x = getattr(out, name)
+        x += 1
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_results_outlive_each_other(gpu):
+    """The results share one allocation: it stays while any of them is used."""
+    z, t = draw_rows(rng(6), 300, 40, np.float32)
+    ref = Rows(z, np.float32)
+    out = nt.token_logprobs(dev(z, True), dev(t), entropy=True, top=4)
+    top = out.top_logprobs
+    del out
+    others = [nt.full(2700, value=7.0, device="cuda") for _ in range(8)]
+    order = np.argsort(-z, 1, kind="stable")[:, :4]
+    within(host(top), np.take_along_axis(ref.logp, order, 1),
+           np.take_along_axis(ref.tol_lp, order, 1))
+    assert all((host(x) == 7).all() for x in others)
+
+
 # ------------------------------------------------------------------- types
 
 

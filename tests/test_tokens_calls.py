@@ -187,3 +187,39 @@ def test_one_row_gradient_reaches_the_backward_pass(lib, i):
     out[i].sum().backward()
     got = lib.args("nt_token_logprobs_bwd")[4:6]
     assert got[i] is not None and got[1 - i] is None
+
+
+NAMES = ["logprob", "entropy", "top_logprobs", "top_tokens"]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("wanted", [NAMES, ["logprob", "top_logprobs", "top_tokens"],
+                                    ["entropy", "top_logprobs"], ["logprob", "entropy"]])
+def test_each_result_has_a_version_of_its_own(lib, wanted, grad):
+    z, t = tensor(40, 20, requires_grad=grad), tensor(40, dtype=Dtype.Int64)
+    out = nt.token_logprobs(z, t if "logprob" in wanted else None, entropy="entropy" in wanted,
+                            top=3 * ("top_logprobs" in wanted))
+    for name in wanted:
+        before = {n: getattr(out, n).version for n in wanted}
+        x = getattr(out, name)
+        with nt.no_grad():
+            x += x
+        after = {n: getattr(out, n).version for n in wanted}
+        assert [n for n in wanted if after[n] != before[n]] == [name]
+
+
+@pytest.mark.parametrize("last", NAMES)
+def test_results_keep_their_memory(lib, last):
+    """The results' allocation goes back with the last of them."""
+    z, t = tensor(40, 20), tensor(40, dtype=Dtype.Int64)
+    with nt.no_grad():
+        out = nt.token_logprobs(z, t, entropy=True, top=3)
+    x = getattr(out, last)
+    used = lib.within(View(x.storage.data_ptr(), x.strides[1], x.dtype, x.shape, None))
+    assert len(used) == x.numel * sizeof(x.dtype)
+    base = used.start // (1 << 40) * (1 << 40)
+    del out
+    assert base not in lib.freed
+    del x
+    assert lib.freed.count(base) == 1
+    assert len(lib.freed) == 2  # the results and the alternatives' tokens
