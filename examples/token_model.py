@@ -48,10 +48,6 @@ class TokenModel(nn.Module):
     def parameters(self):
         return [*self.tokens.parameters(), *self.head.parameters()]
 
-    def train(self, mode: bool = True) -> "TokenModel":
-        self.head.train(mode)
-        return self
-
     def forward(self, context: nt.Tensor) -> nt.Tensor:
         x = self.tokens(context)  # [batch, 2, dim]
         return self.head(x.reshape(x.shape[0], x.shape[1] * x.shape[2]))

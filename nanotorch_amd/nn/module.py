@@ -14,7 +14,7 @@ modules' ``train`` / ``eval`` switch.
 from __future__ import annotations
 
 import math
-from typing import Any, Sequence
+from typing import Any, Iterable, Iterator, Sequence
 
 from ..autograd import EmbeddingOp, ReluOp, SigmoidOp, TanhOp
 from ..autograd.ops_binary import LinearOp
@@ -35,7 +35,18 @@ class Module:
         return self
 
     def train(self, mode: bool = True) -> "Module":
-        """Training (True) or answering (False): only Dropout differs."""
+        """Training (True) or answering (False), for this module and those
+        among its attributes, in lists, tuples and dicts too: only Dropout
+        differs."""
+        own = vars(self)
+        if "_switching" not in own:  # once, where modules refer to each other
+            modules = list(_modules_in(own.values()))
+            own["_switching"] = True
+            try:
+                for m in modules:
+                    m.train(mode)
+            finally:
+                del own["_switching"]
         return self
 
     def eval(self) -> "Module":
@@ -43,6 +54,16 @@ class Module:
 
     def forward(self, *args: Any, **kwargs: Any) -> Any:
         raise NotImplementedError
+
+
+def _modules_in(values: Iterable[Any]) -> Iterator[Module]:
+    for v in values:
+        if isinstance(v, Module):
+            yield v
+        elif isinstance(v, dict):
+            yield from _modules_in(v.values())
+        elif isinstance(v, (list, tuple)):
+            yield from _modules_in(v)
 
 
 class Linear(Module):
@@ -151,12 +172,6 @@ class Sequential(Module):
 
     def to(self, device: Device | str) -> "Sequential":
         self._modules = [m.to(device) for m in self._modules]
-        return self
-
-    def train(self, mode: bool = True) -> "Sequential":
-        for m in self._modules:
-            if isinstance(m, Module):  # a plain function has no mode
-                m.train(mode)
         return self
 
     def forward(self, *args: Any, **kwargs: Any) -> Any:

@@ -61,3 +61,62 @@ def test_rows_in_place(make, in_place):
     assert (rows.storage is x.storage) == in_place
     want = x.numpy().reshape(-1, x.shape[-1])
     assert rows.shape == want.shape and (rows.numpy() == want).all()
+
+
+class Composed(nn.Module):
+    """Holds its modules in every way that an attribute can."""
+
+    def __init__(self):
+        self.drop = nn.Dropout(0.5)
+        self.layers = [nn.Tanh(), (nn.Dropout(0.5), [nn.Dropout(0.5)])]
+        self.heads = {"a": nn.Dropout(0.5), "b": {"c": nn.Sequential(nn.Dropout(0.5))}}
+        self.other = ("a text", 3, None, {"x": 1.0}, nt.ones(2), lambda x: x)
+
+    def dropouts(self):
+        return [self.drop, self.layers[1][0], self.layers[1][1][0], self.heads["a"],
+                self.heads["b"]["c"]._modules[0]]
+
+
+def dropping(m):
+    """Whether a Dropout drops: then it needs the device."""
+    x = nt.ones(3)
+    try:
+        return m(x) is not x
+    except RuntimeError:
+        return True
+
+
+@pytest.mark.parametrize("wrap", [lambda m: m, lambda m: nn.Sequential(nn.Tanh(), m)])
+def test_train_and_eval_reach_the_modules_of_a_composed_one(wrap):
+    inner = Composed()
+    net = wrap(inner)
+    before = dict(vars(inner))
+    assert net.eval() is net
+    assert not any(map(dropping, inner.dropouts()))
+    assert net.train() is net
+    assert all(map(dropping, inner.dropouts()))
+    assert net.train(False) is net
+    assert not any(map(dropping, inner.dropouts()))
+    assert vars(inner) == before
+
+
+def test_train_reaches_modules_that_refer_to_each_other():
+    a, b = Composed(), Composed()
+    a.child, b.parent = b, a
+    b.eval()
+    assert not any(map(dropping, a.dropouts() + b.dropouts()))
+    a.train()
+    assert all(map(dropping, a.dropouts() + b.dropouts()))
+
+
+def test_a_train_of_ones_own_is_called():
+    class Own(nn.Module):
+        def train(self, mode=True):
+            self.modes = getattr(self, "modes", []) + [mode]
+            return self
+
+    own = Own()
+    net = nn.Sequential(own)
+    net.train()
+    net.eval()
+    assert own.modes == [True, False]
