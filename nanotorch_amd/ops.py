@@ -128,17 +128,22 @@ def embedding(table: Tensor, tokens: Tensor, scale: float = 1.0, *,
     return autograd.EmbeddingOp.apply(table, tokens, scale, padding_idx)
 
 
-def dropout(x: Tensor, p: float = 0.5, *, seed: int | None = None, offset: int = 0) -> Tensor:
+def dropout(x: Tensor, p: float = 0.5, *, seed: int | None = None,
+            offset: int | None = None) -> Tensor:
     """x / (1 - p) with each element kept with probability 1 - p, else 0.
 
     Element i (row-major) is kept where word i mod 4 of Philox4x32-10 under the
     64-bit key ``seed`` at the counter (i div 4, ``offset``) is at least
     round(p * 2^32): one seed and offset give one mask, whatever x's strides,
     and the backward pass draws it again.  Without a seed every call takes the
-    next offset of the generator that ``manual_seed`` sets."""
+    next offset of the generator that ``manual_seed`` sets, and none can be
+    given; with one the offset is 0 unless given."""
     if seed is None:
+        if offset is not None:
+            raise ValueError("dropout() takes an offset only with a seed.")
         seed, offset = next_dropout_counter()
-    return autograd.DropoutOp.apply(x, p, int(seed) & (2**64 - 1), int(offset) & (2**64 - 1))
+    return autograd.DropoutOp.apply(x, p, int(seed) & (2**64 - 1),
+                                    int(offset or 0) & (2**64 - 1))
 
 
 class TokenLogProbs(NamedTuple):

@@ -223,3 +223,13 @@ def test_results_keep_their_memory(lib, last):
     del x
     assert lib.freed.count(base) == 1
     assert len(lib.freed) == 2  # the results and the alternatives' tokens
+
+
+def test_dropout_seeds_and_offsets(lib):
+    x = tensor(5)
+    nt.manual_seed(9)
+    for given, want in (({}, (9, 0)), ({"seed": 3}, (3, 0)), ({"seed": 3, "offset": 7}, (3, 7)),
+                        ({"seed": 0, "offset": 0}, (0, 0)), ({}, (9, 1)),
+                        ({"seed": -1, "offset": -1}, (2 ** 64 - 1, 2 ** 64 - 1))):
+        nt.dropout(x, 0.5, **given)
+        assert lib.args("nt_dropout")[2:4] == want

@@ -63,6 +63,14 @@ def test_rows_in_place(make, in_place):
     assert rows.shape == want.shape and (rows.numpy() == want).all()
 
 
+def test_dropout_offset_without_a_seed_is_refused():
+    nt.manual_seed(5)
+    for offset in (0, 7):
+        with pytest.raises(ValueError):
+            nt.dropout(nt.ones(3), 0.5, offset=offset)
+    assert next_dropout_counter() == (5, 0)  # a refused call draws nothing
+
+
 class Composed(nn.Module):
     """Holds its modules in every way that an attribute can."""
 
