@@ -3,7 +3,9 @@ dropout, and the log probabilities of given tokens with the rows' entropies.
 The reference has none of them.
 
 Each backward is one fused pass that writes a new gradient or adds into an
-existing one (``_backward_into``); token numbers have no gradient.
+existing one (``_backward_into``), by way of a new one where that is of
+another float type or its rows cannot be walked; token numbers have no
+gradient.
 """
 
 from __future__ import annotations
@@ -57,8 +59,10 @@ def _as_rows(x: Tensor) -> Tensor:
 
 
 def _added(target: Tensor, storage, shape) -> Tensor:
-    """Adds a new gradient's storage into `target` of any strides."""
-    K.inplace(_lib.ADD, target, Tensor._new_contiguous(storage, shape))
+    """Adds a new gradient's storage into `target` of any strides and float
+    type."""
+    new = Tensor._new_contiguous(storage, shape)
+    K.inplace(_lib.ADD, target, new.to(target._storage._dtype))
     return target
 
 
@@ -98,7 +102,8 @@ class EmbeddingOp(Function):
         shape = self._shape
         g = reshape_view(g.to(self._dtype), (self._flat._shape[0], shape[1]))._to_contiguous()
         into = target
-        if target is not None and shape[1] > 1 and target._strides[1] != 1:
+        if target is not None and ((shape[1] > 1 and target._strides[1] != 1)
+                                   or target._storage._dtype != self._dtype):
             into = None
         st = K.embedding_bwd(g, self._flat, self._scale, self._padding, shape, into)
         if into is not None:
@@ -143,9 +148,14 @@ class DropoutOp(Function):
 
     def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
         g = g.to(self._dtype)
-        st = K.dropout(g, *self._args, target)
-        if target is not None:
+        into = target
+        if target is not None and target._storage._dtype != self._dtype:
+            into = None
+        st = K.dropout(g, *self._args, into)
+        if into is not None:
             return target
+        if target is not None:
+            return _added(target, st, g._shape)
         return Tensor._unchecked_view(st, g._shape, row_major_strides(g._shape), 0)
 
     @classmethod
@@ -204,7 +214,9 @@ class TokenLogProbOp(Function):
             g = reshape_view(g, (2, rows))._to_contiguous()
             ga, gb = _row_of(g, 0), _row_of(g, 1)
         ga, gb = (None if x is None else _vector(x.to(z.dtype)) for x in (ga, gb))
-        into = None if target is None else _rows_in_place(target)
+        into = None
+        if target is not None and target._storage._dtype == z._storage._dtype:
+            into = _rows_in_place(target)
         st = K.token_logprobs_bwd(z, flat, ignore, results, ga, gb, into)
         if into is not None:
             return target

@@ -168,3 +168,25 @@ def test_entropy_is_asked_for_by_its_truth(gpu, flag):
         Rows(z, np.float32).check(out, t, True, 3)
     (out.logprob * dev(a) + out.entropy * dev(b)).sum().backward()
     Rows(z, np.float32).check_grad(host(Z.grad), t, a, b)
+
+
+@pytest.mark.parametrize("op", ["embedding", "dropout", "logprob"])
+@pytest.mark.parametrize("strided", [False, True])
+def test_added_to_a_gradient_of_another_type(gpu, op, strided):
+    """Float32 operators whose input already has a float64 gradient, as one
+    that is also multiplied by float64 weights gets: added to it as they are.
+    The start is a quarter of small integers, the sums exact."""
+    r = rng(seed_of("into", op))
+    x = r.standard_normal((20, 12)).astype(np.float32)
+    t = r.integers(0, 12, 20)
+    start = r.integers(-40, 40, (12, 20) if strided else (20, 12)) / 4.0
+    g = r.integers(-4, 5, (20,) if op == "logprob" else (20, 12)).astype(np.float32)
+    X = dev(x, True)
+    y = {"embedding": lambda: nt.embedding(X, dev(t)),
+         "dropout": lambda: nt.dropout(X, 0.5, seed=3),
+         "logprob": lambda: nt.token_logprobs(X, dev(t)).logprob}[op]()
+    alone = host(y.grad_fn.backward(dev(g))[0])
+    assert alone.dtype == np.float32
+    target = dev(start).T if strided else dev(start)
+    y.grad_fn._backward_into(dev(g), [True, False], [target, None])
+    assert_bitexact(host(target), alone + (start.T if strided else start))
