@@ -364,6 +364,7 @@ def embedding_bwd(g, tokens, scale: float, padding: int, shape, target) -> "Stor
         _lib.call_packed("nt_embedding_bwd", _packed(g), _packed(tokens), scale, padding,
                          _packed_flat(out, shape), 0)
         return out
+    require_device(target)
     _lib.call_packed("nt_embedding_bwd", _packed(g), _packed(tokens), scale, padding,
                      _packed(target), 1)
     target._storage.bump_version()
@@ -379,6 +380,7 @@ def dropout(x, p: float, seed: int, offset: int, target=None) -> "Storage | None
         _lib.call_packed("nt_dropout", _packed(x), p, seed, offset,
                          _packed_flat(out, x._shape), 0)
         return out
+    require_device(target)
     _lib.call_packed("nt_dropout", _packed(x), p, seed, offset, _packed(target), 1)
     target._storage.bump_version()
     return None
@@ -416,6 +418,7 @@ def token_logprobs_bwd(z, tokens, ignore: int, results: Storage, ga, gb,
     probabilities and gb of the entropies (None: zero); added to `target`
     (adjacent elements in each row) when given, else a new storage.  `results`
     is token_logprobs's buffer, the statistics at its end."""
+    require_device(*[x for x in (ga, gb, target) if x is not None])
     rows = int(z._shape[0])
     if target is None:
         out = Storage.allocate(rows * int(z._shape[1]), z._storage._dtype, Device.Cuda)

@@ -233,3 +233,19 @@ def test_dropout_seeds_and_offsets(lib):
                         ({"seed": -1, "offset": -1}, (2 ** 64 - 1, 2 ** 64 - 1))):
         nt.dropout(x, 0.5, **given)
         assert lib.args("nt_dropout")[2:4] == want
+
+
+@pytest.mark.parametrize("op", ["embedding", "dropout", "logprob", "entropy"])
+def test_gradients_on_the_host_are_refused(lib, op):
+    x, t = tensor(6, 5, requires_grad=True), tensor(6, dtype=Dtype.Int64)
+    y = {"embedding": lambda: nt.embedding(x, t), "dropout": lambda: nt.dropout(x, 0.5),
+         "logprob": lambda: nt.token_logprobs(x, t).logprob,
+         "entropy": lambda: nt.token_logprobs(x, entropy=True).entropy}[op]()
+    lib.calls.clear()
+    with pytest.raises(RuntimeError):
+        y.grad_fn.backward(nt.ones(*y.shape))
+    needs = [True] * sum(isinstance(a, Tensor) for a in y.grad_fn.inputs)
+    targets = [nt.ones(6, 5)] + [None] * (len(needs) - 1)
+    with pytest.raises(RuntimeError):
+        y.grad_fn._backward_into(tensor(*y.shape), needs, targets)
+    assert not lib.calls
