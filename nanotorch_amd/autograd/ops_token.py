@@ -133,7 +133,7 @@ class DropoutOp(Function):
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout() needs 0 <= p <= 1, got {p}.")
         self._args = (float(p), seed, offset)
-        self._dtype = x._storage._dtype
+        self._dtype, self._shape = x._storage._dtype, x._shape
         return Tensor._unchecked_view(
             K.dropout(x, *self._args), x._shape, row_major_strides(x._shape), 0)
 
@@ -147,7 +147,7 @@ class DropoutOp(Function):
         return [self._grad(g, targets[0]) if needs[0] else None]
 
     def _grad(self, g: Tensor, target: Tensor | None) -> Tensor:
-        g = g.to(self._dtype)
+        g = reshape_view(g.to(self._dtype), self._shape)
         into = target
         if target is not None and target._storage._dtype != self._dtype:
             into = None

@@ -249,3 +249,18 @@ def test_gradients_on_the_host_are_refused(lib, op):
     with pytest.raises(RuntimeError):
         y.grad_fn._backward_into(tensor(*y.shape), needs, targets)
     assert not lib.calls
+
+
+@pytest.mark.parametrize("op", ["embedding", "dropout", "logprob"])
+def test_gradients_of_another_size_are_refused(lib, op):
+    """Of another shape they are taken in row-major order, as by the other
+    operators."""
+    x, t = tensor(6, 5, requires_grad=True), tensor(6, dtype=Dtype.Int64)
+    y = {"embedding": lambda: nt.embedding(x, t), "dropout": lambda: nt.dropout(x, 0.5),
+         "logprob": lambda: nt.token_logprobs(x, t).logprob}[op]()
+    if op != "logprob":  # its library call checks one gradient per row
+        for shape in ((5, 5), (30, 2), (1,), ()):
+            with pytest.raises((RuntimeError, ValueError)):
+                y.grad_fn.backward(tensor(*shape))
+    (dx, *_) = y.grad_fn.backward(tensor(*y.shape[::-1]))
+    assert dx.shape == (6, 5)
