@@ -190,3 +190,94 @@ def test_added_to_a_gradient_of_another_type(gpu, op, strided):
     target = dev(start).T if strided else dev(start)
     y.grad_fn._backward_into(dev(g), [True, False], [target, None])
     assert_bitexact(host(target), alone + (start.T if strided else start))
+
+
+# ---------------------------------------------------- radix-sorted gradient
+
+
+@pytest.mark.parametrize("left_out", ["some", "most", "all"])
+@pytest.mark.parametrize("N", [17001, 70001, (1 << 21) + 5001])
+@pytest.mark.parametrize("V", [700, 511, 512, 1 << 18])
+def test_radix_sorted_gradient_of_left_out_tokens(gpu, V, N, left_out):
+    """Many tokens, of which some, most or all are padding or lie outside the
+    table; V + 1 sort keys in one, two and three digits, some with a digit bit
+    only for the left-out key; new gradients and added ones, contiguous and
+    with longer rows."""
+    D = 5
+    r = rng(seed_of("radix", V, N, left_out))
+    t = r.integers(0, V, N)
+    hit = r.random(N) < {"some": 0.2, "most": 0.98, "all": 2.0}[left_out]
+    padding = V // 3
+    t[hit] = padding
+    g = r.integers(-8, 9, (N, D)).astype(np.float32)
+    G = dev(g)
+    kept = t != padding
+    want = np.stack([np.bincount(t[kept], g[kept, c], V) for c in range(D)], 1)
+    want = want.astype(np.float32)
+    w = dev(np.zeros((V, D), np.float32), True)
+    y = nt.embedding(w, dev(t), padding_idx=padding)
+    assert_bitexact(host(y.grad_fn.backward(G)[0]), want, "padding")
+    start = r.integers(-8, 9, (V, D + 3)).astype(np.float32)
+    for wide in (False, True):
+        S = dev(start if wide else start[:, :D])
+        into = S[:, 2:D + 2] if wide else S
+        y.grad_fn._backward_into(G, [True, False], [into, None])
+        expect = start.copy() if wide else start[:, :D].copy()
+        (expect[:, 2:D + 2] if wide else expect)[...] += want
+        assert_bitexact(host(S), expect, "added")
+    bad = t.copy()
+    bad[hit] = np.where(np.arange(hit.sum()) % 2, -1, V)
+    kept = (bad >= 0) & (bad < V)
+    want = np.stack([np.bincount(t[kept], g[kept, c], V) for c in range(D)], 1)
+    want = want.astype(np.float32)
+    y = nt.embedding(w, dev(bad))
+    with pytest.raises(IndexError):
+        nt.sync()
+    dw = y.grad_fn.backward(G)[0]
+    with pytest.raises(IndexError):
+        nt.sync()
+    assert_bitexact(host(dw), want, "outside")
+    S = dev(start[:, :D])
+    y.grad_fn._backward_into(G, [True, False], [S, None])
+    with pytest.raises(IndexError):
+        nt.sync()
+    assert_bitexact(host(S), start[:, :D] + want, "outside, added")
+
+
+# --------------------------------------- logits that outgrow the Infinity Cache
+
+
+@pytest.mark.parametrize("dtype,rows,V,top", [
+    (np.float32, 2100000, 33, 0), (np.float32, 700000, 100, 2), (np.float32, 270000, 260, 0),
+    (np.float32, 20000, 4001, 3), (np.float32, 16500, 4101, 0), (np.float32, 16500, 4101, 5),
+    (np.float64, 8300, 4101, 2), (np.float64, 1100000, 31, 0), (np.float64, 270000, 127, 0)])
+def test_logits_larger_than_the_cache(gpu, dtype, rows, V, top):
+    """More than 256 MB: read past the cache, the gradient's last rows first.
+    Rows that differ in logits, tokens and upstream weights, some left out;
+    blocks of rows from the first to the last, new gradients and added ones."""
+    assert rows * V * np.dtype(dtype).itemsize > 256 << 20
+    r = rng(seed_of("cache", rows, V))
+    z = r.standard_normal((rows, V), dtype=dtype)
+    t = r.integers(0, V, rows)
+    t[r.random(rows) < 0.2] = -100
+    a, b = r.standard_normal((2, rows)).astype(dtype)
+    Z = dev(z, True)
+    out = nt.token_logprobs(Z, dev(t), entropy=True, top=top)
+    start = r.standard_normal((16, V)).astype(dtype)
+    added = dev(np.resize(start, (rows, V)))  # row i: start[i % 16]
+    A, B = dev(a), dev(b)
+    (out.logprob * A + out.entropy * B).sum().backward()
+    only = nt.token_logprobs(Z, dev(t)).logprob
+    only.grad_fn._backward_into(A, [True, False], [added, None])
+    blocks = {0, 1, rows // 3, rows // 2, rows - 41, rows - 20} | {
+        int(k) for k in r.integers(0, rows - 20, 6)}
+    for k in sorted(blocks):
+        part = slice(k, k + 20)
+        live = t[part] != -100
+        ref = Rows(z[part], dtype, live)
+        cut = nt.TokenLogProbs(*(None if x is None else x[part] for x in out))
+        ref.check(cut, np.where(live, t[part], 0), True, top)
+        tokens = np.where(live, t[part], 0)
+        ref.check_grad(host(Z.grad[part]), tokens, a[part], b[part])
+        ref.check_grad(host(added[part]), tokens, a[part], None,
+                       extra=start[np.arange(k, min(k + 20, rows)) % 16])

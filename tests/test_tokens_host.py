@@ -128,3 +128,18 @@ def test_a_train_of_ones_own_is_called():
     net.train()
     net.eval()
     assert own.modes == [True, False]
+
+
+@pytest.mark.parametrize("counter,key,want", [
+    ((0, 0, 0, 0), (0, 0), "6627e8d5 e169c58d bc57ac4c 9b00dbd8"),
+    ((2 ** 32 - 1,) * 4, (2 ** 32 - 1,) * 2, "408f276d 41c83b0e a20bc7c6 6d5451fd"),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     "d16cfe09 94fdcceb 5001e420 24126ea1")])
+def test_philox_published_answers(counter, key, want):
+    """What dropout's device results are compared with, against the known
+    answers published with Philox4x32-10: zeros, all ones, digits of pi."""
+    from test_gpu_tokens import words_of
+
+    i = np.array([counter[0] | counter[1] << 32], np.uint64)
+    got = words_of(i, key[0] | key[1] << 32, counter[2] | counter[3] << 32)
+    assert " ".join(f"{int(w):08x}" for w in got) == want
