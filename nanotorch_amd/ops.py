@@ -175,6 +175,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
     if not shape or not is_float(logits._storage._dtype):
         raise ValueError(f"Logits are float with an axis of tokens, got {logits.dtype.name} "
                          f"{shape}.")
+    if not -2**63 <= ignore_index < 2**63:  # the library's 64 bits would wrap round
+        raise ValueError(f"ignore_index must fit 64 bits, got {ignore_index}.")
     if not 0 <= top <= min(shape[-1], 64):
         raise ValueError(f"top must lie in [0, min(V, 64)], got {top} with V = {shape[-1]}.")
     if tokens is None:

@@ -264,3 +264,13 @@ def test_gradients_of_another_size_are_refused(lib, op):
                 y.grad_fn.backward(tensor(*shape))
     (dx, *_) = y.grad_fn.backward(tensor(*y.shape[::-1]))
     assert dx.shape == (6, 5)
+
+
+def test_ignore_index_fits_64_bits(lib):
+    z, t = tensor(6, 5), tensor(6, dtype=Dtype.Int64)
+    for bad in (2 ** 63, 2 ** 64, -2 ** 63 - 1, 2 ** 64 - 100):
+        with pytest.raises(ValueError):
+            nt.token_logprobs(z, t, ignore_index=bad)
+    for good in (-2 ** 63, 2 ** 63 - 1, -100, 0, np.int32(-1)):
+        nt.token_logprobs(z, t, ignore_index=good)
+        assert lib.args("nt_token_logprobs")[2] == good
