@@ -821,7 +821,11 @@ void run_sorted(const nt_view *g, const Tokens &tok, int64_t padding, T scale,
   const uint32_t vectors = row_vectors<T>(D);
   T *const to = typed_ptr<T>(dw);
   // a filling workgroup's rows: 512 workgroups, but 2^12 to 2^15 vectors each,
-  // which take longer to write than the tokens to read
+  // which take longer to write than the tokens to read, and at most RANK_ROWS
+  // rows.  Those bound tall narrow tables, whose many workgroups each read all
+  // tokens (us by ranks and by the radix sort: 1000000 x 4, 1024 tokens 14 and
+  // 45, 16384 54 and 64; 10000000 x 4, 1024 36 and 122, 9000 96 and 103, but
+  // 16384 145 and 107).
   const int64_t fill = std::clamp<int64_t>((V * vectors + 511) / 512, 1 << 12, 1 << 15);
   const uint32_t R = uint32_t(std::clamp<int64_t>(fill / vectors, 1, RANK_ROWS));
   const bool ranked = N <= RANK_MOST && (ACC || (V + R - 1) / R < int64_t(1) << 20);
