@@ -418,7 +418,9 @@ def token_logprobs_bwd(z, tokens, ignore: int, results: Storage, ga, gb,
     probabilities and gb of the entropies (None: zero); added to `target`
     (adjacent elements in each row) when given, else a new storage.  `results`
     is token_logprobs's buffer, the statistics at its end."""
-    require_device(*[x for x in (ga, gb, target) if x is not None])
+    for x in (ga, gb, target):
+        if x is not None and x._storage._device is not Device.Cuda:
+            require_device(x)
     rows = int(z._shape[0])
     if target is None:
         out = Storage.allocate(rows * int(z._shape[1]), z._storage._dtype, Device.Cuda)

@@ -213,9 +213,11 @@ class TokenLogProbOp(Function):
         else:
             g = reshape_view(g, (2, rows))._to_contiguous()
             ga, gb = _row_of(g, 0), _row_of(g, 1)
-        ga, gb = (None if x is None else _vector(x.to(z.dtype)) for x in (ga, gb))
+        dtype = z._storage._dtype
+        ga, gb = [x if x is None else _vector(x if x._storage._dtype == dtype else x.to(dtype))
+                  for x in (ga, gb)]
         into = None
-        if target is not None and target._storage._dtype == z._storage._dtype:
+        if target is not None and target._storage._dtype == dtype:
             into = _rows_in_place(target)
         st = K.token_logprobs_bwd(z, flat, ignore, results, ga, gb, into)
         if into is not None:

@@ -274,3 +274,18 @@ def test_ignore_index_fits_64_bits(lib):
     for good in (-2 ** 63, 2 ** 63 - 1, -100, 0, np.int32(-1)):
         nt.token_logprobs(z, t, ignore_index=good)
         assert lib.args("nt_token_logprobs")[2] == good
+
+
+@pytest.mark.parametrize("i", [0, 1])
+def test_a_row_gradient_is_added_to_a_plain_one(lib, i):
+    """As the ops' contract has it; the engine itself never holds one here."""
+    z, t = tensor(4, 20, requires_grad=True), tensor(4, dtype=Dtype.Int64)
+    op = nt.token_logprobs(z, t, entropy=True)[i].grad_fn
+    both, g = tensor(2, 4), tensor(4)
+    assert op._backward_into(g, [True], [both]) == [both]
+    _, out, other = lib.args("nt_inplace")
+    assert out[:4] == (both.storage.data_ptr(), 4 * i, Dtype.Float32, (4,))
+    assert other.ptr == g.storage.data_ptr()
+    (full,) = op.backward(g)
+    assert full.shape == (2, 4)
+    assert lib.args("nt_copy")[1][:2] == (full.storage.data_ptr(), 4 * i)
