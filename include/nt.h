@@ -2,9 +2,9 @@
  * nt.h -- C ABI of libnt, the MI355X (gfx950) compute library behind the
  * nanotorch_amd Tensor/autograd API.
  *
- * Every entry point but those of the token operators replaces one binding of
- * the reference's pybind11 module `nanotorch._C` (src/cpp/_C.cpp:12-24, typed
- * in src/nanotorch/_C.pyi).  The citation above each declaration names the
+ * Every entry point but those of the token and transformer operators replaces
+ * one binding of the reference's pybind11 module `nanotorch._C`
+ * (src/cpp/_C.cpp:12-24, typed in src/nanotorch/_C.pyi).  The citation above each declaration names the
  * reference interface it stands in for.  Conventions:
  *
  *  - All tensors are described by `nt_view`: a base pointer to device memory,
@@ -399,6 +399,80 @@ int nt_token_logprobs_bwd(const nt_view *logits, const nt_view *tokens,
                           int64_t ignore, const nt_view *stats,
                           const nt_view *g_logprob, const nt_view *g_entropy,
                           const nt_view *dlogits, int32_t accumulate);
+
+/* -------------------------------------------------- transformer operators */
+
+/* No counterpart in the reference: what a transformer's blocks need around
+ * their matrix products, and the step over its parameters. */
+
+/* y = s r w with s = x + residual (x where residual is NULL) and
+ * r = (mean s^2 + eps)^-1/2 over each row of [rows, D]; weight w [D] or NULL
+ * (ones).  sum [rows, D] receives s and rstd [rows] r, each NULL where it is
+ * not wanted.  x and residual need adjacent elements in a row, any row stride;
+ * the others are contiguous; all of one float dtype.  1 <= D < 2^30. */
+int nt_rms_norm(const nt_view *x, const nt_view *residual,
+                const nt_view *weight, double eps, const nt_view *y,
+                const nt_view *sum, const nt_view *rstd);
+
+/* From g, the gradient of y, and g_sum, that of the sum (either NULL: zero;
+ * adjacent elements in a row): d_sum = g_sum + r (g w - n mean(g w n)) with
+ * n = s r, which is the gradient of x and of the residual alike, and d_weight =
+ * the sum of g n over the rows, in an order that the shape alone fixes.
+ * Either output may be NULL.  sum is s, rstd as nt_rms_norm wrote it. */
+int nt_rms_norm_bwd(const nt_view *sum, const nt_view *weight,
+                    const nt_view *rstd, const nt_view *g,
+                    const nt_view *g_sum, const nt_view *d_sum,
+                    const nt_view *d_weight);
+
+/* y = softmax(scale q . k) v over the keys that each query sees.  q is
+ * [B, Tq, H, D], k and v are [B, Tk, Hk, D] with Hk dividing H (head h reads
+ * key head h / (H / Hk)), of one float dtype, with adjacent elements in a head
+ * and any other strides; 1 <= D <= 256.  Query i of sequence b sees the keys
+ * j < lengths[b] (Tk without lengths) and, by `causal`:
+ *   0  all of them;
+ *   1  j <= lengths[b] - Tq + i: the queries end with the sequence;
+ *   2  j <= starts[b] + i, or start + i where starts is NULL.
+ * lengths and starts are 1-D int32 or int64 [B].  A query that sees nothing
+ * gives zeros.  Keys from lengths[b] on are not read.  A length outside
+ * [0, Tk] is taken as the nearer end, and the next nt_sync() or
+ * nt_memcpy_d2h() returns NT_ERR_INDEX.  y is contiguous; lse, which
+ * nt_attention_bwd needs, receives B H Tq statistics or is NULL. */
+int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v,
+                 const nt_view *lengths, const nt_view *starts, int64_t start,
+                 int32_t causal, double scale, const nt_view *y,
+                 const nt_view *lse);
+
+/* The gradients for g, that of y, with the forward call's arguments and
+ * results; g has q's shape and adjacent elements in a head.  dq, dk and dv
+ * are contiguous, of q's, k's and v's shapes, each NULL where it is not
+ * wanted; every element of them is written.  The probabilities are formed
+ * again; sums run in an order that the shapes and lengths alone fix. */
+int nt_attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v,
+                     const nt_view *lengths, const nt_view *starts,
+                     int64_t start, int32_t causal, double scale,
+                     const nt_view *y, const nt_view *lse, const nt_view *g,
+                     const nt_view *dq, const nt_view *dk, const nt_view *dv);
+
+/* One parameter of nt_adamw_step: n contiguous elements at p and their
+ * gradients at g; its moments begin at element `state` of m and v. */
+typedef struct nt_adamw_tensor {
+  void *p;
+  const void *g;
+  int64_t n;
+  int64_t state;
+} nt_adamw_tensor;
+
+/* The AdamW step number `step` (from 1) of `count` parameters of m's dtype
+ * (float32 or float64), in one launch for each 96 of them:
+ *   m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+ *   p = p - lr weight_decay p
+ *         - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * m and v are contiguous 1-D; the parameters come in the order of their
+ * moments.  Parameters may not share memory with one another or with any
+ * gradient (NT_ERR_RUNTIME). */
+int nt_adamw_step(const nt_adamw_tensor *tensors, int64_t count,
+                  const nt_view *m, const nt_view *v, double lr, double beta1,
+                  double beta2, double eps, double weight_decay, int64_t step);
 
 /* ------------------------------------------------------------- host utils */
 

@@ -36,6 +36,7 @@ from .ops import (
     add,
     argmax,
     argmin,
+    attention,
     clone,
     divide,
     dropout,
@@ -59,6 +60,7 @@ from .ops import (
     pow,
     relu,
     reshape,
+    rms_norm,
     sigmoid,
     sqrt,
     subtract,
@@ -78,6 +80,7 @@ __all__ = [
     "arange",
     "argmax",
     "argmin",
+    "attention",
     "bool_",
     "clone",
     "divide",
@@ -111,6 +114,7 @@ __all__ = [
     "randint",
     "relu",
     "reshape",
+    "rms_norm",
     "sigmoid",
     "sqrt",
     "subtract",

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 from . import _lib
 from ._data_type import Dtype
@@ -436,6 +437,86 @@ def token_logprobs_bwd(z, tokens, ignore: int, results: Storage, ga, gb,
     if target is not None:
         target._storage.bump_version()
     return out
+
+
+# --------------------------------------------------- transformer operators
+
+
+def rms_norm(x, residual, weight, eps: float, stats: bool):
+    """(results, rstd) of [rows, D]: results holds y and, with a residual, the
+    sum x + residual behind it; rstd one value per row, or None without stats."""
+    require_device(*[t for t in (x, residual, weight) if t is not None])
+    shape, dtype = (int(x._shape[0]), int(x._shape[1])), x._storage._dtype
+    n = shape[0] * shape[1]
+    out = Storage.allocate(2 * n if residual is not None else n, dtype, Device.Cuda)
+    rstd = Storage.allocate(shape[0], dtype, Device.Cuda) if stats else None
+    ptr, pack, strides = out._ptr, _lib.pack_view, (shape[1], 1)
+    _lib.call_packed(
+        "nt_rms_norm", _packed(x), _packed(residual) if residual is not None else None,
+        _packed(weight) if weight is not None else None, eps,
+        pack(ptr, 0, dtype, shape, strides),
+        pack(ptr, n, dtype, shape, strides) if residual is not None else None,
+        pack(rstd._ptr, 0, dtype, shape[:1], (1,)) if stats else None)
+    return out, rstd
+
+
+def rms_norm_bwd(s, weight, rstd: Storage, g, g_sum, need_sum: bool, need_weight: bool):
+    """(gradient of the sum, gradient of the weight) as new storages, None for
+    what is not needed; g and g_sum may be None (zero)."""
+    require_device(s, *[t for t in (g, g_sum) if t is not None])
+    shape, dtype = s._shape, s._storage._dtype
+    ds = Storage.allocate(shape[0] * shape[1], dtype, Device.Cuda) if need_sum else None
+    dw = Storage.allocate(shape[1], dtype, Device.Cuda) if need_weight else None
+    _lib.call_packed(
+        "nt_rms_norm_bwd", _packed(s), _packed(weight) if weight is not None else None,
+        _packed_flat(rstd, shape[:1]), _packed(g) if g is not None else None,
+        _packed(g_sum) if g_sum is not None else None,
+        _packed_flat(ds, shape) if need_sum else None,
+        _packed_flat(dw, shape[1:]) if need_weight else None)
+    return ds, dw
+
+
+def attention(q, k, v, lengths, starts, start: int, causal: int, scale: float, stats: bool):
+    """(y, lse) of [B, T, heads, D] views; lse None without stats."""
+    require_device(*[t for t in (q, k, v, lengths, starts) if t is not None])
+    shape, dtype = q._shape, q._storage._dtype
+    out = Storage.allocate(_numel(shape), dtype, Device.Cuda)
+    rows = _numel(shape[:3])
+    lse = Storage.allocate(rows, dtype, Device.Cuda) if stats else None
+    _lib.call_packed(
+        "nt_attention", _packed(q), _packed(k), _packed(v),
+        _packed(lengths) if lengths is not None else None,
+        _packed(starts) if starts is not None else None, start, causal, scale,
+        _packed_flat(out, shape), _packed_flat(lse, (rows,)) if stats else None)
+    return out, lse
+
+
+def attention_bwd(q, k, v, lengths, starts, start: int, causal: int, scale: float, y: Storage,
+                  lse: Storage, g, needs) -> list:
+    """New storages of the gradients of q, k and v, None for what is not needed."""
+    require_device(g)
+    dtype = q._storage._dtype
+    out = [Storage.allocate(_numel(x._shape), dtype, Device.Cuda) if need else None
+           for x, need in zip((q, k, v), needs)]
+    views = [None if st is None else _packed_flat(st, x._shape)
+             for st, x in zip(out, (q, k, v))]
+    _lib.call_packed(
+        "nt_attention_bwd", _packed(q), _packed(k), _packed(v),
+        _packed(lengths) if lengths is not None else None,
+        _packed(starts) if starts is not None else None, start, causal, scale,
+        _packed_flat(y, q._shape), _packed_flat(lse, (lse._size,)), _packed(g), *views)
+    return out
+
+
+def adamw_step(tensors: list[int], m, v, lr: float, betas, eps: float, weight_decay: float,
+               step: int) -> None:
+    """One step over many parameters; tensors: (address of the parameter, of its
+    gradient, elements, first moment) of each, one after the other."""
+    n = len(tensors)
+    _lib.call_packed("nt_adamw_step", struct.pack(f"={n}q", *tensors), n // 4, _packed(m),
+                     _packed(v), lr, betas[0], betas[1], eps, weight_decay, step)
+    m._storage.bump_version()
+    v._storage.bump_version()
 
 
 # ------------------------------------------------------------- host helpers

@@ -98,6 +98,18 @@ _SIGNATURES = {
     "nt_dropout": (c_int, [_VP, c_double, c_uint64, c_uint64, _VP, c_int32]),
     "nt_token_logprobs": (c_int, [_VP, _VP, c_int64, _VP, _VP, _VP, _VP, _VP]),
     "nt_token_logprobs_bwd": (c_int, [_VP, _VP, c_int64, _VP, _VP, _VP, _VP, c_int32]),
+    "nt_rms_norm": (c_int, [_VP, _VP, _VP, c_double, _VP, _VP, _VP]),
+    "nt_rms_norm_bwd": (c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "nt_attention": (
+        c_int, [_VP, _VP, _VP, _VP, _VP, c_int64, c_int32, c_double, _VP, _VP]),
+    "nt_attention_bwd": (
+        c_int,
+        [_VP, _VP, _VP, _VP, _VP, c_int64, c_int32, c_double, _VP, _VP, _VP, _VP, _VP, _VP],
+    ),
+    "nt_adamw_step": (
+        c_int,
+        [c_char_p, c_int64, _VP, _VP, c_double, c_double, c_double, c_double, c_double, c_int64],
+    ),
     "nt_manual_seed": (c_int, [c_uint64]),
     "nt_host_uniform": (c_int, [c_void_p, c_int32, c_int64, c_double, c_double]),
     "nt_device_uniform": (c_int, [c_void_p, c_int32, c_int64, c_double, c_double]),

@@ -7,6 +7,7 @@ from .ops_binary import AddOp, MatmulOp, MulOp, SubOp, TrueDivOp
 from .ops_reduction import MaxOp, MeanOp, MinOp, SumOp
 from .ops_special import ExpandOp, ReshapeOp, TOp, TransposeOp
 from .ops_token import DropoutOp, EmbeddingOp, TokenLogProbOp
+from .ops_transformer import AttentionOp, RmsNormOp
 from .ops_unary import ExpOp, LogOp, NegOp, PowOp, ReluOp, SigmoidOp, SqrtOp, TanhOp
 
 ALL_OPS_ = [
@@ -35,6 +36,7 @@ ALL_OPS_ = [
 
 __all__ = [
     "AddOp",
+    "AttentionOp",
     "DropoutOp",
     "EmbeddingOp",
     "ExpandOp",
@@ -50,6 +52,7 @@ __all__ = [
     "PowOp",
     "ReluOp",
     "ReshapeOp",
+    "RmsNormOp",
     "SigmoidOp",
     "SqrtOp",
     "SubOp",

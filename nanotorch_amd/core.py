@@ -666,7 +666,7 @@ def _accumulation_target(x: Tensor) -> Tensor | None:
 
 def _store_first(x: Tensor, r: Tensor, upstream: Tensor) -> None:
     x._grad = r
-    x._grad_owned = r._storage is not upstream._storage
+    x._grad_owned = r._storage is not upstream._storage and not getattr(r, "_shared", False)
 
 
 def _run_backward(fn, grad: Tensor, inputs: tuple) -> None:

@@ -1,0 +1,891 @@
+// Attention, its gradients, and attention over a cache of keys and values.
+//
+//   z = scale q . k over the keys that a query sees,  p = softmax z,  y = sum p v
+//   dv = sum p g,   ds = p (g . v - delta),  delta = g . y
+//   dq = scale sum ds k,   dk = scale sum ds q
+//
+// q, y and g are [B, Tq, H, D], k and v [B, Tk, Hk, D]; head h reads key head
+// h / (H / Hk).  The H / Hk query heads of a key head are rows beside one
+// another here: row R of a (sequence, key head) is query R / G of its head
+// R % G, G = H / Hk, so that one read of a key serves all of them.  The
+// forward pass keeps z's running maximum and sum (base 2) and never stores p;
+// the backward pass forms p again from the rows' maximum plus log sum.
+//
+// The kernels of this file work on tiles of 16 rows by 16 keys, in registers,
+// on the 16x16x4 matrix instructions of float32 and float64.  A lane l has
+// n = l % 16 and h = l / 16.  With
+//
+//   dots   S[item, own] = sum over d of X[item, d] own[own, d]
+//   sums   acc[own, d] += sum over items of a[own, item] X[item, d]
+//
+// the same registers serve as dots' result and as sums' operand: dots leaves a
+// lane the own row n and four items, which is what sums' instruction r (its
+// k index runs over h) takes of it.  So probabilities never leave their lane.
+// Forward: own = queries, items = keys; dots with k, sums with v.  dq: dots
+// with k and with v, sums with k.  dk and dv: own = keys, items = queries,
+// dots with q and g, sums with q and g.  The order of d within dots and of the
+// columns within sums is permuted so that every lane loads 16 bytes.
+//
+// A workgroup's four waves have the same own rows and every fourth block of
+// items; they are joined in LDS in a fixed order, and so are the parts of rows
+// whose keys are split over workgroups (few rows over a long cache).
+//
+// Keys from lengths[b] on are not read.  Within the length, a key that only
+// some rows of a tile see may hold anything: where such a block has a value
+// that is not finite, the sums go over visible pairs one by one (0 times an
+// infinity would be NaN).
+#include <algorithm>
+#include <cmath>
+#include <limits>
+
+#include "tokens.h"
+
+namespace nt {
+
+constexpr int AT_WAVES = 4;
+
+// One head-grouped operand: row R is at outer (R / G) + inner (R % G); keys
+// have G = 1.
+template <class T> struct Rows {
+  T *p;
+  int64_t sB, sOuter, sInner, sHead; // batch, token, head of a group, key head
+};
+
+struct AttnShape {
+  int B, Tq, Tk, Hk, G, D;
+  int rows;      // Tq G
+  FastDivU32 by_group;
+  int causal;    // 0 no, 1 the queries end with the sequence, 2 they begin at `start`
+  int64_t start;
+  Tokens starts, lengths; // p null: none
+  int *err;
+};
+
+template <class T> struct AttnFwd {
+  AttnShape s;
+  Rows<const T> q, k, v;
+  T *y;            // [B, Tq, H, D]
+  T *lse;          // [B, Hk, rows], base 2; null: not wanted
+  T scale2;        // scale log2 e
+  int splits;      // of the keys
+  T *part_acc;     // [tile, split, 16, D]
+  T *part_stat;    // [tile, split, 2, 16]
+  int vec;         // rows of all operands are whole, aligned 16-byte pieces
+};
+
+template <class T> struct AttnBwd {
+  AttnShape s;
+  Rows<const T> q, k, v, g;
+  const T *lse, *delta; // [B, Hk, rows]
+  T *dq;                // [B, Tq, H, D]
+  T *dk, *dv;           // [B, Tk, Hk, D]; either may be null
+  T scale, scale2;
+  int vec;
+};
+
+template <class T> struct Mma;
+template <> struct Mma<float> {
+  typedef float V4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ V4 mma(float a, float b, V4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+  }
+  // Row of a result's element r in lane group h.
+  static __device__ __forceinline__ int row(int h, int r) { return 4 * h + r; }
+  static __device__ __forceinline__ float exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+  static __device__ __forceinline__ float log2(float x) { return ::log2f(x); }
+};
+template <> struct Mma<double> {
+  typedef double V4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ V4 mma(double a, double b, V4 c) {
+    return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int h, int r) { return h + 4 * r; }
+  static __device__ __forceinline__ double exp2(double x) { return ::exp2(x); }
+  static __device__ __forceinline__ double log2(double x) { return ::log2(x); }
+};
+
+template <class T> constexpr T NEG_INF = -std::numeric_limits<T>::infinity();
+
+// Consecutive workgroups' work on one XCD (ids are dealt round-robin to 8).
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
+  const uint32_t q = n / 8, r = n % 8, x = id % 8;
+  return x * q + (x < r ? x : r) + id / 8;
+}
+
+// Keys of sequence b, and the position of its first query among them.
+__device__ __forceinline__ void sequence(const AttnShape &s, int b, bool report, int &n,
+                                         int &first) {
+  n = s.Tk;
+  if (s.lengths.p) {
+    const int64_t v = s.lengths[b];
+    if (report && (v < 0 || v > s.Tk))
+      *s.err = NT_ERR_INDEX;
+    n = int(v < 0 ? 0 : v > s.Tk ? s.Tk : v);
+  }
+  if (s.causal == 1)
+    first = n - s.Tq;
+  else {
+    const int64_t v = s.starts.p ? s.starts[b] : s.start;
+    // beyond these nothing changes
+    first = int(v < -int64_t(s.Tq) ? -int64_t(s.Tq) : v > s.Tk ? s.Tk : v);
+  }
+}
+
+// How many keys query i of a sequence sees.
+__device__ __forceinline__ int seen(const AttnShape &s, int n, int first, int i) {
+  if (!s.causal)
+    return n;
+  const int e = first + i + 1;
+  return e < 0 ? 0 : e < n ? e : n;
+}
+
+// 16 bytes at element d of a row of D elements; zeros past the end or where
+// the row is not `live`.
+template <class T>
+__device__ __forceinline__ typename RowVec<T>::V piece(const T *p, int d, int D, bool live,
+                                                       int vec) {
+  using R = RowVec<T>;
+  typename R::V v{};
+  if (!live)
+    return v;
+  if (vec) {
+    if (d < D)
+      v = *reinterpret_cast<const typename R::V *>(p + d);
+    return v;
+  }
+  if (d + R::N <= D)
+    return R::load(p + d);
+#pragma unroll
+  for (int j = 0; j < R::N; ++j)
+    if (d + j < D)
+      v[j] = p[d + j];
+  return v;
+}
+
+// A row's share of a lane as operand of dots: pieces at 4 N c + N h.
+template <class T, int DP> struct Frag {
+  static constexpr int N = RowVec<T>::N, C = DP / (4 * N);
+  typename RowVec<T>::V v[C];
+  __device__ __forceinline__ void load(const T *row, int D, bool live, int vec, int h) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      v[c] = piece(row, 4 * N * c + N * h, D, live, vec);
+  }
+};
+
+template <class T, int DP>
+__device__ __forceinline__ typename Mma<T>::V4 dots(const Frag<T, DP> &items,
+                                                    const Frag<T, DP> &own) {
+  typename Mma<T>::V4 s{};
+#pragma unroll
+  for (int c = 0; c < Frag<T, DP>::C; ++c)
+#pragma unroll
+    for (int e = 0; e < Frag<T, DP>::N; ++e)
+      s = Mma<T>::mma(items.v[c][e], own.v[c][e], s);
+  return s;
+}
+
+// Items' rows as operand of sums: of the four items row(h, r), pieces at
+// 16 N c + N n.  Result column 4 N c' .. of a lane: see Sums::column.
+template <class T, int DP> struct Items {
+  static constexpr int N = RowVec<T>::N, C = DP / (16 * N);
+  typename RowVec<T>::V v[4][C];
+};
+
+template <class T, int DP> struct Sums {
+  using V4 = typename Mma<T>::V4;
+  static constexpr int N = RowVec<T>::N, C = DP / (16 * N);
+  V4 acc[C][N]; // acc[c][e][r]: column(c, e, r) of the own row n
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        acc[c][e] = V4{};
+  }
+  static __device__ __forceinline__ int column(int c, int e, int h, int r) {
+    return 16 * N * c + N * Mma<T>::row(h, r) + e;
+  }
+  __device__ __forceinline__ void scale(T f) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        acc[c][e] *= f;
+  }
+  __device__ __forceinline__ void add(const T (&a)[4], const Items<T, DP> &x) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          acc[c][e] = Mma<T>::mma(x.v[r][c][e], a[r], acc[c][e]);
+  }
+  // The same over visible pairs only, from memory: `row(item)` is the item's
+  // row, null past the end.
+  template <class F>
+  __device__ __forceinline__ void add_visible(const T (&a)[4], const bool (&vis)[4], int D,
+                                              int lane, F row) {
+    const int n = lane & 15, h = lane >> 4;
+#pragma unroll 1
+    for (int item = 0; item < 16; ++item) {
+      const T *p = row(item);
+      T w = 0;
+      int on = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (Mma<T>::row(g, r) == item) {
+            w = __shfl(a[r], n + 16 * g);
+            on = __shfl(int(vis[r]), n + 16 * g);
+          }
+      if (p == nullptr || !on)
+        continue;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int d = column(c, e, h, r);
+            if (d < D)
+              acc[c][e][r] = fma(w, p[d], acc[c][e][r]);
+          }
+    }
+  }
+};
+
+// Joins the four waves' sums, each first multiplied by its lane's factor
+// (of row n), and hands 16 by 16 N of them at a time to `out(row, column, value)`.
+template <class T, int DP, class F>
+__device__ __forceinline__ void join_waves(Sums<T, DP> &s, T factor, T *lds, F out) {
+  constexpr int N = RowVec<T>::N, W = 16 * N; // columns of a turn
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+#pragma unroll
+  for (int c = 0; c < Sums<T, DP>::C; ++c) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        lds[(wave * 16 + n) * W + N * Mma<T>::row(h, r) + e] = s.acc[c][e][r] * factor;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * W; i += 64 * AT_WAVES) {
+      T v = lds[i];
+#pragma unroll
+      for (int w = 1; w < AT_WAVES; ++w)
+        v += lds[w * 16 * W + i];
+      out(i / W, c * W + i % W, v);
+    }
+  }
+}
+
+template <class T> constexpr int JOIN_ELEMENTS = AT_WAVES * 16 * 16 * RowVec<T>::N;
+
+template <class T> __device__ __forceinline__ bool finite(typename RowVec<T>::V v) {
+  bool f = true;
+#pragma unroll
+  for (int j = 0; j < RowVec<T>::N; ++j)
+    f = f && __builtin_isfinite(v[j]);
+  return f;
+}
+
+template <class T, int DP> __device__ __forceinline__ bool all_finite(const Items<T, DP> &x) {
+  bool f = true;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < Items<T, DP>::C; ++c)
+      f = f && finite<T>(x.v[r][c]);
+  return __all(f);
+}
+
+// ---------------------------------------------------------------- forward
+
+// Tiles of 16 keys that a wave takes at a time: two, as long as their rows fit
+// its registers beside two waves to a SIMD.
+template <class T, int DP> constexpr int FWD_TILES = DP * sizeof(T) <= 512 ? 2 : 1;
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_kernel(
+    const AttnFwd<T> a) {
+  using M = Mma<T>;
+  constexpr int TILES = FWD_TILES<T, DP>;
+  __shared__ T lds[JOIN_ELEMENTS<T>];
+  __shared__ T stat[2][AT_WAVES][16];
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const uint32_t tiles = uint32_t(s.rows + 15) / 16;
+  const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
+  const uint32_t split = id % uint32_t(a.splits), t = id / uint32_t(a.splits);
+  const uint32_t bh = t / tiles;
+  // long rows first: under a causal mask the last tiles see the most keys
+  const int tile = int(tiles - 1 - (t - bh * tiles));
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, threadIdx.x == 0, keys, first);
+  const int row = tile * 16 + n;
+  const bool live = row < s.rows;
+  const uint32_t qi = s.by_group.div(uint32_t(row)), qg = uint32_t(row) - qi * uint32_t(s.G);
+  const int limit = live ? seen(s, keys, first, int(qi)) : 0;
+  const int last = std::min(tile * 16 + 15, s.rows - 1);
+  const int end = seen(s, keys, first, int(s.by_group.div(uint32_t(last)))); // of any row
+  const int all = seen(s, keys, first, int(s.by_group.div(uint32_t(tile * 16)))); // of every row
+  const T *qp = a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
+                int64_t(qg) * a.q.sInner;
+  const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
+  const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
+  Frag<T, DP> q;
+  q.load(qp, s.D, live, a.vec, h);
+  Sums<T, DP> sums;
+  sums.clear();
+  T m = NEG_INF<T>, l = 0;
+  // this workgroup's blocks of keys, dealt to its waves
+  const int blocks = (end + 16 * TILES - 1) / (16 * TILES);
+  const int per = (blocks + a.splits - 1) / a.splits;
+  const int stop = std::min(blocks, int(split + 1) * per);
+  for (int blk = int(split) * per + wave; blk < stop; blk += AT_WAVES) {
+    const int j0 = blk * 16 * TILES;
+    Frag<T, DP> k[TILES];
+    Items<T, DP> v[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+      k[i].load(kp + int64_t(j0 + 16 * i + n) * a.k.sOuter, s.D, j0 + 16 * i + n < end, a.vec,
+                h);
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = j0 + 16 * i + M::row(h, r);
+        const T *p = vp + int64_t(j) * a.v.sOuter;
+#pragma unroll
+        for (int c = 0; c < Items<T, DP>::C; ++c)
+          v[i].v[r][c] = piece(p, RowVec<T>::N * (16 * c + n), s.D, j < end, a.vec);
+      }
+    T z[TILES][4];
+    bool vis[TILES][4];
+    T top = NEG_INF<T>;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      const auto d = dots<T, DP>(k[i], q);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        vis[i][r] = j0 + 16 * i + M::row(h, r) < limit;
+        z[i][r] = vis[i][r] ? d[r] * a.scale2 : NEG_INF<T>;
+        top = fmax(top, z[i][r]);
+      }
+    }
+    top = fmax(top, __shfl_xor(top, 16));
+    top = fmax(top, __shfl_xor(top, 32));
+    const T next = fmax(m, top);
+    // a row that has seen nothing but -inf: exp2(-inf - 0) = 0, not NaN
+    const T base = next == NEG_INF<T> ? T(0) : next;
+    const T shrink = M::exp2(m - base);
+    m = next;
+    l *= shrink;
+    sums.scale(shrink);
+    T sum = 0;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // fmax drops a NaN; here it comes back
+        z[i][r] = vis[i][r] ? M::exp2(z[i][r] - base) : T(0);
+        sum += z[i][r];
+      }
+    l += sum;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      const int j = j0 + 16 * i;
+      if (j + 16 > all && !all_finite<T, DP>(v[i]))
+        sums.add_visible(z[i], vis[i], s.D, lane, [&](int item) {
+          return j + item < end ? vp + int64_t(j + item) * a.v.sOuter : nullptr;
+        });
+      else
+        sums.add(z[i], v[i]);
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (h == 0) {
+    stat[0][wave][n] = m;
+    stat[1][wave][n] = l;
+  }
+  __syncthreads();
+  T top = stat[0][0][n];
+#pragma unroll
+  for (int w = 1; w < AT_WAVES; ++w)
+    top = fmax(top, stat[0][w][n]);
+  const T base = top == NEG_INF<T> ? T(0) : top;
+  T total = 0;
+#pragma unroll
+  for (int w = 0; w < AT_WAVES; ++w)
+    total += stat[1][w][n] * M::exp2(stat[0][w][n] - base);
+  const T mine = M::exp2(m - base);
+  if (a.splits > 1) {
+    const int64_t slot = int64_t(t) * a.splits + split;
+    if (wave == 0 && h == 0) {
+      a.part_stat[slot * 32 + n] = top;
+      a.part_stat[slot * 32 + 16 + n] = total;
+    }
+    join_waves<T, DP>(sums, mine, lds, [&](int r, int d, T v) {
+      if (d < s.D && tile * 16 + r < s.rows)
+        a.part_acc[(slot * 16 + r) * s.D + d] = v;
+    });
+    return;
+  }
+  if (a.lse && wave == 0 && h == 0 && live)
+    a.lse[int64_t(bh) * s.rows + row] = top == NEG_INF<T> ? T(0) : top + M::log2(total);
+  const T factor = limit > 0 ? mine / total : T(0);
+  join_waves<T, DP>(sums, factor, lds, [&](int r, int d, T v) {
+    const int w = tile * 16 + r;
+    if (d >= s.D || w >= s.rows)
+      return;
+    const uint32_t i = s.by_group.div(uint32_t(w));
+    const int64_t head = int64_t(hk) * s.G + (uint32_t(w) - i * uint32_t(s.G));
+    a.y[((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D + d] = v;
+  });
+}
+
+// Rows whose keys were split: each wave one row.
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63;
+  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (item >= int64_t(s.B) * s.Hk * s.rows)
+    return;
+  const int bh = int(item / s.rows), row = int(item % s.rows);
+  const int tiles = (s.rows + 15) / 16, n = row & 15;
+  // the slots are numbered with the tiles backwards, as their workgroups were
+  const int64_t slot = (int64_t(bh) * tiles + (tiles - 1 - row / 16)) * a.splits;
+  T top = NEG_INF<T>;
+  for (int k = 0; k < a.splits; ++k)
+    top = fmax(top, a.part_stat[(slot + k) * 32 + n]);
+  const T base = top == NEG_INF<T> ? T(0) : top;
+  T total = 0;
+  for (int k = 0; k < a.splits; ++k)
+    total += a.part_stat[(slot + k) * 32 + 16 + n] *
+             Mma<T>::exp2(a.part_stat[(slot + k) * 32 + n] - base);
+  int keys, first;
+  sequence(s, bh / s.Hk, false, keys, first);
+  const uint32_t i = s.by_group.div(uint32_t(row));
+  const bool any = seen(s, keys, first, int(i)) > 0;
+  if (a.lse && lane == 0)
+    a.lse[item] = top == NEG_INF<T> ? T(0) : top + Mma<T>::log2(total);
+  const int64_t head = int64_t(bh % s.Hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
+  T *y = a.y + ((int64_t(bh / s.Hk) * s.Tq + i) * s.Hk * s.G + head) * s.D;
+  for (int d = lane; d < s.D; d += 64) {
+    T v = 0;
+    for (int k = 0; k < a.splits; ++k)
+      v = fma(a.part_acc[((slot + k) * 16 + n) * s.D + d],
+              Mma<T>::exp2(a.part_stat[(slot + k) * 32 + n] - base), v);
+    y[d] = any ? v / total : T(0);
+  }
+}
+
+// --------------------------------------------------------------- backward
+
+// delta = g . y of each row; a wave for each.  y is contiguous.
+template <class T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(const AttnShape s, const Rows<const T> g,
+                                                         const T *y, T *delta) {
+  const int lane = threadIdx.x & 63;
+  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (item >= int64_t(s.B) * s.Hk * s.rows)
+    return;
+  const int bh = int(item / s.rows), row = int(item % s.rows), b = bh / s.Hk, hk = bh % s.Hk;
+  const uint32_t i = s.by_group.div(uint32_t(row)), gi = uint32_t(row) - i * uint32_t(s.G);
+  const T *gp = g.p + b * g.sB + hk * g.sHead + int64_t(i) * g.sOuter + int64_t(gi) * g.sInner;
+  const T *yp = y + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + int64_t(hk) * s.G + gi) * s.D;
+  T sum = 0;
+  for (int d = lane; d < s.D; d += 64)
+    sum = fma(gp[d], yp[d], sum);
+#pragma unroll
+  for (int o = 32; o; o >>= 1)
+    sum += __shfl_xor(sum, o);
+  if (lane == 0)
+    delta[item] = sum;
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(const AttnBwd<T> a) {
+  using M = Mma<T>;
+  __shared__ T lds[JOIN_ELEMENTS<T>];
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const uint32_t tiles = uint32_t(s.rows + 15) / 16;
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
+  const int tile = int(tiles - 1 - (t - bh * tiles));
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, false, keys, first);
+  const int row = tile * 16 + n;
+  const bool live = row < s.rows;
+  const uint32_t qi = s.by_group.div(uint32_t(row)), qg = uint32_t(row) - qi * uint32_t(s.G);
+  const int limit = live ? seen(s, keys, first, int(qi)) : 0;
+  const int last = std::min(tile * 16 + 15, s.rows - 1);
+  const int end = seen(s, keys, first, int(s.by_group.div(uint32_t(last))));
+  const int all = seen(s, keys, first, int(s.by_group.div(uint32_t(tile * 16))));
+  const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
+  const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
+  Frag<T, DP> q, g;
+  q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
+             int64_t(qg) * a.q.sInner,
+         s.D, live, a.vec, h);
+  g.load(a.g.p + b * a.g.sB + hk * a.g.sHead + int64_t(qi) * a.g.sOuter +
+             int64_t(qg) * a.g.sInner,
+         s.D, live, a.vec, h);
+  const T lse = live ? a.lse[int64_t(bh) * s.rows + row] : T(0);
+  const T delta = live ? a.delta[int64_t(bh) * s.rows + row] : T(0);
+  Sums<T, DP> sums;
+  sums.clear();
+  for (int j0 = wave * 16; j0 < end; j0 += 16 * AT_WAVES) {
+    Frag<T, DP> k, v;
+    Items<T, DP> x;
+    k.load(kp + int64_t(j0 + n) * a.k.sOuter, s.D, j0 + n < end, a.vec, h);
+    v.load(vp + int64_t(j0 + n) * a.v.sOuter, s.D, j0 + n < end, a.vec, h);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = j0 + M::row(h, r);
+      const T *p = kp + int64_t(j) * a.k.sOuter;
+#pragma unroll
+      for (int c = 0; c < Items<T, DP>::C; ++c)
+        x.v[r][c] = piece(p, RowVec<T>::N * (16 * c + n), s.D, j < end, a.vec);
+    }
+    const auto z = dots<T, DP>(k, q), dp = dots<T, DP>(v, g);
+    T ds[4];
+    bool vis[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vis[r] = j0 + M::row(h, r) < limit;
+      ds[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse) * (dp[r] - delta) : T(0);
+    }
+    if (j0 + 16 > all && !all_finite<T, DP>(x))
+      sums.add_visible(ds, vis, s.D, lane, [&](int item) {
+        return j0 + item < end ? kp + int64_t(j0 + item) * a.k.sOuter : nullptr;
+      });
+    else
+      sums.add(ds, x);
+  }
+  join_waves<T, DP>(sums, a.scale, lds, [&](int r, int d, T v) {
+    const int w = tile * 16 + r;
+    if (d >= s.D || w >= s.rows)
+      return;
+    const uint32_t i = s.by_group.div(uint32_t(w));
+    const int64_t head = int64_t(hk) * s.G + (uint32_t(w) - i * uint32_t(s.G));
+    a.dq[((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D + d] = v;
+  });
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(const AttnBwd<T> a) {
+  using M = Mma<T>;
+  __shared__ T lds[JOIN_ELEMENTS<T>];
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const uint32_t tiles = uint32_t(s.Tk + 15) / 16;
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
+  const int key0 = int(t - bh * tiles) * 16, key = key0 + n;
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, false, keys, first);
+  const T *qp = a.q.p + b * a.q.sB + hk * a.q.sHead;
+  const T *gp = a.g.p + b * a.g.sB + hk * a.g.sHead;
+  auto at = [&](const T *p, const Rows<const T> &x, int row) {
+    const uint32_t i = s.by_group.div(uint32_t(row));
+    return p + int64_t(i) * x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * x.sInner;
+  };
+  Frag<T, DP> k, v;
+  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + int64_t(key) * a.k.sOuter, s.D, key < keys,
+         a.vec, h);
+  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + int64_t(key) * a.v.sOuter, s.D, key < keys,
+         a.vec, h);
+  Sums<T, DP> dk, dv;
+  dk.clear();
+  dv.clear();
+  // rows before the first query that sees any of these keys take no part
+  int row0 = 0;
+  if (key0 >= keys)
+    row0 = s.rows;
+  else if (s.causal && key0 > first)
+    row0 = int(std::min<int64_t>(int64_t(key0 - first) * s.G, s.rows)) & ~15;
+  const int clear = key0 + 16; // a row that sees so many sees all of this tile
+  for (int r0 = row0 + wave * 16; r0 < s.rows; r0 += 16 * AT_WAVES) {
+    Frag<T, DP> q, g;
+    const bool live = r0 + n < s.rows;
+    q.load(at(qp, a.q, live ? r0 + n : 0), s.D, live, a.vec, h);
+    g.load(at(gp, a.g, live ? r0 + n : 0), s.D, live, a.vec, h);
+    Items<T, DP> xq, xg;
+    T lse[4], delta[4];
+    int limit[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = r0 + M::row(h, r);
+      const bool on = row < s.rows;
+      const T *p = at(qp, a.q, on ? row : 0), *o = at(gp, a.g, on ? row : 0);
+#pragma unroll
+      for (int c = 0; c < Items<T, DP>::C; ++c) {
+        xq.v[r][c] = piece(p, RowVec<T>::N * (16 * c + n), s.D, on, a.vec);
+        xg.v[r][c] = piece(o, RowVec<T>::N * (16 * c + n), s.D, on, a.vec);
+      }
+      lse[r] = on ? a.lse[int64_t(bh) * s.rows + row] : T(0);
+      delta[r] = on ? a.delta[int64_t(bh) * s.rows + row] : T(0);
+      limit[r] = on ? seen(s, keys, first, int(s.by_group.div(uint32_t(row)))) : 0;
+    }
+    const auto z = dots<T, DP>(q, k), dp = dots<T, DP>(g, v);
+    T p[4], ds[4];
+    bool vis[4], some = false;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vis[r] = key < limit[r];
+      some = some || limit[r] < clear;
+      p[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse[r]) : T(0);
+      ds[r] = vis[r] ? p[r] * (dp[r] - delta[r]) : T(0);
+    }
+    auto row_of = [&](const T *base, const Rows<const T> &x) {
+      return [&, base](int item) { return r0 + item < s.rows ? at(base, x, r0 + item) : nullptr; };
+    };
+    if (__any(some) && !all_finite<T, DP>(xg))
+      dv.add_visible(p, vis, s.D, lane, row_of(gp, a.g));
+    else
+      dv.add(p, xg);
+    if (__any(some) && !all_finite<T, DP>(xq))
+      dk.add_visible(ds, vis, s.D, lane, row_of(qp, a.q));
+    else
+      dk.add(ds, xq);
+  }
+  auto store = [&](T *out) {
+    return [&, out](int r, int d, T x) {
+      if (d < s.D && key0 + r < s.Tk)
+        out[((int64_t(b) * s.Tk + key0 + r) * s.Hk + hk) * s.D + d] = x;
+    };
+  };
+  if (a.dv)
+    join_waves<T, DP>(dv, T(1), lds, store(a.dv));
+  if (a.dk)
+    join_waves<T, DP>(dk, a.scale, lds, store(a.dk));
+}
+
+// ------------------------------------------------------------------- host
+
+namespace {
+
+constexpr int AT_MAX_D = 256;
+
+void check_heads(const nt_view *v, const nt_view *like, const char *what) {
+  check_view(v, what);
+  if (v->dtype != like->dtype)
+    fail(NT_ERR_VALUE, std::string("attention: ") + what + " has another dtype than q");
+  if (v->ndim != 4)
+    fail(NT_ERR_RUNTIME, std::string("attention: ") + what + " must be [B, T, heads, D]");
+  if (v->shape[0] != like->shape[0] || v->shape[3] != like->shape[3])
+    fail(NT_ERR_RUNTIME, std::string("attention: ") + what + " has another batch or width");
+  if (v->shape[3] > 1 && v->strides[3] != 1)
+    fail(NT_ERR_RUNTIME, std::string("attention: ") + what + " needs adjacent elements in a head");
+}
+
+Tokens per_sequence(const nt_view *v, int64_t B, const char *what) {
+  Tokens t{};
+  if (v == nullptr)
+    return t;
+  t = token_view(v, "attention");
+  if (v->shape[0] != B)
+    fail(NT_ERR_RUNTIME, std::string("attention: one of ") + what + " for each sequence");
+  return t;
+}
+
+AttnShape attn_shape(const nt_view *q, const nt_view *k, const nt_view *v,
+                     const nt_view *lengths, const nt_view *starts, int64_t start,
+                     int32_t causal) {
+  check_heads(q, q, "q");
+  check_heads(k, q, "k");
+  check_heads(v, q, "v");
+  require_same_shape(k, v, "attention");
+  const int64_t B = q->shape[0], Tq = q->shape[1], H = q->shape[2], D = q->shape[3];
+  const int64_t Tk = k->shape[1], Hk = k->shape[2];
+  if (causal < 0 || causal > 2)
+    fail(NT_ERR_VALUE, "attention: causal is 0, 1 or 2");
+  if (D < 1 || D > AT_MAX_D)
+    fail(NT_ERR_VALUE, "attention: heads of 1 to 256 elements");
+  if (Hk < 1 || H < 1 || H % Hk)
+    fail(NT_ERR_VALUE, "attention: the query heads must be a multiple of the key heads");
+  constexpr int64_t MOST = int64_t(1) << 30;
+  const int64_t G = H / Hk;
+  if (B >= MOST || Tk >= MOST || Tq >= MOST || H >= MOST || Tq * G >= MOST || B * Hk >= MOST ||
+      (B * Hk) * ((std::max(Tq * G, Tk) + 15) / 16) >= MOST / 256)
+    fail(NT_ERR_VALUE, "attention: too many rows");
+  AttnShape s{};
+  s.B = int(B), s.Tq = int(Tq), s.Tk = int(Tk), s.Hk = int(Hk), s.G = int(G), s.D = int(D);
+  s.rows = int(Tq * G);
+  s.by_group = FastDivU32(uint32_t(G));
+  s.causal = causal;
+  s.start = start;
+  s.lengths = per_sequence(lengths, B, "lengths");
+  s.starts = per_sequence(starts, B, "starts");
+  s.err = deferred_error_word();
+  return s;
+}
+
+// q, g (G heads to a group) or k, v (G = 1).
+template <class T> Rows<T> rows_of(const nt_view *v, int64_t G) {
+  Rows<T> r;
+  r.p = typed_ptr<T>(v);
+  r.sB = v->strides[0];
+  r.sOuter = v->strides[1];
+  r.sInner = v->strides[2];
+  r.sHead = v->strides[2] * G;
+  return r;
+}
+
+bool whole_pieces(const nt_view *v) {
+  const int64_t n = int64_t(16 / dtype_size(v->dtype));
+  bool ok = v->shape[3] % n == 0 &&
+            (reinterpret_cast<uintptr_t>(v->data) + size_t(v->offset) * dtype_size(v->dtype)) %
+                    16 ==
+                0;
+  for (int i = 0; i < 3; ++i)
+    ok = ok && (v->shape[i] <= 1 || v->strides[i] % n == 0);
+  return ok;
+}
+
+template <class T> T *contiguous_of(const nt_view *v, int64_t n, int dt, const char *what) {
+  check_view(v, what);
+  if (v->dtype != dt)
+    fail(NT_ERR_VALUE, std::string("attention: ") + what + " has another dtype than q");
+  if (numel(v) != n || !is_contiguous(v))
+    fail(NT_ERR_RUNTIME, std::string("attention: ") + what + " must be contiguous, of " +
+                             std::to_string(n) + " elements");
+  return typed_ptr<T>(v);
+}
+
+// The padded width: the matrix instructions' columns come 16 pieces at a time.
+template <class T, class F> void dispatch_width(int D, F &&f) {
+  constexpr int LEAST = 16 * RowVec<T>::N; // 64 float32, 32 float64
+  if (D <= LEAST)
+    f.template operator()<LEAST>();
+  else if (D <= 128)
+    f.template operator()<128>();
+  else
+    f.template operator()<256>();
+}
+
+// Into how many parts each tile's keys are split: as many as fill the chip
+// (eight workgroups a CU), with at least two blocks to a wave.
+int key_splits(const AttnShape &s) {
+  const int64_t groups = int64_t(s.B) * s.Hk * ((s.rows + 15) / 16);
+  const int64_t want = int64_t(device_cu_count()) * 4 / std::max<int64_t>(groups, 1);
+  const int64_t most = s.Tk / (32 * AT_WAVES * 2);
+  return int(std::max<int64_t>(1, std::min({want, most, int64_t(256)})));
+}
+
+template <class T> void run_attention(AttnFwd<T> &a) {
+  const AttnShape &s = a.s;
+  const int64_t tiles = int64_t(s.B) * s.Hk * ((s.rows + 15) / 16);
+  a.splits = key_splits(s);
+  const size_t slots = a.splits > 1 ? size_t(tiles) * size_t(a.splits) : 0;
+  DeviceScratch acc(slots * 16 * size_t(s.D) * sizeof(T)), stat(slots * 32 * sizeof(T));
+  a.part_acc = acc.template get<T>();
+  a.part_stat = stat.template get<T>();
+  dispatch_width<T>(s.D, [&]<int DP>() {
+    attn_fwd_kernel<T, DP>
+        <<<dim3(uint32_t(tiles * a.splits)), 64 * AT_WAVES, 0, stream()>>>(a);
+  });
+  NT_LAUNCH_CHECK();
+  if (a.splits > 1) {
+    attn_join_kernel<T><<<dim3(uint32_t((int64_t(s.B) * s.Hk * s.rows + 3) / 4)), 256, 0,
+                          stream()>>>(a);
+    NT_LAUNCH_CHECK();
+  }
+}
+
+template <class T> void run_attention_bwd(AttnBwd<T> &a, const T *y) {
+  const AttnShape &s = a.s;
+  const int64_t rows = int64_t(s.B) * s.Hk * s.rows;
+  DeviceScratch delta(size_t(rows) * sizeof(T));
+  a.delta = delta.template get<T>();
+  if (rows) {
+    attn_delta_kernel<T>
+        <<<dim3(uint32_t((rows + 3) / 4)), 256, 0, stream()>>>(s, a.g, y, delta.template get<T>());
+    NT_LAUNCH_CHECK();
+  }
+  dispatch_width<T>(s.D, [&]<int DP>() {
+    if (a.dq && rows) {
+      attn_dq_kernel<T, DP><<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.rows + 15) / 16))),
+                              64 * AT_WAVES, 0, stream()>>>(a);
+      NT_LAUNCH_CHECK();
+    }
+    if ((a.dk || a.dv) && s.Tk && s.B) {
+      attn_dkv_kernel<T, DP><<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.Tk + 15) / 16))),
+                               64 * AT_WAVES, 0, stream()>>>(a);
+      NT_LAUNCH_CHECK();
+    }
+  });
+}
+
+} // namespace
+
+} // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v, const nt_view *lengths,
+                 const nt_view *starts, int64_t start, int32_t causal, double scale,
+                 const nt_view *y, const nt_view *lse) {
+  return guard([&] {
+    const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
+    dispatch_float(q->dtype, [&]<class T>() {
+      AttnFwd<T> a{};
+      a.s = s;
+      a.q = rows_of<const T>(q, s.G);
+      a.k = rows_of<const T>(k, 1);
+      a.v = rows_of<const T>(v, 1);
+      a.y = contiguous_of<T>(y, numel(q), q->dtype, "y");
+      const int64_t rows = int64_t(s.B) * s.Hk * s.rows;
+      if (lse)
+        a.lse = contiguous_of<T>(lse, rows, q->dtype, "lse");
+      a.scale2 = T(scale * 1.4426950408889634);
+      a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v);
+      if (rows)
+        run_attention(a);
+    });
+  });
+}
+
+int nt_attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v,
+                     const nt_view *lengths, const nt_view *starts, int64_t start,
+                     int32_t causal, double scale, const nt_view *y, const nt_view *lse,
+                     const nt_view *g, const nt_view *dq, const nt_view *dk,
+                     const nt_view *dv) {
+  return guard([&] {
+    const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
+    check_heads(g, q, "g");
+    require_same_shape(g, q, "attention_bwd");
+    dispatch_float(q->dtype, [&]<class T>() {
+      AttnBwd<T> a{};
+      a.s = s;
+      a.q = rows_of<const T>(q, s.G);
+      a.k = rows_of<const T>(k, 1);
+      a.v = rows_of<const T>(v, 1);
+      a.g = rows_of<const T>(g, s.G);
+      const T *out = contiguous_of<const T>(y, numel(q), q->dtype, "y");
+      a.lse = contiguous_of<const T>(lse, int64_t(s.B) * s.Hk * s.rows, q->dtype, "lse");
+      if (dq)
+        a.dq = contiguous_of<T>(dq, numel(q), q->dtype, "dq");
+      if (dk)
+        a.dk = contiguous_of<T>(dk, numel(k), q->dtype, "dk");
+      if (dv)
+        a.dv = contiguous_of<T>(dv, numel(v), q->dtype, "dv");
+      a.scale = T(scale);
+      a.scale2 = T(scale * 1.4426950408889634);
+      a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v) && whole_pieces(g);
+      run_attention_bwd(a, out);
+    });
+  });
+}
+
+} // extern "C"

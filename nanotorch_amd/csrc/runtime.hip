@@ -262,7 +262,7 @@ void raise_deferred_error() {
   *w = NT_OK;
   fail(code, "an earlier gather/scatter call met an index, or a token operator "
              "a token, outside its axis (found by the device-side check; those "
-             "elements were skipped)");
+             "elements were skipped), or attention a length outside its keys");
 }
 int device_cu_count() { return rt().cu_count; }
 void *device_alloc(size_t nbytes) { return allocator().alloc(nbytes); }

@@ -1,7 +1,19 @@
 """Neural-network modules and optimizers."""
 
-from .module import Dropout, Embedding, Linear, Module, ReLU, Sequential, Sigmoid, Tanh
-from .optimizers import GradientDescent, Optimizer
+from .module import (
+    Attention,
+    Dropout,
+    Embedding,
+    KeyValueCache,
+    Linear,
+    Module,
+    ReLU,
+    RMSNorm,
+    Sequential,
+    Sigmoid,
+    Tanh,
+)
+from .optimizers import AdamW, GradientDescent, Optimizer
 
-__all__ = ["Dropout", "Embedding", "GradientDescent", "Linear", "Module", "Optimizer", "ReLU",
-           "Sequential", "Sigmoid", "Tanh"]
+__all__ = ["AdamW", "Attention", "Dropout", "Embedding", "GradientDescent", "KeyValueCache",
+           "Linear", "Module", "Optimizer", "RMSNorm", "ReLU", "Sequential", "Sigmoid", "Tanh"]

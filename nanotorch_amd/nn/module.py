@@ -8,7 +8,8 @@ Tanh (the reference exposes sigmoid only as a function).  ``Linear.forward``
 on float32 device tensors runs the product and the bias add as one kernel
 (``LinearOp``): same values and gradients as the reference's two ops.
 ``Embedding`` and ``Dropout`` are additions too, and with ``Dropout`` the
-modules' ``train`` / ``eval`` switch.
+modules' ``train`` / ``eval`` switch; so are ``RMSNorm``, ``Attention`` and its
+``KeyValueCache``.
 """
 
 from __future__ import annotations
@@ -16,12 +17,12 @@ from __future__ import annotations
 import math
 from typing import Any, Iterable, Iterator, Sequence
 
-from ..autograd import EmbeddingOp, ReluOp, SigmoidOp, TanhOp
+from ..autograd import EmbeddingOp, ReluOp, SigmoidOp, TanhOp, is_grad_enabled
 from ..autograd.ops_binary import LinearOp
 from ..core import Tensor
 from ..cuda import Device
-from ..factories import rand, zeros
-from ..ops import dropout
+from ..factories import ones, rand, zeros
+from ..ops import attention, dropout, rms_norm
 
 
 class Module:
@@ -143,6 +144,105 @@ class Dropout(Module):
 
     def forward(self, x: Tensor) -> Tensor:
         return dropout(x, self._p) if self._training and self._p > 0.0 else x
+
+
+class RMSNorm(Module):
+    """x (mean x^2 + eps)^-1/2 w over the last axis, w [dim] beginning with
+    ones.  With a residual: (that of x + residual, x + residual)."""
+
+    def __init__(self, dim: int, eps: float = 1e-6, *, device: Device | str = "cuda") -> None:
+        if dim <= 0:
+            raise ValueError(f"Cannot initialize RMSNorm with {dim=} (non-positive).")
+        self._w = ones(dim, requires_grad=True, device=device)
+        self._eps = eps
+
+    def parameters(self) -> Sequence[Tensor]:
+        return [self._w]
+
+    def to(self, device: Device | str) -> "RMSNorm":
+        self._w = self._w.to(device)
+        return self
+
+    def forward(self, x: Tensor, residual: Tensor | None = None):
+        return rms_norm(x, self._w, residual=residual, eps=self._eps)
+
+
+class KeyValueCache:
+    """Keys and values of up to max_tokens tokens of some sequences, which
+    Attention fills and reads: every call's tokens come behind those before."""
+
+    def __init__(self, sequences: int, max_tokens: int, kv_heads: int, head_dim: int) -> None:
+        shape = (sequences, max_tokens, kv_heads, head_dim)
+        self.keys = zeros(*shape, device="cuda")
+        self.values = zeros(*shape, device="cuda")
+        self.tokens = 0
+
+    def append(self, k: Tensor, v: Tensor) -> tuple[Tensor, Tensor]:
+        """Stores [sequences, n, kv_heads, head_dim] and returns views of all so
+        far."""
+        B, most, heads, dim = self.keys.shape
+        n, end = k.shape[1], self.tokens + k.shape[1]
+        if k.shape != (B, n, heads, dim) or v.shape != k.shape:
+            raise ValueError(f"A cache of {self.keys.shape} cannot take {k.shape}, {v.shape}.")
+        if end > most:
+            raise ValueError(f"A cache of {most} tokens cannot hold {end}.")
+        self.keys[:, self.tokens:end] = k
+        self.values[:, self.tokens:end] = v
+        self.tokens = end
+        return self.keys[:, :end], self.values[:, :end]
+
+
+class Attention(Module):
+    """Self-attention of x [B, T, dim]: projections to `heads` query heads and
+    `kv_heads` key heads (as many unless given), attention, projection back.
+
+    Causal unless told otherwise.  `lengths` [B] are the texts' own tokens where
+    they are padded at their ends.  With a cache, x holds the tokens after those
+    that it has; nothing is differentiated through it."""
+
+    def __init__(self, dim: int, heads: int, kv_heads: int | None = None, *, causal: bool = True,
+                 device: Device | str = "cuda") -> None:
+        kv_heads = heads if kv_heads is None else kv_heads
+        if min(dim, heads, kv_heads) <= 0 or dim % heads or heads % kv_heads:
+            raise ValueError(f"Cannot initialize Attention with {dim=}, {heads=}, {kv_heads=}.")
+        self._heads, self._kv_heads, self._head_dim = heads, kv_heads, dim // heads
+        self._causal = causal
+        self._q = Linear(dim, dim, False, device=device)
+        self._k = Linear(dim, kv_heads * self._head_dim, False, device=device)
+        self._v = Linear(dim, kv_heads * self._head_dim, False, device=device)
+        self._out = Linear(dim, dim, False, device=device)
+
+    def parameters(self) -> Sequence[Tensor]:
+        return [p for m in (self._q, self._k, self._v, self._out) for p in m.parameters()]
+
+    def to(self, device: Device | str) -> "Attention":
+        for m in (self._q, self._k, self._v, self._out):
+            m.to(device)
+        return self
+
+    def cache(self, sequences: int, max_tokens: int) -> KeyValueCache:
+        return KeyValueCache(sequences, max_tokens, self._kv_heads, self._head_dim)
+
+    def forward(self, x: Tensor, lengths: Tensor | None = None,
+                cache: KeyValueCache | None = None) -> Tensor:
+        if x.ndim != 3:
+            raise ValueError(f"Attention takes [B, T, dim], got {x.shape}.")
+        B, T, dim = x.shape
+        flat = x.reshape(B * T, dim)
+        q = self._q(flat).reshape(B, T, self._heads, self._head_dim)
+        k = self._k(flat).reshape(B, T, self._kv_heads, self._head_dim)
+        v = self._v(flat).reshape(B, T, self._kv_heads, self._head_dim)
+        if cache is None:
+            starts = 0 if self._causal else None
+        else:
+            if lengths is not None or not self._causal:
+                raise ValueError("A cache is for causal attention without padding.")
+            if is_grad_enabled() and any([t.requires_grad for t in (q, k, v)]):
+                raise RuntimeError("A cache is not differentiated: use no_grad().")
+            starts = cache.tokens
+            k, v = cache.append(k, v)
+        y = attention(q, k, v, causal=self._causal, lengths=lengths, starts=starts)
+        return self._out(y.reshape(B * T, dim)).reshape(B, T, dim)
 
 
 class ReLU(Module):

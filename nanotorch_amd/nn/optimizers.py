@@ -9,7 +9,8 @@ import struct
 
 from .. import _kernels as K
 from .. import autograd as ag
-from .._data_type import Dtype
+from .._data_type import Dtype, is_float
+from .._indexing import row_major_strides
 from ..core import Tensor
 from ..cuda import Device
 
@@ -61,3 +62,117 @@ class GradientDescent(Optimizer):
                         K.sgd_step(p, g, lr32)
                     else:
                         p -= g * self._lr
+
+
+class AdamW(Optimizer):
+    """Adam with decoupled weight decay, over all parameters in one launch for
+    each 96 of them:
+
+        m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2
+        p <- p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+
+    Parameters are device tensors of one float type, and so are the moments,
+    which lie in two vectors, the parameters' parts one after the other (each
+    beginning at a multiple of 64 elements).  A parameter listed twice is
+    stepped once; different ones may not share memory."""
+
+    _ALIGN = 64
+
+    def __init__(self, parameters: Sequence[Tensor], lr: float, *,
+                 betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01) -> None:
+        parameters = list(parameters)
+        super().__init__(parameters)
+        lr, eps, weight_decay = float(lr), float(eps), float(weight_decay)
+        b1, b2 = [float(b) for b in betas]
+        if not (math.isfinite(lr) and 0.0 <= eps < math.inf and 0.0 <= weight_decay < math.inf
+                and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW needs a finite lr, 0 <= betas < 1, eps >= 0 and "
+                             f"weight_decay >= 0, got {lr=}, {betas=}, {eps=}, {weight_decay=}.")
+        self.lr = lr
+        self._betas, self._eps, self._decay = (b1, b2), eps, weight_decay
+        self._step = 0
+        unique: dict[int, Tensor] = {id(p): p for p in parameters}
+        self._slots: list[tuple[Tensor, int]] = []  # and where its moments begin
+        self._dtype, n = Dtype.Float32, 0
+        for i, p in enumerate(unique.values()):
+            dtype = p._storage._dtype
+            if not is_float(dtype) or (i and dtype != self._dtype):
+                raise ValueError(f"AdamW needs parameters of one float type, got "
+                                 f"{dtype.name} at {i}.")
+            self._dtype = dtype
+            self._slots.append((p, n))
+            n += -(-p.numel // self._ALIGN) * self._ALIGN
+        self._size = n
+        self._m: Tensor | None = None  # made with the first step
+        self._v: Tensor | None = None
+
+    @property
+    def steps(self) -> int:
+        """How many steps were taken."""
+        return self._step
+
+    def moments(self) -> tuple[Tensor, Tensor]:
+        """The first and second moments of all parameters, as the two vectors
+        that the steps update."""
+        if self._m is None:
+            self._m, self._v = [Tensor._new_contiguous(
+                K.fill(self._size, 0.0, self._dtype, Device.Cuda), (self._size,))
+                for _ in range(2)]
+        return self._m, self._v
+
+    def moments_of(self, i: int) -> tuple[Tensor, Tensor]:
+        """The moments of parameter i, as views of its shape."""
+        p = list(self._parameters)[i]
+        at = next(at for q, at in self._slots if q is p)
+        return tuple([Tensor._new_view(t._storage, p._shape, None, at)
+                      for t in self.moments()])
+
+    def load_moments(self, m: Tensor, v: Tensor, steps: int) -> None:
+        """Continues from moments() and steps of an earlier optimizer of the
+        same parameters; the vectors are copied."""
+        for t in (m, v):
+            if t._shape != (self._size,) or t._storage._dtype != self._dtype:
+                raise ValueError(f"The moments are vectors of {self._size} {self._dtype.name}, "
+                                 f"got {t.dtype.name} {t.shape}.")
+        if steps < 0:
+            raise ValueError(f"steps cannot be negative, got {steps}.")
+        self._m, self._v = [t.to(Device.Cuda)._to_contiguous(force=True) for t in (m, v)]
+        self._step = int(steps)
+
+    def step(self) -> None:
+        tensors: list[int] = []
+        written: list[Tensor] = []
+        copies: list[tuple[Tensor, Tensor]] = []  # views: stepped as a copy
+        keep = []  # temporaries live until the call
+        dtype = self._dtype
+        for p, at in self._slots:
+            if not p.requires_grad:
+                continue
+            g = p._grad
+            if g is None:
+                raise RuntimeError("Gradients not set, did you call backward?")
+            if p._storage._device is not Device.Cuda or g._storage._device is not Device.Cuda:
+                K.require_device(p, g)
+            if p._storage._dtype is not dtype or g._shape != p._shape:
+                raise ValueError(f"A parameter {dtype.name} {p.shape} became {p.dtype.name}, or "
+                                 f"its gradient has another shape: {g.shape}.")
+            strides = row_major_strides(p._shape)
+            if g._storage._dtype is not dtype or g._strides != strides:
+                g = g.to(dtype)._to_contiguous()
+                keep.append(g)
+            to = p
+            if p._strides != strides:
+                to = p._to_contiguous(force=True)
+                copies.append((to, p))
+            item = 4 if dtype is Dtype.Float32 else 8
+            tensors += (to._storage._ptr + to._offset * item, g._storage._ptr + g._offset * item,
+                        p.numel, at)
+            written.append(p)
+        m, v = self.moments()
+        K.adamw_step(tensors, m, v, self.lr, self._betas, self._eps, self._decay, self._step + 1)
+        self._step += 1
+        for new, p in copies:
+            K.copy_view(new, p)
+        for p in written:
+            p._storage.bump_version()

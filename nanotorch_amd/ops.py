@@ -11,6 +11,7 @@ from . import autograd
 from ._data_type import Dtype, is_float, promote_dtypes
 from ._indexing import broadcast_shapes
 from .autograd.ops_token import RowOp, _as_rows, _check_tokens, result_row, top_views
+from .autograd.ops_transformer import NormRowOp, check_attention
 from .core import Tensor
 from .factories import next_dropout_counter
 
@@ -203,6 +204,60 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, entropy: boo
             row = RowOp.apply if tracked else result_row
             logprob, ent = row(out, 0), row(out, 1)
     return TokenLogProbs(logprob, ent, *extras)
+
+
+def rms_norm(x: Tensor, weight: Tensor | None = None, *, residual: Tensor | None = None,
+             eps: float = 1e-6) -> Tensor | tuple[Tensor, Tensor]:
+    """x (mean x^2 + eps)^-1/2 weight over the last axis of a float tensor.
+
+    With a ``residual`` of x's shape, the sum s = x + residual takes x's place,
+    and (y, s) is returned: s is what the next block adds to.  ``weight`` is
+    1-D.  One pass forward; one backward for the gradients of both results,
+    with the weight's summed in an order that the shape alone fixes."""
+    out = autograd.RmsNormOp.apply(x, weight, residual, eps)
+    if residual is None:
+        return out
+    rows = out._rows
+    if out._grad_fn is None:
+        return rows
+    return NormRowOp.apply(out, 0), NormRowOp.apply(out, 1)
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False,
+              lengths: Tensor | None = None, starts: Tensor | int | None = None,
+              scale: float | None = None) -> Tensor:
+    """softmax(scale q . k) v: queries [B, Tq, H, D] over keys and values
+    [B, Tk, Hk, D], or all without B; returns [B, Tq, H, D].
+
+    Hk divides H: query head h reads key head h // (H // Hk).  D is at most
+    256, ``scale`` D**-0.5 unless given.  Query i of sequence b sees key j where
+
+    * j < ``lengths[b]`` (int32 or int64 [B]; Tk unless given), and
+    * if ``causal``, j <= ``starts[b]`` + i, with starts an int for all or an
+      int32 or int64 tensor [B].  Unless given, the queries are the last ones of
+      their sequences: starts = lengths - Tq.  (A batch of texts padded at
+      their ends has starts=0.)
+
+    A query that sees no key gives zeros and has no gradient.  Keys and values
+    from lengths[b] on are not read, and what a query does not see does not
+    reach its result, whatever it holds.  Lengths are checked on the device: one
+    outside [0, Tk] is taken as the nearer end, and the next synchronisation
+    (``sync``, ``cpu``) raises IndexError.
+
+    The probabilities are never stored: the backward pass forms them again.
+    Every result comes out the same every time."""
+    check_attention(q, k, v, lengths, starts)
+    start, mode = 0, 0
+    if starts is not None and not causal:
+        raise ValueError("attention() takes starts only with causal=True.")
+    if causal:
+        mode = 1 if starts is None else 2
+        if starts is not None and not isinstance(starts, Tensor):
+            start, starts = int(starts), None
+            if not -2**63 <= start < 2**63:  # the library's 64 bits would wrap round
+                raise ValueError(f"starts must fit 64 bits, got {start}.")
+    scale = q._shape[-1] ** -0.5 if scale is None else float(scale)
+    return autograd.AttentionOp.apply(q, k, v, mode, lengths, starts, start, scale)
 
 
 def _arg_reduce(op: int, name: str, x: Tensor, axis, keepdim: bool) -> Tensor:

@@ -1,0 +1,184 @@
+"""The AdamW step against plain numpy in 64 bits (long double for float64).
+
+Tolerances, u the unit roundoff.  m is a product and a fused sum with rounded
+coefficients: 4 u (|b1 m| + |c1 g|); v the same with one factor more, 6 u of
+itself.  The update's own relative error beside m's is v's half and 12 u for the
+root, the coefficients, the sum with eps, the quotient and the product; p: that
+and 3 u |p|.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from helpers import assert_bitexact, dev, host, rng, seed_of
+
+import nanotorch_amd as nt
+from nanotorch_amd import nn
+
+pytestmark = pytest.mark.gpu
+
+U = {np.float32: 2.0 ** -24, np.float64: 2.0 ** -53}
+FLOATS = [np.float32, np.float64]
+B1, B2 = 0.9, 0.999
+
+
+def step(p, g, m, v, t, lr, eps, wd, u, betas=(B1, B2)):
+    """[(value, tolerance)] of p, m, v."""
+    b1, b2 = betas
+    wide = np.longdouble if p.dtype == np.float64 else np.float64
+    p, g, m, v = [x.astype(wide) for x in (p, g, m, v)]
+    em = 4 * u * (np.abs(b1 * m) + np.abs((1 - b1) * g))
+    m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    den = np.sqrt(v / (1 - wide(b2) ** t)) + eps
+    rate = lr / (1 - wide(b1) ** t)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        upd = np.where(m == 0, 0, rate * m / den)
+        eu = np.where(m == 0, 0, abs(rate) * em / den) + 15 * u * np.abs(upd)
+    new = p - lr * wd * p - upd
+    return [(new, eu + 3 * u * (np.abs(p) + np.abs(new))), (m, em), (v, 6 * u * v)]
+
+
+def check(got, want, what):
+    value, tol = want
+    err = np.abs(got.astype(np.longdouble) - value)
+    bad = ~(err <= tol + 1e-300)
+    assert not bad.any(), (what, int(bad.sum()), float(np.nanmax(err / (tol + 1e-300))))
+
+
+def leaf(a):
+    return dev(a, True)
+
+
+def with_grad(p, g):
+    """p.grad = g, through the engine."""
+    p.zero_grad()
+    (p * dev(g)).sum().backward()
+
+
+SIZES = [(1,), (3, 5), (), (64, 64), (1, 0), (4097,), (100, 333), (8192,), (2, 3, 7), (4096, 5)]
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("count", [1, 7, 250])
+def test_steps(gpu, dtype, count):
+    """Several steps of tensors of all kinds of sizes, each step against the
+    state that the last one left; over 96 tensors take several launches."""
+    r = rng(seed_of("adamw", count, dtype.__name__))
+    values = [np.asarray(r.standard_normal(SIZES[i % len(SIZES)]) * 0.1).astype(dtype)
+              for i in range(count)]
+    ps = [leaf(a) for a in values]
+    opt = nn.AdamW(ps, 1e-2, weight_decay=0.1)
+    state = [(a, np.zeros_like(a), np.zeros_like(a)) for a in values]
+    for t in range(1, 4):
+        gs = [np.asarray(r.standard_normal(a.shape)).astype(dtype) for a in values]
+        for p, g in zip(ps, gs):
+            with_grad(p, g)
+        versions = [p.version for p in ps]
+        opt.step()
+        assert opt.steps == t and all(p.version > n for p, n in zip(ps, versions))
+        for i, (p, g) in enumerate(zip(ps, gs)):
+            got = (host(p), *[host(x) for x in opt.moments_of(i)])
+            for x, want, name in zip(got, step(state[i][0], g, *state[i][1:], t, 1e-2, 1e-8, 0.1,
+                                               U[dtype]), "pmv"):
+                check(x.reshape(values[i].shape), want, (t, i, name))
+            state[i] = tuple(x.reshape(values[i].shape) for x in got)
+
+
+@pytest.mark.parametrize("t", [1, 1000, 10**7])
+def test_coefficients(gpu, t):
+    """Late steps, where 1 - b^t is 1, betas of 0 and next to 1, no decay."""
+    r = rng(seed_of("late", t))
+    a, g = [r.standard_normal(500).astype(np.float32) for _ in range(2)]
+    for betas in ((0.9, 0.999), (0.0, 0.0), (0.99, 1 - 1e-6)):
+        p = leaf(a)
+        opt = nn.AdamW([p], 0.1, betas=betas, eps=1e-3, weight_decay=0.0)
+        m = r.standard_normal(512).astype(np.float32)
+        opt.load_moments(dev(m), dev(m * m), t - 1)
+        with_grad(p, g)
+        opt.step()
+        b1, b2 = betas
+        want = step(a, g, m[:500], (m * m)[:500], t, 0.1, 1e-3, 0.0, U[np.float32], betas)
+        check(host(p), want[0], betas)
+        check(host(opt.moments_of(0)[0]), want[1], betas)
+        check(host(opt.moments_of(0)[1]), want[2], betas)
+        # what lies between the parameters' moments stays
+        assert_bitexact(host(opt.moments()[0])[500:], m[500:])
+
+
+def test_continues_bit_for_bit(gpu):
+    r = rng(3)
+    a = r.standard_normal((30, 40)).astype(np.float32)
+    gs = [r.standard_normal((30, 40)).astype(np.float32) for _ in range(4)]
+    p = leaf(a)
+    opt = nn.AdamW([p], 1e-2)
+    for i, g in enumerate(gs):
+        if i == 2:
+            saved = [host(x) for x in opt.moments()]
+            q, n = leaf(host(p)), opt.steps
+        with_grad(p, g)
+        opt.step()
+    again = nn.AdamW([q], 1e-2)
+    again.load_moments(dev(saved[0]), dev(saved[1]), n)
+    for g in gs[2:]:
+        with_grad(q, g)
+        again.step()
+    assert_bitexact(host(q), host(p))
+    for x, y in zip(again.moments(), opt.moments()):
+        assert_bitexact(host(x), host(y))
+
+
+def test_views_doubles_and_tied(gpu):
+    """A parameter that is a transposed view or starts at any element, a gradient
+    of other strides or float type, a parameter listed twice, one without a
+    gradient of its own (frozen)."""
+    r = rng(5)
+    a, g = [r.standard_normal((9, 14)).astype(np.float32) for _ in range(2)]
+    want = step(a, g, np.zeros_like(a), np.zeros_like(a), 1, 0.1, 1e-8, 0.01, U[np.float32])[0]
+    buf = dev(np.ascontiguousarray(a.T))
+    view = nt.Tensor._new_view(buf.storage, (9, 14), (1, 9), 0)
+    view.enable_grad()
+    wide = dev(np.concatenate([np.full(3, 7, np.float32), a.reshape(-1), np.full(3, 7,
+                                                                                 np.float32)]))
+    shifted = nt.Tensor._new_view(wide.storage, (9, 14), None, 3)
+    shifted.enable_grad()
+    plain, frozen = leaf(a), dev(a)
+    other = leaf(a)
+    for p in (view, shifted, plain):
+        with_grad(p, g)
+    other._grad = dev(np.ascontiguousarray(g.T.astype(np.float64))).T
+    nn.AdamW([view, shifted, plain, frozen, plain, other], 0.1).step()
+    for p in (view, shifted, plain, other):
+        check(host(p), want, "p")
+    assert_bitexact(host(frozen), a)
+    assert (host(wide)[:3] == 7).all() and (host(wide)[-3:] == 7).all()
+
+
+def test_not_numbers_stay_where_they_are(gpu):
+    a, g = np.ones(5000, np.float32), np.ones(5000, np.float32)
+    g[7], g[11], g[4500] = np.nan, np.inf, 0
+    p = leaf(a)
+    with_grad(p, np.ones_like(a))
+    p._grad = dev(g)
+    opt = nn.AdamW([p], 0.1)
+    opt.step()
+    got = host(p)
+    assert np.isnan(got[7]) and np.isnan(got[11])
+    assert np.isfinite(np.delete(got, [7, 11])).all()
+
+
+def test_shared_memory_is_refused(gpu):
+    buf = dev(np.zeros(100, np.float32))
+    one, two = [nt.Tensor._new_view(buf.storage, (60,), None, at) for at in (0, 40)]
+    for p in (one, two):
+        p.enable_grad()
+        p._grad = dev(np.ones(60, np.float32))
+    opt = nn.AdamW([one, two], 0.1)
+    with pytest.raises(RuntimeError, match="share memory"):
+        opt.step()
+    assert opt.steps == 0 and (host(buf) == 0).all()
+    one._grad = two
+    with pytest.raises(RuntimeError, match="share memory"):
+        nn.AdamW([one], 0.1).step()
+    nn.AdamW([], 0.1).step()
