@@ -1,0 +1,131 @@
+// What the attention kernels share: the operands' description, the rows and keys
+// of a sequence, and the hand-over between the kernels on half-precision planes
+// (attention_split.hip) and those on tiles in registers (attention.hip).
+#pragma once
+
+#include "tokens.h"
+
+namespace nt {
+
+// One head-grouped operand: row R is at outer (R / G) + inner (R % G); keys
+// have G = 1.
+template <class T> struct Rows {
+  T *p;
+  int64_t sB, sOuter, sInner, sHead; // batch, token, head of a group, key head
+};
+
+struct AttnShape {
+  int B, Tq, Tk, Hk, G, D;
+  int rows;      // Tq G
+  FastDivU32 by_group;
+  int causal;    // 0 no, 1 the queries end with the sequence, 2 they begin at `start`
+  int64_t start;
+  Tokens starts, lengths; // p null: none
+  int *err;
+};
+
+// Which of the two kinds of kernels computes a (sequence, key head): the packing
+// kernel leaves a word for each of its tiles, not 0 where half precision cannot
+// hold the tile's values.  words null: no packing took place.
+struct AttnGate {
+  const uint32_t *words;
+  int per; // of each (sequence, key head)
+};
+
+// Whether any word is set; the same for all work-items of the workgroup.
+__device__ __forceinline__ bool gate_set(const AttnGate &g, uint32_t bh) {
+  uint32_t any = 0;
+  for (int i = threadIdx.x; i < g.per; i += blockDim.x)
+    any |= g.words[int64_t(bh) * g.per + i];
+  return __syncthreads_or(int(any)) != 0;
+}
+
+template <class T> struct AttnFwd {
+  AttnShape s;
+  Rows<const T> q, k, v;
+  T *y;            // [B, Tq, H, D]
+  T *lse;          // [B, Hk, rows], base 2; null: not wanted
+  T scale2;        // scale log2 e
+  int splits;      // of the keys
+  T *part_acc;     // [tile, split, 16, D]
+  T *part_stat;    // [tile, split, 2, 16]
+  int vec;         // rows of all operands are whole, aligned 16-byte pieces
+  AttnGate gate;
+};
+
+template <class T> struct AttnBwd {
+  AttnShape s;
+  Rows<const T> q, k, v, g;
+  const T *lse, *delta; // [B, Hk, rows]
+  T *dq;                // [B, Tq, H, D]
+  T *dk, *dv;           // [B, Tk, Hk, D]; either may be null
+  T scale, scale2;
+  int vec;
+  AttnGate gate;
+};
+
+// Consecutive workgroups' work on one XCD (ids are dealt round-robin to 8).
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
+  const uint32_t q = n / 8, r = n % 8, x = id % 8;
+  return x * q + (x < r ? x : r) + id / 8;
+}
+
+// Keys of sequence b, and the position of its first query among them.
+__device__ __forceinline__ void sequence(const AttnShape &s, int b, bool report, int &n,
+                                         int &first) {
+  n = s.Tk;
+  if (s.lengths.p) {
+    const int64_t v = s.lengths[b];
+    if (report && (v < 0 || v > s.Tk))
+      *s.err = NT_ERR_INDEX;
+    n = int(v < 0 ? 0 : v > s.Tk ? s.Tk : v);
+  }
+  if (s.causal == 1)
+    first = n - s.Tq;
+  else {
+    const int64_t v = s.starts.p ? s.starts[b] : s.start;
+    // beyond these nothing changes
+    first = int(v < -int64_t(s.Tq) ? -int64_t(s.Tq) : v > s.Tk ? s.Tk : v);
+  }
+}
+
+// How many keys query i of a sequence sees.
+__device__ __forceinline__ int seen(const AttnShape &s, int n, int first, int i) {
+  if (!s.causal)
+    return n;
+  const int e = first + i + 1;
+  return e < 0 ? 0 : e < n ? e : n;
+}
+
+// 16 bytes at element d of a row of D elements; zeros past the end or where
+// the row is not `live`.
+template <class T>
+__device__ __forceinline__ typename RowVec<T>::V piece(const T *p, int d, int D, bool live,
+                                                       int vec) {
+  using R = RowVec<T>;
+  typename R::V v{};
+  if (!live)
+    return v;
+  if (vec) {
+    if (d < D)
+      v = *reinterpret_cast<const typename R::V *>(p + d);
+    return v;
+  }
+  if (d + R::N <= D)
+    return R::load(p + d);
+#pragma unroll
+  for (int j = 0; j < R::N; ++j)
+    if (d + j < D)
+      v[j] = p[d + j];
+  return v;
+}
+
+// attention_split.hip: whether its kernels take a product of this shape, and
+// their launches.  The forward launch leaves a.gate for the kernels that follow
+// it; `words` is its memory, which must outlive them.
+bool split_takes(const AttnShape &s);
+size_t split_gate_words(const AttnShape &s, bool backward);
+void run_split(AttnFwd<float> &a, uint32_t *words);
+void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words);
+
+} // namespace nt

@@ -37,51 +37,13 @@
 #include <algorithm>
 #include <cmath>
 #include <limits>
+#include <type_traits>
 
-#include "tokens.h"
+#include "attention.h"
 
 namespace nt {
 
 constexpr int AT_WAVES = 4;
-
-// One head-grouped operand: row R is at outer (R / G) + inner (R % G); keys
-// have G = 1.
-template <class T> struct Rows {
-  T *p;
-  int64_t sB, sOuter, sInner, sHead; // batch, token, head of a group, key head
-};
-
-struct AttnShape {
-  int B, Tq, Tk, Hk, G, D;
-  int rows;      // Tq G
-  FastDivU32 by_group;
-  int causal;    // 0 no, 1 the queries end with the sequence, 2 they begin at `start`
-  int64_t start;
-  Tokens starts, lengths; // p null: none
-  int *err;
-};
-
-template <class T> struct AttnFwd {
-  AttnShape s;
-  Rows<const T> q, k, v;
-  T *y;            // [B, Tq, H, D]
-  T *lse;          // [B, Hk, rows], base 2; null: not wanted
-  T scale2;        // scale log2 e
-  int splits;      // of the keys
-  T *part_acc;     // [tile, split, 16, D]
-  T *part_stat;    // [tile, split, 2, 16]
-  int vec;         // rows of all operands are whole, aligned 16-byte pieces
-};
-
-template <class T> struct AttnBwd {
-  AttnShape s;
-  Rows<const T> q, k, v, g;
-  const T *lse, *delta; // [B, Hk, rows]
-  T *dq;                // [B, Tq, H, D]
-  T *dk, *dv;           // [B, Tk, Hk, D]; either may be null
-  T scale, scale2;
-  int vec;
-};
 
 template <class T> struct Mma;
 template <> struct Mma<float> {
@@ -105,62 +67,6 @@ template <> struct Mma<double> {
 };
 
 template <class T> constexpr T NEG_INF = -std::numeric_limits<T>::infinity();
-
-// Consecutive workgroups' work on one XCD (ids are dealt round-robin to 8).
-__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
-  const uint32_t q = n / 8, r = n % 8, x = id % 8;
-  return x * q + (x < r ? x : r) + id / 8;
-}
-
-// Keys of sequence b, and the position of its first query among them.
-__device__ __forceinline__ void sequence(const AttnShape &s, int b, bool report, int &n,
-                                         int &first) {
-  n = s.Tk;
-  if (s.lengths.p) {
-    const int64_t v = s.lengths[b];
-    if (report && (v < 0 || v > s.Tk))
-      *s.err = NT_ERR_INDEX;
-    n = int(v < 0 ? 0 : v > s.Tk ? s.Tk : v);
-  }
-  if (s.causal == 1)
-    first = n - s.Tq;
-  else {
-    const int64_t v = s.starts.p ? s.starts[b] : s.start;
-    // beyond these nothing changes
-    first = int(v < -int64_t(s.Tq) ? -int64_t(s.Tq) : v > s.Tk ? s.Tk : v);
-  }
-}
-
-// How many keys query i of a sequence sees.
-__device__ __forceinline__ int seen(const AttnShape &s, int n, int first, int i) {
-  if (!s.causal)
-    return n;
-  const int e = first + i + 1;
-  return e < 0 ? 0 : e < n ? e : n;
-}
-
-// 16 bytes at element d of a row of D elements; zeros past the end or where
-// the row is not `live`.
-template <class T>
-__device__ __forceinline__ typename RowVec<T>::V piece(const T *p, int d, int D, bool live,
-                                                       int vec) {
-  using R = RowVec<T>;
-  typename R::V v{};
-  if (!live)
-    return v;
-  if (vec) {
-    if (d < D)
-      v = *reinterpret_cast<const typename R::V *>(p + d);
-    return v;
-  }
-  if (d + R::N <= D)
-    return R::load(p + d);
-#pragma unroll
-  for (int j = 0; j < R::N; ++j)
-    if (d + j < D)
-      v[j] = p[d + j];
-  return v;
-}
 
 // A row's share of a lane as operand of dots: pieces at 4 N c + N h.
 template <class T, int DP> struct Frag {
@@ -308,9 +214,9 @@ template <class T, int DP> __device__ __forceinline__ bool all_finite(const Item
 // its registers beside two waves to a SIMD.
 template <class T, int DP> constexpr int FWD_TILES = DP * sizeof(T) <= 512 ? 2 : 1;
 
+// Tile t of all, numbered (sequence, key head) by (sequence, key head).
 template <class T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_kernel(
-    const AttnFwd<T> a) {
+__device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, uint32_t split) {
   using M = Mma<T>;
   constexpr int TILES = FWD_TILES<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
@@ -318,8 +224,6 @@ __global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_ke
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
   const uint32_t tiles = uint32_t(s.rows + 15) / 16;
-  const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
-  const uint32_t split = id % uint32_t(a.splits), t = id / uint32_t(a.splits);
   const uint32_t bh = t / tiles;
   // long rows first: under a causal mask the last tiles see the most keys
   const int tile = int(tiles - 1 - (t - bh * tiles));
@@ -449,6 +353,28 @@ __global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_ke
   });
 }
 
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_kernel(
+    const AttnFwd<T> a) {
+  const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
+  attn_fwd_tile<T, DP>(a, id / uint32_t(a.splits), id % uint32_t(a.splits));
+}
+
+// What the kernels on half-precision planes left: the tiles of each (sequence,
+// key head) dealt to `groups` workgroups.
+template <int DP>
+__global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<float, DP>)) void attn_fwd_left_kernel(
+    const AttnFwd<float> a, uint32_t groups) {
+  const uint32_t bh = blockIdx.x / groups;
+  if (!gate_set(a.gate, bh))
+    return;
+  const uint32_t tiles = uint32_t(a.s.rows + 15) / 16;
+  for (uint32_t t = blockIdx.x % groups; t < tiles; t += groups) {
+    __syncthreads();
+    attn_fwd_tile<float, DP>(a, bh * tiles + t, 0);
+  }
+}
+
 // Rows whose keys were split: each wave one row.
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
@@ -511,13 +437,13 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const AttnShape s, cons
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(const AttnBwd<T> a) {
+__device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t t) {
   using M = Mma<T>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
   const uint32_t tiles = uint32_t(s.rows + 15) / 16;
-  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
+  const uint32_t bh = t / tiles;
   const int tile = int(tiles - 1 - (t - bh * tiles));
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
@@ -581,13 +507,13 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(const AttnBwd<T>
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(const AttnBwd<T> a) {
+__device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t t) {
   using M = Mma<T>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
   const uint32_t tiles = uint32_t(s.Tk + 15) / 16;
-  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
+  const uint32_t bh = t / tiles;
   const int key0 = int(t - bh * tiles) * 16, key = key0 + n;
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
@@ -667,6 +593,36 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(const AttnBwd<T
     join_waves<T, DP>(dv, T(1), lds, store(a.dv));
   if (a.dk)
     join_waves<T, DP>(dk, a.scale, lds, store(a.dk));
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(const AttnBwd<T> a) {
+  attn_dq_tile<T, DP>(a, xcd_run(blockIdx.x, gridDim.x));
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(const AttnBwd<T> a) {
+  attn_dkv_tile<T, DP>(a, xcd_run(blockIdx.x, gridDim.x));
+}
+
+// As attn_fwd_left_kernel.
+template <int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const AttnBwd<float> a,
+                                                                     uint32_t groups) {
+  const uint32_t bh = blockIdx.x / groups;
+  if (!gate_set(a.gate, bh))
+    return;
+  const uint32_t rows = uint32_t(a.s.rows + 15) / 16, keys = uint32_t(a.s.Tk + 15) / 16;
+  if (a.dq)
+    for (uint32_t t = blockIdx.x % groups; t < rows; t += groups) {
+      __syncthreads();
+      attn_dq_tile<float, DP>(a, bh * rows + t);
+    }
+  if (a.dk || a.dv)
+    for (uint32_t t = blockIdx.x % groups; t < keys; t += groups) {
+      __syncthreads();
+      attn_dkv_tile<float, DP>(a, bh * keys + t);
+    }
 }
 
 // ------------------------------------------------------------------- host
@@ -781,8 +737,25 @@ int key_splits(const AttnShape &s) {
   return int(std::max<int64_t>(1, std::min({want, most, int64_t(256)})));
 }
 
+// Workgroups for each (sequence, key head) that the other kernels left, or not.
+uint32_t left_groups(uint32_t bhs) { return std::clamp<uint32_t>(2048 / bhs, 1, 32); }
+
 template <class T> void run_attention(AttnFwd<T> &a) {
   const AttnShape &s = a.s;
+  if constexpr (std::is_same_v<T, float>)
+    if (split_takes(s)) {
+      DeviceScratch words(split_gate_words(s, false) * sizeof(uint32_t));
+      run_split(a, words.get<uint32_t>());
+      a.splits = 1;
+      const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk), groups = left_groups(bhs);
+      dispatch_width<float>(s.D, [&]<int DP>() {
+        if constexpr (DP <= 128)
+          attn_fwd_left_kernel<DP>
+              <<<dim3(groups * bhs), 64 * AT_WAVES, 0, stream()>>>(a, groups);
+      });
+      NT_LAUNCH_CHECK();
+      return;
+    }
   const int64_t tiles = int64_t(s.B) * s.Hk * ((s.rows + 15) / 16);
   a.splits = key_splits(s);
   const size_t slots = a.splits > 1 ? size_t(tiles) * size_t(a.splits) : 0;
@@ -806,6 +779,19 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a, const T *y) {
   const int64_t rows = int64_t(s.B) * s.Hk * s.rows;
   DeviceScratch delta(size_t(rows) * sizeof(T));
   a.delta = delta.template get<T>();
+  if constexpr (std::is_same_v<T, float>)
+    if (split_takes(s)) {
+      DeviceScratch words(split_gate_words(s, true) * sizeof(uint32_t));
+      run_split_bwd(a, y, words.get<uint32_t>());
+      const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk), groups = left_groups(bhs);
+      dispatch_width<float>(s.D, [&]<int DP>() {
+        if constexpr (DP <= 128)
+          attn_bwd_left_kernel<DP>
+              <<<dim3(groups * bhs), 64 * AT_WAVES, 0, stream()>>>(a, groups);
+      });
+      NT_LAUNCH_CHECK();
+      return;
+    }
   if (rows) {
     attn_delta_kernel<T>
         <<<dim3(uint32_t((rows + 3) / 4)), 256, 0, stream()>>>(s, a.g, y, delta.template get<T>());

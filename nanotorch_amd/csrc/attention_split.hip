@@ -1,0 +1,915 @@
+// Attention and its gradients in float32 on the half-precision matrix cores, for
+// products large enough that arithmetic bounds them (attention.hip has the
+// mathematics, and the kernels for all others).
+//
+// A float32 x, scaled by a power of two to below 2^15, is hi + lo with hi the
+// nearest half and lo the nearest half of the rest: off by 2^-22 of x at most,
+// 2^-24 in the root mean square, where a float32 itself is off by 2^-24 at most.
+// Products of halves are exact in float32, so a . b is lo hi' + hi lo' + hi hi'
+// on v_mfma_f32_32x32x16_f16, which does sixteen times the work of the float32
+// instructions: 5.3 times their rate with three products for one.  What is left
+// out, lo lo', is 2^-22 of a b at most.
+//
+// The matrix cores do not round their running sums to nearest, so no long sum
+// stays in them: the products of 32 or 64 rows are summed there, the small ones
+// apart from or before the large ones, and the vector unit adds that to the
+// running result.
+//
+// A packing kernel writes the operands as planes of halves in the order in which
+// the other kernels' LDS and registers hold them, 32 rows to a unit:
+//   row form  pieces of 32 rows by 16 d: lane l has row l % 32, 8 d's from
+//             8 (l / 32), 16 bytes; an operand of sums over d
+//   col form  pieces of 32 d by 16 rows: lane l has column l % 32 and rows
+//             4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3, h = l / 32, which are the
+//             rows that a lane of a 32 by 32 result holds: probabilities go from
+//             one matrix instruction into the next without leaving their lane
+// A unit is a plane of hi pieces and one of lo pieces.  Keys, values and queries
+// have one power of two to a tile of 64 rows, gradients one to a row.  A tile with
+// a value that is not finite, or whose rows' largest values lie further apart than
+// 2^12 (the small ones would lose bits), is reported in a word, and the whole
+// (sequence, key head) is then left to attention.hip's kernels, queued behind.
+// So a masked key's value never coarsens the others.
+//
+// Every kernel's own rows (queries forward and for dq, keys for dk and dv) are the
+// lanes of a result, l % 32, and the other operand's units stream through two
+// stages of LDS, loaded there directly.  Row statistics, rescaling and masks are
+// then a lane's own, and sums over own rows' columns need no exchange.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.h"
+
+namespace nt {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr int SA_UNIT = 32, SA_TILE = 64; // rows of a unit, of a packed tile
+constexpr float SA_INF = std::numeric_limits<float>::infinity();
+// Row statistics of a unit for the gradients: [lse, delta / scale, scale, limit][32].
+constexpr int SA_STATS = 4 * SA_UNIT;
+
+// Bytes of a unit's form, DB = padded width / 32.
+template <int DB> constexpr int SA_CHUNK = DB * 4096;
+
+__device__ __forceinline__ float pow2(int k) { // -126 <= k <= 127
+  return __uint_as_float(uint32_t(127 + k) << 23);
+}
+
+// The power of two that takes a largest magnitude into [2^14, 2^15), as an
+// exponent; 0 for 0.
+__device__ __forceinline__ int up_exponent(float most) {
+  if (most == 0.f)
+    return 0;
+  const int e = int(__float_as_uint(most) >> 23) - 127; // subnormals: -127
+  return min(14 - e, 126);
+}
+
+__device__ __forceinline__ void split8(const float (&x)[8], half8 &hi, half8 &lo) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    hi[j] = _Float16(x[j]);
+    lo[j] = _Float16(x[j] - float(hi[j]));
+  }
+}
+
+__device__ __forceinline__ floatx16 mma(half8 a, half8 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Row of a 32 by 32 result's element r in lane half h.
+__device__ __forceinline__ int row32(int h, int r) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// ---------------------------------------------------------------- packing
+
+struct PackTensor {
+  Rows<const float> x;
+  char *row, *col;   // units of all (sequence, key head)s; null: not wanted
+  float *scale;      // [bh, tiles]; null: one to a row, in `stats`
+  int rows, tiles;
+  int keys;          // rows from the sequence's length on are zeros
+  uint32_t blocks;   // first workgroup of the next tensor
+  int word;          // where its words begin among a (sequence, key head)'s
+};
+
+struct PackArgs {
+  AttnShape s;
+  PackTensor t[4];
+  int count, vec;
+  uint32_t *words;
+  int per;
+  // the gradient's: y, the forward statistics, and what becomes of them
+  const float *y, *lse;
+  float *stats, *delta;
+};
+
+// A workgroup packs a tile of 64 rows, by way of LDS.  HBM bound: 4 bytes read,
+// 4 written for each form.
+template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const PackArgs a) {
+  constexpr int DP = 32 * DB, PITCH = DP + 4, CH = SA_CHUNK<DB>;
+  __shared__ float x[SA_TILE * PITCH];
+  __shared__ float factor[SA_TILE];
+  __shared__ int wave_most[4], wave_least[4];
+  int which = 0;
+  while (blockIdx.x >= a.t[which].blocks)
+    ++which;
+  const PackTensor &t = a.t[which];
+  const AttnShape &s = a.s;
+  const uint32_t id = blockIdx.x - (which ? a.t[which - 1].blocks : 0);
+  const int bh = int(id / uint32_t(t.tiles)), tile = int(id - uint32_t(bh) * uint32_t(t.tiles));
+  const int b = bh / s.Hk, hk = bh % s.Hk;
+  int n, first;
+  sequence(s, b, false, n, first);
+  const int rows = t.keys ? min(n, t.rows) : t.rows;
+  const float *base = t.x.p + b * t.x.sB + hk * t.x.sHead;
+  auto address = [&](int row) {
+    if (t.keys)
+      return base + int64_t(row) * t.x.sOuter;
+    const uint32_t i = s.by_group.div(uint32_t(row));
+    return base + int64_t(i) * t.x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * t.x.sInner;
+  };
+  for (int i = threadIdx.x; i < SA_TILE * (DP / 4); i += 256) {
+    const int r = i / (DP / 4), d = i % (DP / 4) * 4, row = tile * SA_TILE + r;
+    const bool live = row < rows;
+    const auto v = piece(live ? address(row) : base, d, s.D, live, a.vec);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[r * PITCH + d + j] = v[j];
+  }
+  __syncthreads();
+  // four work-items to a row: its largest magnitude (NaN above infinity)
+  const int r = threadIdx.x / 4, part = threadIdx.x % 4;
+  uint32_t top = 0;
+  for (int d = part; d < DP; d += 4)
+    top = max(top, __float_as_uint(x[r * PITCH + d]) & 0x7fffffffu);
+  top = max(top, uint32_t(__shfl_xor(int(top), 1)));
+  top = max(top, uint32_t(__shfl_xor(int(top), 2)));
+  // the tile's largest, and its smallest that is not 0
+  int hi = int(top), lo = top ? int(top) : 0x7fffffff;
+#pragma unroll
+  for (int o = 4; o < 64; o <<= 1) {
+    hi = max(hi, __shfl_xor(hi, o));
+    lo = min(lo, __shfl_xor(lo, o));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    wave_most[threadIdx.x >> 6] = hi;
+    wave_least[threadIdx.x >> 6] = lo;
+  }
+  __syncthreads();
+  hi = max(max(wave_most[0], wave_most[1]), max(wave_most[2], wave_most[3]));
+  lo = min(min(wave_least[0], wave_least[1]), min(wave_least[2], wave_least[3]));
+  // a gradient's row of zeros counts least among the rows that it is summed with
+  const int up = !t.scale && top == 0 ? 126 : up_exponent(__int_as_float(t.scale ? hi : int(top)));
+  bool bad = hi >= 0x7f800000;
+  if (t.scale) {
+    bad = bad || (hi > lo && (hi >> 23) - (lo >> 23) > 12);
+    if (threadIdx.x == 0)
+      t.scale[int64_t(bh) * t.tiles + tile] = pow2(-up);
+  } else { // the gradient: its rows' statistics
+    const int row = tile * SA_TILE + r;
+    float dot = 0.f;
+    uint32_t i = 0;
+    if (row < rows) {
+      i = s.by_group.div(uint32_t(row));
+      const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
+      const float *y = a.y + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D;
+      for (int d = part * 4; d < s.D; d += 16)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d + j < s.D)
+            dot = fmaf(x[r * PITCH + d + j], y[d + j], dot);
+    }
+    dot += __shfl_xor(dot, 1);
+    dot += __shfl_xor(dot, 2);
+    if (part == 0) {
+      const int limit = row < rows ? seen(s, n, first, int(i)) : 0;
+      float *st = a.stats + (int64_t(bh) * t.tiles * 2 + tile * 2 + r / SA_UNIT) * SA_STATS +
+                  r % SA_UNIT;
+      // a row that sees nothing: exp2(z - inf) = 0
+      st[0] = limit > 0 ? a.lse[int64_t(bh) * t.rows + row] : SA_INF;
+      st[SA_UNIT] = dot * pow2(up);
+      st[2 * SA_UNIT] = pow2(-up);
+      reinterpret_cast<int *>(st)[3 * SA_UNIT] = limit;
+      if (row < rows)
+        a.delta[int64_t(bh) * t.rows + row] = dot;
+    }
+  }
+  if (part == 0)
+    factor[r] = pow2(up);
+  if (threadIdx.x == 0)
+    a.words[int64_t(bh) * a.per + t.word + tile] = bad;
+  __syncthreads();
+  const int64_t unit0 = (int64_t(bh) * t.tiles + tile) * 2;
+  // pieces of both units, a wave for each
+  const int lane = threadIdx.x & 63, l = lane & 31, h = lane >> 5;
+  for (int p = threadIdx.x >> 6; p < 4 * DB; p += 4) {
+    const int unit = p / (2 * DB), f = p % (2 * DB);
+    float v[8];
+    half8 vh, vl;
+    if (t.row) {
+      const int rr = unit * SA_UNIT + l;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = x[rr * PITCH + f * 16 + 8 * h + j] * factor[rr];
+      split8(v, vh, vl);
+      char *to = t.row + (unit0 + unit) * CH + f * 1024 + lane * 16;
+      *reinterpret_cast<half8 *>(to) = vh;
+      *reinterpret_cast<half8 *>(to + CH / 2) = vl;
+    }
+    if (t.col) {
+      const int db = f / 2, ks = f % 2;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int rr = unit * SA_UNIT + ks * 16 + (j < 4 ? 4 * h + j : 4 + 4 * h + j);
+        v[j] = x[rr * PITCH + db * 32 + l] * factor[rr];
+      }
+      split8(v, vh, vl);
+      char *to = t.col + (unit0 + unit) * CH + f * 1024 + lane * 16;
+      *reinterpret_cast<half8 *>(to) = vh;
+      *reinterpret_cast<half8 *>(to + CH / 2) = vl;
+    }
+  }
+}
+
+// ----------------------------------------------------------------- shared
+
+__device__ __forceinline__ void load_lds(const char *from, char *to, int lane) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void *)(from + lane * 16),
+      (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// This wave's direct loads have landed, and every wave is past the stage before.
+__device__ __forceinline__ void stage_ready() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+__device__ __forceinline__ half8 frag(const char *p, int lane) {
+  return *reinterpret_cast<const half8 *>(p + lane * 16);
+}
+
+// items' row form (a unit) . own rows: result[item, own].
+template <int DB>
+__device__ __forceinline__ floatx16 dots32(const char *unit, const half8 (&hi)[2 * DB],
+                                           const half8 (&lo)[2 * DB], int lane) {
+  constexpr int CH = SA_CHUNK<DB>;
+  floatx16 top{}, low{};
+#pragma unroll
+  for (int f = 0; f < 2 * DB; ++f) {
+    const half8 xh = frag(unit + f * 1024, lane), xl = frag(unit + CH / 2 + f * 1024, lane);
+    low = mma(xl, hi[f], low);
+    top = mma(xh, hi[f], top);
+    low = mma(xh, lo[f], low);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    top[r] += low[r];
+  return top;
+}
+
+// The lane's 16 results of a unit as operand: two groups of 16 items.
+__device__ __forceinline__ void split16(const floatx16 &x, half8 (&hi)[2], half8 (&lo)[2]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = x[8 * k + j];
+    split8(v, hi[k], lo[k]);
+  }
+}
+
+// A power of two that takes the 32 items' largest magnitude in this lane's column
+// (both halves') below 2^15, and its inverse.
+__device__ __forceinline__ float column_factor(const floatx16 &x, float &inverse) {
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    most = fmaxf(most, fabsf(x[r]));
+  most = fmaxf(most, __shfl_xor(most, 32));
+  const int e = int(__float_as_uint(most) >> 23);
+  const int up = min(268 - e, 253);
+  inverse = __uint_as_float(uint32_t(254 - up) << 23);
+  return __uint_as_float(uint32_t(up) << 23);
+}
+
+// acc = acc + k (items' col form (a unit) . x) for one block of 32 columns.
+template <int DB>
+__device__ __forceinline__ void sums32(floatx16 &acc, const char *unit, int db,
+                                       const half8 (&hi)[2], const half8 (&lo)[2], float k,
+                                       int lane) {
+  constexpr int CH = SA_CHUNK<DB>;
+  floatx16 t{};
+  half8 xh[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    xh[i] = frag(unit + (2 * db + i) * 1024, lane);
+    t = mma(frag(unit + CH / 2 + (2 * db + i) * 1024, lane), hi[i], t);
+    t = mma(xh[i], lo[i], t);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    t = mma(xh[i], hi[i], t);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    acc[r] = fmaf(t[r], k, acc[r]);
+}
+
+// Stores a lane's own row of 32 DB columns, times k.
+template <int DB>
+__device__ __forceinline__ void store_row(float *p, const floatx16 (&acc)[DB], float k, int D,
+                                          int h) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * db + 8 * q + 4 * h;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = acc[db][4 * q + j] * k;
+      if (d + 4 <= D)
+        RowVec<float>::store(p + d, RowVec<float>::V{v[0], v[1], v[2], v[3]});
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d + j < D)
+            p[d + j] = v[j];
+    }
+}
+
+// ---------------------------------------------------------------- forward
+
+constexpr int SF_WAVES = 8, SF_ROWS = SF_WAVES * SA_UNIT;
+
+struct SplitFwd {
+  AttnShape s;
+  Rows<const float> q;
+  const char *k, *v;             // row form, col form
+  const float *k_scale, *v_scale;
+  int tiles;                     // of 64 keys
+  float *y, *lse;
+  float scale2;
+  int vec;
+  AttnGate gate;
+};
+
+template <int DB>
+__global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const SplitFwd a) {
+  constexpr int CH = SA_CHUNK<DB>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][4 * CH];
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tiles = uint32_t(s.rows + SF_ROWS - 1) / SF_ROWS;
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
+  const int tile = int(tiles - 1 - (t - bh * tiles)); // the most keys first
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, threadIdx.x == 0, keys, first);
+  if (gate_set(a.gate, bh))
+    return;
+  auto limit_of = [&](int row) {
+    return seen(s, keys, first, int(s.by_group.div(uint32_t(row))));
+  };
+  const int row0 = tile * SF_ROWS + wave * SA_UNIT, row = row0 + n;
+  const bool live = row < s.rows;
+  const int limit = live ? limit_of(row) : 0;
+  const int end = row0 < s.rows ? limit_of(min(row0 + SA_UNIT, s.rows) - 1) : 0; // of any row
+  const int all = row0 < s.rows ? limit_of(row0) : 0;                           // of every row
+  const int group_end = limit_of(min((tile + 1) * SF_ROWS, s.rows) - 1);
+  const char *kp = a.k + int64_t(bh) * a.tiles * 2 * CH, *vp = a.v + int64_t(bh) * a.tiles * 2 * CH;
+  auto issue = [&](char *stage, int it) {
+#pragma unroll
+    for (int j = 0; j < 2 * DB; ++j) {
+      const int p = j < DB ? j * 8 + wave : (j - DB) * 8 + wave;
+      load_lds((j < DB ? kp : vp) + int64_t(it) * 2 * CH + p * 1024,
+               stage + (j < DB ? 0 : 2 * CH) + p * 1024, lane);
+    }
+  };
+  const int steps = (group_end + SA_TILE - 1) / SA_TILE;
+  if (steps)
+    issue(lds[0], 0);
+  // own row: one power of two, and the sign of the scale
+  half8 qh[2 * DB], ql[2 * DB];
+  float q_scale;
+  {
+    const uint32_t i = s.by_group.div(uint32_t(row));
+    const float *qp = a.q.p + b * a.q.sB + hk * a.q.sHead;
+    if (live)
+      qp += int64_t(i) * a.q.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * a.q.sInner;
+    float v[2 * DB][8];
+    float most = 0.f;
+#pragma unroll
+    for (int f = 0; f < 2 * DB; ++f)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const auto x = piece(qp, 16 * f + 8 * h + 4 * u, s.D, live, a.vec);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[f][4 * u + j] = x[j];
+          most = fmaxf(most, fabsf(x[j]));
+        }
+      }
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int up = up_exponent(most < SA_INF ? most : 0.f);
+    const float k = a.scale2 > 0.f ? pow2(up) : a.scale2 < 0.f ? -pow2(up) : 0.f;
+    q_scale = pow2(-up);
+#pragma unroll
+    for (int f = 0; f < 2 * DB; ++f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[f][j] *= k;
+      split8(v[f], qh[f], ql[f]);
+    }
+  }
+  const float c = fabsf(a.scale2);
+  floatx16 acc[DB]{};
+  float m = -SA_INF, l = 0.f;
+  for (int it = 0; it < steps; ++it) {
+    stage_ready();
+    if (it + 1 < steps)
+      issue(lds[(it + 1) & 1], it + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (it * SA_TILE >= end)
+      continue;
+    const char *st = lds[it & 1];
+    // positive and finite, so that it takes -inf to -inf
+    const float cz = fminf(fmaxf(c * q_scale * a.k_scale[int64_t(bh) * a.tiles + it], 1.2e-38f),
+                           3.4e38f);
+    const float v_scale = a.v_scale[int64_t(bh) * a.tiles + it];
+    floatx16 z[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      z[u] = dots32<DB>(st + u * CH, qh, ql, lane);
+    if (it * SA_TILE + SA_TILE > all)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          z[u][r] = it * SA_TILE + u * SA_UNIT + row32(h, r) < limit ? z[u][r] : -SA_INF;
+    float top = -SA_INF;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        top = fmaxf(top, z[u][r]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float next = fmaxf(m, top * cz), base = next == -SA_INF ? 0.f : next;
+    const float shrink = __builtin_amdgcn_exp2f(m - base);
+    m = next;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        // times 2^14, which the quotient by l takes out again
+        z[u][r] = __builtin_amdgcn_exp2f(fmaf(z[u][r], cz, 14.f - base));
+        sum += z[u][r];
+      }
+    l = fmaf(l, shrink, sum);
+    half8 ph[2][2], pl[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      split16(z[u], ph[u], pl[u]);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      floatx16 o{};
+      half8 vh[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const char *p = st + (2 + i / 2) * CH + (2 * db + i % 2) * 1024;
+        vh[i] = frag(p, lane);
+        o = mma(frag(p + CH / 2, lane), ph[i / 2][i % 2], o);
+        o = mma(vh[i], pl[i / 2][i % 2], o);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o = mma(vh[i], ph[i / 2][i % 2], o);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        acc[db][r] = fmaf(o[r], v_scale, acc[db][r] * shrink);
+    }
+  }
+  if (!live)
+    return;
+  l += __shfl_xor(l, 32);
+  const uint32_t i = s.by_group.div(uint32_t(row));
+  const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
+  store_row<DB>(a.y + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D, acc,
+                limit > 0 ? 1.f / l : 0.f, s.D, h);
+  if (a.lse && h == 0)
+    a.lse[int64_t(bh) * s.rows + row] = m == -SA_INF ? 0.f : m + (log2f(l) - 14.f);
+}
+
+// --------------------------------------------------------------- backward
+
+constexpr int SB_WAVES = 4, SB_ROWS = SB_WAVES * SA_UNIT;
+
+struct SplitBwd {
+  AttnShape s;
+  const char *q_row, *q_col, *g_row, *g_col, *k_row, *k_col, *v_row;
+  const float *q_scale, *k_scale, *v_scale; // [bh, tiles]
+  const float *stats;                       // [bh, units][SA_STATS]
+  int q_tiles, k_tiles;                     // of 64 rows
+  float *dq, *dk, *dv;                      // dk, dv: [parts] of the result's size
+  int parts;
+  float scale, scale2;
+  AttnGate gate;
+};
+
+template <int DB>
+__device__ __forceinline__ void load_own(const char *unit, half8 (&hi)[2 * DB],
+                                         half8 (&lo)[2 * DB], int lane) {
+#pragma unroll
+  for (int f = 0; f < 2 * DB; ++f) {
+    hi[f] = frag(unit + f * 1024, lane);
+    lo[f] = frag(unit + SA_CHUNK<DB> / 2 + f * 1024, lane);
+  }
+}
+
+template <int DB>
+__global__ __launch_bounds__(64 * SB_WAVES, (DB <= 2 ? 2 : 1)) void attn_split_dq_kernel(
+    const SplitBwd a) {
+  constexpr int CH = SA_CHUNK<DB>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][3 * CH];
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tiles = uint32_t(s.rows + SB_ROWS - 1) / SB_ROWS;
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
+  const int tile = int(tiles - 1 - (t - bh * tiles));
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, false, keys, first);
+  if (gate_set(a.gate, bh))
+    return;
+  auto limit_of = [&](int row) {
+    return seen(s, keys, first, int(s.by_group.div(uint32_t(row))));
+  };
+  const int row0 = tile * SB_ROWS + wave * SA_UNIT, row = row0 + n;
+  const bool on = row0 < s.rows; // of the wave
+  const int end = on ? limit_of(min(row0 + SA_UNIT, s.rows) - 1) : 0;
+  const int all = on ? limit_of(row0) : 0;
+  const int group_end = limit_of(min((tile + 1) * SB_ROWS, s.rows) - 1);
+  const int64_t kv = int64_t(bh) * a.k_tiles * 2 * CH;
+  auto issue = [&](char *stage, int it) {
+#pragma unroll
+    for (int j = 0; j < 3 * DB; ++j) {
+      const int p = (j % DB) * 4 + wave;
+      const char *from = j < DB ? a.k_row : j < 2 * DB ? a.v_row : a.k_col;
+      load_lds(from + kv + int64_t(it) * CH + p * 1024, stage + j / DB * CH + p * 1024, lane);
+    }
+  };
+  const int steps = (group_end + SA_UNIT - 1) / SA_UNIT;
+  if (steps)
+    issue(lds[0], 0);
+  half8 qh[2 * DB], ql[2 * DB], gh[2 * DB], gl[2 * DB];
+  const int64_t unit = int64_t(bh) * a.q_tiles * 2 + (on ? row0 / SA_UNIT : 0);
+  load_own<DB>(a.q_row + unit * CH, qh, ql, lane);
+  load_own<DB>(a.g_row + unit * CH, gh, gl, lane);
+  const float *st = a.stats + unit * SA_STATS + n;
+  const float lse = st[0], delta = st[SA_UNIT], g_scale = st[2 * SA_UNIT];
+  const int limit = reinterpret_cast<const int *>(st)[3 * SA_UNIT];
+  const float c = a.scale2 * a.q_scale[unit / 2];
+  floatx16 acc[DB]{};
+  for (int it = 0; it < steps; ++it) {
+    stage_ready();
+    if (it + 1 < steps)
+      issue(lds[(it + 1) & 1], it + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (it * SA_UNIT >= end)
+      continue;
+    const char *stage = lds[it & 1];
+    const float k_scale = a.k_scale[int64_t(bh) * a.k_tiles + it / 2];
+    const float v_scale = a.v_scale[int64_t(bh) * a.k_tiles + it / 2];
+    const floatx16 z = dots32<DB>(stage, qh, ql, lane);
+    floatx16 ds = dots32<DB>(stage + CH, gh, gl, lane);
+    const float cz = c * k_scale;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(z[r], cz, -lse));
+      ds[r] = p * fmaf(ds[r], v_scale, -delta);
+    }
+    if (it * SA_UNIT + SA_UNIT > all)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ds[r] = it * SA_UNIT + row32(h, r) < limit ? ds[r] : 0.f;
+    float inverse;
+    const float k = column_factor(ds, inverse);
+    ds *= k;
+    half8 hi[2], lo[2];
+    split16(ds, hi, lo);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      sums32<DB>(acc[db], stage + 2 * CH, db, hi, lo, inverse * k_scale, lane);
+  }
+  if (row >= s.rows)
+    return;
+  const uint32_t i = s.by_group.div(uint32_t(row));
+  const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
+  store_row<DB>(a.dq + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D, acc,
+                a.scale * g_scale, s.D, h);
+}
+
+template <int DB>
+__global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_dkv_kernel(
+    const SplitBwd a) {
+  constexpr int CH = SA_CHUNK<DB>, STAT = SA_STATS * 4;
+  __shared__ __attribute__((aligned(1024))) char lds[2][4 * CH + STAT];
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tiles = uint32_t(s.Tk + SB_ROWS - 1) / SB_ROWS;
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x);
+  const uint32_t bh = t / (tiles * uint32_t(a.parts)), u = t - bh * tiles * uint32_t(a.parts);
+  const int tile = int(u / uint32_t(a.parts)), part = int(u % uint32_t(a.parts));
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, false, keys, first);
+  if (gate_set(a.gate, bh))
+    return;
+  auto limit_of = [&](int row) {
+    return seen(s, keys, first, int(s.by_group.div(uint32_t(row))));
+  };
+  const int key0 = tile * SB_ROWS, own0 = key0 + wave * SA_UNIT, key = own0 + n;
+  // units from the first query that sees any of these keys on, this part of them
+  const int units = (s.rows + SA_UNIT - 1) / SA_UNIT;
+  int from = 0;
+  if (key0 >= keys)
+    from = units;
+  else if (s.causal && key0 > first)
+    from = int(min(int64_t(key0 - first) * s.G / SA_UNIT, int64_t(units)));
+  const int per = (units - from + a.parts - 1) / a.parts;
+  const int u0 = min(from + part * per, units), u1 = min(u0 + per, units);
+  const int64_t base = int64_t(bh) * a.q_tiles * 2;
+  auto issue = [&](char *stage, int it) {
+    const int64_t at = (base + it) * CH;
+#pragma unroll
+    for (int j = 0; j < 4 * DB; ++j) {
+      const int p = (j % DB) * 4 + wave;
+      const char *x = j < DB ? a.q_row : j < 2 * DB ? a.q_col : j < 3 * DB ? a.g_row : a.g_col;
+      load_lds(x + at + p * 1024, stage + j / DB * CH + p * 1024, lane);
+    }
+    if (wave < 2) // the rows' statistics, 4 bytes a lane
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(a.stats + (base + it) * SA_STATS +
+                                                           wave * 64 + lane),
+          (__attribute__((address_space(3))) void *)(stage + 4 * CH + wave * 256), 4, 0, 0);
+  };
+  if (u0 < u1)
+    issue(lds[0], u0);
+  half8 kh[2 * DB], kl[2 * DB], vh[2 * DB], vl[2 * DB];
+  const bool on = own0 < keys;
+  const int64_t unit = int64_t(bh) * a.k_tiles * 2 + (on ? own0 / SA_UNIT : 0);
+  load_own<DB>(a.k_row + unit * CH, kh, kl, lane);
+  load_own<DB>(a.v_row + unit * CH, vh, vl, lane);
+  const float v_scale = a.v_scale[unit / 2], c = a.scale2 * a.k_scale[unit / 2];
+  floatx16 dk[DB]{}, dv[DB]{};
+  for (int it = u0; it < u1; ++it) {
+    const int buf = (it - u0) & 1;
+    stage_ready();
+    if (it + 1 < u1)
+      issue(lds[buf ^ 1], it + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const int r0 = it * SA_UNIT;
+    if (!on || limit_of(min(r0 + SA_UNIT, s.rows) - 1) <= own0)
+      continue;
+    const char *stage = lds[buf];
+    const float *st = reinterpret_cast<const float *>(stage + 4 * CH);
+    const float q_scale = a.q_scale[int64_t(bh) * a.q_tiles + it / 2], cz = c * q_scale;
+    floatx16 w = dots32<DB>(stage, kh, kl, lane);
+    floatx16 ds = dots32<DB>(stage + 2 * CH, vh, vl, lane);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 lse = *reinterpret_cast<const float4 *>(st + 8 * q + 4 * h);
+      const float4 delta = *reinterpret_cast<const float4 *>(st + SA_UNIT + 8 * q + 4 * h);
+      const float4 g = *reinterpret_cast<const float4 *>(st + 2 * SA_UNIT + 8 * q + 4 * h);
+      const float ls[4] = {lse.x, lse.y, lse.z, lse.w};
+      const float de[4] = {delta.x, delta.y, delta.z, delta.w};
+      const float gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * q + j;
+        // p times the row's scale: what multiplies its packed gradient
+        w[r] = __builtin_amdgcn_exp2f(fmaf(w[r], cz, -ls[j])) * gs[j];
+        ds[r] = w[r] * fmaf(ds[r], v_scale, -de[j]);
+      }
+    }
+    if (limit_of(r0) < own0 + SA_UNIT)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int4 limit =
+            *reinterpret_cast<const int4 *>(st + 3 * SA_UNIT + 8 * q + 4 * h);
+        const int li[4] = {limit.x, limit.y, limit.z, limit.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[4 * q + j] = key < li[j] ? w[4 * q + j] : 0.f;
+          ds[4 * q + j] = key < li[j] ? ds[4 * q + j] : 0.f;
+        }
+      }
+    half8 hi[2], lo[2];
+    float inverse;
+    {
+      const float k = column_factor(w, inverse);
+      w *= k;
+      split16(w, hi, lo);
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      sums32<DB>(dv[db], stage + 3 * CH, db, hi, lo, inverse, lane);
+    {
+      const float k = column_factor(ds, inverse);
+      ds *= k;
+      split16(ds, hi, lo);
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      sums32<DB>(dk[db], stage + CH, db, hi, lo, inverse * q_scale, lane);
+  }
+  if (key >= s.Tk)
+    return;
+  const int64_t size = int64_t(s.B) * s.Tk * s.Hk * s.D;
+  const int64_t at = part * size + ((int64_t(b) * s.Tk + key) * s.Hk + hk) * s.D;
+  if (a.dk)
+    store_row<DB>(a.dk + at, dk, a.scale, s.D, h);
+  if (a.dv)
+    store_row<DB>(a.dv + at, dv, 1.f, s.D, h);
+}
+
+// The parts of dk and dv added up in order.  What the gate left to other kernels
+// is not written.
+__global__ __launch_bounds__(256) void attn_split_parts_kernel(const SplitBwd a, float *dk,
+                                                               float *dv) {
+  const AttnShape &s = a.s;
+  const int64_t size = int64_t(s.B) * s.Tk * s.Hk * s.D;
+  const uint32_t bh = blockIdx.y;
+  if (gate_set(a.gate, bh))
+    return;
+  const int64_t b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t key = i / s.D;
+  if (key >= s.Tk)
+    return;
+  const int64_t at = ((b * s.Tk + key) * s.Hk + hk) * s.D + i % s.D;
+  float x = 0.f, y = 0.f;
+  for (int p = 0; p < a.parts; ++p) {
+    if (dk)
+      x += a.dk[p * size + at];
+    if (dv)
+      y += a.dv[p * size + at];
+  }
+  if (dk)
+    dk[at] = x;
+  if (dv)
+    dv[at] = y;
+}
+
+// ------------------------------------------------------------------- host
+
+namespace {
+
+int tiles_of(int rows) { return (rows + SA_TILE - 1) / SA_TILE; }
+
+template <class F> void dispatch_blocks(int D, F &&f) {
+  switch ((D + 31) / 32) {
+  case 1:
+    return f.template operator()<1>();
+  case 2:
+    return f.template operator()<2>();
+  case 3:
+    return f.template operator()<3>();
+  default:
+    return f.template operator()<4>();
+  }
+}
+
+} // namespace
+
+// Float32 with heads of up to 128 elements (a wider one's planes outgrow the
+// registers), from the size on at which packing and half-empty tiles cost less than
+// the matrix cores save.
+bool split_takes(const AttnShape &s) {
+  if (s.D > 128 || s.rows < 64 || s.Tk < 64)
+    return false;
+  const double pairs = double(s.B) * s.Hk * s.rows * s.Tk * s.D;
+  return pairs >= double(1 << 24);
+}
+
+size_t split_gate_words(const AttnShape &s, bool backward) {
+  const size_t k = size_t(tiles_of(s.Tk)), q = size_t(tiles_of(s.rows));
+  return size_t(s.B) * size_t(s.Hk) * (2 * k + (backward ? 2 * q : 0));
+}
+
+void run_split(AttnFwd<float> &a, uint32_t *words) {
+  const AttnShape &s = a.s;
+  const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
+  const int tiles = tiles_of(s.Tk);
+  a.gate = {words, 2 * tiles};
+  dispatch_blocks(s.D, [&]<int DB>() {
+    const size_t form = size_t(bhs) * size_t(tiles) * 2 * SA_CHUNK<DB>;
+    DeviceScratch planes(2 * form + 2 * size_t(bhs) * size_t(tiles) * sizeof(float));
+    char *k = planes.get<char>(), *v = k + form;
+    float *k_scale = reinterpret_cast<float *>(v + form), *v_scale = k_scale + bhs * size_t(tiles);
+    PackArgs p{};
+    p.s = s;
+    p.count = 2;
+    p.vec = a.vec;
+    p.words = words;
+    p.per = a.gate.per;
+    p.t[0] = {a.k, k, nullptr, k_scale, s.Tk, tiles, 1, bhs * uint32_t(tiles), 0};
+    p.t[1] = {a.v, nullptr, v, v_scale, s.Tk, tiles, 1, 2 * bhs * uint32_t(tiles), tiles};
+    attn_pack_kernel<DB><<<dim3(p.t[1].blocks), 256, 0, stream()>>>(p);
+    NT_LAUNCH_CHECK();
+    SplitFwd f{};
+    f.s = s;
+    f.q = a.q;
+    f.k = k, f.v = v;
+    f.k_scale = k_scale, f.v_scale = v_scale;
+    f.tiles = tiles;
+    f.y = a.y, f.lse = a.lse;
+    f.scale2 = a.scale2;
+    f.vec = a.vec;
+    f.gate = a.gate;
+    attn_split_fwd_kernel<DB><<<dim3(bhs * uint32_t((s.rows + SF_ROWS - 1) / SF_ROWS)),
+                                64 * SF_WAVES, 0, stream()>>>(f);
+    NT_LAUNCH_CHECK();
+  });
+}
+
+void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
+  const AttnShape &s = a.s;
+  const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
+  const int kt = tiles_of(s.Tk), qt = tiles_of(s.rows);
+  a.gate = {words, 2 * kt + 2 * qt};
+  dispatch_blocks(s.D, [&]<int DB>() {
+    const size_t kform = size_t(bhs) * size_t(kt) * 2 * SA_CHUNK<DB>;
+    const size_t qform = size_t(bhs) * size_t(qt) * 2 * SA_CHUNK<DB>;
+    const size_t rows = size_t(bhs) * size_t(qt) * 2 * SA_STATS;
+    DeviceScratch planes(3 * kform + 4 * qform);
+    DeviceScratch scales((size_t(bhs) * size_t(2 * kt + qt) + rows) * sizeof(float));
+    SplitBwd f{};
+    f.s = s;
+    char *at = planes.get<char>();
+    auto take = [&](size_t n) { return (at += n) - n; };
+    char *q_row = take(qform), *q_col = take(qform), *g_row = take(qform), *g_col = take(qform);
+    char *k_row = take(kform), *k_col = take(kform), *v_row = take(kform);
+    float *stats = scales.get<float>(), *k_scale = stats + rows;
+    float *v_scale = k_scale + size_t(bhs) * size_t(kt), *q_scale = v_scale + size_t(bhs) * size_t(kt);
+    PackArgs p{};
+    p.s = s;
+    p.count = 4;
+    p.vec = a.vec;
+    p.words = words;
+    p.per = a.gate.per;
+    p.y = y;
+    p.lse = a.lse;
+    p.stats = stats;
+    p.delta = const_cast<float *>(a.delta);
+    const uint32_t kb = bhs * uint32_t(kt), qb = bhs * uint32_t(qt);
+    p.t[0] = {a.k, k_row, k_col, k_scale, s.Tk, kt, 1, kb, 0};
+    p.t[1] = {a.v, v_row, nullptr, v_scale, s.Tk, kt, 1, 2 * kb, kt};
+    p.t[2] = {a.q, q_row, q_col, q_scale, s.rows, qt, 0, 2 * kb + qb, 2 * kt};
+    p.t[3] = {a.g, g_row, g_col, nullptr, s.rows, qt, 0, 2 * kb + 2 * qb, 2 * kt + qt};
+    attn_pack_kernel<DB><<<dim3(p.t[3].blocks), 256, 0, stream()>>>(p);
+    NT_LAUNCH_CHECK();
+    f.q_row = q_row, f.q_col = q_col, f.g_row = g_row, f.g_col = g_col;
+    f.k_row = k_row, f.k_col = k_col, f.v_row = v_row;
+    f.q_scale = q_scale, f.k_scale = k_scale, f.v_scale = v_scale;
+    f.stats = stats;
+    f.q_tiles = qt, f.k_tiles = kt;
+    f.scale = a.scale, f.scale2 = a.scale2;
+    f.gate = a.gate;
+    f.parts = 1;
+    if (a.dq) {
+      f.dq = a.dq;
+      attn_split_dq_kernel<DB><<<dim3(bhs * uint32_t((s.rows + SB_ROWS - 1) / SB_ROWS)),
+                                 64 * SB_WAVES, 0, stream()>>>(f);
+      NT_LAUNCH_CHECK();
+    }
+    if (a.dk || a.dv) {
+      // Workgroups of different lengths, one to two at a time on a CU: four for
+      // each CU even them out.  Fewer key tiles than that share their rows.
+      const int64_t groups = int64_t(bhs) * ((s.Tk + SB_ROWS - 1) / SB_ROWS);
+      const int units = (s.rows + SA_UNIT - 1) / SA_UNIT;
+      f.parts = int(std::max<int64_t>(
+          1, std::min<int64_t>({int64_t(device_cu_count()) * 4 / groups, units / 8, 16})));
+      const size_t size = size_t(s.B) * size_t(s.Tk) * size_t(s.Hk) * size_t(s.D);
+      DeviceScratch sums(f.parts > 1 ? 2 * size * size_t(f.parts) * sizeof(float) : 0);
+      f.dk = a.dk && f.parts > 1 ? sums.get<float>() : a.dk;
+      f.dv = a.dv && f.parts > 1 ? sums.get<float>() + size * size_t(f.parts) : a.dv;
+      attn_split_dkv_kernel<DB>
+          <<<dim3(uint32_t(groups * f.parts)), 64 * SB_WAVES, 0, stream()>>>(f);
+      NT_LAUNCH_CHECK();
+      if (f.parts > 1) {
+        const int64_t each = int64_t(s.Tk) * s.D;
+        attn_split_parts_kernel<<<dim3(uint32_t((each + 255) / 256), bhs), 256, 0, stream()>>>(
+            f, a.dk, a.dv);
+        NT_LAUNCH_CHECK();
+      }
+    }
+  });
+}
+
+} // namespace nt

@@ -149,6 +149,78 @@ def test_attention(gpu, shape, causal, dtype):
     check_all(q, k, v, g, visible(B, Tq, Tk, causal), dtype, causal=causal)
 
 
+LARGE = [  # as many products as the half-precision planes are used for
+    (1, 520, 520, 4, 2, 64), (2, 300, 470, 6, 3, 128), (1, 1000, 997, 2, 2, 33),
+    (3, 257, 640, 3, 1, 80), (1, 64, 2049, 8, 2, 32), (1, 1300, 130, 2, 1, 96),
+    (2, 777, 777, 1, 1, 100),
+]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", LARGE)
+def test_large(gpu, shape, causal):
+    B, Tq, Tk, H, Hk, D = shape
+    r = rng(seed_of("large", shape, causal))
+    q, k, v, g = inputs(r, *shape, np.float32, sharp=2.0)
+    check_all(q, k, v, g, visible(B, Tq, Tk, causal), np.float32, causal=causal)
+
+
+@pytest.mark.parametrize("causal,starts", [(False, None), (True, None), (True, 0),
+                                           (True, [5, -700, 300, 64, 0])])
+def test_large_lengths_and_starts(gpu, causal, starts):
+    B, Tq, Tk, H, Hk, D = 5, 330, 350, 2, 2, 64
+    lengths = np.array([350, 0, 1, 193, 320])
+    r = rng(seed_of("large len", causal, str(starts)))
+    q, k, v, g = inputs(r, B, Tq, Tk, H, Hk, D, np.float32)
+    for b, n in enumerate(lengths):
+        k[b, n:] = np.nan
+        v[b, n:] = np.inf
+    see = visible(B, Tq, Tk, causal, lengths, starts)
+    given = dev(np.array(starts)) if isinstance(starts, list) else starts
+    check_all(q, k, v, g, see, np.float32, causal=causal, lengths=dev(lengths), starts=given)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e15])
+@pytest.mark.parametrize("what", ["v", "g", "qk"])
+def test_large_of_any_magnitude(gpu, what, size):
+    """Values far from 1, and rows of gradients of very different sizes: nothing
+    is lost to the range of half precision."""
+    r = rng(seed_of("magnitude", what, size))
+    q, k, v, g = inputs(r, 1, 420, 420, 2, 1, 64, np.float32)
+    if what == "v":
+        v *= np.float32(size)
+    elif what == "g":
+        g *= np.float32(size)
+        g *= (10.0 ** r.uniform(-6, 6, (1, 420, 1, 1))).astype(np.float32)
+        g[0, ::7] = 0
+    else:
+        q *= np.float32(size)
+        k /= np.float32(size)
+    check_all(q, k, v, g, visible(1, 420, 420, True), np.float32, causal=True)
+
+
+@pytest.mark.parametrize("what", ["k", "v", "q"])
+def test_large_with_an_outlier(gpu, what):
+    """One row 2^13 times and more above its neighbours, where most rows do not
+    see it: the others keep their bits."""
+    r = rng(seed_of("outlier", what))
+    T = 420
+    q, k, v, g = inputs(r, 1, T, T, 2, 1, 64, np.float32)
+    see = visible(1, T, T, True)
+    clean = reference(q, k, v, g, see, 0.125, U[np.float32])
+    x = {"q": q, "k": k, "v": v}[what]
+    at = T - 20
+    x[0, at] *= np.float32(1e12)
+    y, (dq, dk, dv) = run(q, k, v, g, causal=True)
+    if what == "q":
+        keep = np.arange(T) != at
+        check(y[:, keep], [t[:, keep] for t in clean["y"]], "y")
+        check(dq[:, keep], [t[:, keep] for t in clean["dq"]], "dq")
+    else:
+        check(y[:, :at], [t[:, :at] for t in clean["y"]], "y")
+        check(dq[:, :at], [t[:, :at] for t in clean["dq"]], "dq")
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("wide", [np.int32, np.int64])
 @pytest.mark.parametrize("causal,starts", [(False, None), (True, None), (True, 0), (True, -3),
@@ -179,7 +251,7 @@ def test_lengths_and_starts(gpu, causal, starts, wide, dtype):
 
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("T,D", [(37, 24), (150, 64)])
+@pytest.mark.parametrize("T,D", [(37, 24), (150, 64), (460, 64)])
 def test_what_is_not_seen_does_not_matter(gpu, dtype, bad, T, D):
     """A key, value, query or gradient that is no number reaches the rows that
     see it and no other."""
