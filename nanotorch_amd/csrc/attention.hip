@@ -91,11 +91,59 @@ __device__ __forceinline__ typename Mma<T>::V4 dots(const Frag<T, DP> &items,
   return s;
 }
 
+// Own rows of up to 512 bytes stay in registers.  Longer ones are read again with
+// every tile of items, 256 bytes at a time, and a workgroup keeps only 512 bytes
+// of its sums' columns: several workgroups form the same probabilities, each for
+// columns of its own (in one kernel, wide float64 rows needed a thousand registers
+// a lane).
+template <class T, int DP> constexpr bool IN_REGISTERS = DP * sizeof(T) <= 512;
+template <class T, int DP>
+constexpr int COLUMNS = IN_REGISTERS<T, DP> ? DP : int(512 / sizeof(T));
+template <class T, int DP> constexpr int COLUMN_GROUPS = DP / COLUMNS<T, DP>;
+
+template <class T, int DP> struct Own {
+  Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> f;
+  const T *row;
+  bool live;
+  __device__ __forceinline__ void load(const T *p, int D, bool on, int vec, int h) {
+    row = p;
+    live = on;
+    if constexpr (IN_REGISTERS<T, DP>)
+      f.load(p, D, on, vec, h);
+  }
+  // With the lane's item row.
+  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, int D, bool on, int vec,
+                                                      int h) const {
+    if constexpr (IN_REGISTERS<T, DP>) {
+      Frag<T, DP> x;
+      x.load(item, D, on, vec, h);
+      return nt::dots<T, DP>(x, f);
+    } else {
+      constexpr int W = 256 / sizeof(T);
+      typename Mma<T>::V4 s{};
+#pragma unroll 1
+      for (int d = 0; d < D; d += W) {
+        Frag<T, W> x, o;
+        x.load(item + d, D - d, on, vec, h);
+        o.load(row + d, D - d, live, vec, h);
+        s += nt::dots<T, W>(x, o);
+      }
+      return s;
+    }
+  }
+};
+
 // Items' rows as operand of sums: of the four items row(h, r), pieces at
-// 16 N c + N n.  Result column 4 N c' .. of a lane: see Sums::column.
+// 16 N c + N n of a workgroup's columns.  Where a result's columns are: see
+// Sums::column.
 template <class T, int DP> struct Items {
   static constexpr int N = RowVec<T>::N, C = DP / (16 * N);
   typename RowVec<T>::V v[4][C];
+  __device__ __forceinline__ void load(int r, const T *p, int D, bool on, int vec, int n) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      v[r][c] = piece(p, N * (16 * c + n), D, on, vec);
+  }
 };
 
 template <class T, int DP> struct Sums {
@@ -212,21 +260,23 @@ template <class T, int DP> __device__ __forceinline__ bool all_finite(const Item
 
 // Tiles of 16 keys that a wave takes at a time: two, as long as their rows fit
 // its registers beside two waves to a SIMD.
-template <class T, int DP> constexpr int FWD_TILES = DP * sizeof(T) <= 512 ? 2 : 1;
-
-// Tile t of all, numbered (sequence, key head) by (sequence, key head).
 template <class T, int DP>
-__device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, uint32_t split) {
+constexpr int FWD_TILES = DP * sizeof(T) <= (sizeof(T) == 4 ? 512 : 256) ? 2 : 1;
+
+// Tile `item` of a (sequence, key head).
+template <class T, int DP>
+__device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, uint32_t item,
+                                              uint32_t split, int col0) {
   using M = Mma<T>;
+  constexpr int SC = COLUMNS<T, DP>;
   constexpr int TILES = FWD_TILES<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   __shared__ T stat[2][AT_WAVES][16];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
   const uint32_t tiles = uint32_t(s.rows + 15) / 16;
-  const uint32_t bh = t / tiles;
   // long rows first: under a causal mask the last tiles see the most keys
-  const int tile = int(tiles - 1 - (t - bh * tiles));
+  const int tile = int(tiles - 1 - item);
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, threadIdx.x == 0, keys, first);
@@ -241,9 +291,9 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, u
                 int64_t(qg) * a.q.sInner;
   const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
   const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
-  Frag<T, DP> q;
+  Own<T, DP> q;
   q.load(qp, s.D, live, a.vec, h);
-  Sums<T, DP> sums;
+  Sums<T, SC> sums;
   sums.clear();
   T m = NEG_INF<T>, l = 0;
   // this workgroup's blocks of keys, dealt to its waves
@@ -252,28 +302,21 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, u
   const int stop = std::min(blocks, int(split + 1) * per);
   for (int blk = int(split) * per + wave; blk < stop; blk += AT_WAVES) {
     const int j0 = blk * 16 * TILES;
-    Frag<T, DP> k[TILES];
-    Items<T, DP> v[TILES];
-#pragma unroll
-    for (int i = 0; i < TILES; ++i)
-      k[i].load(kp + int64_t(j0 + 16 * i + n) * a.k.sOuter, s.D, j0 + 16 * i + n < end, a.vec,
-                h);
+    Items<T, SC> v[TILES];
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = j0 + 16 * i + M::row(h, r);
-        const T *p = vp + int64_t(j) * a.v.sOuter;
-#pragma unroll
-        for (int c = 0; c < Items<T, DP>::C; ++c)
-          v[i].v[r][c] = piece(p, RowVec<T>::N * (16 * c + n), s.D, j < end, a.vec);
+        v[i].load(r, vp + int64_t(j) * a.v.sOuter + col0, s.D - col0, j < end, a.vec, n);
       }
     T z[TILES][4];
     bool vis[TILES][4];
     T top = NEG_INF<T>;
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
-      const auto d = dots<T, DP>(k[i], q);
+      const int j = j0 + 16 * i + n;
+      const auto d = q.dots(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         vis[i][r] = j0 + 16 * i + M::row(h, r) < limit;
@@ -303,9 +346,9 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, u
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i;
-      if (j + 16 > all && !all_finite<T, DP>(v[i]))
-        sums.add_visible(z[i], vis[i], s.D, lane, [&](int item) {
-          return j + item < end ? vp + int64_t(j + item) * a.v.sOuter : nullptr;
+      if (j + 16 > all && !all_finite<T, SC>(v[i]))
+        sums.add_visible(z[i], vis[i], s.D - col0, lane, [&](int item) {
+          return j + item < end ? vp + int64_t(j + item) * a.v.sOuter + col0 : nullptr;
         });
       else
         sums.add(z[i], v[i]);
@@ -329,22 +372,24 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, u
     total += stat[1][w][n] * M::exp2(stat[0][w][n] - base);
   const T mine = M::exp2(m - base);
   if (a.splits > 1) {
-    const int64_t slot = int64_t(t) * a.splits + split;
-    if (wave == 0 && h == 0) {
+    const int64_t slot = (int64_t(bh) * tiles + item) * a.splits + split;
+    if (wave == 0 && h == 0 && col0 == 0) {
       a.part_stat[slot * 32 + n] = top;
       a.part_stat[slot * 32 + 16 + n] = total;
     }
-    join_waves<T, DP>(sums, mine, lds, [&](int r, int d, T v) {
+    join_waves<T, SC>(sums, mine, lds, [&](int r, int d, T v) {
+      d += col0;
       if (d < s.D && tile * 16 + r < s.rows)
         a.part_acc[(slot * 16 + r) * s.D + d] = v;
     });
     return;
   }
-  if (a.lse && wave == 0 && h == 0 && live)
+  if (a.lse && wave == 0 && h == 0 && live && col0 == 0)
     a.lse[int64_t(bh) * s.rows + row] = top == NEG_INF<T> ? T(0) : top + M::log2(total);
   const T factor = limit > 0 ? mine / total : T(0);
-  join_waves<T, DP>(sums, factor, lds, [&](int r, int d, T v) {
+  join_waves<T, SC>(sums, factor, lds, [&](int r, int d, T v) {
     const int w = tile * 16 + r;
+    d += col0;
     if (d >= s.D || w >= s.rows)
       return;
     const uint32_t i = s.by_group.div(uint32_t(w));
@@ -356,8 +401,15 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t t, u
 template <class T, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_kernel(
     const AttnFwd<T> a) {
-  const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
-  attn_fwd_tile<T, DP>(a, id / uint32_t(a.splits), id % uint32_t(a.splits));
+  constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
+  const uint32_t splits = uint32_t(a.splits);
+  uint32_t bh, item;
+  head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk),
+            uint32_t(a.s.rows + 15) / 16 * splits * GROUPS, bh, item);
+  const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
+  item /= GROUPS;
+  if (col0 < a.s.D)
+    attn_fwd_tile<T, DP>(a, bh, item / splits, item % splits, col0);
 }
 
 // What the kernels on half-precision planes left: the tiles of each (sequence,
@@ -371,7 +423,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<float, DP>)) void attn_fw
   const uint32_t tiles = uint32_t(a.s.rows + 15) / 16;
   for (uint32_t t = blockIdx.x % groups; t < tiles; t += groups) {
     __syncthreads();
-    attn_fwd_tile<float, DP>(a, bh * tiles + t, 0);
+    attn_fwd_tile<float, DP>(a, bh, t, 0, 0);
   }
 }
 
@@ -437,14 +489,15 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const AttnShape s, cons
 }
 
 template <class T, int DP>
-__device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t t) {
+__device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
+                                             int col0) {
   using M = Mma<T>;
+  constexpr int SC = COLUMNS<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
   const uint32_t tiles = uint32_t(s.rows + 15) / 16;
-  const uint32_t bh = t / tiles;
-  const int tile = int(tiles - 1 - (t - bh * tiles));
+  const int tile = int(tiles - 1 - item);
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, false, keys, first);
@@ -457,7 +510,7 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t t) {
   const int all = seen(s, keys, first, int(s.by_group.div(uint32_t(tile * 16))));
   const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
   const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
-  Frag<T, DP> q, g;
+  Own<T, DP> q, g;
   q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
              int64_t(qg) * a.q.sInner,
          s.D, live, a.vec, h);
@@ -466,22 +519,18 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t t) {
          s.D, live, a.vec, h);
   const T lse = live ? a.lse[int64_t(bh) * s.rows + row] : T(0);
   const T delta = live ? a.delta[int64_t(bh) * s.rows + row] : T(0);
-  Sums<T, DP> sums;
+  Sums<T, SC> sums;
   sums.clear();
   for (int j0 = wave * 16; j0 < end; j0 += 16 * AT_WAVES) {
-    Frag<T, DP> k, v;
-    Items<T, DP> x;
-    k.load(kp + int64_t(j0 + n) * a.k.sOuter, s.D, j0 + n < end, a.vec, h);
-    v.load(vp + int64_t(j0 + n) * a.v.sOuter, s.D, j0 + n < end, a.vec, h);
+    Items<T, SC> x;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = j0 + M::row(h, r);
-      const T *p = kp + int64_t(j) * a.k.sOuter;
-#pragma unroll
-      for (int c = 0; c < Items<T, DP>::C; ++c)
-        x.v[r][c] = piece(p, RowVec<T>::N * (16 * c + n), s.D, j < end, a.vec);
+      x.load(r, kp + int64_t(j) * a.k.sOuter + col0, s.D - col0, j < end, a.vec, n);
     }
-    const auto z = dots<T, DP>(k, q), dp = dots<T, DP>(v, g);
+    const int j = j0 + n;
+    const auto z = q.dots(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
+    const auto dp = g.dots(vp + int64_t(j) * a.v.sOuter, s.D, j < end, a.vec, h);
     T ds[4];
     bool vis[4];
 #pragma unroll
@@ -489,15 +538,16 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t t) {
       vis[r] = j0 + M::row(h, r) < limit;
       ds[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse) * (dp[r] - delta) : T(0);
     }
-    if (j0 + 16 > all && !all_finite<T, DP>(x))
-      sums.add_visible(ds, vis, s.D, lane, [&](int item) {
-        return j0 + item < end ? kp + int64_t(j0 + item) * a.k.sOuter : nullptr;
+    if (j0 + 16 > all && !all_finite<T, SC>(x))
+      sums.add_visible(ds, vis, s.D - col0, lane, [&](int item) {
+        return j0 + item < end ? kp + int64_t(j0 + item) * a.k.sOuter + col0 : nullptr;
       });
     else
       sums.add(ds, x);
   }
-  join_waves<T, DP>(sums, a.scale, lds, [&](int r, int d, T v) {
+  join_waves<T, SC>(sums, a.scale, lds, [&](int r, int d, T v) {
     const int w = tile * 16 + r;
+    d += col0;
     if (d >= s.D || w >= s.rows)
       return;
     const uint32_t i = s.by_group.div(uint32_t(w));
@@ -507,14 +557,14 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t t) {
 }
 
 template <class T, int DP>
-__device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t t) {
+__device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
+                                              int col0) {
   using M = Mma<T>;
+  constexpr int SC = COLUMNS<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
-  const uint32_t tiles = uint32_t(s.Tk + 15) / 16;
-  const uint32_t bh = t / tiles;
-  const int key0 = int(t - bh * tiles) * 16, key = key0 + n;
+  const int key0 = int(item) * 16, key = key0 + n;
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, false, keys, first);
@@ -524,12 +574,12 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t t) {
     const uint32_t i = s.by_group.div(uint32_t(row));
     return p + int64_t(i) * x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * x.sInner;
   };
-  Frag<T, DP> k, v;
+  Own<T, DP> k, v;
   k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + int64_t(key) * a.k.sOuter, s.D, key < keys,
          a.vec, h);
   v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + int64_t(key) * a.v.sOuter, s.D, key < keys,
          a.vec, h);
-  Sums<T, DP> dk, dv;
+  Sums<T, SC> dk, dv;
   dk.clear();
   dv.clear();
   // rows before the first query that sees any of these keys take no part
@@ -540,28 +590,23 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t t) {
     row0 = int(std::min<int64_t>(int64_t(key0 - first) * s.G, s.rows)) & ~15;
   const int clear = key0 + 16; // a row that sees so many sees all of this tile
   for (int r0 = row0 + wave * 16; r0 < s.rows; r0 += 16 * AT_WAVES) {
-    Frag<T, DP> q, g;
-    const bool live = r0 + n < s.rows;
-    q.load(at(qp, a.q, live ? r0 + n : 0), s.D, live, a.vec, h);
-    g.load(at(gp, a.g, live ? r0 + n : 0), s.D, live, a.vec, h);
-    Items<T, DP> xq, xg;
+    Items<T, SC> xq, xg;
     T lse[4], delta[4];
     int limit[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = r0 + M::row(h, r);
       const bool on = row < s.rows;
-      const T *p = at(qp, a.q, on ? row : 0), *o = at(gp, a.g, on ? row : 0);
-#pragma unroll
-      for (int c = 0; c < Items<T, DP>::C; ++c) {
-        xq.v[r][c] = piece(p, RowVec<T>::N * (16 * c + n), s.D, on, a.vec);
-        xg.v[r][c] = piece(o, RowVec<T>::N * (16 * c + n), s.D, on, a.vec);
-      }
+      xq.load(r, at(qp, a.q, on ? row : 0) + col0, s.D - col0, on, a.vec, n);
+      xg.load(r, at(gp, a.g, on ? row : 0) + col0, s.D - col0, on, a.vec, n);
       lse[r] = on ? a.lse[int64_t(bh) * s.rows + row] : T(0);
       delta[r] = on ? a.delta[int64_t(bh) * s.rows + row] : T(0);
       limit[r] = on ? seen(s, keys, first, int(s.by_group.div(uint32_t(row)))) : 0;
     }
-    const auto z = dots<T, DP>(q, k), dp = dots<T, DP>(g, v);
+    const bool live = r0 + n < s.rows;
+    const int own = live ? r0 + n : 0;
+    const auto z = k.dots(at(qp, a.q, own), s.D, live, a.vec, h);
+    const auto dp = v.dots(at(gp, a.g, own), s.D, live, a.vec, h);
     T p[4], ds[4];
     bool vis[4], some = false;
 #pragma unroll
@@ -572,37 +617,52 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t t) {
       ds[r] = vis[r] ? p[r] * (dp[r] - delta[r]) : T(0);
     }
     auto row_of = [&](const T *base, const Rows<const T> &x) {
-      return [&, base](int item) { return r0 + item < s.rows ? at(base, x, r0 + item) : nullptr; };
+      return [&, base](int item) {
+        return r0 + item < s.rows ? at(base, x, r0 + item) + col0 : nullptr;
+      };
     };
-    if (__any(some) && !all_finite<T, DP>(xg))
-      dv.add_visible(p, vis, s.D, lane, row_of(gp, a.g));
+    if (__any(some) && !all_finite<T, SC>(xg))
+      dv.add_visible(p, vis, s.D - col0, lane, row_of(gp, a.g));
     else
       dv.add(p, xg);
-    if (__any(some) && !all_finite<T, DP>(xq))
-      dk.add_visible(ds, vis, s.D, lane, row_of(qp, a.q));
+    if (__any(some) && !all_finite<T, SC>(xq))
+      dk.add_visible(ds, vis, s.D - col0, lane, row_of(qp, a.q));
     else
       dk.add(ds, xq);
   }
   auto store = [&](T *out) {
     return [&, out](int r, int d, T x) {
+      d += col0;
       if (d < s.D && key0 + r < s.Tk)
         out[((int64_t(b) * s.Tk + key0 + r) * s.Hk + hk) * s.D + d] = x;
     };
   };
   if (a.dv)
-    join_waves<T, DP>(dv, T(1), lds, store(a.dv));
+    join_waves<T, SC>(dv, T(1), lds, store(a.dv));
   if (a.dk)
-    join_waves<T, DP>(dk, a.scale, lds, store(a.dk));
+    join_waves<T, SC>(dk, a.scale, lds, store(a.dk));
 }
 
 template <class T, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(const AttnBwd<T> a) {
-  attn_dq_tile<T, DP>(a, xcd_run(blockIdx.x, gridDim.x));
+  constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
+  uint32_t bh, item;
+  head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk), uint32_t(a.s.rows + 15) / 16 * GROUPS, bh,
+            item);
+  const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
+  if (col0 < a.s.D)
+    attn_dq_tile<T, DP>(a, bh, item / GROUPS, col0);
 }
 
 template <class T, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(const AttnBwd<T> a) {
-  attn_dkv_tile<T, DP>(a, xcd_run(blockIdx.x, gridDim.x));
+  constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
+  uint32_t bh, item;
+  head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk), uint32_t(a.s.Tk + 15) / 16 * GROUPS, bh,
+            item);
+  const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
+  if (col0 < a.s.D)
+    attn_dkv_tile<T, DP>(a, bh, item / GROUPS, col0);
 }
 
 // As attn_fwd_left_kernel.
@@ -616,12 +676,12 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const Attn
   if (a.dq)
     for (uint32_t t = blockIdx.x % groups; t < rows; t += groups) {
       __syncthreads();
-      attn_dq_tile<float, DP>(a, bh * rows + t);
+      attn_dq_tile<float, DP>(a, bh, t, 0);
     }
   if (a.dk || a.dv)
     for (uint32_t t = blockIdx.x % groups; t < keys; t += groups) {
       __syncthreads();
-      attn_dkv_tile<float, DP>(a, bh * keys + t);
+      attn_dkv_tile<float, DP>(a, bh, t, 0);
     }
 }
 
@@ -671,7 +731,7 @@ AttnShape attn_shape(const nt_view *q, const nt_view *k, const nt_view *v,
   constexpr int64_t MOST = int64_t(1) << 30;
   const int64_t G = H / Hk;
   if (B >= MOST || Tk >= MOST || Tq >= MOST || H >= MOST || Tq * G >= MOST || B * Hk >= MOST ||
-      (B * Hk) * ((std::max(Tq * G, Tk) + 15) / 16) >= MOST / 256)
+      (B * Hk) * ((std::max(Tq * G, Tk) + 15) / 16) >= MOST / 1024)
     fail(NT_ERR_VALUE, "attention: too many rows");
   AttnShape s{};
   s.B = int(B), s.Tq = int(Tq), s.Tk = int(Tk), s.Hk = int(Hk), s.G = int(G), s.D = int(D);
@@ -719,9 +779,10 @@ template <class T> T *contiguous_of(const nt_view *v, int64_t n, int dt, const c
 
 // The padded width: the matrix instructions' columns come 16 pieces at a time.
 template <class T, class F> void dispatch_width(int D, F &&f) {
-  constexpr int LEAST = 16 * RowVec<T>::N; // 64 float32, 32 float64
-  if (D <= LEAST)
-    f.template operator()<LEAST>();
+  if (D <= 32 && sizeof(T) == 8)
+    f.template operator()<sizeof(T) == 8 ? 32 : 64>();
+  else if (D <= 64)
+    f.template operator()<64>();
   else if (D <= 128)
     f.template operator()<128>();
   else
@@ -764,7 +825,8 @@ template <class T> void run_attention(AttnFwd<T> &a) {
   a.part_stat = stat.template get<T>();
   dispatch_width<T>(s.D, [&]<int DP>() {
     attn_fwd_kernel<T, DP>
-        <<<dim3(uint32_t(tiles * a.splits)), 64 * AT_WAVES, 0, stream()>>>(a);
+        <<<dim3(uint32_t(tiles * a.splits * COLUMN_GROUPS<T, DP>)), 64 * AT_WAVES, 0,
+           stream()>>>(a);
   });
   NT_LAUNCH_CHECK();
   if (a.splits > 1) {
@@ -799,13 +861,15 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a, const T *y) {
   }
   dispatch_width<T>(s.D, [&]<int DP>() {
     if (a.dq && rows) {
-      attn_dq_kernel<T, DP><<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.rows + 15) / 16))),
-                              64 * AT_WAVES, 0, stream()>>>(a);
+      attn_dq_kernel<T, DP>
+          <<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.rows + 15) / 16) * COLUMN_GROUPS<T, DP>)),
+             64 * AT_WAVES, 0, stream()>>>(a);
       NT_LAUNCH_CHECK();
     }
     if ((a.dk || a.dv) && s.Tk && s.B) {
-      attn_dkv_kernel<T, DP><<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.Tk + 15) / 16))),
-                               64 * AT_WAVES, 0, stream()>>>(a);
+      attn_dkv_kernel<T, DP>
+          <<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.Tk + 15) / 16) * COLUMN_GROUPS<T, DP>)),
+             64 * AT_WAVES, 0, stream()>>>(a);
       NT_LAUNCH_CHECK();
     }
   });

@@ -363,8 +363,9 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = uint32_t(s.rows + SF_ROWS - 1) / SF_ROWS;
-  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
-  const int tile = int(tiles - 1 - (t - bh * tiles)); // the most keys first
+  uint32_t bh, item;
+  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles, bh, item);
+  const int tile = int(tiles - 1 - item); // the most keys first
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, threadIdx.x == 0, keys, first);
@@ -538,8 +539,9 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 2 ? 2 : 1)) void attn_split_d
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = uint32_t(s.rows + SB_ROWS - 1) / SB_ROWS;
-  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), bh = t / tiles;
-  const int tile = int(tiles - 1 - (t - bh * tiles));
+  uint32_t bh, item;
+  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles, bh, item);
+  const int tile = int(tiles - 1 - item);
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, false, keys, first);
@@ -622,8 +624,8 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = uint32_t(s.Tk + SB_ROWS - 1) / SB_ROWS;
-  const uint32_t t = xcd_run(blockIdx.x, gridDim.x);
-  const uint32_t bh = t / (tiles * uint32_t(a.parts)), u = t - bh * tiles * uint32_t(a.parts);
+  uint32_t bh, u;
+  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles * uint32_t(a.parts), bh, u);
   const int tile = int(u / uint32_t(a.parts)), part = int(u % uint32_t(a.parts));
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
