@@ -64,25 +64,22 @@ template <class T> struct AttnBwd {
   AttnGate gate;
 };
 
-// Workgroup id -> (sequence, key head) of `heads`, item of `items` each, items
-// rising in the order of dispatch.  Workgroups are dealt to the 8 XCDs round-
-// robin; eight heads at a time are walked together, so that an XCD has one of
-// them, whose keys its L2 then holds, and every XCD the same mixture of long
-// items (the first, under a causal mask) and short ones.  (Consecutive ids on one
-// XCD left a third of the CUs without work: 8192 tokens, 4 key heads, forward
-// 1.01 ms.)  The last heads % 8 share the XCDs.
+// Workgroup id -> (sequence, key head) of `heads`, item of `items` each; items
+// rise in the order of dispatch, the longest first under a causal mask.
+// Workgroups are dealt to the 8 XCDs round-robin.  Some heads at a time are walked
+// together, a multiple of 8: every XCD then has heads of its own, whose keys its L2
+// holds, and the same mixture of long items and short ones; enough of them that
+// an XCD's 32 CUs have two rounds of items, so that short ones fill the gaps that
+// long ones leave.  (Consecutive ids on one XCD left a third of the CUs without
+// work: 8192 tokens, 4 key heads, forward 1.01 ms for 0.77; 8 heads at a time of 64
+// with 8 items each nearly half.)  The last heads % 8 share the XCDs.
 __device__ __forceinline__ void head_item(uint32_t id, uint32_t heads, uint32_t items,
                                           uint32_t &head, uint32_t &item) {
-  const uint32_t whole = heads / 8 * 8, even = whole * items;
-  if (id < even) {
-    const uint32_t r = id / 8;
-    head = r / items * 8 + id % 8;
-    item = r % items;
-  } else {
-    const uint32_t left = heads - whole;
-    head = whole + (id - even) % left;
-    item = (id - even) / left;
-  }
+  const uint32_t together = items >= 64 ? 8 : (64 + items - 1) / items * 8;
+  const uint32_t turn = id / (together * items), r = id - turn * together * items;
+  const uint32_t left = heads - turn * together, n = left < together ? left : together;
+  item = r / n;
+  head = turn * together + (r - item * n);
 }
 
 // Keys of sequence b, and the position of its first query among them.
