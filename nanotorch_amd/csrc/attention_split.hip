@@ -65,11 +65,20 @@ __device__ __forceinline__ int up_exponent(float most) {
   return min(14 - e, 126);
 }
 
+// Two values to an instruction where they are rounded; the rest x - hi, which is
+// exact, as a sum of mixed types: two instructions a value.
 __device__ __forceinline__ void split8(const float (&x)[8], half8 &hi, half8 &lo) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+  float minus = -1.f;
+  asm("" : "+s"(minus)); // a known -1 would make it a conversion and a difference
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    hi[j] = _Float16(x[j]);
-    lo[j] = _Float16(x[j] - float(hi[j]));
+  for (int j = 0; j < 8; j += 2) {
+    const half2v h = __builtin_convertvector(float2v{x[j], x[j + 1]}, half2v);
+    const float2v rest = {fmaf(float(h.x), minus, x[j]), fmaf(float(h.y), minus, x[j + 1])};
+    const half2v l = __builtin_convertvector(rest, half2v);
+    hi[j] = h.x, hi[j + 1] = h.y;
+    lo[j] = l.x, lo[j + 1] = l.y;
   }
 }
 
@@ -249,23 +258,27 @@ __device__ __forceinline__ half8 frag(const char *p, int lane) {
   return *reinterpret_cast<const half8 *>(p + lane * 16);
 }
 
-// items' row form (a unit) . own rows: result[item, own].
+// items' row form (a unit) . own rows: result[item, own].  The small products come
+// first, so that their sum is not rounded as the large ones' is; the hi pieces wait
+// for their turn in registers, or are read again where those are few.
 template <int DB>
 __device__ __forceinline__ floatx16 dots32(const char *unit, const half8 (&hi)[2 * DB],
                                            const half8 (&lo)[2 * DB], int lane) {
   constexpr int CH = SA_CHUNK<DB>;
-  floatx16 top{}, low{};
+  constexpr bool KEEP = DB <= 3;
+  floatx16 s{};
+  half8 xh[KEEP ? 2 * DB : 1];
 #pragma unroll
   for (int f = 0; f < 2 * DB; ++f) {
-    const half8 xh = frag(unit + f * 1024, lane), xl = frag(unit + CH / 2 + f * 1024, lane);
-    low = mma(xl, hi[f], low);
-    top = mma(xh, hi[f], top);
-    low = mma(xh, lo[f], low);
+    half8 &x = xh[KEEP ? f : 0];
+    x = frag(unit + f * 1024, lane);
+    s = mma(frag(unit + CH / 2 + f * 1024, lane), hi[f], s);
+    s = mma(x, lo[f], s);
   }
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    top[r] += low[r];
-  return top;
+  for (int f = 0; f < 2 * DB; ++f)
+    s = mma(KEEP ? xh[KEEP ? f : 0] : frag(unit + f * 1024, lane), hi[f], s);
+  return s;
 }
 
 // The lane's 16 results of a unit as operand: two groups of 16 items.
@@ -506,7 +519,10 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
 
 // --------------------------------------------------------------- backward
 
-constexpr int SB_WAVES = 4, SB_ROWS = SB_WAVES * SA_UNIT;
+// Two waves to a SIMD: two workgroups of four on a CU, or where the stages fill more
+// than half of its LDS one of eight.
+template <int DB> constexpr int SB_WAVES = DB <= 2 ? 4 : 8;
+template <int DB> constexpr int SB_ROWS = SB_WAVES<DB> * SA_UNIT;
 
 struct SplitBwd {
   AttnShape s;
@@ -531,14 +547,14 @@ __device__ __forceinline__ void load_own(const char *unit, half8 (&hi)[2 * DB],
 }
 
 template <int DB>
-__global__ __launch_bounds__(64 * SB_WAVES, (DB <= 2 ? 2 : 1)) void attn_split_dq_kernel(
+__global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
     const SplitBwd a) {
-  constexpr int CH = SA_CHUNK<DB>;
+  constexpr int CH = SA_CHUNK<DB>, WAVES = SB_WAVES<DB>;
   __shared__ __attribute__((aligned(1024))) char lds[2][3 * CH];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tiles = uint32_t(s.rows + SB_ROWS - 1) / SB_ROWS;
+  const uint32_t tiles = uint32_t(s.rows + SB_ROWS<DB> - 1) / SB_ROWS<DB>;
   uint32_t bh, item;
   head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles, bh, item);
   const int tile = int(tiles - 1 - item);
@@ -550,18 +566,20 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 2 ? 2 : 1)) void attn_split_d
   auto limit_of = [&](int row) {
     return seen(s, keys, first, int(s.by_group.div(uint32_t(row))));
   };
-  const int row0 = tile * SB_ROWS + wave * SA_UNIT, row = row0 + n;
+  const int row0 = tile * SB_ROWS<DB> + wave * SA_UNIT, row = row0 + n;
   const bool on = row0 < s.rows; // of the wave
   const int end = on ? limit_of(min(row0 + SA_UNIT, s.rows) - 1) : 0;
   const int all = on ? limit_of(row0) : 0;
-  const int group_end = limit_of(min((tile + 1) * SB_ROWS, s.rows) - 1);
+  const int group_end = limit_of(min((tile + 1) * SB_ROWS<DB>, s.rows) - 1);
   const int64_t kv = int64_t(bh) * a.k_tiles * 2 * CH;
   auto issue = [&](char *stage, int it) {
 #pragma unroll
-    for (int j = 0; j < 3 * DB; ++j) {
-      const int p = (j % DB) * 4 + wave;
-      const char *from = j < DB ? a.k_row : j < 2 * DB ? a.v_row : a.k_col;
-      load_lds(from + kv + int64_t(it) * CH + p * 1024, stage + j / DB * CH + p * 1024, lane);
+    for (int j = 0; j < 12 * DB; j += WAVES) {
+      const int p = j + wave, form = (4 * DB % WAVES ? p : j) / (4 * DB);
+      if (p < 12 * DB)
+        load_lds((form == 0 ? a.k_row : form == 1 ? a.v_row : a.k_col) + kv + int64_t(it) * CH +
+                     (p - form * 4 * DB) * 1024,
+                 stage + p * 1024, lane);
     }
   };
   const int steps = (group_end + SA_UNIT - 1) / SA_UNIT;
@@ -615,15 +633,22 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 2 ? 2 : 1)) void attn_split_d
                 a.scale * g_scale, s.D, h);
 }
 
-template <int DB>
-__global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_dkv_kernel(
+// DK, DV: which of the two.  Both in one kernel share the probabilities; of heads
+// over 64 wide both sums and both own operands do not fit the registers of two
+// waves to a SIMD, and one wave leaves the matrix cores idle while it forms
+// probabilities: 8192 tokens, 16 heads over 4 of 128, in one kernel 2.53 ms.
+template <int DB, bool DK, bool DV>
+__global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
     const SplitBwd a) {
-  constexpr int CH = SA_CHUNK<DB>, STAT = SA_STATS * 4;
-  __shared__ __attribute__((aligned(1024))) char lds[2][4 * CH + STAT];
+  constexpr int CH = SA_CHUNK<DB>, STAT = SA_STATS * 4, WAVES = SB_WAVES<DB>;
+  // a stage: q's rows; g's (DK); g's columns (DV); q's columns (DK)
+  constexpr int FORMS = 1 + 2 * DK + DV, G_ROW = CH, G_COL = DK ? 2 * CH : CH,
+                Q_COL = (2 + DV) * CH;
+  __shared__ __attribute__((aligned(1024))) char lds[2][FORMS * CH + STAT];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tiles = uint32_t(s.Tk + SB_ROWS - 1) / SB_ROWS;
+  const uint32_t tiles = uint32_t(s.Tk + SB_ROWS<DB> - 1) / SB_ROWS<DB>;
   uint32_t bh, u;
   head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles * uint32_t(a.parts), bh, u);
   const int tile = int(u / uint32_t(a.parts)), part = int(u % uint32_t(a.parts));
@@ -635,7 +660,7 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
   auto limit_of = [&](int row) {
     return seen(s, keys, first, int(s.by_group.div(uint32_t(row))));
   };
-  const int key0 = tile * SB_ROWS, own0 = key0 + wave * SA_UNIT, key = own0 + n;
+  const int key0 = tile * SB_ROWS<DB>, own0 = key0 + wave * SA_UNIT, key = own0 + n;
   // units from the first query that sees any of these keys on, this part of them
   const int units = (s.rows + SA_UNIT - 1) / SA_UNIT;
   int from = 0;
@@ -649,16 +674,20 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
   auto issue = [&](char *stage, int it) {
     const int64_t at = (base + it) * CH;
 #pragma unroll
-    for (int j = 0; j < 4 * DB; ++j) {
-      const int p = (j % DB) * 4 + wave;
-      const char *x = j < DB ? a.q_row : j < 2 * DB ? a.q_col : j < 3 * DB ? a.g_row : a.g_col;
-      load_lds(x + at + p * 1024, stage + j / DB * CH + p * 1024, lane);
+    for (int j = 0; j < FORMS * 4 * DB; j += WAVES) {
+      const int p = j + wave, to = (4 * DB % WAVES ? p : j) / (4 * DB) * CH;
+      const char *x = to == 0             ? a.q_row
+                      : DK && to == G_ROW ? a.g_row
+                      : DV && to == G_COL ? a.g_col
+                                          : a.q_col;
+      if (p < FORMS * 4 * DB)
+        load_lds(x + at + p * 1024 - to, stage + p * 1024, lane);
     }
     if (wave < 2) // the rows' statistics, 4 bytes a lane
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void *)(a.stats + (base + it) * SA_STATS +
                                                            wave * 64 + lane),
-          (__attribute__((address_space(3))) void *)(stage + 4 * CH + wave * 256), 4, 0, 0);
+          (__attribute__((address_space(3))) void *)(stage + FORMS * CH + wave * 256), 4, 0, 0);
   };
   if (u0 < u1)
     issue(lds[0], u0);
@@ -666,7 +695,8 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
   const bool on = own0 < keys;
   const int64_t unit = int64_t(bh) * a.k_tiles * 2 + (on ? own0 / SA_UNIT : 0);
   load_own<DB>(a.k_row + unit * CH, kh, kl, lane);
-  load_own<DB>(a.v_row + unit * CH, vh, vl, lane);
+  if constexpr (DK)
+    load_own<DB>(a.v_row + unit * CH, vh, vl, lane);
   const float v_scale = a.v_scale[unit / 2], c = a.scale2 * a.k_scale[unit / 2];
   floatx16 dk[DB]{}, dv[DB]{};
   for (int it = u0; it < u1; ++it) {
@@ -679,10 +709,12 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
     if (!on || limit_of(min(r0 + SA_UNIT, s.rows) - 1) <= own0)
       continue;
     const char *stage = lds[buf];
-    const float *st = reinterpret_cast<const float *>(stage + 4 * CH);
+    const float *st = reinterpret_cast<const float *>(stage + FORMS * CH);
     const float q_scale = a.q_scale[int64_t(bh) * a.q_tiles + it / 2], cz = c * q_scale;
     floatx16 w = dots32<DB>(stage, kh, kl, lane);
-    floatx16 ds = dots32<DB>(stage + 2 * CH, vh, vl, lane);
+    floatx16 ds{};
+    if constexpr (DK)
+      ds = dots32<DB>(stage + G_ROW, vh, vl, lane);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4 lse = *reinterpret_cast<const float4 *>(st + 8 * q + 4 * h);
@@ -696,7 +728,8 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
         const int r = 4 * q + j;
         // p times the row's scale: what multiplies its packed gradient
         w[r] = __builtin_amdgcn_exp2f(fmaf(w[r], cz, -ls[j])) * gs[j];
-        ds[r] = w[r] * fmaf(ds[r], v_scale, -de[j]);
+        if constexpr (DK)
+          ds[r] = w[r] * fmaf(ds[r], v_scale, -de[j]);
       }
     }
     if (limit_of(r0) < own0 + SA_UNIT)
@@ -708,35 +741,36 @@ __global__ __launch_bounds__(64 * SB_WAVES, (DB <= 1 ? 2 : 1)) void attn_split_d
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           w[4 * q + j] = key < li[j] ? w[4 * q + j] : 0.f;
-          ds[4 * q + j] = key < li[j] ? ds[4 * q + j] : 0.f;
+          if constexpr (DK)
+            ds[4 * q + j] = key < li[j] ? ds[4 * q + j] : 0.f;
         }
       }
     half8 hi[2], lo[2];
     float inverse;
-    {
+    if constexpr (DV) {
       const float k = column_factor(w, inverse);
       w *= k;
       split16(w, hi, lo);
-    }
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-      sums32<DB>(dv[db], stage + 3 * CH, db, hi, lo, inverse, lane);
-    {
+      for (int db = 0; db < DB; ++db)
+        sums32<DB>(dv[db], stage + G_COL, db, hi, lo, inverse, lane);
+    }
+    if constexpr (DK) {
       const float k = column_factor(ds, inverse);
       ds *= k;
       split16(ds, hi, lo);
-    }
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-      sums32<DB>(dk[db], stage + CH, db, hi, lo, inverse * q_scale, lane);
+      for (int db = 0; db < DB; ++db)
+        sums32<DB>(dk[db], stage + Q_COL, db, hi, lo, inverse * q_scale, lane);
+    }
   }
   if (key >= s.Tk)
     return;
   const int64_t size = int64_t(s.B) * s.Tk * s.Hk * s.D;
   const int64_t at = part * size + ((int64_t(b) * s.Tk + key) * s.Hk + hk) * s.D;
-  if (a.dk)
+  if (DK && a.dk)
     store_row<DB>(a.dk + at, dk, a.scale, s.D, h);
-  if (a.dv)
+  if (DV && a.dv)
     store_row<DB>(a.dv + at, dv, 1.f, s.D, h);
 }
 
@@ -886,14 +920,14 @@ void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
     f.parts = 1;
     if (a.dq) {
       f.dq = a.dq;
-      attn_split_dq_kernel<DB><<<dim3(bhs * uint32_t((s.rows + SB_ROWS - 1) / SB_ROWS)),
-                                 64 * SB_WAVES, 0, stream()>>>(f);
+      attn_split_dq_kernel<DB><<<dim3(bhs * uint32_t((s.rows + SB_ROWS<DB> - 1) / SB_ROWS<DB>)),
+                                 64 * SB_WAVES<DB>, 0, stream()>>>(f);
       NT_LAUNCH_CHECK();
     }
     if (a.dk || a.dv) {
       // Workgroups of different lengths, one to two at a time on a CU: four for
       // each CU even them out.  Fewer key tiles than that share their rows.
-      const int64_t groups = int64_t(bhs) * ((s.Tk + SB_ROWS - 1) / SB_ROWS);
+      const int64_t groups = int64_t(bhs) * ((s.Tk + SB_ROWS<DB> - 1) / SB_ROWS<DB>);
       const int units = (s.rows + SA_UNIT - 1) / SA_UNIT;
       f.parts = int(std::max<int64_t>(
           1, std::min<int64_t>({int64_t(device_cu_count()) * 4 / groups, units / 8, 16})));
@@ -901,9 +935,20 @@ void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
       DeviceScratch sums(f.parts > 1 ? 2 * size * size_t(f.parts) * sizeof(float) : 0);
       f.dk = a.dk && f.parts > 1 ? sums.get<float>() : a.dk;
       f.dv = a.dv && f.parts > 1 ? sums.get<float>() + size * size_t(f.parts) : a.dv;
-      attn_split_dkv_kernel<DB>
-          <<<dim3(uint32_t(groups * f.parts)), 64 * SB_WAVES, 0, stream()>>>(f);
-      NT_LAUNCH_CHECK();
+      const dim3 grid(uint32_t(groups * f.parts));
+      if constexpr (DB <= 2) {
+        attn_split_dkv_kernel<DB, true, true><<<grid, 64 * SB_WAVES<DB>, 0, stream()>>>(f);
+        NT_LAUNCH_CHECK();
+      } else {
+        if (a.dv) {
+          attn_split_dkv_kernel<DB, false, true><<<grid, 64 * SB_WAVES<DB>, 0, stream()>>>(f);
+          NT_LAUNCH_CHECK();
+        }
+        if (a.dk) {
+          attn_split_dkv_kernel<DB, true, false><<<grid, 64 * SB_WAVES<DB>, 0, stream()>>>(f);
+          NT_LAUNCH_CHECK();
+        }
+      }
       if (f.parts > 1) {
         const int64_t each = int64_t(s.Tk) * s.D;
         attn_split_parts_kernel<<<dim3(uint32_t((each + 255) / 256), bhs), 256, 0, stream()>>>(
