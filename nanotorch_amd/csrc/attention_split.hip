@@ -258,31 +258,80 @@ __device__ __forceinline__ half8 frag(const char *p, int lane) {
   return *reinterpret_cast<const half8 *>(p + lane * 16);
 }
 
-// items' row form (a unit) . own rows: result[item, own].  The small products come
-// first, so that their sum is not rounded as the large ones' is; the hi pieces wait
-// for their turn in registers, or are read again where those are few.
-template <int DB>
-__device__ __forceinline__ floatx16 dots32(const char *unit, const half8 (&hi)[2 * DB],
-                                           const half8 (&lo)[2 * DB], int lane) {
-  constexpr int CH = SA_CHUNK<DB>;
-  constexpr bool KEEP = DB <= 3;
+// A hi piece and the lo piece that belongs to it.
+struct Pair {
+  half8 h, l;
+};
+
+// Pieces are read two pairs ahead of the matrix instructions that take them, across
+// the ends of sums too: the reads stay where they are written, and only other
+// work moves past them.  (The compiler put each right before its use; the wait on
+// LDS was a third of the waves' time.)
+__device__ __forceinline__ void keep_order() {
+  __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x10); // vector, scalar, global memory
+}
+
+// sum over NF pieces of (pieces . operand), pieces at at(0) ..; pre holds the first
+// two pairs and gets those at next(0) and next(1).  The small products come first,
+// so that their sum is not rounded as the large ones' is; the hi pieces wait for
+// their turn in registers (KEEP), or are read again where those are few.
+template <int NF, bool KEEP, int HALF, class At, class Next>
+__device__ __forceinline__ floatx16 stream_sum(At at, Next next, const half8 *hi, const half8 *lo,
+                                               Pair (&pre)[2], int lane) {
   floatx16 s{};
-  half8 xh[KEEP ? 2 * DB : 1];
+  half8 xh[KEEP ? NF : 2];
+  auto pair = [&](const char *p) { return Pair{frag(p, lane), frag(p + HALF, lane)}; };
 #pragma unroll
-  for (int f = 0; f < 2 * DB; ++f) {
-    half8 &x = xh[KEEP ? f : 0];
-    x = frag(unit + f * 1024, lane);
-    s = mma(frag(unit + CH / 2 + f * 1024, lane), hi[f], s);
-    s = mma(x, lo[f], s);
+  for (int f = 0; f < NF; ++f) {
+    const Pair x = pre[f & 1];
+    if constexpr (KEEP) {
+      xh[f] = x.h;
+      pre[f & 1] = pair(f + 2 < NF ? at(f + 2) : next(f + 2 - NF));
+    } else if (f + 2 < NF) {
+      pre[f & 1] = pair(at(f + 2));
+    } else {
+      xh[f & 1] = frag(at(f & 1), lane);
+    }
+    keep_order();
+    s = mma(x.l, hi[f], s);
+    s = mma(x.h, lo[f], s);
+    keep_order();
   }
 #pragma unroll
-  for (int f = 0; f < 2 * DB; ++f)
-    s = mma(KEEP ? xh[KEEP ? f : 0] : frag(unit + f * 1024, lane), hi[f], s);
+  for (int f = 0; f < NF; ++f) {
+    const half8 x = xh[KEEP ? f : f & 1];
+    if constexpr (!KEEP) {
+      if (f + 2 < NF)
+        xh[f & 1] = frag(at(f + 2), lane);
+      else
+        pre[f & 1] = pair(next(f & 1));
+      keep_order();
+    }
+    s = mma(x, hi[f], s);
+  }
+  keep_order();
   return s;
 }
 
+// items' row form (a unit) . own rows: result[item, own]; pre and next as above.
+template <int DB, class Next>
+__device__ __forceinline__ floatx16 dots32(const char *unit, const half8 (&hi)[2 * DB],
+                                           const half8 (&lo)[2 * DB], Pair (&pre)[2], Next next,
+                                           int lane) {
+  return stream_sum<2 * DB, DB <= 3, SA_CHUNK<DB> / 2>(
+      [&](int f) { return unit + f * 1024; }, next, hi, lo, pre, lane);
+}
+
+// The first two pairs of a form.
+template <int DB> __device__ __forceinline__ void first_pairs(Pair (&pre)[2], const char *p,
+                                                              int lane) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    pre[i] = {frag(p + i * 1024, lane), frag(p + SA_CHUNK<DB> / 2 + i * 1024, lane)};
+}
+
 // The lane's 16 results of a unit as operand: two groups of 16 items.
-__device__ __forceinline__ void split16(const floatx16 &x, half8 (&hi)[2], half8 (&lo)[2]) {
+__device__ __forceinline__ void split16(const floatx16 &x, half8 *hi, half8 *lo) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     float v[8];
@@ -307,26 +356,22 @@ __device__ __forceinline__ float column_factor(const floatx16 &x, float &inverse
   return __uint_as_float(uint32_t(up) << 23);
 }
 
-// acc = acc + k (items' col form (a unit) . x) for one block of 32 columns.
+// acc = acc + k (items' col form (a unit) . x); pre holds its first pairs and gets
+// those at `after`.
 template <int DB>
-__device__ __forceinline__ void sums32(floatx16 &acc, const char *unit, int db,
-                                       const half8 (&hi)[2], const half8 (&lo)[2], float k,
-                                       int lane) {
-  constexpr int CH = SA_CHUNK<DB>;
-  floatx16 t{};
-  half8 xh[2];
+__device__ __forceinline__ void sums32(floatx16 (&acc)[DB], const char *unit, const half8 (&hi)[2],
+                                       const half8 (&lo)[2], float k, Pair (&pre)[2],
+                                       const char *after, int lane) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    xh[i] = frag(unit + (2 * db + i) * 1024, lane);
-    t = mma(frag(unit + CH / 2 + (2 * db + i) * 1024, lane), hi[i], t);
-    t = mma(xh[i], lo[i], t);
+  for (int db = 0; db < DB; ++db) {
+    const floatx16 t = stream_sum<2, true, SA_CHUNK<DB> / 2>(
+        [&](int f) { return unit + (2 * db + f) * 1024; },
+        [&](int f) { return (db + 1 < DB ? unit + (2 * db + 2) * 1024 : after) + f * 1024; }, hi,
+        lo, pre, lane);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      acc[db][r] = fmaf(t[r], k, acc[db][r]);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    t = mma(xh[i], hi[i], t);
-#pragma unroll
-  for (int r = 0; r < 16; ++r)
-    acc[r] = fmaf(t[r], k, acc[r]);
 }
 
 // Stores a lane's own row of 32 DB columns, times k.
@@ -454,9 +499,12 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
                            3.4e38f);
     const float v_scale = a.v_scale[int64_t(bh) * a.tiles + it];
     floatx16 z[2];
+    Pair pre[2];
+    first_pairs<DB>(pre, st, lane);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      z[u] = dots32<DB>(st + u * CH, qh, ql, lane);
+      z[u] = dots32<DB>(st + u * CH, qh, ql, pre,
+                        [&](int f) { return st + (u + 1) * CH + f * 1024; }, lane);
     if (it * SA_TILE + SA_TILE > all)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -483,24 +531,16 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
         sum += z[u][r];
       }
     l = fmaf(l, shrink, sum);
-    half8 ph[2][2], pl[2][2];
+    half8 ph[4], pl[4];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      split16(z[u], ph[u], pl[u]);
+      split16(z[u], ph + 2 * u, pl + 2 * u);
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
-      floatx16 o{};
-      half8 vh[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const char *p = st + (2 + i / 2) * CH + (2 * db + i % 2) * 1024;
-        vh[i] = frag(p, lane);
-        o = mma(frag(p + CH / 2, lane), ph[i / 2][i % 2], o);
-        o = mma(vh[i], pl[i / 2][i % 2], o);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o = mma(vh[i], ph[i / 2][i % 2], o);
+      const floatx16 o = stream_sum<4, true, CH / 2>(
+          [&](int f) { return st + (2 + f / 2) * CH + (2 * db + f % 2) * 1024; },
+          [&](int f) { return st + 2 * CH + (2 * (db + 1 < DB ? db + 1 : 0) + f) * 1024; }, ph, pl,
+          pre, lane);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         acc[db][r] = fmaf(o[r], v_scale, acc[db][r] * shrink);
@@ -604,8 +644,12 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
     const char *stage = lds[it & 1];
     const float k_scale = a.k_scale[int64_t(bh) * a.k_tiles + it / 2];
     const float v_scale = a.v_scale[int64_t(bh) * a.k_tiles + it / 2];
-    const floatx16 z = dots32<DB>(stage, qh, ql, lane);
-    floatx16 ds = dots32<DB>(stage + CH, gh, gl, lane);
+    Pair pre[2];
+    first_pairs<DB>(pre, stage, lane);
+    const floatx16 z = dots32<DB>(stage, qh, ql, pre,
+                                  [&](int f) { return stage + CH + f * 1024; }, lane);
+    floatx16 ds = dots32<DB>(stage + CH, gh, gl, pre,
+                             [&](int f) { return stage + 2 * CH + f * 1024; }, lane);
     const float cz = c * k_scale;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -621,9 +665,7 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
     ds *= k;
     half8 hi[2], lo[2];
     split16(ds, hi, lo);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-      sums32<DB>(acc[db], stage + 2 * CH, db, hi, lo, inverse * k_scale, lane);
+    sums32<DB>(acc, stage + 2 * CH, hi, lo, inverse * k_scale, pre, stage, lane);
   }
   if (row >= s.rows)
     return;
@@ -711,10 +753,14 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
     const char *stage = lds[buf];
     const float *st = reinterpret_cast<const float *>(stage + FORMS * CH);
     const float q_scale = a.q_scale[int64_t(bh) * a.q_tiles + it / 2], cz = c * q_scale;
-    floatx16 w = dots32<DB>(stage, kh, kl, lane);
+    Pair pre[2];
+    first_pairs<DB>(pre, stage, lane);
+    floatx16 w = dots32<DB>(stage, kh, kl, pre,
+                            [&](int f) { return stage + CH + f * 1024; }, lane);
     floatx16 ds{};
     if constexpr (DK)
-      ds = dots32<DB>(stage + G_ROW, vh, vl, lane);
+      ds = dots32<DB>(stage + G_ROW, vh, vl, pre,
+                      [&](int f) { return stage + 2 * CH + f * 1024; }, lane);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4 lse = *reinterpret_cast<const float4 *>(st + 8 * q + 4 * h);
@@ -751,17 +797,13 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
       const float k = column_factor(w, inverse);
       w *= k;
       split16(w, hi, lo);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        sums32<DB>(dv[db], stage + G_COL, db, hi, lo, inverse, lane);
+      sums32<DB>(dv, stage + G_COL, hi, lo, inverse, pre, DK ? stage + Q_COL : stage, lane);
     }
     if constexpr (DK) {
       const float k = column_factor(ds, inverse);
       ds *= k;
       split16(ds, hi, lo);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        sums32<DB>(dk[db], stage + Q_COL, db, hi, lo, inverse * q_scale, lane);
+      sums32<DB>(dk, stage + Q_COL, hi, lo, inverse * q_scale, pre, stage, lane);
     }
   }
   if (key >= s.Tk)
