@@ -66,16 +66,18 @@ class RmsNormOp(Function):
         return y
 
     def backward(self, grad_out: Tensor) -> tuple:
-        n = sum(self._given)
-        return tuple(self._grad(grad_out, [True] * n, [None] * n))
+        n = sum(self._given)  # x and the residual get one tensor, as those of a sum do
+        return tuple(self._grad(grad_out, [True] * n, [None] * n, True))
 
     def fused_ok(self) -> bool:
         return True
 
     def _backward_into(self, g: Tensor, needs, targets):
-        return self._grad(g, needs, targets)
+        tensors = [t for t in self._inputs if isinstance(t, Tensor)]
+        leaf = any([t.is_leaf for t, need in zip(tensors, needs) if need])
+        return self._grad(g, needs, targets, not leaf)
 
-    def _grad(self, g: Tensor, needs, targets) -> list:
+    def _grad(self, g: Tensor, needs, targets, share: bool) -> list:
         self.saved_tensors  # raises if the sum or the weight was modified in place
         s, w, rstd = self._call
         _, weighted, residual = self._given
@@ -95,17 +97,15 @@ class RmsNormOp(Function):
         if weighted and needs[1]:
             out[1] = _give(dw, shape[-1:], targets[1])
         for k, i in enumerate(summed):
-            if k and targets[i] is None:
+            if k and targets[i] is None and targets[summed[0]] is None:
                 # x and the residual have one gradient: one memory for both, but
                 # where a leaf keeps it
-                new = out[summed[0]]
-                tensors = [t for t in self._inputs if isinstance(t, Tensor)]
-                if targets[summed[0]] is not None or any(tensors[j].is_leaf for j in summed):
-                    ds = ds.clone() if targets[summed[0]] is None else ds
-                    out[i] = _give(ds, shape, None)
+                first = out[summed[0]]
+                if share:
+                    out[i] = first._alias()
+                    first._shared = out[i]._shared = True
                 else:
-                    out[i] = new._alias()
-                    new._shared = out[i]._shared = True
+                    out[i] = _give(ds.clone(), shape, None)
             else:
                 out[i] = _give(ds, shape, targets[i])
         return out

@@ -258,10 +258,12 @@ template <class T, int DP> __device__ __forceinline__ bool all_finite(const Item
 
 // ---------------------------------------------------------------- forward
 
-// Tiles of 16 keys that a wave takes at a time: two, as long as their rows fit
-// its registers beside two waves to a SIMD.
+// Tiles of 16 keys that a wave takes at a time, two blocks of which fit its registers
+// beside two waves to a SIMD.
+template <class T, int DP> constexpr int FWD_TILES = DP * sizeof(T) <= 256 ? 2 : 1;
+// Float64 rows of 512 bytes need the registers of one wave to a SIMD.
 template <class T, int DP>
-constexpr int FWD_TILES = DP * sizeof(T) <= (sizeof(T) == 4 ? 512 : 256) ? 2 : 1;
+constexpr int FWD_WAVES = sizeof(T) == 8 && DP * sizeof(T) == 512 ? 1 : 2;
 
 // Tile `item` of a (sequence, key head).
 template <class T, int DP>
@@ -300,23 +302,39 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   const int blocks = (end + 16 * TILES - 1) / (16 * TILES);
   const int per = (blocks + a.splits - 1) / a.splits;
   const int stop = std::min(blocks, int(split + 1) * per);
-  for (int blk = int(split) * per + wave; blk < stop; blk += AT_WAVES) {
-    const int j0 = blk * 16 * TILES;
+  // A block's keys (rows in registers only) and values.
+  struct Block {
+    Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> k[TILES];
     Items<T, SC> v[TILES];
+  };
+  auto load = [&](Block &x, int j0, int to) {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      const int j = j0 + 16 * i + n;
+      if constexpr (IN_REGISTERS<T, DP>)
+        x.k[i].load(kp + int64_t(j) * a.k.sOuter, s.D, j < to, a.vec, h);
+    }
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = j0 + 16 * i + M::row(h, r);
-        v[i].load(r, vp + int64_t(j) * a.v.sOuter + col0, s.D - col0, j < end, a.vec, n);
+        x.v[i].load(r, vp + int64_t(j) * a.v.sOuter + col0, s.D - col0, j < to, a.vec, n);
       }
+  };
+  auto take = [&](const Block &x, int j0) {
     T z[TILES][4];
     bool vis[TILES][4];
     T top = NEG_INF<T>;
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
-      const int j = j0 + 16 * i + n;
-      const auto d = q.dots(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
+      typename M::V4 d;
+      if constexpr (IN_REGISTERS<T, DP>) {
+        d = dots<T, DP>(x.k[i], q.f);
+      } else {
+        const int j = j0 + 16 * i + n;
+        d = q.dots(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         vis[i][r] = j0 + 16 * i + M::row(h, r) < limit;
@@ -346,12 +364,31 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i;
-      if (j + 16 > all && !all_finite<T, SC>(v[i]))
+      if (j + 16 > all && !all_finite<T, SC>(x.v[i]))
         sums.add_visible(z[i], vis[i], s.D - col0, lane, [&](int item) {
           return j + item < end ? vp + int64_t(j + item) * a.v.sOuter + col0 : nullptr;
         });
       else
-        sums.add(z[i], v[i]);
+        sums.add(z[i], x.v[i]);
+    }
+  };
+  // The next block is on its way while one is computed with: few rows over many
+  // keys wait for memory.  (A block past the last one loads nothing.)
+  constexpr int STEP = 16 * TILES;
+  auto bound = [&](int blk) { return blk < stop ? end : 0; };
+  int blk = int(split) * per + wave;
+  if (blk < stop) {
+    Block x, y;
+    load(x, blk * STEP, end);
+    for (;;) {
+      load(y, (blk + AT_WAVES) * STEP, bound(blk + AT_WAVES));
+      take(x, blk * STEP);
+      if ((blk += AT_WAVES) >= stop)
+        break;
+      load(x, (blk + AT_WAVES) * STEP, bound(blk + AT_WAVES));
+      take(y, blk * STEP);
+      if ((blk += AT_WAVES) >= stop)
+        break;
     }
   }
   l += __shfl_xor(l, 16);
@@ -399,7 +436,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_kernel(
+__global__ __launch_bounds__(64 * AT_WAVES, (FWD_WAVES<T, DP>)) void attn_fwd_kernel(
     const AttnFwd<T> a) {
   constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
   const uint32_t splits = uint32_t(a.splits);
@@ -415,7 +452,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<T, DP>)) void attn_fwd_ke
 // What the kernels on half-precision planes left: the tiles of each (sequence,
 // key head) dealt to `groups` workgroups.
 template <int DP>
-__global__ __launch_bounds__(64 * AT_WAVES, (FWD_TILES<float, DP>)) void attn_fwd_left_kernel(
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_left_kernel(
     const AttnFwd<float> a, uint32_t groups) {
   const uint32_t bh = blockIdx.x / groups;
   if (!gate_set(a.gate, bh))
@@ -439,14 +476,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
   const int tiles = (s.rows + 15) / 16, n = row & 15;
   // the slots are numbered with the tiles backwards, as their workgroups were
   const int64_t slot = (int64_t(bh) * tiles + (tiles - 1 - row / 16)) * a.splits;
-  T top = NEG_INF<T>;
-  for (int k = 0; k < a.splits; ++k)
-    top = fmax(top, a.part_stat[(slot + k) * 32 + n]);
-  const T base = top == NEG_INF<T> ? T(0) : top;
-  T total = 0;
-  for (int k = 0; k < a.splits; ++k)
-    total += a.part_stat[(slot + k) * 32 + 16 + n] *
-             Mma<T>::exp2(a.part_stat[(slot + k) * 32 + n] - base);
+  // a lane for each part, of at most 64
+  T m = NEG_INF<T>, l = 0;
+  if (lane < a.splits) {
+    m = a.part_stat[(slot + lane) * 32 + n];
+    l = a.part_stat[(slot + lane) * 32 + 16 + n];
+  }
+  T top = m;
+#pragma unroll
+  for (int o = 32; o; o >>= 1)
+    top = fmax(top, __shfl_xor(top, o));
+  const T weight = Mma<T>::exp2(m - (top == NEG_INF<T> ? T(0) : top));
+  T total = l * weight;
+#pragma unroll
+  for (int o = 32; o; o >>= 1)
+    total += __shfl_xor(total, o);
   int keys, first;
   sequence(s, bh / s.Hk, false, keys, first);
   const uint32_t i = s.by_group.div(uint32_t(row));
@@ -455,12 +499,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
     a.lse[item] = top == NEG_INF<T> ? T(0) : top + Mma<T>::log2(total);
   const int64_t head = int64_t(bh % s.Hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
   T *y = a.y + ((int64_t(bh / s.Hk) * s.Tq + i) * s.Hk * s.G + head) * s.D;
-  for (int d = lane; d < s.D; d += 64) {
+  for (int d0 = 0; d0 < s.D; d0 += 64) {
+    const int d = std::min(d0 + lane, s.D - 1);
     T v = 0;
+#pragma unroll 8
     for (int k = 0; k < a.splits; ++k)
-      v = fma(a.part_acc[((slot + k) * 16 + n) * s.D + d],
-              Mma<T>::exp2(a.part_stat[(slot + k) * 32 + n] - base), v);
-    y[d] = any ? v / total : T(0);
+      v = fma(a.part_acc[((slot + k) * 16 + n) * s.D + d], __shfl(weight, k), v);
+    if (d0 + lane < s.D)
+      y[d] = any ? v / total : T(0);
   }
 }
 
@@ -795,11 +841,11 @@ int key_splits(const AttnShape &s) {
   const int64_t groups = int64_t(s.B) * s.Hk * ((s.rows + 15) / 16);
   const int64_t want = int64_t(device_cu_count()) * 4 / std::max<int64_t>(groups, 1);
   const int64_t most = s.Tk / (32 * AT_WAVES * 2);
-  return int(std::max<int64_t>(1, std::min({want, most, int64_t(256)})));
+  return int(std::max<int64_t>(1, std::min({want, most, int64_t(64)})));
 }
 
 // Workgroups for each (sequence, key head) that the other kernels left, or not.
-uint32_t left_groups(uint32_t bhs) { return std::clamp<uint32_t>(2048 / bhs, 1, 32); }
+uint32_t left_groups(uint32_t bhs) { return std::clamp<uint32_t>(1024 / bhs, 1, 32); }
 
 template <class T> void run_attention(AttnFwd<T> &a) {
   const AttnShape &s = a.s;

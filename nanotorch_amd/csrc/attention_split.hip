@@ -411,6 +411,8 @@ struct SplitFwd {
   float scale2;
   int vec;
   AttnGate gate;
+  int parts;                     // of the keys; over one: sums [part][bh, row][D] and
+  float *sums, *tops;            // maxima, sums of p [part][2][bh, row]
 };
 
 template <int DB>
@@ -421,9 +423,11 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = uint32_t(s.rows + SF_ROWS - 1) / SF_ROWS;
+  const uint32_t parts = uint32_t(a.parts);
   uint32_t bh, item;
-  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles, bh, item);
-  const int tile = int(tiles - 1 - item); // the most keys first
+  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles * parts, bh, item);
+  const int tile = int(tiles - 1 - item / parts); // the most keys first
+  const int part = int(item % parts);
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, threadIdx.x == 0, keys, first);
@@ -447,9 +451,11 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
                stage + (j < DB ? 0 : 2 * CH) + p * 1024, lane);
     }
   };
-  const int steps = (group_end + SA_TILE - 1) / SA_TILE;
-  if (steps)
-    issue(lds[0], 0);
+  const int all_steps = (group_end + SA_TILE - 1) / SA_TILE;
+  const int per = (all_steps + a.parts - 1) / a.parts;
+  const int begin = min(part * per, all_steps), steps = min(begin + per, all_steps);
+  if (begin < steps)
+    issue(lds[begin & 1], begin);
   // own row: one power of two, and the sign of the scale
   half8 qh[2 * DB], ql[2 * DB];
   float q_scale;
@@ -486,7 +492,7 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
   const float c = fabsf(a.scale2);
   floatx16 acc[DB]{};
   float m = -SA_INF, l = 0.f;
-  for (int it = 0; it < steps; ++it) {
+  for (int it = begin; it < steps; ++it) {
     stage_ready();
     if (it + 1 < steps)
       issue(lds[(it + 1) & 1], it + 1);
@@ -549,12 +555,66 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
   if (!live)
     return;
   l += __shfl_xor(l, 32);
+  if (a.parts > 1) {
+    const int64_t rows = int64_t(s.B) * s.Hk * s.rows, at = int64_t(bh) * s.rows + row;
+    store_row<DB>(a.sums + (part * rows + at) * s.D, acc, 1.f, s.D, h);
+    if (h == 0) {
+      a.tops[2 * part * rows + at] = m;
+      a.tops[(2 * part + 1) * rows + at] = l;
+    }
+    return;
+  }
   const uint32_t i = s.by_group.div(uint32_t(row));
   const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
   store_row<DB>(a.y + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D, acc,
                 limit > 0 ? 1.f / l : 0.f, s.D, h);
   if (a.lse && h == 0)
     a.lse[int64_t(bh) * s.rows + row] = m == -SA_INF ? 0.f : m + (log2f(l) - 14.f);
+}
+
+// Rows whose keys were split into at most 64 parts: a wave for each row.
+__global__ __launch_bounds__(256) void attn_split_join_kernel(const SplitFwd a) {
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63;
+  // a workgroup's rows belong to one (sequence, key head)
+  const uint32_t groups = uint32_t(s.rows + 3) / 4, bh = blockIdx.x / groups;
+  if (gate_set(a.gate, bh))
+    return;
+  const int row = int(blockIdx.x - bh * groups) * 4 + int(threadIdx.x >> 6);
+  if (row >= s.rows)
+    return;
+  const int64_t rows = int64_t(s.B) * s.Hk * s.rows, at = int64_t(bh) * s.rows + row;
+  float m = -SA_INF, l = 0.f;
+  if (lane < a.parts) {
+    m = a.tops[2 * lane * rows + at];
+    l = a.tops[(2 * lane + 1) * rows + at];
+  }
+  float top = m;
+#pragma unroll
+  for (int o = 32; o; o >>= 1)
+    top = fmaxf(top, __shfl_xor(top, o));
+  const float weight = __builtin_amdgcn_exp2f(m - (top == -SA_INF ? 0.f : top));
+  float total = l * weight;
+#pragma unroll
+  for (int o = 32; o; o >>= 1)
+    total += __shfl_xor(total, o);
+  int keys, first;
+  sequence(s, int(bh) / s.Hk, false, keys, first);
+  const uint32_t i = s.by_group.div(uint32_t(row));
+  const float k = seen(s, keys, first, int(i)) > 0 ? 1.f / total : 0.f;
+  const int64_t head = int64_t(bh % uint32_t(s.Hk)) * s.G + (uint32_t(row) - i * uint32_t(s.G));
+  float *y = a.y + ((int64_t(bh / uint32_t(s.Hk)) * s.Tq + i) * s.Hk * s.G + head) * s.D;
+  for (int d0 = 0; d0 < s.D; d0 += 64) {
+    const int d = min(d0 + lane, s.D - 1);
+    float v = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < a.parts; ++p)
+      v = fmaf(a.sums[(p * rows + at) * s.D + d], __shfl(weight, p), v);
+    if (d0 + lane < s.D)
+      y[d] = v * k;
+  }
+  if (a.lse && lane == 0)
+    a.lse[at] = top == -SA_INF ? 0.f : top + (log2f(total) - 14.f);
 }
 
 // --------------------------------------------------------------- backward
@@ -570,8 +630,8 @@ struct SplitBwd {
   const float *q_scale, *k_scale, *v_scale; // [bh, tiles]
   const float *stats;                       // [bh, units][SA_STATS]
   int q_tiles, k_tiles;                     // of 64 rows
-  float *dq, *dk, *dv;                      // dk, dv: [parts] of the result's size
-  int parts;
+  float *dq, *dk, *dv;                      // [parts] of the result's size each
+  int q_parts, parts;                       // of dq's keys, of dk's and dv's rows
   float scale, scale2;
   AttnGate gate;
 };
@@ -595,9 +655,10 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles = uint32_t(s.rows + SB_ROWS<DB> - 1) / SB_ROWS<DB>;
+  const uint32_t parts = uint32_t(a.q_parts);
   uint32_t bh, item;
-  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles, bh, item);
-  const int tile = int(tiles - 1 - item);
+  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles * parts, bh, item);
+  const int tile = int(tiles - 1 - item / parts), part = int(item % parts);
   const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
   int keys, first;
   sequence(s, b, false, keys, first);
@@ -622,9 +683,11 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
                  stage + p * 1024, lane);
     }
   };
-  const int steps = (group_end + SA_UNIT - 1) / SA_UNIT;
-  if (steps)
-    issue(lds[0], 0);
+  const int all_steps = (group_end + SA_UNIT - 1) / SA_UNIT;
+  const int per = (all_steps + a.q_parts - 1) / a.q_parts;
+  const int begin = min(part * per, all_steps), steps = min(begin + per, all_steps);
+  if (begin < steps)
+    issue(lds[begin & 1], begin);
   half8 qh[2 * DB], ql[2 * DB], gh[2 * DB], gl[2 * DB];
   const int64_t unit = int64_t(bh) * a.q_tiles * 2 + (on ? row0 / SA_UNIT : 0);
   load_own<DB>(a.q_row + unit * CH, qh, ql, lane);
@@ -634,7 +697,7 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
   const int limit = reinterpret_cast<const int *>(st)[3 * SA_UNIT];
   const float c = a.scale2 * a.q_scale[unit / 2];
   floatx16 acc[DB]{};
-  for (int it = 0; it < steps; ++it) {
+  for (int it = begin; it < steps; ++it) {
     stage_ready();
     if (it + 1 < steps)
       issue(lds[(it + 1) & 1], it + 1);
@@ -671,7 +734,8 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
     return;
   const uint32_t i = s.by_group.div(uint32_t(row));
   const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
-  store_row<DB>(a.dq + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D, acc,
+  const int64_t size = int64_t(s.B) * s.Hk * s.rows * s.D;
+  store_row<DB>(a.dq + part * size + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D, acc,
                 a.scale * g_scale, s.D, h);
 }
 
@@ -816,32 +880,26 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
     store_row<DB>(a.dv + at, dv, 1.f, s.D, h);
 }
 
-// The parts of dk and dv added up in order.  What the gate left to other kernels
-// is not written.
-__global__ __launch_bounds__(256) void attn_split_parts_kernel(const SplitBwd a, float *dk,
-                                                               float *dv) {
-  const AttnShape &s = a.s;
-  const int64_t size = int64_t(s.B) * s.Tk * s.Hk * s.D;
-  const uint32_t bh = blockIdx.y;
-  if (gate_set(a.gate, bh))
+// The parts of a gradient [B, T, Hk G, D] added up in order; what the gate left to
+// other kernels is not written.
+__global__ __launch_bounds__(256) void attn_split_parts_kernel(const float *parts, float *out,
+                                                               int count, int B, int T, int Hk,
+                                                               int GD, AttnGate gate) {
+  const uint32_t groups = uint32_t((int64_t(T) * GD + 255) / 256), bh = blockIdx.x / groups;
+  if (gate_set(gate, bh))
     return;
-  const int64_t b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t key = i / s.D;
-  if (key >= s.Tk)
+  const int64_t i = int64_t(blockIdx.x - bh * groups) * 256 + threadIdx.x;
+  const int64_t t = i / GD;
+  if (t >= T)
     return;
-  const int64_t at = ((b * s.Tk + key) * s.Hk + hk) * s.D + i % s.D;
-  float x = 0.f, y = 0.f;
-  for (int p = 0; p < a.parts; ++p) {
-    if (dk)
-      x += a.dk[p * size + at];
-    if (dv)
-      y += a.dv[p * size + at];
-  }
-  if (dk)
-    dk[at] = x;
-  if (dv)
-    dv[at] = y;
+  const int64_t b = bh / uint32_t(Hk), hk = bh % uint32_t(Hk);
+  const int64_t at = ((b * T + t) * Hk + hk) * GD + (i - t * GD);
+  const int64_t size = int64_t(B) * T * Hk * GD;
+  float x = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < count; ++p)
+    x += parts[p * size + at];
+  out[at] = x;
 }
 
 // ------------------------------------------------------------------- host
@@ -849,6 +907,21 @@ __global__ __launch_bounds__(256) void attn_split_parts_kernel(const SplitBwd a,
 namespace {
 
 int tiles_of(int rows) { return (rows + SA_TILE - 1) / SA_TILE; }
+
+// Into how many parts `groups` workgroups' `steps` steps are split: one where there
+// are two for each CU, else as many as make that, of at least four steps.
+int parts_of(int64_t groups, int64_t steps) {
+  const int64_t want = 2 * int64_t(device_cu_count()) / groups;
+  return int(std::max<int64_t>(1, std::min<int64_t>({want, steps / 4, 32})));
+}
+
+void add_parts(const float *parts, float *out, int count, const AttnShape &s, int T, int G,
+               const AttnGate &gate) {
+  const int64_t groups = (int64_t(T) * G * s.D + 255) / 256;
+  attn_split_parts_kernel<<<dim3(uint32_t(groups * s.B * s.Hk)), 256, 0, stream()>>>(
+      parts, out, count, s.B, T, s.Hk, G * s.D, gate);
+  NT_LAUNCH_CHECK();
+}
 
 template <class F> void dispatch_blocks(int D, F &&f) {
   switch ((D + 31) / 32) {
@@ -910,9 +983,19 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     f.scale2 = a.scale2;
     f.vec = a.vec;
     f.gate = a.gate;
-    attn_split_fwd_kernel<DB><<<dim3(bhs * uint32_t((s.rows + SF_ROWS - 1) / SF_ROWS)),
-                                64 * SF_WAVES, 0, stream()>>>(f);
+    const uint32_t groups = bhs * uint32_t((s.rows + SF_ROWS - 1) / SF_ROWS);
+    f.parts = parts_of(groups, tiles);
+    const size_t rows = size_t(bhs) * size_t(s.rows), kept = f.parts > 1 ? size_t(f.parts) : 0;
+    DeviceScratch sums(kept * rows * size_t(s.D + 2) * sizeof(float));
+    f.sums = sums.get<float>();
+    f.tops = f.sums + kept * rows * size_t(s.D);
+    attn_split_fwd_kernel<DB>
+        <<<dim3(groups * uint32_t(f.parts)), 64 * SF_WAVES, 0, stream()>>>(f);
     NT_LAUNCH_CHECK();
+    if (f.parts > 1) {
+      attn_split_join_kernel<<<dim3(bhs * uint32_t((s.rows + 3) / 4)), 256, 0, stream()>>>(f);
+      NT_LAUNCH_CHECK();
+    }
   });
 }
 
@@ -959,25 +1042,28 @@ void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
     f.q_tiles = qt, f.k_tiles = kt;
     f.scale = a.scale, f.scale2 = a.scale2;
     f.gate = a.gate;
-    f.parts = 1;
     if (a.dq) {
-      f.dq = a.dq;
-      attn_split_dq_kernel<DB><<<dim3(bhs * uint32_t((s.rows + SB_ROWS<DB> - 1) / SB_ROWS<DB>)),
-                                 64 * SB_WAVES<DB>, 0, stream()>>>(f);
+      const uint32_t groups = bhs * uint32_t((s.rows + SB_ROWS<DB> - 1) / SB_ROWS<DB>);
+      f.q_parts = parts_of(groups, 2 * kt);
+      const size_t size = size_t(bhs) * size_t(s.rows) * size_t(s.D);
+      DeviceScratch sums(f.q_parts > 1 ? size * size_t(f.q_parts) * sizeof(float) : 0);
+      f.dq = f.q_parts > 1 ? sums.get<float>() : a.dq;
+      attn_split_dq_kernel<DB>
+          <<<dim3(groups * uint32_t(f.q_parts)), 64 * SB_WAVES<DB>, 0, stream()>>>(f);
       NT_LAUNCH_CHECK();
+      if (f.q_parts > 1)
+        add_parts(f.dq, a.dq, f.q_parts, s, s.Tq, s.G, a.gate);
     }
     if (a.dk || a.dv) {
-      // Workgroups of different lengths, one to two at a time on a CU: four for
-      // each CU even them out.  Fewer key tiles than that share their rows.
-      const int64_t groups = int64_t(bhs) * ((s.Tk + SB_ROWS<DB> - 1) / SB_ROWS<DB>);
-      const int units = (s.rows + SA_UNIT - 1) / SA_UNIT;
-      f.parts = int(std::max<int64_t>(
-          1, std::min<int64_t>({int64_t(device_cu_count()) * 4 / groups, units / 8, 16})));
+      // Few tiles of keys under a causal mask, each of another length, even out
+      // with shorter parts.
+      const uint32_t groups = bhs * uint32_t((s.Tk + SB_ROWS<DB> - 1) / SB_ROWS<DB>);
+      f.parts = parts_of(s.causal ? (groups + 1) / 2 : groups, 2 * qt);
       const size_t size = size_t(s.B) * size_t(s.Tk) * size_t(s.Hk) * size_t(s.D);
       DeviceScratch sums(f.parts > 1 ? 2 * size * size_t(f.parts) * sizeof(float) : 0);
       f.dk = a.dk && f.parts > 1 ? sums.get<float>() : a.dk;
       f.dv = a.dv && f.parts > 1 ? sums.get<float>() + size * size_t(f.parts) : a.dv;
-      const dim3 grid(uint32_t(groups * f.parts));
+      const dim3 grid(groups * uint32_t(f.parts));
       if constexpr (DB <= 2) {
         attn_split_dkv_kernel<DB, true, true><<<grid, 64 * SB_WAVES<DB>, 0, stream()>>>(f);
         NT_LAUNCH_CHECK();
@@ -992,10 +1078,10 @@ void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
         }
       }
       if (f.parts > 1) {
-        const int64_t each = int64_t(s.Tk) * s.D;
-        attn_split_parts_kernel<<<dim3(uint32_t((each + 255) / 256), bhs), 256, 0, stream()>>>(
-            f, a.dk, a.dv);
-        NT_LAUNCH_CHECK();
+        if (a.dk)
+          add_parts(f.dk, a.dk, f.parts, s, s.Tk, 1, a.gate);
+        if (a.dv)
+          add_parts(f.dv, a.dv, f.parts, s, s.Tk, 1, a.gate);
       }
     }
   });
