@@ -44,6 +44,7 @@
 namespace nt {
 
 constexpr int AT_WAVES = 4;
+constexpr int AT_MAX_D = 256;
 
 template <class T> struct Mma;
 template <> struct Mma<float> {
@@ -76,6 +77,12 @@ template <class T, int DP> struct Frag {
 #pragma unroll
     for (int c = 0; c < C; ++c)
       v[c] = piece(row, 4 * N * c + N * h, D, live, vec);
+  }
+  // A row of DP elements, aligned: no branch, so that many loads go out together.
+  __device__ __forceinline__ void load_whole(const T *row, int h) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      v[c] = *reinterpret_cast<const typename RowVec<T>::V *>(row + 4 * N * c + N * h);
   }
 };
 
@@ -143,6 +150,11 @@ template <class T, int DP> struct Items {
 #pragma unroll
     for (int c = 0; c < C; ++c)
       v[r][c] = piece(p, N * (16 * c + n), D, on, vec);
+  }
+  __device__ __forceinline__ void load_whole(int r, const T *p, int n) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      v[r][c] = *reinterpret_cast<const typename RowVec<T>::V *>(p + N * (16 * c + n));
   }
 };
 
@@ -307,7 +319,22 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
     Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> k[TILES];
     Items<T, SC> v[TILES];
   };
+  constexpr int STEP = 16 * TILES;
+  const bool whole = a.vec && s.D == DP;
   auto load = [&](Block &x, int j0, int to) {
+    if (whole && j0 + STEP <= to) {
+#pragma unroll
+      for (int i = 0; i < TILES; ++i)
+        if constexpr (IN_REGISTERS<T, DP>)
+          x.k[i].load_whole(kp + int64_t(j0 + 16 * i + n) * a.k.sOuter, h);
+#pragma unroll
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x.v[i].load_whole(
+              r, vp + int64_t(j0 + 16 * i + M::row(h, r)) * a.v.sOuter + col0, n);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i + n;
@@ -374,7 +401,6 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   };
   // The next block is on its way while one is computed with: few rows over many
   // keys wait for memory.  (A block past the last one loads nothing.)
-  constexpr int STEP = 16 * TILES;
   auto bound = [&](int blk) { return blk < stop ? end : 0; };
   int blk = int(split) * per + wave;
   if (blk < stop) {
@@ -464,19 +490,17 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_left_kernel(
   }
 }
 
-// Rows whose keys were split: each wave one row.
+// Rows whose keys were split into at most 64 parts: a workgroup for each row, its
+// waves every fourth part, joined in order.
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
   const AttnShape &s = a.s;
-  const int lane = threadIdx.x & 63;
-  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= int64_t(s.B) * s.Hk * s.rows)
-    return;
-  const int bh = int(item / s.rows), row = int(item % s.rows);
+  __shared__ T lds[3][AT_MAX_D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int bh = int(blockIdx.x / uint32_t(s.rows)), row = int(blockIdx.x % uint32_t(s.rows));
   const int tiles = (s.rows + 15) / 16, n = row & 15;
   // the slots are numbered with the tiles backwards, as their workgroups were
   const int64_t slot = (int64_t(bh) * tiles + (tiles - 1 - row / 16)) * a.splits;
-  // a lane for each part, of at most 64
   T m = NEG_INF<T>, l = 0;
   if (lane < a.splits) {
     m = a.part_stat[(slot + lane) * 32 + n];
@@ -491,22 +515,39 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
 #pragma unroll
   for (int o = 32; o; o >>= 1)
     total += __shfl_xor(total, o);
+  T v[AT_MAX_D / 64];
+#pragma unroll
+  for (int c = 0; c < AT_MAX_D / 64; ++c) {
+    v[c] = 0;
+    const int d = c * 64 + lane;
+#pragma unroll 4
+    for (int k = wave; k < a.splits; k += 4) {
+      const T w = __shfl(weight, k);
+      if (d < s.D)
+        v[c] = fma(a.part_acc[((slot + k) * 16 + n) * s.D + d], w, v[c]);
+    }
+    if (wave && d < s.D)
+      lds[wave - 1][d] = v[c];
+  }
+  __syncthreads();
+  if (wave)
+    return;
   int keys, first;
   sequence(s, bh / s.Hk, false, keys, first);
   const uint32_t i = s.by_group.div(uint32_t(row));
   const bool any = seen(s, keys, first, int(i)) > 0;
   if (a.lse && lane == 0)
-    a.lse[item] = top == NEG_INF<T> ? T(0) : top + Mma<T>::log2(total);
+    a.lse[int64_t(bh) * s.rows + row] = top == NEG_INF<T> ? T(0) : top + Mma<T>::log2(total);
   const int64_t head = int64_t(bh % s.Hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
   T *y = a.y + ((int64_t(bh / s.Hk) * s.Tq + i) * s.Hk * s.G + head) * s.D;
-  for (int d0 = 0; d0 < s.D; d0 += 64) {
-    const int d = std::min(d0 + lane, s.D - 1);
-    T v = 0;
-#pragma unroll 8
-    for (int k = 0; k < a.splits; ++k)
-      v = fma(a.part_acc[((slot + k) * 16 + n) * s.D + d], __shfl(weight, k), v);
-    if (d0 + lane < s.D)
-      y[d] = any ? v / total : T(0);
+#pragma unroll
+  for (int c = 0; c < AT_MAX_D / 64; ++c) {
+    const int d = c * 64 + lane;
+    if (d < s.D) {
+      for (int w = 0; w < 3; ++w)
+        v[c] += lds[w][d];
+      y[d] = any ? v[c] / total : T(0);
+    }
   }
 }
 
@@ -735,8 +776,6 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const Attn
 
 namespace {
 
-constexpr int AT_MAX_D = 256;
-
 void check_heads(const nt_view *v, const nt_view *like, const char *what) {
   check_view(v, what);
   if (v->dtype != like->dtype)
@@ -876,8 +915,8 @@ template <class T> void run_attention(AttnFwd<T> &a) {
   });
   NT_LAUNCH_CHECK();
   if (a.splits > 1) {
-    attn_join_kernel<T><<<dim3(uint32_t((int64_t(s.B) * s.Hk * s.rows + 3) / 4)), 256, 0,
-                          stream()>>>(a);
+    attn_join_kernel<T>
+        <<<dim3(uint32_t(int64_t(s.B) * s.Hk * s.rows)), 256, 0, stream()>>>(a);
     NT_LAUNCH_CHECK();
   }
 }

@@ -604,15 +604,19 @@ __global__ __launch_bounds__(256) void attn_split_join_kernel(const SplitFwd a) 
   const float k = seen(s, keys, first, int(i)) > 0 ? 1.f / total : 0.f;
   const int64_t head = int64_t(bh % uint32_t(s.Hk)) * s.G + (uint32_t(row) - i * uint32_t(s.G));
   float *y = a.y + ((int64_t(bh / uint32_t(s.Hk)) * s.Tq + i) * s.Hk * s.G + head) * s.D;
-  for (int d0 = 0; d0 < s.D; d0 += 64) {
-    const int d = min(d0 + lane, s.D - 1);
-    float v = 0.f;
+  // both halves of a row of up to 128 at once
+  float v[2] = {0.f, 0.f};
 #pragma unroll 8
-    for (int p = 0; p < a.parts; ++p)
-      v = fmaf(a.sums[(p * rows + at) * s.D + d], __shfl(weight, p), v);
-    if (d0 + lane < s.D)
-      y[d] = v * k;
+  for (int p = 0; p < a.parts; ++p) {
+    const float w = __shfl(weight, p);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      v[c] = fmaf(a.sums[(p * rows + at) * s.D + min(64 * c + lane, s.D - 1)], w, v[c]);
   }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (64 * c + lane < s.D)
+      y[64 * c + lane] = v[c] * k;
   if (a.lse && lane == 0)
     a.lse[at] = top == -SA_INF ? 0.f : top + (log2f(total) - 14.f);
 }
