@@ -135,7 +135,7 @@ __device__ __forceinline__ typename RowVec<T>::V piece(const T *p, int d, int D,
 // attention_split.hip: whether its kernels take a product of this shape, and
 // their launches.  The forward launch leaves a.gate for the kernels that follow
 // it; `words` is its memory, which must outlive them.
-bool split_takes(const AttnShape &s);
+bool split_takes(const AttnShape &s, bool backward);
 size_t split_gate_words(const AttnShape &s, bool backward);
 void run_split(AttnFwd<float> &a, uint32_t *words);
 void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words);

@@ -889,7 +889,7 @@ uint32_t left_groups(uint32_t bhs) { return std::clamp<uint32_t>(1024 / bhs, 1, 
 template <class T> void run_attention(AttnFwd<T> &a) {
   const AttnShape &s = a.s;
   if constexpr (std::is_same_v<T, float>)
-    if (split_takes(s)) {
+    if (split_takes(s, false)) {
       DeviceScratch words(split_gate_words(s, false) * sizeof(uint32_t));
       run_split(a, words.get<uint32_t>());
       a.splits = 1;
@@ -927,7 +927,7 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a, const T *y) {
   DeviceScratch delta(size_t(rows) * sizeof(T));
   a.delta = delta.template get<T>();
   if constexpr (std::is_same_v<T, float>)
-    if (split_takes(s)) {
+    if (split_takes(s, true)) {
       DeviceScratch words(split_gate_words(s, true) * sizeof(uint32_t));
       run_split_bwd(a, y, words.get<uint32_t>());
       const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk), groups = left_groups(bhs);

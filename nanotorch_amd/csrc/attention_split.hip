@@ -943,13 +943,17 @@ template <class F> void dispatch_blocks(int D, F &&f) {
 } // namespace
 
 // Float32 with heads of up to 128 elements (a wider one's planes outgrow the
-// registers), from the size on at which packing and half-empty tiles cost less than
-// the matrix cores save.
-bool split_takes(const AttnShape &s) {
-  if (s.D > 128 || s.rows < 64 || s.Tk < 64)
+// registers), from the size on at which packing, another launch or two and half-empty
+// tiles cost less than the matrix cores save.  Both sides in us, B, Tq, Tk, H, Hk, D,
+// this kind second.  Forward: 8 256 256 8 8 64 24 and 29, 1 1024 1024 4 4 64 30 and
+// 31, 4 2048 2048 16 16 64 about 470 and 165; of few rows 4 16 4096 32 8 128 85 and
+// 110.  Backward: 1 256 256 16 16 64 33 and 48, 16 128 128 8 8 64 48 and 46, 1 512 512
+// 8 8 64 52 and 52, 1 1024 1024 4 4 64 89 and 53, 8 1 8192 64 2 128 870 and 237.
+bool split_takes(const AttnShape &s, bool backward) {
+  if (s.D > 128)
     return false;
-  const double pairs = double(s.B) * s.Hk * s.rows * s.Tk * s.D;
-  return pairs >= double(1 << 24);
+  const double work = double(s.B) * s.Hk * s.rows * s.Tk * s.D;
+  return backward ? work >= double(1 << 27) : s.rows >= 128 && work >= 3.0 * double(1 << 27);
 }
 
 size_t split_gate_words(const AttnShape &s, bool backward) {
