@@ -277,8 +277,8 @@ template <class T, int DP> constexpr int FWD_TILES = DP * sizeof(T) <= 256 ? 2 :
 template <class T, int DP>
 constexpr int FWD_WAVES = sizeof(T) == 8 && DP * sizeof(T) == 512 ? 1 : 2;
 
-// Tile `item` of a (sequence, key head).
-template <class T, int DP>
+// Tile `item` of a (sequence, key head).  WHOLE: rows of DP elements, aligned.
+template <class T, int DP, bool WHOLE>
 __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, uint32_t item,
                                               uint32_t split, int col0) {
   using M = Mma<T>;
@@ -314,42 +314,37 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   const int blocks = (end + 16 * TILES - 1) / (16 * TILES);
   const int per = (blocks + a.splits - 1) / a.splits;
   const int stop = std::min(blocks, int(split + 1) * per);
-  // A block's keys (rows in registers only) and values.
-  struct Block {
+  // A block's keys (of rows in registers) and its values.
+  struct Keys {
     Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> k[TILES];
-    Items<T, SC> v[TILES];
   };
   constexpr int STEP = 16 * TILES;
-  const bool whole = a.vec && s.D == DP;
-  auto load = [&](Block &x, int j0, int to) {
-    if (whole && j0 + STEP <= to) {
+  // WHOLE: past the end the last key again, which no row sees there
+  auto load_keys = [&](Keys &x, int j0) {
 #pragma unroll
-      for (int i = 0; i < TILES; ++i)
-        if constexpr (IN_REGISTERS<T, DP>)
-          x.k[i].load_whole(kp + int64_t(j0 + 16 * i + n) * a.k.sOuter, h);
-#pragma unroll
-      for (int i = 0; i < TILES; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x.v[i].load_whole(
-              r, vp + int64_t(j0 + 16 * i + M::row(h, r)) * a.v.sOuter + col0, n);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-      const int j = j0 + 16 * i + n;
-      if constexpr (IN_REGISTERS<T, DP>)
-        x.k[i].load(kp + int64_t(j) * a.k.sOuter, s.D, j < to, a.vec, h);
-    }
+    for (int i = 0; i < TILES; ++i)
+      if constexpr (IN_REGISTERS<T, DP>) {
+        const int j = j0 + 16 * i + n;
+        if constexpr (WHOLE)
+          x.k[i].load_whole(kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, h);
+        else
+          x.k[i].load(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
+      }
+  };
+  Items<T, SC> v[TILES];
+  auto load_values = [&](int j0) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = j0 + 16 * i + M::row(h, r);
-        x.v[i].load(r, vp + int64_t(j) * a.v.sOuter + col0, s.D - col0, j < to, a.vec, n);
+        if constexpr (WHOLE)
+          v[i].load_whole(r, vp + int64_t(std::min(j, end - 1)) * a.v.sOuter + col0, n);
+        else
+          v[i].load(r, vp + int64_t(j) * a.v.sOuter + col0, s.D - col0, j < end, a.vec, n);
       }
   };
-  auto take = [&](const Block &x, int j0) {
+  auto take = [&](const Keys &x, int j0) {
     T z[TILES][4];
     bool vis[TILES][4];
     T top = NEG_INF<T>;
@@ -391,31 +386,31 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i;
-      if (j + 16 > all && !all_finite<T, SC>(x.v[i]))
+      if (j + 16 > all && !all_finite<T, SC>(v[i]))
         sums.add_visible(z[i], vis[i], s.D - col0, lane, [&](int item) {
           return j + item < end ? vp + int64_t(j + item) * a.v.sOuter + col0 : nullptr;
         });
       else
-        sums.add(z[i], x.v[i]);
+        sums.add(z[i], v[i]);
     }
   };
-  // The next block is on its way while one is computed with: few rows over many
-  // keys wait for memory.  (A block past the last one loads nothing.)
-  auto bound = [&](int blk) { return blk < stop ? end : 0; };
+  // A block's values and the next block's keys are on their way while its scores
+  // are formed: few rows over many keys wait for memory.
   int blk = int(split) * per + wave;
   if (blk < stop) {
-    Block x, y;
-    load(x, blk * STEP, end);
-    for (;;) {
-      load(y, (blk + AT_WAVES) * STEP, bound(blk + AT_WAVES));
-      take(x, blk * STEP);
-      if ((blk += AT_WAVES) >= stop)
-        break;
-      load(x, (blk + AT_WAVES) * STEP, bound(blk + AT_WAVES));
-      take(y, blk * STEP);
-      if ((blk += AT_WAVES) >= stop)
-        break;
-    }
+    Keys x, y;
+    load_keys(x, blk * STEP);
+    auto turn = [&](const Keys &now, Keys &next) {
+      const bool more = blk + AT_WAVES < stop;
+      load_values(blk * STEP);
+      if (more)
+        load_keys(next, (blk + AT_WAVES) * STEP);
+      take(now, blk * STEP);
+      blk += AT_WAVES;
+      return more;
+    };
+    while (turn(x, y) && turn(y, x))
+      ;
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -461,7 +456,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   });
 }
 
-template <class T, int DP>
+template <class T, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * AT_WAVES, (FWD_WAVES<T, DP>)) void attn_fwd_kernel(
     const AttnFwd<T> a) {
   constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
@@ -472,7 +467,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, (FWD_WAVES<T, DP>)) void attn_fwd_ke
   const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
   item /= GROUPS;
   if (col0 < a.s.D)
-    attn_fwd_tile<T, DP>(a, bh, item / splits, item % splits, col0);
+    attn_fwd_tile<T, DP, WHOLE>(a, bh, item / splits, item % splits, col0);
 }
 
 // What the kernels on half-precision planes left: the tiles of each (sequence,
@@ -486,7 +481,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_left_kernel(
   const uint32_t tiles = uint32_t(a.s.rows + 15) / 16;
   for (uint32_t t = blockIdx.x % groups; t < tiles; t += groups) {
     __syncthreads();
-    attn_fwd_tile<float, DP>(a, bh, t, 0, 0);
+    attn_fwd_tile<float, DP, false>(a, bh, t, 0, 0);
   }
 }
 
@@ -909,9 +904,11 @@ template <class T> void run_attention(AttnFwd<T> &a) {
   a.part_acc = acc.template get<T>();
   a.part_stat = stat.template get<T>();
   dispatch_width<T>(s.D, [&]<int DP>() {
-    attn_fwd_kernel<T, DP>
-        <<<dim3(uint32_t(tiles * a.splits * COLUMN_GROUPS<T, DP>)), 64 * AT_WAVES, 0,
-           stream()>>>(a);
+    const dim3 grid(uint32_t(tiles * a.splits * COLUMN_GROUPS<T, DP>));
+    if (a.vec && s.D == DP)
+      attn_fwd_kernel<T, DP, true><<<grid, 64 * AT_WAVES, 0, stream()>>>(a);
+    else
+      attn_fwd_kernel<T, DP, false><<<grid, 64 * AT_WAVES, 0, stream()>>>(a);
   });
   NT_LAUNCH_CHECK();
   if (a.splits > 1) {

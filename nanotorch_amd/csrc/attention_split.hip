@@ -948,11 +948,14 @@ template <class F> void dispatch_blocks(int D, F &&f) {
 // this kind second.  Forward: 8 256 256 8 8 64 24 and 29, 1 1024 1024 4 4 64 30 and
 // 31, 4 2048 2048 16 16 64 about 470 and 165; of few rows 4 16 4096 32 8 128 85 and
 // 110.  Backward: 1 256 256 16 16 64 33 and 48, 16 128 128 8 8 64 48 and 46, 1 512 512
-// 8 8 64 52 and 52, 1 1024 1024 4 4 64 89 and 53, 8 1 8192 64 2 128 870 and 237.
+// 8 8 64 52 and 52, 1 1024 1024 4 4 64 89 and 53, 8 1 8192 64 2 128 870 and 237; of
+// long axes with little beside them 1 64 2000 8 8 64 88 and 38.
 bool split_takes(const AttnShape &s, bool backward) {
   if (s.D > 128)
     return false;
   const double work = double(s.B) * s.Hk * s.rows * s.Tk * s.D;
+  if (backward && std::max(s.rows, s.Tk) >= 640 && work >= double(1 << 25))
+    return true;
   return backward ? work >= double(1 << 27) : s.rows >= 128 && work >= 3.0 * double(1 << 27);
 }
 
