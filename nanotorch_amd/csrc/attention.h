@@ -55,8 +55,8 @@ template <class T> struct AttnFwd {
 
 template <class T> struct AttnBwd {
   AttnShape s;
-  Rows<const T> q, k, v, g;
-  const T *lse, *delta; // [B, Hk, rows]
+  Rows<const T> q, k, v, g, y;
+  const T *lse;         // [B, Hk, rows]
   T *dq;                // [B, Tq, H, D]
   T *dk, *dv;           // [B, Tk, Hk, D]; either may be null
   T scale, scale2;
@@ -138,6 +138,6 @@ __device__ __forceinline__ typename RowVec<T>::V piece(const T *p, int d, int D,
 bool split_takes(const AttnShape &s, bool backward);
 size_t split_gate_words(const AttnShape &s, bool backward);
 void run_split(AttnFwd<float> &a, uint32_t *words);
-void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words);
+void run_split_bwd(AttnBwd<float> &a, uint32_t *words);
 
 } // namespace nt

@@ -98,6 +98,18 @@ __device__ __forceinline__ typename Mma<T>::V4 dots(const Frag<T, DP> &items,
   return s;
 }
 
+// The sum of a lane's elements' products.
+template <class T, int DP>
+__device__ __forceinline__ T times(const Frag<T, DP> &a, const Frag<T, DP> &b) {
+  T sum = 0;
+#pragma unroll
+  for (int c = 0; c < Frag<T, DP>::C; ++c)
+#pragma unroll
+    for (int e = 0; e < Frag<T, DP>::N; ++e)
+      sum = fma(a.v[c][e], b.v[c][e], sum);
+  return sum;
+}
+
 // Own rows of up to 512 bytes stay in registers.  Longer ones are read again with
 // every tile of items, 256 bytes at a time, and a workgroup keeps only 512 bytes
 // of its sums' columns: several workgroups form the same probabilities, each for
@@ -137,6 +149,29 @@ template <class T, int DP> struct Own {
       }
       return s;
     }
+  }
+  // As dots, and the lane's item row times `other`, elements of its own.
+  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, const T *other, int D, bool on,
+                                                      int vec, int h, T &product) const {
+    constexpr int W = IN_REGISTERS<T, DP> ? DP : int(256 / sizeof(T));
+    typename Mma<T>::V4 s{};
+    product = 0;
+#pragma unroll 1
+    for (int d = 0; d < D; d += W) {
+      Frag<T, W> x, y, o;
+      x.load(item + d, D - d, on, vec, h);
+      y.load(other + d, D - d, on, vec, h);
+      if constexpr (IN_REGISTERS<T, DP>) {
+        s = nt::dots<T, W>(x, f);
+      } else {
+        o.load(row + d, D - d, live, vec, h);
+        s += nt::dots<T, W>(x, o);
+      }
+      product += times<T, W>(x, y);
+      if constexpr (IN_REGISTERS<T, DP>)
+        break;
+    }
+    return s;
   }
 };
 
@@ -548,27 +583,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
 
 // --------------------------------------------------------------- backward
 
-// delta = g . y of each row; a wave for each.  y is contiguous.
-template <class T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(const AttnShape s, const Rows<const T> g,
-                                                         const T *y, T *delta) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= int64_t(s.B) * s.Hk * s.rows)
-    return;
-  const int bh = int(item / s.rows), row = int(item % s.rows), b = bh / s.Hk, hk = bh % s.Hk;
-  const uint32_t i = s.by_group.div(uint32_t(row)), gi = uint32_t(row) - i * uint32_t(s.G);
-  const T *gp = g.p + b * g.sB + hk * g.sHead + int64_t(i) * g.sOuter + int64_t(gi) * g.sInner;
-  const T *yp = y + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + int64_t(hk) * s.G + gi) * s.D;
-  T sum = 0;
-  for (int d = lane; d < s.D; d += 64)
-    sum = fma(gp[d], yp[d], sum);
-#pragma unroll
-  for (int o = 32; o; o >>= 1)
-    sum += __shfl_xor(sum, o);
-  if (lane == 0)
-    delta[item] = sum;
-}
+// A row's delta = g . y is formed where it is needed: a launch less, for one more
+// row read with each of g.
 
 template <class T, int DP>
 __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
@@ -600,7 +616,18 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
              int64_t(qg) * a.g.sInner,
          s.D, live, a.vec, h);
   const T lse = live ? a.lse[int64_t(bh) * s.rows + row] : T(0);
-  const T delta = live ? a.delta[int64_t(bh) * s.rows + row] : T(0);
+  const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead + int64_t(qi) * a.y.sOuter +
+                int64_t(qg) * a.y.sInner;
+  T delta = 0;
+#pragma unroll 1
+  for (int d = 0; d < s.D; d += 4 * RowVec<T>::N * 4) {
+    Frag<T, 16 * RowVec<T>::N> x, y;
+    x.load(g.row + d, s.D - d, live, a.vec, h);
+    y.load(yp + d, s.D - d, live, a.vec, h);
+    delta += times<T, 16 * RowVec<T>::N>(x, y);
+  }
+  delta += __shfl_xor(delta, 16);
+  delta += __shfl_xor(delta, 32);
   Sums<T, SC> sums;
   sums.clear();
   for (int j0 = wave * 16; j0 < end; j0 += 16 * AT_WAVES) {
@@ -652,6 +679,7 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
   sequence(s, b, false, keys, first);
   const T *qp = a.q.p + b * a.q.sB + hk * a.q.sHead;
   const T *gp = a.g.p + b * a.g.sB + hk * a.g.sHead;
+  const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead;
   auto at = [&](const T *p, const Rows<const T> &x, int row) {
     const uint32_t i = s.by_group.div(uint32_t(row));
     return p + int64_t(i) * x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * x.sInner;
@@ -682,13 +710,19 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
       xq.load(r, at(qp, a.q, on ? row : 0) + col0, s.D - col0, on, a.vec, n);
       xg.load(r, at(gp, a.g, on ? row : 0) + col0, s.D - col0, on, a.vec, n);
       lse[r] = on ? a.lse[int64_t(bh) * s.rows + row] : T(0);
-      delta[r] = on ? a.delta[int64_t(bh) * s.rows + row] : T(0);
       limit[r] = on ? seen(s, keys, first, int(s.by_group.div(uint32_t(row)))) : 0;
     }
     const bool live = r0 + n < s.rows;
     const int own = live ? r0 + n : 0;
     const auto z = k.dots(at(qp, a.q, own), s.D, live, a.vec, h);
-    const auto dp = v.dots(at(gp, a.g, own), s.D, live, a.vec, h);
+    T product;
+    const auto dp =
+        v.dots(at(gp, a.g, own), at(yp, a.y, own), s.D, live, a.vec, h, product);
+    product += __shfl_xor(product, 16);
+    product += __shfl_xor(product, 32);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      delta[r] = __shfl(product, M::row(h, r));
     T p[4], ds[4];
     bool vis[4], some = false;
 #pragma unroll
@@ -725,26 +759,23 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
     join_waves<T, SC>(dk, a.scale, lds, store(a.dk));
 }
 
+// Both gradients in one launch: tiles of keys, then tiles of rows.
 template <class T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(const AttnBwd<T> a) {
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_kernel(const AttnBwd<T> a,
+                                                                 uint32_t key_blocks) {
   constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
+  const AttnShape &s = a.s;
+  const bool keys = blockIdx.x < key_blocks;
   uint32_t bh, item;
-  head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk), uint32_t(a.s.rows + 15) / 16 * GROUPS, bh,
-            item);
+  head_item(keys ? blockIdx.x : blockIdx.x - key_blocks, uint32_t(s.B) * uint32_t(s.Hk),
+            uint32_t((keys ? s.Tk : s.rows) + 15) / 16 * GROUPS, bh, item);
   const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
-  if (col0 < a.s.D)
-    attn_dq_tile<T, DP>(a, bh, item / GROUPS, col0);
-}
-
-template <class T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(const AttnBwd<T> a) {
-  constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
-  uint32_t bh, item;
-  head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk), uint32_t(a.s.Tk + 15) / 16 * GROUPS, bh,
-            item);
-  const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
-  if (col0 < a.s.D)
+  if (col0 >= s.D)
+    return;
+  if (keys)
     attn_dkv_tile<T, DP>(a, bh, item / GROUPS, col0);
+  else
+    attn_dq_tile<T, DP>(a, bh, item / GROUPS, col0);
 }
 
 // As attn_fwd_left_kernel.
@@ -918,15 +949,12 @@ template <class T> void run_attention(AttnFwd<T> &a) {
   }
 }
 
-template <class T> void run_attention_bwd(AttnBwd<T> &a, const T *y) {
+template <class T> void run_attention_bwd(AttnBwd<T> &a) {
   const AttnShape &s = a.s;
-  const int64_t rows = int64_t(s.B) * s.Hk * s.rows;
-  DeviceScratch delta(size_t(rows) * sizeof(T));
-  a.delta = delta.template get<T>();
   if constexpr (std::is_same_v<T, float>)
     if (split_takes(s, true)) {
       DeviceScratch words(split_gate_words(s, true) * sizeof(uint32_t));
-      run_split_bwd(a, y, words.get<uint32_t>());
+      run_split_bwd(a, words.get<uint32_t>());
       const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk), groups = left_groups(bhs);
       dispatch_width<float>(s.D, [&]<int DP>() {
         if constexpr (DP <= 128)
@@ -936,24 +964,14 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a, const T *y) {
       NT_LAUNCH_CHECK();
       return;
     }
-  if (rows) {
-    attn_delta_kernel<T>
-        <<<dim3(uint32_t((rows + 3) / 4)), 256, 0, stream()>>>(s, a.g, y, delta.template get<T>());
-    NT_LAUNCH_CHECK();
-  }
   dispatch_width<T>(s.D, [&]<int DP>() {
-    if (a.dq && rows) {
-      attn_dq_kernel<T, DP>
-          <<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.rows + 15) / 16) * COLUMN_GROUPS<T, DP>)),
-             64 * AT_WAVES, 0, stream()>>>(a);
-      NT_LAUNCH_CHECK();
-    }
-    if ((a.dk || a.dv) && s.Tk && s.B) {
-      attn_dkv_kernel<T, DP>
-          <<<dim3(uint32_t(int64_t(s.B) * s.Hk * ((s.Tk + 15) / 16) * COLUMN_GROUPS<T, DP>)),
-             64 * AT_WAVES, 0, stream()>>>(a);
-      NT_LAUNCH_CHECK();
-    }
+    const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk) * COLUMN_GROUPS<T, DP>;
+    const uint32_t keys = a.dk || a.dv ? bhs * uint32_t((s.Tk + 15) / 16) : 0;
+    const uint32_t rows = a.dq ? bhs * uint32_t((s.rows + 15) / 16) : 0;
+    if (keys + rows == 0)
+      return;
+    attn_bwd_kernel<T, DP><<<dim3(keys + rows), 64 * AT_WAVES, 0, stream()>>>(a, keys);
+    NT_LAUNCH_CHECK();
   });
 }
 
@@ -1004,7 +1022,11 @@ int nt_attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v,
       a.k = rows_of<const T>(k, 1);
       a.v = rows_of<const T>(v, 1);
       a.g = rows_of<const T>(g, s.G);
-      const T *out = contiguous_of<const T>(y, numel(q), q->dtype, "y");
+      a.y.p = contiguous_of<const T>(y, numel(q), q->dtype, "y");
+      a.y.sInner = s.D;
+      a.y.sHead = int64_t(s.D) * s.G;
+      a.y.sOuter = a.y.sHead * s.Hk;
+      a.y.sB = a.y.sOuter * s.Tq;
       a.lse = contiguous_of<const T>(lse, int64_t(s.B) * s.Hk * s.rows, q->dtype, "lse");
       if (dq)
         a.dq = contiguous_of<T>(dq, numel(q), q->dtype, "dq");
@@ -1014,8 +1036,9 @@ int nt_attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v,
         a.dv = contiguous_of<T>(dv, numel(v), q->dtype, "dv");
       a.scale = T(scale);
       a.scale2 = T(scale * 1.4426950408889634);
-      a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v) && whole_pieces(g);
-      run_attention_bwd(a, out);
+      a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v) && whole_pieces(g) &&
+              reinterpret_cast<uintptr_t>(a.y.p) % 16 == 0;
+      run_attention_bwd(a);
     });
   });
 }

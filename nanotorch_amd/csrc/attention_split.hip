@@ -109,7 +109,7 @@ struct PackArgs {
   int per;
   // the gradient's: y, the forward statistics, and what becomes of them
   const float *y, *lse;
-  float *stats, *delta;
+  float *stats;
 };
 
 // A workgroup packs a tile of 64 rows, by way of LDS.  HBM bound: 4 bytes read,
@@ -199,8 +199,6 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
       st[SA_UNIT] = dot * pow2(up);
       st[2 * SA_UNIT] = pow2(-up);
       reinterpret_cast<int *>(st)[3 * SA_UNIT] = limit;
-      if (row < rows)
-        a.delta[int64_t(bh) * t.rows + row] = dot;
     }
   }
   if (part == 0)
@@ -1010,7 +1008,7 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
   });
 }
 
-void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
+void run_split_bwd(AttnBwd<float> &a, uint32_t *words) {
   const AttnShape &s = a.s;
   const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
   const int kt = tiles_of(s.Tk), qt = tiles_of(s.rows);
@@ -1035,10 +1033,9 @@ void run_split_bwd(AttnBwd<float> &a, const float *y, uint32_t *words) {
     p.vec = a.vec;
     p.words = words;
     p.per = a.gate.per;
-    p.y = y;
+    p.y = a.y.p;
     p.lse = a.lse;
     p.stats = stats;
-    p.delta = const_cast<float *>(a.delta);
     const uint32_t kb = bhs * uint32_t(kt), qb = bhs * uint32_t(qt);
     p.t[0] = {a.k, k_row, k_col, k_scale, s.Tk, kt, 1, kb, 0};
     p.t[1] = {a.v, v_row, nullptr, v_scale, s.Tk, kt, 1, 2 * kb, kt};
