@@ -3,6 +3,8 @@
 // (attention_split.hip) and those on tiles in registers (attention.hip).
 #pragma once
 
+#include <algorithm>
+
 #include "tokens.h"
 
 namespace nt {
@@ -16,6 +18,7 @@ template <class T> struct Rows {
 
 struct AttnShape {
   int B, Tq, Tk, Hk, G, D;
+  int W;         // elements of the operands' rows, D to whole 16 bytes
   int rows;      // Tq G
   FastDivU32 by_group;
   int causal;    // 0 no, 1 the queries end with the sequence, 2 they begin at `start`
@@ -60,7 +63,6 @@ template <class T> struct AttnBwd {
   T *dq;                // [B, Tq, H, D]
   T *dk, *dv;           // [B, Tk, Hk, D]; either may be null
   T scale, scale2;
-  int vec;
   AttnGate gate;
 };
 
@@ -109,26 +111,18 @@ __device__ __forceinline__ int seen(const AttnShape &s, int n, int first, int i)
   return e < 0 ? 0 : e < n ? e : n;
 }
 
-// 16 bytes at element d of a row of D elements; zeros past the end or where
-// the row is not `live`.
+// 16 bytes at element d of a row of W elements, a multiple of 16 bytes; zeros past
+// its end or where the row is not `live`, which must be one that can be read all the
+// same.  No branches (one for each load kept the loads apart and filled the scalar
+// registers with lane masks).
 template <class T>
-__device__ __forceinline__ typename RowVec<T>::V piece(const T *p, int d, int D, bool live,
-                                                       int vec) {
+__device__ __forceinline__ typename RowVec<T>::V piece(const T *row, int d, int W, bool live) {
   using R = RowVec<T>;
-  typename R::V v{};
-  if (!live)
-    return v;
-  if (vec) {
-    if (d < D)
-      v = *reinterpret_cast<const typename R::V *>(p + d);
-    return v;
-  }
-  if (d + R::N <= D)
-    return R::load(p + d);
+  typename R::V v = R::load(row + std::min(d, W - R::N));
+  live = live && d < W;
 #pragma unroll
   for (int j = 0; j < R::N; ++j)
-    if (d + j < D)
-      v[j] = p[d + j];
+    v[j] = live ? v[j] : T(0);
   return v;
 }
 

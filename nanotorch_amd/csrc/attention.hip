@@ -73,10 +73,11 @@ template <class T> constexpr T NEG_INF = -std::numeric_limits<T>::infinity();
 template <class T, int DP> struct Frag {
   static constexpr int N = RowVec<T>::N, C = DP / (4 * N);
   typename RowVec<T>::V v[C];
-  __device__ __forceinline__ void load(const T *row, int D, bool live, int vec, int h) {
+  // From element d0 of a row of D on.
+  __device__ __forceinline__ void load(const T *row, int d0, int D, bool live, int h) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      v[c] = piece(row, 4 * N * c + N * h, D, live, vec);
+      v[c] = piece(row, d0 + 4 * N * c + N * h, D, live);
   }
   // A row of DP elements, aligned: no branch, so that many loads go out together.
   __device__ __forceinline__ void load_whole(const T *row, int h) {
@@ -110,32 +111,37 @@ __device__ __forceinline__ T times(const Frag<T, DP> &a, const Frag<T, DP> &b) {
   return sum;
 }
 
-// Own rows of up to 512 bytes stay in registers.  Longer ones are read again with
-// every tile of items, 256 bytes at a time, and a workgroup keeps only 512 bytes
-// of its sums' columns: several workgroups form the same probabilities, each for
-// columns of its own (in one kernel, wide float64 rows needed a thousand registers
-// a lane).
-template <class T, int DP> constexpr bool IN_REGISTERS = DP * sizeof(T) <= 512;
+// Own rows of up to 1 KB stay in registers (those over 512 bytes with one wave to a
+// SIMD).  Longer ones, float64 over 128 wide, are read again with every tile of
+// items, 256 bytes at a time.  A workgroup keeps at most so many bytes of its sums'
+// columns; where that is less than a row, several workgroups form the same
+// probabilities, each for columns of its own (in one, wide float64 rows would need a
+// thousand registers a lane).
+template <class T, int DP> constexpr bool IN_REGISTERS = DP * sizeof(T) <= 1024;
+template <class T, int DP> constexpr int COLUMNS_OF(int bytes) {
+  return std::min(DP, bytes / int(sizeof(T)));
+}
+// y and dq; dk and dv.
 template <class T, int DP>
-constexpr int COLUMNS = IN_REGISTERS<T, DP> ? DP : int(512 / sizeof(T));
-template <class T, int DP> constexpr int COLUMN_GROUPS = DP / COLUMNS<T, DP>;
+constexpr int COLUMNS = COLUMNS_OF<T, DP>(IN_REGISTERS<T, DP> ? 1024 : 512);
+template <class T, int DP> constexpr int KEY_COLUMNS = COLUMNS_OF<T, DP>(512);
 
 template <class T, int DP> struct Own {
   Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> f;
   const T *row;
   bool live;
-  __device__ __forceinline__ void load(const T *p, int D, bool on, int vec, int h) {
+  __device__ __forceinline__ void load(const T *p, int D, bool on, int h) {
     row = p;
     live = on;
     if constexpr (IN_REGISTERS<T, DP>)
-      f.load(p, D, on, vec, h);
+      f.load(p, 0, D, on, h);
   }
   // With the lane's item row.
-  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, int D, bool on, int vec,
+  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, int D, bool on,
                                                       int h) const {
     if constexpr (IN_REGISTERS<T, DP>) {
       Frag<T, DP> x;
-      x.load(item, D, on, vec, h);
+      x.load(item, 0, D, on, h);
       return nt::dots<T, DP>(x, f);
     } else {
       constexpr int W = 256 / sizeof(T);
@@ -143,8 +149,8 @@ template <class T, int DP> struct Own {
 #pragma unroll 1
       for (int d = 0; d < D; d += W) {
         Frag<T, W> x, o;
-        x.load(item + d, D - d, on, vec, h);
-        o.load(row + d, D - d, live, vec, h);
+        x.load(item, d, D, on, h);
+        o.load(row, d, D, live, h);
         s += nt::dots<T, W>(x, o);
       }
       return s;
@@ -152,19 +158,19 @@ template <class T, int DP> struct Own {
   }
   // As dots, and the lane's item row times `other`, elements of its own.
   __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, const T *other, int D, bool on,
-                                                      int vec, int h, T &product) const {
+                                                      int h, T &product) const {
     constexpr int W = IN_REGISTERS<T, DP> ? DP : int(256 / sizeof(T));
     typename Mma<T>::V4 s{};
     product = 0;
 #pragma unroll 1
     for (int d = 0; d < D; d += W) {
       Frag<T, W> x, y, o;
-      x.load(item + d, D - d, on, vec, h);
-      y.load(other + d, D - d, on, vec, h);
+      x.load(item, d, D, on, h);
+      y.load(other, d, D, on, h);
       if constexpr (IN_REGISTERS<T, DP>) {
         s = nt::dots<T, W>(x, f);
       } else {
-        o.load(row + d, D - d, live, vec, h);
+        o.load(row, d, D, live, h);
         s += nt::dots<T, W>(x, o);
       }
       product += times<T, W>(x, y);
@@ -181,10 +187,11 @@ template <class T, int DP> struct Own {
 template <class T, int DP> struct Items {
   static constexpr int N = RowVec<T>::N, C = DP / (16 * N);
   typename RowVec<T>::V v[4][C];
-  __device__ __forceinline__ void load(int r, const T *p, int D, bool on, int vec, int n) {
+  // The columns from d0 on of a row of D.
+  __device__ __forceinline__ void load(int r, const T *row, int d0, int D, bool on, int n) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      v[r][c] = piece(p, N * (16 * c + n), D, on, vec);
+      v[r][c] = piece(row, d0 + N * (16 * c + n), D, on);
   }
   __device__ __forceinline__ void load_whole(int r, const T *p, int n) {
 #pragma unroll
@@ -308,9 +315,10 @@ template <class T, int DP> __device__ __forceinline__ bool all_finite(const Item
 // Tiles of 16 keys that a wave takes at a time, two blocks of which fit its registers
 // beside two waves to a SIMD.
 template <class T, int DP> constexpr int FWD_TILES = DP * sizeof(T) <= 256 ? 2 : 1;
-// Float64 rows of 512 bytes need the registers of one wave to a SIMD.
+// Rows of 1 KB, and of 512 bytes in float64, need the registers of one wave to a SIMD.
 template <class T, int DP>
-constexpr int FWD_WAVES = sizeof(T) == 8 && DP * sizeof(T) == 512 ? 1 : 2;
+constexpr int FWD_WAVES =
+    DP * sizeof(T) == 1024 || (sizeof(T) == 8 && DP * sizeof(T) == 512) ? 1 : 2;
 
 // Tile `item` of a (sequence, key head).  WHOLE: rows of DP elements, aligned.
 template <class T, int DP, bool WHOLE>
@@ -331,7 +339,8 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   sequence(s, b, threadIdx.x == 0, keys, first);
   const int row = tile * 16 + n;
   const bool live = row < s.rows;
-  const uint32_t qi = s.by_group.div(uint32_t(row)), qg = uint32_t(row) - qi * uint32_t(s.G);
+  const uint32_t at = uint32_t(std::min(row, s.rows - 1));
+  const uint32_t qi = s.by_group.div(at), qg = at - qi * uint32_t(s.G);
   const int limit = live ? seen(s, keys, first, int(qi)) : 0;
   const int last = std::min(tile * 16 + 15, s.rows - 1);
   const int end = seen(s, keys, first, int(s.by_group.div(uint32_t(last)))); // of any row
@@ -341,7 +350,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
   const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
   Own<T, DP> q;
-  q.load(qp, s.D, live, a.vec, h);
+  q.load(qp, s.W, live, h);
   Sums<T, SC> sums;
   sums.clear();
   T m = NEG_INF<T>, l = 0;
@@ -354,16 +363,17 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
     Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> k[TILES];
   };
   constexpr int STEP = 16 * TILES;
-  // WHOLE: past the end the last key again, which no row sees there
+  // past the end the last key again, which no row sees there
   auto load_keys = [&](Keys &x, int j0) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
       if constexpr (IN_REGISTERS<T, DP>) {
         const int j = j0 + 16 * i + n;
+        const T *p = kp + int64_t(std::min(j, end - 1)) * a.k.sOuter;
         if constexpr (WHOLE)
-          x.k[i].load_whole(kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, h);
+          x.k[i].load_whole(p, h);
         else
-          x.k[i].load(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
+          x.k[i].load(p, 0, s.W, j < end, h);
       }
   };
   Items<T, SC> v[TILES];
@@ -373,10 +383,11 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = j0 + 16 * i + M::row(h, r);
+        const T *p = vp + int64_t(std::min(j, end - 1)) * a.v.sOuter;
         if constexpr (WHOLE)
-          v[i].load_whole(r, vp + int64_t(std::min(j, end - 1)) * a.v.sOuter + col0, n);
+          v[i].load_whole(r, p + col0, n);
         else
-          v[i].load(r, vp + int64_t(j) * a.v.sOuter + col0, s.D - col0, j < end, a.vec, n);
+          v[i].load(r, p, col0, s.W, j < end, n);
       }
   };
   auto take = [&](const Keys &x, int j0) {
@@ -390,7 +401,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
         d = dots<T, DP>(x.k[i], q.f);
       } else {
         const int j = j0 + 16 * i + n;
-        d = q.dots(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
+        d = q.dots(kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, s.W, j < end, h);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -494,7 +505,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 template <class T, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * AT_WAVES, (FWD_WAVES<T, DP>)) void attn_fwd_kernel(
     const AttnFwd<T> a) {
-  constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
+  constexpr uint32_t GROUPS = DP / COLUMNS<T, DP>;
   const uint32_t splits = uint32_t(a.splits);
   uint32_t bh, item;
   head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk),
@@ -601,7 +612,8 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
   sequence(s, b, false, keys, first);
   const int row = tile * 16 + n;
   const bool live = row < s.rows;
-  const uint32_t qi = s.by_group.div(uint32_t(row)), qg = uint32_t(row) - qi * uint32_t(s.G);
+  const uint32_t at = uint32_t(std::min(row, s.rows - 1));
+  const uint32_t qi = s.by_group.div(at), qg = at - qi * uint32_t(s.G);
   const int limit = live ? seen(s, keys, first, int(qi)) : 0;
   const int last = std::min(tile * 16 + 15, s.rows - 1);
   const int end = seen(s, keys, first, int(s.by_group.div(uint32_t(last))));
@@ -611,19 +623,19 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
   Own<T, DP> q, g;
   q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
              int64_t(qg) * a.q.sInner,
-         s.D, live, a.vec, h);
+         s.W, live, h);
   g.load(a.g.p + b * a.g.sB + hk * a.g.sHead + int64_t(qi) * a.g.sOuter +
              int64_t(qg) * a.g.sInner,
-         s.D, live, a.vec, h);
-  const T lse = live ? a.lse[int64_t(bh) * s.rows + row] : T(0);
+         s.W, live, h);
+  const T lse = a.lse[int64_t(bh) * s.rows + at];
   const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead + int64_t(qi) * a.y.sOuter +
                 int64_t(qg) * a.y.sInner;
   T delta = 0;
 #pragma unroll 1
-  for (int d = 0; d < s.D; d += 4 * RowVec<T>::N * 4) {
+  for (int d = 0; d < s.W; d += 4 * RowVec<T>::N * 4) {
     Frag<T, 16 * RowVec<T>::N> x, y;
-    x.load(g.row + d, s.D - d, live, a.vec, h);
-    y.load(yp + d, s.D - d, live, a.vec, h);
+    x.load(g.row, d, s.W, live, h);
+    y.load(yp, d, s.W, live, h);
     delta += times<T, 16 * RowVec<T>::N>(x, y);
   }
   delta += __shfl_xor(delta, 16);
@@ -635,11 +647,11 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = j0 + M::row(h, r);
-      x.load(r, kp + int64_t(j) * a.k.sOuter + col0, s.D - col0, j < end, a.vec, n);
+      x.load(r, kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, col0, s.W, j < end, n);
     }
-    const int j = j0 + n;
-    const auto z = q.dots(kp + int64_t(j) * a.k.sOuter, s.D, j < end, a.vec, h);
-    const auto dp = g.dots(vp + int64_t(j) * a.v.sOuter, s.D, j < end, a.vec, h);
+    const int64_t j = std::min(j0 + n, end - 1);
+    const auto z = q.dots(kp + j * a.k.sOuter, s.W, j0 + n < end, h);
+    const auto dp = g.dots(vp + j * a.v.sOuter, s.W, j0 + n < end, h);
     T ds[4];
     bool vis[4];
 #pragma unroll
@@ -669,7 +681,7 @@ template <class T, int DP>
 __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
                                               int col0) {
   using M = Mma<T>;
-  constexpr int SC = COLUMNS<T, DP>;
+  constexpr int SC = KEY_COLUMNS<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
@@ -685,10 +697,9 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
     return p + int64_t(i) * x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * x.sInner;
   };
   Own<T, DP> k, v;
-  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + int64_t(key) * a.k.sOuter, s.D, key < keys,
-         a.vec, h);
-  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + int64_t(key) * a.v.sOuter, s.D, key < keys,
-         a.vec, h);
+  const int64_t own_key = std::min(key, s.Tk - 1);
+  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + own_key * a.k.sOuter, s.W, key < keys, h);
+  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + own_key * a.v.sOuter, s.W, key < keys, h);
   Sums<T, SC> dk, dv;
   dk.clear();
   dv.clear();
@@ -707,17 +718,17 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
     for (int r = 0; r < 4; ++r) {
       const int row = r0 + M::row(h, r);
       const bool on = row < s.rows;
-      xq.load(r, at(qp, a.q, on ? row : 0) + col0, s.D - col0, on, a.vec, n);
-      xg.load(r, at(gp, a.g, on ? row : 0) + col0, s.D - col0, on, a.vec, n);
-      lse[r] = on ? a.lse[int64_t(bh) * s.rows + row] : T(0);
+      xq.load(r, at(qp, a.q, on ? row : 0), col0, s.W, on, n);
+      xg.load(r, at(gp, a.g, on ? row : 0), col0, s.W, on, n);
+      lse[r] = a.lse[int64_t(bh) * s.rows + (on ? row : 0)];
       limit[r] = on ? seen(s, keys, first, int(s.by_group.div(uint32_t(row)))) : 0;
     }
     const bool live = r0 + n < s.rows;
     const int own = live ? r0 + n : 0;
-    const auto z = k.dots(at(qp, a.q, own), s.D, live, a.vec, h);
+    const auto z = k.dots(at(qp, a.q, own), s.W, live, h);
     T product;
     const auto dp =
-        v.dots(at(gp, a.g, own), at(yp, a.y, own), s.D, live, a.vec, h, product);
+        v.dots(at(gp, a.g, own), at(yp, a.y, own), s.W, live, h, product);
     product += __shfl_xor(product, 16);
     product += __shfl_xor(product, 32);
 #pragma unroll
@@ -763,19 +774,21 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
 template <class T, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_kernel(const AttnBwd<T> a,
                                                                  uint32_t key_blocks) {
-  constexpr uint32_t GROUPS = COLUMN_GROUPS<T, DP>;
+  constexpr uint32_t GROUPS = DP / COLUMNS<T, DP>, KEY_GROUPS = DP / KEY_COLUMNS<T, DP>;
   const AttnShape &s = a.s;
-  const bool keys = blockIdx.x < key_blocks;
+  const uint32_t heads = uint32_t(s.B) * uint32_t(s.Hk);
   uint32_t bh, item;
-  head_item(keys ? blockIdx.x : blockIdx.x - key_blocks, uint32_t(s.B) * uint32_t(s.Hk),
-            uint32_t((keys ? s.Tk : s.rows) + 15) / 16 * GROUPS, bh, item);
-  const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
-  if (col0 >= s.D)
-    return;
-  if (keys)
-    attn_dkv_tile<T, DP>(a, bh, item / GROUPS, col0);
-  else
-    attn_dq_tile<T, DP>(a, bh, item / GROUPS, col0);
+  if (blockIdx.x < key_blocks) {
+    head_item(blockIdx.x, heads, uint32_t(s.Tk + 15) / 16 * KEY_GROUPS, bh, item);
+    const int col0 = int(item % KEY_GROUPS) * KEY_COLUMNS<T, DP>;
+    if (col0 < s.D)
+      attn_dkv_tile<T, DP>(a, bh, item / KEY_GROUPS, col0);
+  } else {
+    head_item(blockIdx.x - key_blocks, heads, uint32_t(s.rows + 15) / 16 * GROUPS, bh, item);
+    const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
+    if (col0 < s.D)
+      attn_dq_tile<T, DP>(a, bh, item / GROUPS, col0);
+  }
 }
 
 // As attn_fwd_left_kernel.
@@ -796,6 +809,26 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const Attn
       __syncthreads();
       attn_dkv_tile<float, DP>(a, bh, t, 0);
     }
+}
+
+// x [B, tokens, heads, D] -> contiguous rows of W elements, zeros past D.
+template <class T>
+__global__ __launch_bounds__(256) void attn_pad_kernel(const Rows<const T> x, T *to, int64_t rows,
+                                                       int tokens, int heads, int D, int W) {
+  using R = RowVec<T>;
+  const int per = W / R::N;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, row = i / per;
+  if (row >= rows)
+    return;
+  const int d = int(i - row * per) * R::N;
+  const int64_t t = row / heads;
+  const T *p = x.p + t / tokens * x.sB + t % tokens * x.sOuter + row % heads * x.sInner;
+  typename R::V v{};
+#pragma unroll
+  for (int j = 0; j < R::N; ++j)
+    if (d + j < D)
+      v[j] = p[d + j];
+  R::store(to + row * W + d, v);
 }
 
 // ------------------------------------------------------------------- host
@@ -846,6 +879,7 @@ AttnShape attn_shape(const nt_view *q, const nt_view *k, const nt_view *v,
     fail(NT_ERR_VALUE, "attention: too many rows");
   AttnShape s{};
   s.B = int(B), s.Tq = int(Tq), s.Tk = int(Tk), s.Hk = int(Hk), s.G = int(G), s.D = int(D);
+  s.W = int((D * int64_t(dtype_size(q->dtype)) + 15) / 16 * 16 / int64_t(dtype_size(q->dtype)));
   s.rows = int(Tq * G);
   s.by_group = FastDivU32(uint32_t(G));
   s.causal = causal;
@@ -887,6 +921,33 @@ template <class T> T *contiguous_of(const nt_view *v, int64_t n, int dt, const c
                              std::to_string(n) + " elements");
   return typed_ptr<T>(v);
 }
+
+// Rows whose length is no multiple of 16 bytes are copied with zeros behind them:
+// the kernels read whole pieces only.
+template <class T> struct Padded {
+  DeviceScratch memory;
+  static size_t bytes(const AttnShape &s, int64_t tokens, int64_t heads) {
+    return s.W == s.D ? 0 : size_t(s.B) * size_t(tokens) * size_t(heads) * size_t(s.W) * sizeof(T);
+  }
+  Padded(const AttnShape &s, Rows<const T> &x, int tokens, int heads, int G)
+      : memory(bytes(s, tokens, heads)) {
+    if (s.W == s.D)
+      return;
+    const int64_t rows = int64_t(s.B) * tokens * heads;
+    T *to = memory.template get<T>();
+    if (rows) {
+      const int64_t pieces = rows * (s.W / RowVec<T>::N);
+      attn_pad_kernel<T><<<dim3(uint32_t((pieces + 255) / 256)), 256, 0, stream()>>>(
+          x, to, rows, tokens, heads, s.D, s.W);
+      NT_LAUNCH_CHECK();
+    }
+    x.p = to;
+    x.sInner = s.W;
+    x.sHead = int64_t(s.W) * G;
+    x.sOuter = int64_t(s.W) * heads;
+    x.sB = x.sOuter * tokens;
+  }
+};
 
 // The padded width: the matrix instructions' columns come 16 pieces at a time.
 template <class T, class F> void dispatch_width(int D, F &&f) {
@@ -935,7 +996,7 @@ template <class T> void run_attention(AttnFwd<T> &a) {
   a.part_acc = acc.template get<T>();
   a.part_stat = stat.template get<T>();
   dispatch_width<T>(s.D, [&]<int DP>() {
-    const dim3 grid(uint32_t(tiles * a.splits * COLUMN_GROUPS<T, DP>));
+    const dim3 grid(uint32_t(tiles * a.splits * (DP / COLUMNS<T, DP>)));
     if (a.vec && s.D == DP)
       attn_fwd_kernel<T, DP, true><<<grid, 64 * AT_WAVES, 0, stream()>>>(a);
     else
@@ -965,9 +1026,10 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a) {
       return;
     }
   dispatch_width<T>(s.D, [&]<int DP>() {
-    const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk) * COLUMN_GROUPS<T, DP>;
-    const uint32_t keys = a.dk || a.dv ? bhs * uint32_t((s.Tk + 15) / 16) : 0;
-    const uint32_t rows = a.dq ? bhs * uint32_t((s.rows + 15) / 16) : 0;
+    const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
+    const uint32_t keys =
+        a.dk || a.dv ? bhs * uint32_t((s.Tk + 15) / 16) * (DP / KEY_COLUMNS<T, DP>) : 0;
+    const uint32_t rows = a.dq ? bhs * uint32_t((s.rows + 15) / 16) * (DP / COLUMNS<T, DP>) : 0;
     if (keys + rows == 0)
       return;
     attn_bwd_kernel<T, DP><<<dim3(keys + rows), 64 * AT_WAVES, 0, stream()>>>(a, keys);
@@ -1000,8 +1062,11 @@ int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v, const nt_
         a.lse = contiguous_of<T>(lse, rows, q->dtype, "lse");
       a.scale2 = T(scale * 1.4426950408889634);
       a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v);
-      if (rows)
-        run_attention(a);
+      if (rows == 0)
+        return;
+      const int H = s.Hk * s.G;
+      Padded<T> pq(s, a.q, s.Tq, H, s.G), pk(s, a.k, s.Tk, s.Hk, 1), pv(s, a.v, s.Tk, s.Hk, 1);
+      run_attention(a);
     });
   });
 }
@@ -1036,8 +1101,9 @@ int nt_attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v,
         a.dv = contiguous_of<T>(dv, numel(v), q->dtype, "dv");
       a.scale = T(scale);
       a.scale2 = T(scale * 1.4426950408889634);
-      a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v) && whole_pieces(g) &&
-              reinterpret_cast<uintptr_t>(a.y.p) % 16 == 0;
+      const int H = s.Hk * s.G;
+      Padded<T> pq(s, a.q, s.Tq, H, s.G), pk(s, a.k, s.Tk, s.Hk, 1), pv(s, a.v, s.Tk, s.Hk, 1);
+      Padded<T> pg(s, a.g, s.Tq, H, s.G), py(s, a.y, s.Tq, H, s.G);
       run_attention_bwd(a);
     });
   });

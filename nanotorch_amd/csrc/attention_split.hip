@@ -104,11 +104,12 @@ struct PackTensor {
 struct PackArgs {
   AttnShape s;
   PackTensor t[4];
-  int count, vec;
+  int count;
   uint32_t *words;
   int per;
   // the gradient's: y, the forward statistics, and what becomes of them
-  const float *y, *lse;
+  Rows<const float> y;
+  const float *lse;
   float *stats;
 };
 
@@ -140,7 +141,7 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
   for (int i = threadIdx.x; i < SA_TILE * (DP / 4); i += 256) {
     const int r = i / (DP / 4), d = i % (DP / 4) * 4, row = tile * SA_TILE + r;
     const bool live = row < rows;
-    const auto v = piece(live ? address(row) : base, d, s.D, live, a.vec);
+    const auto v = piece(live ? address(row) : base, d, s.W, live);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       x[r * PITCH + d + j] = v[j];
@@ -180,13 +181,14 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
     uint32_t i = 0;
     if (row < rows) {
       i = s.by_group.div(uint32_t(row));
-      const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
-      const float *y = a.y + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D;
-      for (int d = part * 4; d < s.D; d += 16)
+      const float *y = a.y.p + b * a.y.sB + hk * a.y.sHead + int64_t(i) * a.y.sOuter +
+                       int64_t(uint32_t(row) - i * uint32_t(s.G)) * a.y.sInner;
+      for (int d = part * 4; d < s.W; d += 16) {
+        const auto v = RowVec<float>::load(y + d);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (d + j < s.D)
-            dot = fmaf(x[r * PITCH + d + j], y[d + j], dot);
+          dot = fmaf(x[r * PITCH + d + j], v[j], dot);
+      }
     }
     dot += __shfl_xor(dot, 1);
     dot += __shfl_xor(dot, 2);
@@ -407,7 +409,6 @@ struct SplitFwd {
   int tiles;                     // of 64 keys
   float *y, *lse;
   float scale2;
-  int vec;
   AttnGate gate;
   int parts;                     // of the keys; over one: sums [part][bh, row][D] and
   float *sums, *tops;            // maxima, sums of p [part][2][bh, row]
@@ -468,7 +469,7 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
     for (int f = 0; f < 2 * DB; ++f)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const auto x = piece(qp, 16 * f + 8 * h + 4 * u, s.D, live, a.vec);
+        const auto x = piece(qp, 16 * f + 8 * h + 4 * u, s.W, live);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v[f][4 * u + j] = x[j];
@@ -975,7 +976,6 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     PackArgs p{};
     p.s = s;
     p.count = 2;
-    p.vec = a.vec;
     p.words = words;
     p.per = a.gate.per;
     p.t[0] = {a.k, k, nullptr, k_scale, s.Tk, tiles, 1, bhs * uint32_t(tiles), 0};
@@ -990,7 +990,6 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     f.tiles = tiles;
     f.y = a.y, f.lse = a.lse;
     f.scale2 = a.scale2;
-    f.vec = a.vec;
     f.gate = a.gate;
     const uint32_t groups = bhs * uint32_t((s.rows + SF_ROWS - 1) / SF_ROWS);
     f.parts = parts_of(groups, tiles);
@@ -1030,10 +1029,9 @@ void run_split_bwd(AttnBwd<float> &a, uint32_t *words) {
     PackArgs p{};
     p.s = s;
     p.count = 4;
-    p.vec = a.vec;
     p.words = words;
     p.per = a.gate.per;
-    p.y = a.y.p;
+    p.y = a.y;
     p.lse = a.lse;
     p.stats = stats;
     const uint32_t kb = bhs * uint32_t(kt), qb = bhs * uint32_t(qt);
