@@ -112,17 +112,16 @@ __device__ __forceinline__ int seen(const AttnShape &s, int n, int first, int i)
 }
 
 // 16 bytes at element d of a row of W elements, a multiple of 16 bytes; zeros past
-// its end or where the row is not `live`, which must be one that can be read all the
-// same.  No branches (one for each load kept the loads apart and filled the scalar
-// registers with lane masks).
+// its end.  No branches (one for each load kept the loads apart and filled the scalar
+// registers with lane masks): in place of a row that is not there, callers read one
+// that is, and leave out what comes of it.
 template <class T>
-__device__ __forceinline__ typename RowVec<T>::V piece(const T *row, int d, int W, bool live) {
+__device__ __forceinline__ typename RowVec<T>::V piece(const T *row, int d, int W) {
   using R = RowVec<T>;
   typename R::V v = R::load(row + std::min(d, W - R::N));
-  live = live && d < W;
 #pragma unroll
   for (int j = 0; j < R::N; ++j)
-    v[j] = live ? v[j] : T(0);
+    v[j] = d < W ? v[j] : T(0);
   return v;
 }
 

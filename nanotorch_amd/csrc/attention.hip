@@ -73,11 +73,11 @@ template <class T> constexpr T NEG_INF = -std::numeric_limits<T>::infinity();
 template <class T, int DP> struct Frag {
   static constexpr int N = RowVec<T>::N, C = DP / (4 * N);
   typename RowVec<T>::V v[C];
-  // From element d0 of a row of D on.
-  __device__ __forceinline__ void load(const T *row, int d0, int D, bool live, int h) {
+  // From element d0 of a row of W on.
+  __device__ __forceinline__ void load(const T *row, int d0, int W, int h) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      v[c] = piece(row, d0 + 4 * N * c + N * h, D, live);
+      v[c] = piece(row, d0 + 4 * N * c + N * h, W);
   }
   // A row of DP elements, aligned: no branch, so that many loads go out together.
   __device__ __forceinline__ void load_whole(const T *row, int h) {
@@ -129,51 +129,49 @@ template <class T, int DP> constexpr int KEY_COLUMNS = COLUMNS_OF<T, DP>(512);
 template <class T, int DP> struct Own {
   Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> f;
   const T *row;
-  bool live;
-  __device__ __forceinline__ void load(const T *p, int D, bool on, int h) {
+  __device__ __forceinline__ void load(const T *p, int W, int h) {
     row = p;
-    live = on;
     if constexpr (IN_REGISTERS<T, DP>)
-      f.load(p, 0, D, on, h);
+      f.load(p, 0, W, h);
   }
   // With the lane's item row.
-  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, int D, bool on,
-                                                      int h) const {
+  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, int W, int h) const {
     if constexpr (IN_REGISTERS<T, DP>) {
       Frag<T, DP> x;
-      x.load(item, 0, D, on, h);
+      x.load(item, 0, W, h);
       return nt::dots<T, DP>(x, f);
     } else {
-      constexpr int W = 256 / sizeof(T);
+      constexpr int PART = 256 / sizeof(T);
       typename Mma<T>::V4 s{};
 #pragma unroll 1
-      for (int d = 0; d < D; d += W) {
-        Frag<T, W> x, o;
-        x.load(item, d, D, on, h);
-        o.load(row, d, D, live, h);
-        s += nt::dots<T, W>(x, o);
+      for (int d = 0; d < W; d += PART) {
+        Frag<T, PART> x, o;
+        x.load(item, d, W, h);
+        o.load(row, d, W, h);
+        s += nt::dots<T, PART>(x, o);
       }
       return s;
     }
   }
   // As dots, and the lane's item row times `other`, elements of its own.
-  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, const T *other, int D, bool on,
-                                                      int h, T &product) const {
-    constexpr int W = IN_REGISTERS<T, DP> ? DP : int(256 / sizeof(T));
+  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, const T *other, int W, int h,
+                                                      T &product) const {
+    constexpr int PART = IN_REGISTERS<T, DP> ? DP : int(256 / sizeof(T));
     typename Mma<T>::V4 s{};
     product = 0;
 #pragma unroll 1
-    for (int d = 0; d < D; d += W) {
-      Frag<T, W> x, y, o;
-      x.load(item, d, D, on, h);
-      y.load(other, d, D, on, h);
+    for (int d = 0; d < W; d += PART) {
+      Frag<T, PART> x, y, o;
+      x.load(item, d, W, h);
+      y.load(other, d, W, h);
       if constexpr (IN_REGISTERS<T, DP>) {
-        s = nt::dots<T, W>(x, f);
+        s = nt::dots<T, PART>(x, f);
       } else {
-        o.load(row, d, D, live, h);
-        s += nt::dots<T, W>(x, o);
+        o.load(row, d, W, h);
+        s += nt::dots<T, PART>(x, o);
       }
-      product += times<T, W>(x, y);
+      product += times<T, PART>(x, y);
+      // (the loads of what follows wait, where the registers are full)
       if constexpr (IN_REGISTERS<T, DP>)
         break;
     }
@@ -187,11 +185,11 @@ template <class T, int DP> struct Own {
 template <class T, int DP> struct Items {
   static constexpr int N = RowVec<T>::N, C = DP / (16 * N);
   typename RowVec<T>::V v[4][C];
-  // The columns from d0 on of a row of D.
-  __device__ __forceinline__ void load(int r, const T *row, int d0, int D, bool on, int n) {
+  // The columns from d0 on of a row of W.
+  __device__ __forceinline__ void load(int r, const T *row, int d0, int W, int n) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      v[r][c] = piece(row, d0 + N * (16 * c + n), D, on);
+      v[r][c] = piece(row, d0 + N * (16 * c + n), W);
   }
   __device__ __forceinline__ void load_whole(int r, const T *p, int n) {
 #pragma unroll
@@ -350,7 +348,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
   const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
   Own<T, DP> q;
-  q.load(qp, s.W, live, h);
+  q.load(qp, s.W, h);
   Sums<T, SC> sums;
   sums.clear();
   T m = NEG_INF<T>, l = 0;
@@ -373,7 +371,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
         if constexpr (WHOLE)
           x.k[i].load_whole(p, h);
         else
-          x.k[i].load(p, 0, s.W, j < end, h);
+          x.k[i].load(p, 0, s.W, h);
       }
   };
   Items<T, SC> v[TILES];
@@ -387,7 +385,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
         if constexpr (WHOLE)
           v[i].load_whole(r, p + col0, n);
         else
-          v[i].load(r, p, col0, s.W, j < end, n);
+          v[i].load(r, p, col0, s.W, n);
       }
   };
   auto take = [&](const Keys &x, int j0) {
@@ -401,7 +399,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
         d = dots<T, DP>(x.k[i], q.f);
       } else {
         const int j = j0 + 16 * i + n;
-        d = q.dots(kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, s.W, j < end, h);
+        d = q.dots(kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, s.W, h);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -443,20 +441,31 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   // A block's values and the next block's keys are on their way while its scores
   // are formed: few rows over many keys wait for memory.
   int blk = int(split) * per + wave;
-  if (blk < stop) {
-    Keys x, y;
-    load_keys(x, blk * STEP);
-    auto turn = [&](const Keys &now, Keys &next) {
-      const bool more = blk + AT_WAVES < stop;
+  // (not of rows that leave no registers for two blocks of keys)
+  constexpr bool AHEAD = WHOLE || DP * sizeof(T) < 512 || (sizeof(T) == 4 && DP == 256);
+  if constexpr (AHEAD) {
+    if (blk < stop) {
+      Keys x, y;
+      load_keys(x, blk * STEP);
+      auto turn = [&](const Keys &now, Keys &next) {
+        const bool more = blk + AT_WAVES < stop;
+        load_values(blk * STEP);
+        if (more)
+          load_keys(next, (blk + AT_WAVES) * STEP);
+        take(now, blk * STEP);
+        blk += AT_WAVES;
+        return more;
+      };
+      while (turn(x, y) && turn(y, x))
+        ;
+    }
+  } else {
+    for (; blk < stop; blk += AT_WAVES) {
+      Keys x;
+      load_keys(x, blk * STEP);
       load_values(blk * STEP);
-      if (more)
-        load_keys(next, (blk + AT_WAVES) * STEP);
-      take(now, blk * STEP);
-      blk += AT_WAVES;
-      return more;
-    };
-    while (turn(x, y) && turn(y, x))
-      ;
+      take(x, blk * STEP);
+    }
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -623,10 +632,10 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
   Own<T, DP> q, g;
   q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
              int64_t(qg) * a.q.sInner,
-         s.W, live, h);
+         s.W, h);
   g.load(a.g.p + b * a.g.sB + hk * a.g.sHead + int64_t(qi) * a.g.sOuter +
              int64_t(qg) * a.g.sInner,
-         s.W, live, h);
+         s.W, h);
   const T lse = a.lse[int64_t(bh) * s.rows + at];
   const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead + int64_t(qi) * a.y.sOuter +
                 int64_t(qg) * a.y.sInner;
@@ -634,8 +643,8 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
 #pragma unroll 1
   for (int d = 0; d < s.W; d += 4 * RowVec<T>::N * 4) {
     Frag<T, 16 * RowVec<T>::N> x, y;
-    x.load(g.row, d, s.W, live, h);
-    y.load(yp, d, s.W, live, h);
+    x.load(g.row, d, s.W, h);
+    y.load(yp, d, s.W, h);
     delta += times<T, 16 * RowVec<T>::N>(x, y);
   }
   delta += __shfl_xor(delta, 16);
@@ -647,11 +656,11 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = j0 + M::row(h, r);
-      x.load(r, kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, col0, s.W, j < end, n);
+      x.load(r, kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, col0, s.W, n);
     }
     const int64_t j = std::min(j0 + n, end - 1);
-    const auto z = q.dots(kp + j * a.k.sOuter, s.W, j0 + n < end, h);
-    const auto dp = g.dots(vp + j * a.v.sOuter, s.W, j0 + n < end, h);
+    const auto z = q.dots(kp + j * a.k.sOuter, s.W, h);
+    const auto dp = g.dots(vp + j * a.v.sOuter, s.W, h);
     T ds[4];
     bool vis[4];
 #pragma unroll
@@ -698,8 +707,8 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
   };
   Own<T, DP> k, v;
   const int64_t own_key = std::min(key, s.Tk - 1);
-  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + own_key * a.k.sOuter, s.W, key < keys, h);
-  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + own_key * a.v.sOuter, s.W, key < keys, h);
+  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + own_key * a.k.sOuter, s.W, h);
+  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + own_key * a.v.sOuter, s.W, h);
   Sums<T, SC> dk, dv;
   dk.clear();
   dv.clear();
@@ -712,23 +721,36 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
   const int clear = key0 + 16; // a row that sees so many sees all of this tile
   for (int r0 = row0 + wave * 16; r0 < s.rows; r0 += 16 * AT_WAVES) {
     Items<T, SC> xq, xg;
+    auto load = [&](Items<T, SC> &x, const T *base, const Rows<const T> &of) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = r0 + M::row(h, r);
+        x.load(r, at(base, of, row < s.rows ? row : 0), col0, s.W, n);
+      }
+    };
+    // float64 rows of 1 KB leave no registers for them yet
+    constexpr bool LATE = sizeof(T) == 8 && DP * sizeof(T) == 1024;
+    if constexpr (!LATE) {
+      load(xq, qp, a.q);
+      load(xg, gp, a.g);
+    }
     T lse[4], delta[4];
     int limit[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = r0 + M::row(h, r);
       const bool on = row < s.rows;
-      xq.load(r, at(qp, a.q, on ? row : 0), col0, s.W, on, n);
-      xg.load(r, at(gp, a.g, on ? row : 0), col0, s.W, on, n);
       lse[r] = a.lse[int64_t(bh) * s.rows + (on ? row : 0)];
       limit[r] = on ? seen(s, keys, first, int(s.by_group.div(uint32_t(row)))) : 0;
     }
     const bool live = r0 + n < s.rows;
     const int own = live ? r0 + n : 0;
-    const auto z = k.dots(at(qp, a.q, own), s.W, live, h);
+    const auto z = k.dots(at(qp, a.q, own), s.W, h);
+    if constexpr (DP * sizeof(T) == 1024)
+      __builtin_amdgcn_sched_barrier(0);
     T product;
     const auto dp =
-        v.dots(at(gp, a.g, own), at(yp, a.y, own), s.W, live, h, product);
+        v.dots(at(gp, a.g, own), at(yp, a.y, own), s.W, h, product);
     product += __shfl_xor(product, 16);
     product += __shfl_xor(product, 32);
 #pragma unroll
@@ -748,10 +770,18 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
         return r0 + item < s.rows ? at(base, x, r0 + item) + col0 : nullptr;
       };
     };
+    if constexpr (LATE) {
+      __builtin_amdgcn_sched_barrier(0);
+      load(xg, gp, a.g);
+    }
     if (__any(some) && !all_finite<T, SC>(xg))
       dv.add_visible(p, vis, s.D - col0, lane, row_of(gp, a.g));
     else
       dv.add(p, xg);
+    if constexpr (LATE) {
+      __builtin_amdgcn_sched_barrier(0);
+      load(xq, qp, a.q);
+    }
     if (__any(some) && !all_finite<T, SC>(xq))
       dk.add_visible(ds, vis, s.D - col0, lane, row_of(qp, a.q));
     else

@@ -141,10 +141,10 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
   for (int i = threadIdx.x; i < SA_TILE * (DP / 4); i += 256) {
     const int r = i / (DP / 4), d = i % (DP / 4) * 4, row = tile * SA_TILE + r;
     const bool live = row < rows;
-    const auto v = piece(live ? address(row) : base, d, s.W, live);
+    const auto v = piece(live ? address(row) : base, d, s.W);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      x[r * PITCH + d + j] = v[j];
+      x[r * PITCH + d + j] = live ? v[j] : 0.f;
   }
   __syncthreads();
   // four work-items to a row: its largest magnitude (NaN above infinity)
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
     for (int f = 0; f < 2 * DB; ++f)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const auto x = piece(qp, 16 * f + 8 * h + 4 * u, s.W, live);
+        const auto x = piece(qp, 16 * f + 8 * h + 4 * u, s.W);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v[f][4 * u + j] = x[j];
