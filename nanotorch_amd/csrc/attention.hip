@@ -319,7 +319,8 @@ constexpr int FWD_WAVES =
     DP * sizeof(T) == 1024 || (sizeof(T) == 8 && DP * sizeof(T) == 512) ? 1 : 2;
 
 // Tile `item` of a (sequence, key head).  WHOLE: rows of DP elements, aligned.
-template <class T, int DP, bool WHOLE>
+// MAY_AHEAD: the next keys may be loaded under a block.
+template <class T, int DP, bool WHOLE, bool MAY_AHEAD>
 __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, uint32_t item,
                                               uint32_t split, int col0) {
   using M = Mma<T>;
@@ -442,7 +443,8 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   // are formed: few rows over many keys wait for memory.
   int blk = int(split) * per + wave;
   // (not of rows that leave no registers for two blocks of keys)
-  constexpr bool AHEAD = WHOLE || DP * sizeof(T) < 512 || (sizeof(T) == 4 && DP == 256);
+  constexpr bool AHEAD =
+      MAY_AHEAD && (WHOLE || DP * sizeof(T) < 512 || (sizeof(T) == 4 && DP == 256));
   if constexpr (AHEAD) {
     if (blk < stop) {
       Keys x, y;
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, (FWD_WAVES<T, DP>)) void attn_fwd_ke
   const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
   item /= GROUPS;
   if (col0 < a.s.D)
-    attn_fwd_tile<T, DP, WHOLE>(a, bh, item / splits, item % splits, col0);
+    attn_fwd_tile<T, DP, WHOLE, true>(a, bh, item / splits, item % splits, col0);
 }
 
 // What the kernels on half-precision planes left: the tiles of each (sequence,
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_left_kernel(
   const uint32_t tiles = uint32_t(a.s.rows + 15) / 16;
   for (uint32_t t = blockIdx.x % groups; t < tiles; t += groups) {
     __syncthreads();
-    attn_fwd_tile<float, DP, false>(a, bh, t, 0, 0);
+    attn_fwd_tile<float, DP, false, false>(a, bh, t, 0, 0);
   }
 }
 
@@ -822,22 +824,24 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_kernel(const AttnBwd<T
 }
 
 // As attn_fwd_left_kernel.
-template <int DP>
+template <int DP, bool DQ, bool DKV>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const AttnBwd<float> a,
                                                                      uint32_t groups) {
   const uint32_t bh = blockIdx.x / groups;
   if (!gate_set(a.gate, bh))
     return;
   const uint32_t rows = uint32_t(a.s.rows + 15) / 16, keys = uint32_t(a.s.Tk + 15) / 16;
-  if (a.dq)
+  if (DQ && a.dq)
     for (uint32_t t = blockIdx.x % groups; t < rows; t += groups) {
       __syncthreads();
       attn_dq_tile<float, DP>(a, bh, t, 0);
     }
-  if (a.dk || a.dv)
+  if (DKV && (a.dk || a.dv))
     for (uint32_t t = blockIdx.x % groups; t < keys; t += groups) {
-      __syncthreads();
-      attn_dkv_tile<float, DP>(a, bh, t, 0);
+      for (int col0 = 0; col0 < a.s.D; col0 += KEY_COLUMNS<float, DP>) {
+        __syncthreads();
+        attn_dkv_tile<float, DP>(a, bh, t, col0);
+      }
     }
 }
 
@@ -1012,9 +1016,8 @@ template <class T> void run_attention(AttnFwd<T> &a) {
       a.splits = 1;
       const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk), groups = left_groups(bhs);
       dispatch_width<float>(s.D, [&]<int DP>() {
-        if constexpr (DP <= 128)
-          attn_fwd_left_kernel<DP>
-              <<<dim3(groups * bhs), 64 * AT_WAVES, 0, stream()>>>(a, groups);
+        attn_fwd_left_kernel<DP>
+            <<<dim3(groups * bhs), 64 * AT_WAVES, 0, stream()>>>(a, groups);
       });
       NT_LAUNCH_CHECK();
       return;
@@ -1048,8 +1051,11 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a) {
       run_split_bwd(a, words.get<uint32_t>());
       const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk), groups = left_groups(bhs);
       dispatch_width<float>(s.D, [&]<int DP>() {
-        if constexpr (DP <= 128)
-          attn_bwd_left_kernel<DP>
+        // (one kernel for both keeps too much of wide rows)
+        attn_bwd_left_kernel<DP, true, (DP <= 128)>
+            <<<dim3(groups * bhs), 64 * AT_WAVES, 0, stream()>>>(a, groups);
+        if constexpr (DP > 128)
+          attn_bwd_left_kernel<DP, false, true>
               <<<dim3(groups * bhs), 64 * AT_WAVES, 0, stream()>>>(a, groups);
       });
       NT_LAUNCH_CHECK();

@@ -399,7 +399,11 @@ __device__ __forceinline__ void store_row(float *p, const floatx16 (&acc)[DB], f
 
 // ---------------------------------------------------------------- forward
 
-constexpr int SF_WAVES = 8, SF_ROWS = SF_WAVES * SA_UNIT;
+// Eight waves, two to a SIMD, and 64 keys a step; of heads over 128 wide four waves,
+// which need the registers of two, and 32 keys, as many as LDS holds twice.
+template <int DB> constexpr int SF_WAVES = DB <= 4 ? 8 : 4;
+template <int DB> constexpr int SF_ROWS = SF_WAVES<DB> * SA_UNIT;
+template <int DB> constexpr int SF_UNITS = DB <= 4 ? 2 : 1;
 
 struct SplitFwd {
   AttnShape s;
@@ -415,13 +419,13 @@ struct SplitFwd {
 };
 
 template <int DB>
-__global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const SplitFwd a) {
-  constexpr int CH = SA_CHUNK<DB>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][4 * CH];
+__global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_split_fwd_kernel(const SplitFwd a) {
+  constexpr int CH = SA_CHUNK<DB>, UNITS = SF_UNITS<DB>, STEP = UNITS * SA_UNIT;
+  __shared__ __attribute__((aligned(1024))) char lds[2][2 * UNITS * CH];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tiles = uint32_t(s.rows + SF_ROWS - 1) / SF_ROWS;
+  const uint32_t tiles = uint32_t(s.rows + SF_ROWS<DB> - 1) / SF_ROWS<DB>;
   const uint32_t parts = uint32_t(a.parts);
   uint32_t bh, item;
   head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles * parts, bh, item);
@@ -435,22 +439,22 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
   auto limit_of = [&](int row) {
     return seen(s, keys, first, int(s.by_group.div(uint32_t(row))));
   };
-  const int row0 = tile * SF_ROWS + wave * SA_UNIT, row = row0 + n;
+  const int row0 = tile * SF_ROWS<DB> + wave * SA_UNIT, row = row0 + n;
   const bool live = row < s.rows;
   const int limit = live ? limit_of(row) : 0;
   const int end = row0 < s.rows ? limit_of(min(row0 + SA_UNIT, s.rows) - 1) : 0; // of any row
   const int all = row0 < s.rows ? limit_of(row0) : 0;                           // of every row
-  const int group_end = limit_of(min((tile + 1) * SF_ROWS, s.rows) - 1);
+  const int group_end = limit_of(min((tile + 1) * SF_ROWS<DB>, s.rows) - 1);
   const char *kp = a.k + int64_t(bh) * a.tiles * 2 * CH, *vp = a.v + int64_t(bh) * a.tiles * 2 * CH;
   auto issue = [&](char *stage, int it) {
 #pragma unroll
     for (int j = 0; j < 2 * DB; ++j) {
-      const int p = j < DB ? j * 8 + wave : (j - DB) * 8 + wave;
-      load_lds((j < DB ? kp : vp) + int64_t(it) * 2 * CH + p * 1024,
-               stage + (j < DB ? 0 : 2 * CH) + p * 1024, lane);
+      const int p = j % DB * SF_WAVES<DB> + wave;
+      load_lds((j < DB ? kp : vp) + int64_t(it) * UNITS * CH + p * 1024,
+               stage + (j < DB ? 0 : UNITS * CH) + p * 1024, lane);
     }
   };
-  const int all_steps = (group_end + SA_TILE - 1) / SA_TILE;
+  const int all_steps = (group_end + STEP - 1) / STEP;
   const int per = (all_steps + a.parts - 1) / a.parts;
   const int begin = min(part * per, all_steps), steps = min(begin + per, all_steps);
   if (begin < steps)
@@ -496,29 +500,29 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
     if (it + 1 < steps)
       issue(lds[(it + 1) & 1], it + 1);
     __builtin_amdgcn_sched_barrier(0);
-    if (it * SA_TILE >= end)
+    if (it * STEP >= end)
       continue;
     const char *st = lds[it & 1];
     // positive and finite, so that it takes -inf to -inf
-    const float cz = fminf(fmaxf(c * q_scale * a.k_scale[int64_t(bh) * a.tiles + it], 1.2e-38f),
+    const float cz = fminf(fmaxf(c * q_scale * a.k_scale[int64_t(bh) * a.tiles + it * UNITS / 2], 1.2e-38f),
                            3.4e38f);
-    const float v_scale = a.v_scale[int64_t(bh) * a.tiles + it];
-    floatx16 z[2];
+    const float v_scale = a.v_scale[int64_t(bh) * a.tiles + it * UNITS / 2];
+    floatx16 z[UNITS];
     Pair pre[2];
     first_pairs<DB>(pre, st, lane);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < UNITS; ++u)
       z[u] = dots32<DB>(st + u * CH, qh, ql, pre,
                         [&](int f) { return st + (u + 1) * CH + f * 1024; }, lane);
-    if (it * SA_TILE + SA_TILE > all)
+    if (it * STEP + STEP > all)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < UNITS; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          z[u][r] = it * SA_TILE + u * SA_UNIT + row32(h, r) < limit ? z[u][r] : -SA_INF;
+          z[u][r] = it * STEP + u * SA_UNIT + row32(h, r) < limit ? z[u][r] : -SA_INF;
     float top = -SA_INF;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < UNITS; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         top = fmaxf(top, z[u][r]);
@@ -528,7 +532,7 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
     m = next;
     float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < UNITS; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         // times 2^14, which the quotient by l takes out again
@@ -536,15 +540,15 @@ __global__ __launch_bounds__(64 * SF_WAVES, 2) void attn_split_fwd_kernel(const 
         sum += z[u][r];
       }
     l = fmaf(l, shrink, sum);
-    half8 ph[4], pl[4];
+    half8 ph[2 * UNITS], pl[2 * UNITS];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < UNITS; ++u)
       split16(z[u], ph + 2 * u, pl + 2 * u);
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
-      const floatx16 o = stream_sum<4, true, CH / 2>(
-          [&](int f) { return st + (2 + f / 2) * CH + (2 * db + f % 2) * 1024; },
-          [&](int f) { return st + 2 * CH + (2 * (db + 1 < DB ? db + 1 : 0) + f) * 1024; }, ph, pl,
+      const floatx16 o = stream_sum<2 * UNITS, true, CH / 2>(
+          [&](int f) { return st + (UNITS + f / 2) * CH + (2 * db + f % 2) * 1024; },
+          [&](int f) { return st + UNITS * CH + (2 * (db + 1 < DB ? db + 1 : 0) + f) * 1024; }, ph, pl,
           pre, lane);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -603,17 +607,18 @@ __global__ __launch_bounds__(256) void attn_split_join_kernel(const SplitFwd a) 
   const float k = seen(s, keys, first, int(i)) > 0 ? 1.f / total : 0.f;
   const int64_t head = int64_t(bh % uint32_t(s.Hk)) * s.G + (uint32_t(row) - i * uint32_t(s.G));
   float *y = a.y + ((int64_t(bh / uint32_t(s.Hk)) * s.Tq + i) * s.Hk * s.G + head) * s.D;
-  // both halves of a row of up to 128 at once
-  float v[2] = {0.f, 0.f};
+  // a row of up to 256 at once
+  float v[4] = {};
 #pragma unroll 8
   for (int p = 0; p < a.parts; ++p) {
     const float w = __shfl(weight, p);
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      v[c] = fmaf(a.sums[(p * rows + at) * s.D + min(64 * c + lane, s.D - 1)], w, v[c]);
+    for (int c = 0; c < 4; ++c)
+      if (64 * c < s.D)
+        v[c] = fmaf(a.sums[(p * rows + at) * s.D + min(64 * c + lane, s.D - 1)], w, v[c]);
   }
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+  for (int c = 0; c < 4; ++c)
     if (64 * c + lane < s.D)
       y[64 * c + lane] = v[c] * k;
   if (a.lse && lane == 0)
@@ -623,9 +628,12 @@ __global__ __launch_bounds__(256) void attn_split_join_kernel(const SplitFwd a) 
 // --------------------------------------------------------------- backward
 
 // Two waves to a SIMD: two workgroups of four on a CU, or where the stages fill more
-// than half of its LDS one of eight.
-template <int DB> constexpr int SB_WAVES = DB <= 2 ? 4 : 8;
+// than half of its LDS one of eight; of heads over 128 wide one wave to a SIMD.
+template <int DB> constexpr int SB_WAVES = DB <= 2 || DB > 4 ? 4 : 8;
 template <int DB> constexpr int SB_ROWS = SB_WAVES<DB> * SA_UNIT;
+// Stages of so many bytes: two, or as LDS (160 KB) has it one, loaded when all waves
+// are done with it.
+constexpr int SB_STAGES(int bytes) { return 2 * bytes <= 150 * 1024 ? 2 : 1; }
 
 struct SplitBwd {
   AttnShape s;
@@ -650,10 +658,11 @@ __device__ __forceinline__ void load_own(const char *unit, half8 (&hi)[2 * DB],
 }
 
 template <int DB>
-__global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
+__global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_split_dq_kernel(
     const SplitBwd a) {
   constexpr int CH = SA_CHUNK<DB>, WAVES = SB_WAVES<DB>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][3 * CH];
+  constexpr int STAGES = SB_STAGES(3 * CH);
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES][3 * CH];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -689,8 +698,8 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
   const int all_steps = (group_end + SA_UNIT - 1) / SA_UNIT;
   const int per = (all_steps + a.q_parts - 1) / a.q_parts;
   const int begin = min(part * per, all_steps), steps = min(begin + per, all_steps);
-  if (begin < steps)
-    issue(lds[begin & 1], begin);
+  if (STAGES == 2 && begin < steps)
+    issue(lds[begin & (STAGES - 1)], begin);
   half8 qh[2 * DB], ql[2 * DB], gh[2 * DB], gl[2 * DB];
   const int64_t unit = int64_t(bh) * a.q_tiles * 2 + (on ? row0 / SA_UNIT : 0);
   load_own<DB>(a.q_row + unit * CH, qh, ql, lane);
@@ -701,13 +710,17 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
   const float c = a.scale2 * a.q_scale[unit / 2];
   floatx16 acc[DB]{};
   for (int it = begin; it < steps; ++it) {
+    if constexpr (STAGES == 1) {
+      __syncthreads();
+      issue(lds[0], it);
+    }
     stage_ready();
-    if (it + 1 < steps)
-      issue(lds[(it + 1) & 1], it + 1);
+    if (STAGES == 2 && it + 1 < steps)
+      issue(lds[(it + 1) & (STAGES - 1)], it + 1);
     __builtin_amdgcn_sched_barrier(0);
     if (it * SA_UNIT >= end)
       continue;
-    const char *stage = lds[it & 1];
+    const char *stage = lds[it & (STAGES - 1)];
     const float k_scale = a.k_scale[int64_t(bh) * a.k_tiles + it / 2];
     const float v_scale = a.v_scale[int64_t(bh) * a.k_tiles + it / 2];
     Pair pre[2];
@@ -747,13 +760,14 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dq_kernel(
 // waves to a SIMD, and one wave leaves the matrix cores idle while it forms
 // probabilities: 8192 tokens, 16 heads over 4 of 128, in one kernel 2.53 ms.
 template <int DB, bool DK, bool DV>
-__global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
+__global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_split_dkv_kernel(
     const SplitBwd a) {
   constexpr int CH = SA_CHUNK<DB>, STAT = SA_STATS * 4, WAVES = SB_WAVES<DB>;
   // a stage: q's rows; g's (DK); g's columns (DV); q's columns (DK)
   constexpr int FORMS = 1 + 2 * DK + DV, G_ROW = CH, G_COL = DK ? 2 * CH : CH,
                 Q_COL = (2 + DV) * CH;
-  __shared__ __attribute__((aligned(1024))) char lds[2][FORMS * CH + STAT];
+  constexpr int STAGES = SB_STAGES(FORMS * CH + STAT);
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES][FORMS * CH + STAT];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -798,7 +812,7 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
                                                            wave * 64 + lane),
           (__attribute__((address_space(3))) void *)(stage + FORMS * CH + wave * 256), 4, 0, 0);
   };
-  if (u0 < u1)
+  if (STAGES == 2 && u0 < u1)
     issue(lds[0], u0);
   half8 kh[2 * DB], kl[2 * DB], vh[2 * DB], vl[2 * DB];
   const bool on = own0 < keys;
@@ -809,10 +823,14 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, 2) void attn_split_dkv_kernel(
   const float v_scale = a.v_scale[unit / 2], c = a.scale2 * a.k_scale[unit / 2];
   floatx16 dk[DB]{}, dv[DB]{};
   for (int it = u0; it < u1; ++it) {
-    const int buf = (it - u0) & 1;
+    const int buf = (it - u0) & (STAGES - 1);
+    if constexpr (STAGES == 1) {
+      __syncthreads();
+      issue(lds[0], it);
+    }
     stage_ready();
-    if (it + 1 < u1)
-      issue(lds[buf ^ 1], it + 1);
+    if (STAGES == 2 && it + 1 < u1)
+      issue(lds[buf ^ (STAGES - 1)], it + 1);
     __builtin_amdgcn_sched_barrier(0);
     const int r0 = it * SA_UNIT;
     if (!on || limit_of(min(r0 + SA_UNIT, s.rows) - 1) <= own0)
@@ -934,15 +952,20 @@ template <class F> void dispatch_blocks(int D, F &&f) {
     return f.template operator()<2>();
   case 3:
     return f.template operator()<3>();
-  default:
+  case 4:
     return f.template operator()<4>();
+  case 5:
+    return f.template operator()<5>();
+  case 6:
+    return f.template operator()<6>();
+  default:
+    return f.template operator()<8>();
   }
 }
 
 } // namespace
 
-// Float32 with heads of up to 128 elements (a wider one's planes outgrow the
-// registers), from the size on at which packing, another launch or two and half-empty
+// From the size on at which packing, another launch or two and half-empty
 // tiles cost less than the matrix cores save.  Both sides in us, B, Tq, Tk, H, Hk, D,
 // this kind second.  Forward: 8 256 256 8 8 64 24 and 29, 1 1024 1024 4 4 64 30 and
 // 31, 4 2048 2048 16 16 64 about 470 and 165; of few rows 4 16 4096 32 8 128 85 and
@@ -950,8 +973,6 @@ template <class F> void dispatch_blocks(int D, F &&f) {
 // 8 8 64 52 and 52, 1 1024 1024 4 4 64 89 and 53, 8 1 8192 64 2 128 870 and 237; of
 // long axes with little beside them 1 64 2000 8 8 64 88 and 38.
 bool split_takes(const AttnShape &s, bool backward) {
-  if (s.D > 128)
-    return false;
   const double work = double(s.B) * s.Hk * s.rows * s.Tk * s.D;
   if (backward && std::max(s.rows, s.Tk) >= 640 && work >= double(1 << 25))
     return true;
@@ -991,14 +1012,14 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     f.y = a.y, f.lse = a.lse;
     f.scale2 = a.scale2;
     f.gate = a.gate;
-    const uint32_t groups = bhs * uint32_t((s.rows + SF_ROWS - 1) / SF_ROWS);
-    f.parts = parts_of(groups, tiles);
+    const uint32_t groups = bhs * uint32_t((s.rows + SF_ROWS<DB> - 1) / SF_ROWS<DB>);
+    f.parts = parts_of(groups, tiles * 2 / SF_UNITS<DB>);
     const size_t rows = size_t(bhs) * size_t(s.rows), kept = f.parts > 1 ? size_t(f.parts) : 0;
     DeviceScratch sums(kept * rows * size_t(s.D + 2) * sizeof(float));
     f.sums = sums.get<float>();
     f.tops = f.sums + kept * rows * size_t(s.D);
     attn_split_fwd_kernel<DB>
-        <<<dim3(groups * uint32_t(f.parts)), 64 * SF_WAVES, 0, stream()>>>(f);
+        <<<dim3(groups * uint32_t(f.parts)), 64 * SF_WAVES<DB>, 0, stream()>>>(f);
     NT_LAUNCH_CHECK();
     if (f.parts > 1) {
       attn_split_join_kernel<<<dim3(bhs * uint32_t((s.rows + 3) / 4)), 256, 0, stream()>>>(f);

@@ -162,6 +162,8 @@ LARGE = [  # as many products as the half-precision planes are used for
     (1, 1100, 1100, 6, 3, 128), (2, 1030, 1470, 6, 3, 96), (2, 1600, 1601, 3, 3, 33),
     (3, 657, 1640, 2, 1, 80), (1, 70, 9001, 8, 1, 100), (1, 3333, 330, 4, 1, 96),
     (9, 777, 777, 2, 2, 64), (1, 1777, 1777, 4, 4, 32),
+    (1, 1300, 1200, 2, 1, 160), (1, 900, 1150, 4, 2, 190), (2, 700, 700, 3, 3, 256),
+    (1, 140, 5000, 6, 1, 131),
     # the backward pass alone
     (1, 20, 9049, 8, 1, 96), (1, 520, 520, 8, 4, 64), (8, 1, 4100, 40, 4, 32),
     (2, 300, 470, 6, 6, 128), (1, 1300, 1300, 2, 2, 40),
@@ -211,15 +213,16 @@ def test_large_of_any_magnitude(gpu, what, size):
     check_all(q, k, v, g, visible(1, 1820, 1820, True), np.float32, causal=True)
 
 
-@pytest.mark.parametrize("what", ["k", "v", "q"])
-def test_large_with_an_outlier(gpu, what):
+@pytest.mark.parametrize("what,D", [("k", 64), ("v", 64), ("q", 64), ("k", 256), ("v", 200),
+                                    ("q", 132)])
+def test_large_with_an_outlier(gpu, what, D):
     """One row 2^13 times and more above its neighbours, where most rows do not
     see it: the others keep their bits."""
     r = rng(seed_of("outlier", what))
     T = 1820
-    q, k, v, g = inputs(r, 1, T, T, 2, 1, 64, np.float32)
+    q, k, v, g = inputs(r, 1, T, T, 2, 1, D, np.float32)
     see = visible(1, T, T, True)
-    clean = reference(q, k, v, g, see, 0.125, U[np.float32])
+    clean = reference(q, k, v, g, see, D ** -0.5, U[np.float32])
     x = {"q": q, "k": k, "v": v}[what]
     at = T - 20
     x[0, at] *= np.float32(1e12)
