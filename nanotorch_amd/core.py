@@ -604,39 +604,56 @@ def _basic_index_view(x: Tensor, index: tuple):
 # ---------------------------------------------------------------- autograd
 
 
+def _backward_order(seed: Tensor) -> list[tuple[Tensor, Any, tuple]]:
+    """(tensor, function, its tensor inputs) of every node below `seed`, each after
+    all that consume it, in the order in which a breadth-first walk along every
+    path meets them last (reference: core.py:840-860, which takes that walk; with a
+    residual in every block its length doubles from one to the next).
+
+    Last met means at the end of the longest path: nodes go by its length, and
+    those of one length by the consumers that are one step shorter, the last of
+    them first, then by the last place among its inputs."""
+    nodes: dict[int, tuple[Tensor, Any, tuple]] = {}
+    uses: dict[int, int] = {}  # edges from consumers not yet done
+    todo = [seed]
+    while todo:
+        f_x = todo.pop()
+        if id(f_x) in nodes or f_x._grad_fn is None:
+            continue
+        inputs = tuple([x for x in f_x._grad_fn.inputs if isinstance(x, Tensor)])
+        nodes[id(f_x)] = (f_x, f_x._grad_fn, inputs)
+        for x in inputs:
+            if x._grad_fn is not None:
+                uses[id(x)] = uses.get(id(x), 0) + 1
+                todo.append(x)
+    order: list[tuple[Tensor, Any, tuple]] = []
+    level = [id(seed)] if id(seed) in nodes else []
+    while level:
+        # a node's last consumer is done in the level before its own; met again,
+        # it goes to the end
+        following: dict[int, None] = {}
+        for key in level:
+            order.append(nodes[key])
+            for x in nodes[key][2]:
+                if x._grad_fn is not None:
+                    uses[id(x)] -= 1
+                    following.pop(id(x), None)
+                    following[id(x)] = None
+        level = [key for key in following if uses[key] == 0]
+    return order
+
+
 def _backpropagate_grad(seed: Tensor) -> None:
     """Backpropagation engine (reference: core.py:836-872).
 
-    Nodes are gathered breadth-first while counting, for every tensor, how
-    many graph edges consume it; a node's backward runs when its count drops
-    to zero.  Gradients land in ``x._grad``: the first one is stored as is,
-    later ones are added (``old + new``).  Functions that implement
-    ``_backward_into`` compute and accumulate in one fused pass; others go
-    through ``backward`` plus an in-place add.
+    A node's backward runs when all its consumers' have.  Gradients land in
+    ``x._grad``: the first one is stored as is, later ones are added (``old +
+    new``).  Functions that implement ``_backward_into`` compute and accumulate
+    in one fused pass; others go through ``backward`` plus an in-place add.
     """
-    to_visit = [seed]
-    ncons = {id(seed): 0}
-    order: list[tuple[Tensor, Any, tuple]] = []
-    while to_visit:
-        f_x = to_visit.pop(0)
-        fn = f_x._grad_fn
-        if fn is None:
-            continue
-        inputs = []
-        for x in fn.inputs:
-            if isinstance(x, Tensor):
-                if x._requires_grad or x._grad_fn is not None:
-                    ncons[id(x)] = ncons.get(id(x), 0) + 1
-                    to_visit.append(x)
-                inputs.append(x)
-        order.append((f_x, fn, tuple(inputs)))
-
-    for f_x, fn, inputs in order:
+    for f_x, fn, inputs in _backward_order(seed):
         if f_x._grad is None:
             raise RuntimeError("f_x.grad is None.")
-        ncons[id(f_x)] -= 1
-        if ncons[id(f_x)] > 0:
-            continue
         _run_backward(fn, f_x._grad, inputs)
         f_x._grad = None
 
