@@ -93,7 +93,8 @@ class AdamW(Optimizer):
         self._betas, self._eps, self._decay = (b1, b2), eps, weight_decay
         self._step = 0
         unique: dict[int, Tensor] = {id(p): p for p in parameters}
-        self._slots: list[tuple[Tensor, int]] = []  # and where its moments begin
+        # each parameter, where its moments begin, its shape, strides and size
+        self._slots: list[tuple[Tensor, int, tuple, tuple, int]] = []
         self._dtype, n = Dtype.Float32, 0
         for i, p in enumerate(unique.values()):
             dtype = p._storage._dtype
@@ -101,7 +102,7 @@ class AdamW(Optimizer):
                 raise ValueError(f"AdamW needs parameters of one float type, got "
                                  f"{dtype.name} at {i}.")
             self._dtype = dtype
-            self._slots.append((p, n))
+            self._slots.append((p, n, p._shape, row_major_strides(p._shape), p.numel))
             n += -(-p.numel // self._ALIGN) * self._ALIGN
         self._size = n
         self._m: Tensor | None = None  # made with the first step
@@ -124,7 +125,7 @@ class AdamW(Optimizer):
     def moments_of(self, i: int) -> tuple[Tensor, Tensor]:
         """The moments of parameter i, as views of its shape."""
         p = list(self._parameters)[i]
-        at = next(at for q, at in self._slots if q is p)
+        at = next(slot[1] for slot in self._slots if slot[0] is p)
         return tuple([Tensor._new_view(t._storage, p._shape, None, at)
                       for t in self.moments()])
 
@@ -142,37 +143,38 @@ class AdamW(Optimizer):
 
     def step(self) -> None:
         tensors: list[int] = []
-        written: list[Tensor] = []
+        written = []
         copies: list[tuple[Tensor, Tensor]] = []  # views: stepped as a copy
         keep = []  # temporaries live until the call
-        dtype = self._dtype
-        for p, at in self._slots:
-            if not p.requires_grad:
+        dtype, cuda = self._dtype, Device.Cuda
+        item = 4 if dtype is Dtype.Float32 else 8
+        for p, at, shape, strides, n in self._slots:
+            if not p._requires_grad and p._grad_fn is None:
                 continue
             g = p._grad
             if g is None:
                 raise RuntimeError("Gradients not set, did you call backward?")
-            if p._storage._device is not Device.Cuda or g._storage._device is not Device.Cuda:
+            to, ps, gs = p, p._storage, g._storage
+            if not (ps._dtype is dtype and gs._dtype is dtype and ps._device is cuda
+                    and gs._device is cuda and p._strides == strides and g._strides == strides
+                    and p._shape == shape and g._shape == shape):
                 K.require_device(p, g)
-            if p._storage._dtype is not dtype or g._shape != p._shape:
-                raise ValueError(f"A parameter {dtype.name} {p.shape} became {p.dtype.name}, or "
-                                 f"its gradient has another shape: {g.shape}.")
-            strides = row_major_strides(p._shape)
-            if g._storage._dtype is not dtype or g._strides != strides:
-                g = g.to(dtype)._to_contiguous()
-                keep.append(g)
-            to = p
-            if p._strides != strides:
-                to = p._to_contiguous(force=True)
-                copies.append((to, p))
-            item = 4 if dtype is Dtype.Float32 else 8
+                if ps._dtype != dtype or p._shape != shape or g._shape != shape:
+                    raise ValueError(f"A parameter {dtype.name} {shape} became {p.dtype.name} "
+                                     f"{p.shape}, or its gradient has another shape: {g.shape}.")
+                if gs._dtype != dtype or g._strides != strides:
+                    g = g.to(dtype)._to_contiguous()
+                    keep.append(g)
+                if p._strides != strides:
+                    to = p._to_contiguous(force=True)
+                    copies.append((to, p))
             tensors += (to._storage._ptr + to._offset * item, g._storage._ptr + g._offset * item,
-                        p.numel, at)
-            written.append(p)
+                        n, at)
+            written.append(ps)
         m, v = self.moments()
         K.adamw_step(tensors, m, v, self.lr, self._betas, self._eps, self._decay, self._step + 1)
         self._step += 1
         for new, p in copies:
             K.copy_view(new, p)
-        for p in written:
-            p._storage.bump_version()
+        for storage in written:
+            storage.version += 1
