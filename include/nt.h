@@ -433,10 +433,11 @@ int nt_rms_norm_bwd(const nt_view *sum, const nt_view *weight,
  *   1  j <= lengths[b] - Tq + i: the queries end with the sequence;
  *   2  j <= starts[b] + i, or start + i where starts is NULL.
  * lengths and starts are 1-D int32 or int64 [B].  A query that sees nothing
- * gives zeros.  Keys from lengths[b] on are not read.  A length outside
- * [0, Tk] is taken as the nearer end, and the next nt_sync() or
- * nt_memcpy_d2h() returns NT_ERR_INDEX.  y is contiguous; lse, which
- * nt_attention_bwd needs, receives B H Tq statistics or is NULL. */
+ * gives zeros.  What lies from lengths[b] on has no influence, nor has anything
+ * else that a query does not see, whatever it holds.  A length outside [0, Tk] is taken
+ * as the nearer end, and the next nt_sync() or nt_memcpy_d2h() returns
+ * NT_ERR_INDEX.  y is contiguous; lse, which nt_attention_bwd needs, receives
+ * B H Tq statistics or is NULL.  Hk max(Tq H / Hk, Tk) is below 2^25. */
 int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v,
                  const nt_view *lengths, const nt_view *starts, int64_t start,
                  int32_t causal, double scale, const nt_view *y,

@@ -6,7 +6,10 @@
 //
 // Seven streams of the parameters' size (p, g, m, v read, p, m, v written)
 // and some 60 instructions an element: bound by HBM from a few million
-// elements on, by the launch below.  Coefficients are formed on the host in
+// elements on, by the launch below.  184 million in 122 parameters take 905 us,
+// 287 million in 12 1375: 5.7 and 5.85 TB/s.  (Two 16-byte pieces of each stream to a
+// work-item, or eight, or workgroups of 512 took 2 to 5% longer, loads and stores
+// without the streaming hint 8%.)  Coefficients are formed on the host in
 // 64 bits and rounded once; the element's own arithmetic is in its type.
 #include <algorithm>
 #include <cmath>

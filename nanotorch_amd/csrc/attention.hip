@@ -30,10 +30,18 @@
 // items; they are joined in LDS in a fixed order, and so are the parts of rows
 // whose keys are split over workgroups (few rows over a long cache).
 //
-// Keys from lengths[b] on are not read.  Within the length, a key that only
-// some rows of a tile see may hold anything: where such a block has a value
+// What lies from lengths[b] on has no influence.  Within the length, a key that
+// only some rows of a tile see may hold anything: where such a block has a value
 // that is not finite, the sums go over visible pairs one by one (0 times an
 // infinity would be NaN).
+//
+// What bounds them: few rows over a long cache, HBM (8 tokens of 32 heads over caches
+// of up to 8192 x 8 x 128: 80 us for 403 MB and 7 for joining the 16 parts, 5.0 TB/s;
+// of rows that four heads share, 12 of each instruction's 16 are empty, which costs
+// nothing here); small texts, latency (4 x 128 tokens, 4 heads of 64: 8 us forward,
+// 12 backward, of which an empty launch is 3); float64, loads that nothing hides (one
+// or two waves to a SIMD): 1024 x 8 heads of 64 both passes 17 TFLOP/s of the 71 that
+// a large product reaches.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -891,6 +899,44 @@ Tokens per_sequence(const nt_view *v, int64_t B, const char *what) {
   return t;
 }
 
+// Tiles of 16 rows of one launch: its work-items are counted in 32 bits, with four
+// workgroups of 256 at most for a tile of rows and one of keys.
+constexpr int64_t MOST_TILES = int64_t(1) << 21;
+
+// Some of the sequences of a view [B, ...], or of a contiguous array of B parts.
+nt_view sequences(const nt_view *v, int64_t b, int64_t n) {
+  nt_view p = *v;
+  p.offset += b * p.strides[0];
+  p.shape[0] = n;
+  return p;
+}
+nt_view parts(const nt_view *v, int64_t B, int64_t b, int64_t n) {
+  nt_view p = *v;
+  const int64_t each = numel(v) / B;
+  p.offset += b * each;
+  p.ndim = 1;
+  p.shape[0] = n * each;
+  p.strides[0] = 1;
+  return p;
+}
+
+// Into how many launches' worth of sequences a call goes: one but for very many
+// rows.  0: the views are not what they should be, which attn_shape reports.
+int64_t sequences_at_once(const nt_view *q, const nt_view *k) {
+  if (q == nullptr || k == nullptr || q->ndim != 4 || k->ndim != 4 || q->shape[0] < 2 ||
+      k->shape[2] < 1)
+    return 0;
+  for (const nt_view *v : {q, k})
+    for (int i = 0; i < 4; ++i)
+      if (v->shape[i] < 0 || v->shape[i] >= (int64_t(1) << 30))
+        return 0;
+  const int64_t Hk = k->shape[2];
+  const int64_t rows = std::max(q->shape[1] * (q->shape[2] / Hk), k->shape[1]);
+  if (rows >= (int64_t(1) << 30))
+    return 0;
+  return std::max<int64_t>(1, (MOST_TILES - 1) / std::max<int64_t>(1, Hk * ((rows + 15) / 16)));
+}
+
 AttnShape attn_shape(const nt_view *q, const nt_view *k, const nt_view *v,
                      const nt_view *lengths, const nt_view *starts, int64_t start,
                      int32_t causal) {
@@ -909,7 +955,7 @@ AttnShape attn_shape(const nt_view *q, const nt_view *k, const nt_view *v,
   constexpr int64_t MOST = int64_t(1) << 30;
   const int64_t G = H / Hk;
   if (B >= MOST || Tk >= MOST || Tq >= MOST || H >= MOST || Tq * G >= MOST || B * Hk >= MOST ||
-      (B * Hk) * ((std::max(Tq * G, Tk) + 15) / 16) >= MOST / 1024)
+      (B * Hk) * ((std::max(Tq * G, Tk) + 15) / 16) >= MOST_TILES)
     fail(NT_ERR_VALUE, "attention: too many rows");
   AttnShape s{};
   s.B = int(B), s.Tq = int(Tq), s.Tk = int(Tk), s.Hk = int(Hk), s.G = int(G), s.D = int(D);
@@ -1077,6 +1123,102 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a) {
 
 } // namespace nt
 
+namespace nt {
+namespace {
+
+void attention(const nt_view *q, const nt_view *k, const nt_view *v, const nt_view *lengths,
+               const nt_view *starts, int64_t start, int32_t causal, double scale,
+               const nt_view *y, const nt_view *lse) {
+  const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
+  dispatch_float(q->dtype, [&]<class T>() {
+    AttnFwd<T> a{};
+    a.s = s;
+    a.q = rows_of<const T>(q, s.G);
+    a.k = rows_of<const T>(k, 1);
+    a.v = rows_of<const T>(v, 1);
+    a.y = contiguous_of<T>(y, numel(q), q->dtype, "y");
+    const int64_t rows = int64_t(s.B) * s.Hk * s.rows;
+    if (lse)
+      a.lse = contiguous_of<T>(lse, rows, q->dtype, "lse");
+    a.scale2 = T(scale * 1.4426950408889634);
+    a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v);
+    if (rows == 0)
+      return;
+    const int H = s.Hk * s.G;
+    Padded<T> pq(s, a.q, s.Tq, H, s.G), pk(s, a.k, s.Tk, s.Hk, 1), pv(s, a.v, s.Tk, s.Hk, 1);
+    run_attention(a);
+  });
+}
+
+void attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v, const nt_view *lengths,
+                   const nt_view *starts, int64_t start, int32_t causal, double scale,
+                   const nt_view *y, const nt_view *lse, const nt_view *g, const nt_view *dq,
+                   const nt_view *dk, const nt_view *dv) {
+  const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
+  check_heads(g, q, "g");
+  require_same_shape(g, q, "attention_bwd");
+  dispatch_float(q->dtype, [&]<class T>() {
+    AttnBwd<T> a{};
+    a.s = s;
+    a.q = rows_of<const T>(q, s.G);
+    a.k = rows_of<const T>(k, 1);
+    a.v = rows_of<const T>(v, 1);
+    a.g = rows_of<const T>(g, s.G);
+    a.y.p = contiguous_of<const T>(y, numel(q), q->dtype, "y");
+    a.y.sInner = s.D;
+    a.y.sHead = int64_t(s.D) * s.G;
+    a.y.sOuter = a.y.sHead * s.Hk;
+    a.y.sB = a.y.sOuter * s.Tq;
+    a.lse = contiguous_of<const T>(lse, int64_t(s.B) * s.Hk * s.rows, q->dtype, "lse");
+    if (dq)
+      a.dq = contiguous_of<T>(dq, numel(q), q->dtype, "dq");
+    if (dk)
+      a.dk = contiguous_of<T>(dk, numel(k), q->dtype, "dk");
+    if (dv)
+      a.dv = contiguous_of<T>(dv, numel(v), q->dtype, "dv");
+    a.scale = T(scale);
+    a.scale2 = T(scale * 1.4426950408889634);
+    const int H = s.Hk * s.G;
+    Padded<T> pq(s, a.q, s.Tq, H, s.G), pk(s, a.k, s.Tk, s.Hk, 1), pv(s, a.v, s.Tk, s.Hk, 1);
+    Padded<T> pg(s, a.g, s.Tq, H, s.G), py(s, a.y, s.Tq, H, s.G);
+    run_attention_bwd(a);
+  });
+}
+
+// Calls `f` with the views' sequences, as many at a time as one launch holds.
+// Views of the whole call, some of them null: q, k and others with a sequence to
+// each first index; from `first_array` on contiguous ones of as many equal parts.
+template <size_t N, class F>
+void by_sequences(const nt_view *(&views)[N], size_t first_array, F &&f) {
+  const nt_view *q = views[0], *k = views[1];
+  const int64_t most = sequences_at_once(q, k), B = most ? q->shape[0] : 0;
+  bool whole = most == 0 || B <= most;
+  for (size_t i = 0; i < N && !whole; ++i) { // not of one batch: reported by the whole call
+    const nt_view *v = views[i];
+    if (v && (v->ndim < 1 || v->ndim > NT_MAX_DIMS ||
+              (i < first_array ? v->shape[0] != B : numel(v) % B != 0)))
+      whole = true;
+  }
+  if (whole)
+    return f(views);
+  for (int64_t b = 0; b < B; b += most) {
+    const int64_t n = std::min(most, B - b);
+    nt_view some[N];
+    const nt_view *at[N];
+    for (size_t i = 0; i < N; ++i) {
+      at[i] = nullptr;
+      if (views[i]) {
+        some[i] = i < first_array ? sequences(views[i], b, n) : parts(views[i], B, b, n);
+        at[i] = &some[i];
+      }
+    }
+    f(at);
+  }
+}
+
+} // namespace
+} // namespace nt
+
 using namespace nt;
 
 extern "C" {
@@ -1085,24 +1227,9 @@ int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v, const nt_
                  const nt_view *starts, int64_t start, int32_t causal, double scale,
                  const nt_view *y, const nt_view *lse) {
   return guard([&] {
-    const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
-    dispatch_float(q->dtype, [&]<class T>() {
-      AttnFwd<T> a{};
-      a.s = s;
-      a.q = rows_of<const T>(q, s.G);
-      a.k = rows_of<const T>(k, 1);
-      a.v = rows_of<const T>(v, 1);
-      a.y = contiguous_of<T>(y, numel(q), q->dtype, "y");
-      const int64_t rows = int64_t(s.B) * s.Hk * s.rows;
-      if (lse)
-        a.lse = contiguous_of<T>(lse, rows, q->dtype, "lse");
-      a.scale2 = T(scale * 1.4426950408889634);
-      a.vec = whole_pieces(q) && whole_pieces(k) && whole_pieces(v);
-      if (rows == 0)
-        return;
-      const int H = s.Hk * s.G;
-      Padded<T> pq(s, a.q, s.Tq, H, s.G), pk(s, a.k, s.Tk, s.Hk, 1), pv(s, a.v, s.Tk, s.Hk, 1);
-      run_attention(a);
+    const nt_view *views[] = {q, k, v, lengths, starts, y, lse};
+    by_sequences(views, 5, [&](const nt_view *const *x) {
+      attention(x[0], x[1], x[2], x[3], x[4], start, causal, scale, x[5], x[6]);
     });
   });
 }
@@ -1113,34 +1240,10 @@ int nt_attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v,
                      const nt_view *g, const nt_view *dq, const nt_view *dk,
                      const nt_view *dv) {
   return guard([&] {
-    const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
-    check_heads(g, q, "g");
-    require_same_shape(g, q, "attention_bwd");
-    dispatch_float(q->dtype, [&]<class T>() {
-      AttnBwd<T> a{};
-      a.s = s;
-      a.q = rows_of<const T>(q, s.G);
-      a.k = rows_of<const T>(k, 1);
-      a.v = rows_of<const T>(v, 1);
-      a.g = rows_of<const T>(g, s.G);
-      a.y.p = contiguous_of<const T>(y, numel(q), q->dtype, "y");
-      a.y.sInner = s.D;
-      a.y.sHead = int64_t(s.D) * s.G;
-      a.y.sOuter = a.y.sHead * s.Hk;
-      a.y.sB = a.y.sOuter * s.Tq;
-      a.lse = contiguous_of<const T>(lse, int64_t(s.B) * s.Hk * s.rows, q->dtype, "lse");
-      if (dq)
-        a.dq = contiguous_of<T>(dq, numel(q), q->dtype, "dq");
-      if (dk)
-        a.dk = contiguous_of<T>(dk, numel(k), q->dtype, "dk");
-      if (dv)
-        a.dv = contiguous_of<T>(dv, numel(v), q->dtype, "dv");
-      a.scale = T(scale);
-      a.scale2 = T(scale * 1.4426950408889634);
-      const int H = s.Hk * s.G;
-      Padded<T> pq(s, a.q, s.Tq, H, s.G), pk(s, a.k, s.Tk, s.Hk, 1), pv(s, a.v, s.Tk, s.Hk, 1);
-      Padded<T> pg(s, a.g, s.Tq, H, s.G), py(s, a.y, s.Tq, H, s.G);
-      run_attention_bwd(a);
+    const nt_view *views[] = {q, k, v, lengths, starts, g, y, lse, dq, dk, dv};
+    by_sequences(views, 6, [&](const nt_view *const *x) {
+      attention_bwd(x[0], x[1], x[2], x[3], x[4], start, causal, scale, x[6], x[7], x[5], x[8],
+                    x[9], x[10]);
     });
   });
 }

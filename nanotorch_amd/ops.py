@@ -238,9 +238,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False,
       their sequences: starts = lengths - Tq.  (A batch of texts padded at
       their ends has starts=0.)
 
-    A query that sees no key gives zeros and has no gradient.  Keys and values
-    from lengths[b] on are not read, and what a query does not see does not
-    reach its result, whatever it holds.  Lengths are checked on the device: one
+    A query that sees no key gives zeros and has no gradient.  What a query does
+    not see, behind a length or later than itself, does not reach its result,
+    whatever it holds.  Lengths are checked on the device: one
     outside [0, Tk] is taken as the nearer end, and the next synchronisation
     (``sync``, ``cpu``) raises IndexError.
 

@@ -440,16 +440,38 @@ def test_in_place_changes_are_caught(gpu):
         y.backward()
 
 
-def test_a_length_outside_is_reported(gpu):
-    q = dev(np.ones((2, 1, 1, 4), np.float32))
-    k = dev(np.ones((2, 6, 1, 4), np.float32))
-    for bad in ([7, 3], [3, -1]):
+@pytest.mark.parametrize("T", [1, 4000])  # of either kind of kernels
+def test_a_length_outside_is_reported(gpu, T):
+    q = dev(np.ones((2, T, 1, 4), np.float32))
+    k = dev(np.ones((2, 6 * T, 1, 4), np.float32))
+    for bad in ([6 * T + 1, 3], [3, -1]):
         y = nt.attention(q, k, k, lengths=dev(np.array(bad)))
         with pytest.raises(IndexError):
             nt.sync()
         got = host(y)
         assert (got[[b < 0 for b in bad]] == 0).all()
         assert (got[[b >= 0 for b in bad]] == 1).all()
+
+
+def test_more_sequences_than_one_launch_holds(gpu):
+    """Over 2^21 tiles of 16 rows: taken some sequences at a time, each as alone."""
+    B, T, H, D = 42000, 100, 8, 4
+    nt.manual_seed(4)
+    q, k, v = [nt.rand(B, T, H, D, device="cuda") for _ in range(3)]
+    lengths = dev(np.arange(B) % (T + 1))
+    for t in (q, k, v):
+        t.enable_grad()
+    y = nt.attention(q, k, v, causal=True, lengths=lengths, starts=0)
+    grads = y.grad_fn.backward(v)[:3]
+    for beg in (0, 37000, 37440, B - 50):  # about the border and at the ends
+        some = slice(beg, beg + 50)
+        parts = [dev(host(t[some]), True) for t in (q, k, v)]
+        y1 = nt.attention(*parts, causal=True, lengths=lengths[some], starts=0)
+        assert_bitexact(host(y[some]), host(y1))
+        want = reference(*[host(t) for t in parts], host(parts[2]),
+                         visible(50, T, T, True, host(lengths[some]), 0), 0.5, U[np.float32])
+        for name, got in zip(("dq", "dk", "dv"), grads):
+            check(host(got[some]), want[name], name)
 
 
 def test_no_memory_is_kept_by_a_cycle(gpu):
