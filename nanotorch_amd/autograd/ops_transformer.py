@@ -205,7 +205,11 @@ def check_attention(q: Tensor, k: Tensor, v: Tensor, lengths, starts) -> int:
         raise ValueError(f"Heads have 1 to 256 elements, got {q.shape[-1]}.")
     sequences = math.prod(q._shape[:-3])
     for what, t in (("lengths", lengths), ("starts", starts)):
-        if isinstance(t, Tensor) and (not is_int(t._storage._dtype) or t._shape != (sequences,)):
+        if t is None or what == "starts" and not isinstance(t, Tensor):
+            continue
+        if not isinstance(t, Tensor):
+            raise TypeError(f"{what} are a Tensor, got {type(t).__name__}.")
+        if not is_int(t._storage._dtype) or t._shape != (sequences,):
             raise ValueError(f"{what} are int32 or int64, one for each of {sequences} "
                              f"sequences, got {t.dtype.name} {t.shape}.")
     return sequences

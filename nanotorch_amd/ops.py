@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+import operator
 from typing import NamedTuple
 
 from . import _kernels as K
@@ -253,7 +254,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False,
     if causal:
         mode = 1 if starts is None else 2
         if starts is not None and not isinstance(starts, Tensor):
-            start, starts = int(starts), None
+            start, starts = operator.index(starts), None  # TypeError for a float or a list
             if not -2**63 <= start < 2**63:  # the library's 64 bits would wrap round
                 raise ValueError(f"starts must fit 64 bits, got {start}.")
     scale = q._shape[-1] ** -0.5 if scale is None else float(scale)

@@ -62,6 +62,25 @@ def test_attention_refuses_types_and_masks(lib):  # noqa: F811
     assert not [n for n, _ in lib.calls if n == "nt_attention"]
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("bad", [[1, 2], 2, np.array([1, 2])])
+def test_attention_refuses_lengths_that_are_no_tensor(lib, bad, causal):  # noqa: F811
+    q = heads(2, 4, 2, 8)
+    with pytest.raises(TypeError):
+        nt.attention(q, q, q, causal=causal, lengths=bad)
+    assert not [n for n, _ in lib.calls if n == "nt_attention"]
+
+
+@pytest.mark.parametrize("bad", [[1, 2], 2.5, np.array([1, 2]), "3"])
+def test_attention_refuses_starts_that_are_no_whole_number(lib, bad):  # noqa: F811
+    q = heads(2, 4, 2, 8)
+    with pytest.raises(TypeError):
+        nt.attention(q, q, q, causal=True, starts=bad)
+    assert not [n for n, _ in lib.calls if n == "nt_attention"]
+    nt.attention(q, q, q, causal=True, starts=np.int64(3))
+    assert [n for n, _ in lib.calls if n == "nt_attention"]
+
+
 def test_host_tensors_are_refused():
     x = nt.Tensor(np.ones((1, 3, 2, 4), np.float32))
     with pytest.raises(RuntimeError, match="GPU"):
