@@ -341,17 +341,17 @@ __global__ __launch_bounds__(256) void rms_norm_dw_long_kernel(const NormBackArg
   a.part[blockIdx.y * a.D + col] = sum;
 }
 
-// dw = the partial sums added up in order: 32 columns to a workgroup, each half wave
+// dw = the partial sums [parts, D] added up in order, for `cols` columns: 32 columns to a workgroup, each half wave
 // a 32nd of the parts, eight loads of it on their way at a time.
 template <class T>
 __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const T *part, T *dw, int parts,
-                                                           int64_t D) {
+                                                           int64_t D, int64_t cols) {
   __shared__ T sums[32][32];
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
   const int64_t col = int64_t(blockIdx.x) * 32 + lane;
   const int run = (parts + 31) / 32, end = min(parts, (group + 1) * run);
   T sum = 0;
-  if (col < D) {
+  if (col < cols) {
     int i = group * run;
     for (; i + 8 <= end; i += 8) {
       T v[8];
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const T *part, T *dw,
   }
   sums[group][lane] = sum;
   __syncthreads();
-  if (group || col >= D)
+  if (group || col >= cols)
     return;
 #pragma unroll
   for (int k = 1; k < 32; ++k)
@@ -440,7 +440,11 @@ void check_rows(const nt_view *x) {
     fail(NT_ERR_VALUE, "rms_norm: rows of 1 to 2^30 - 1 elements, fewer than 2^30 of them");
 }
 
-template <class T> void run_norm(const NormArgs<T> &a) {
+// Rows of one launch, whose work-items (up to 1024 a row) are counted in 32 bits.
+constexpr int64_t RN_MOST_ROWS = int64_t(1) << 21;
+constexpr int64_t RN_MOST_COLUMNS = int64_t(1) << 26; // of rms_norm_dw_kernel: 32 a column
+
+template <class T> void launch_norm(const NormArgs<T> &a) {
   const bool held = norm_shape<T>(a.D, [&]<int TPR, int PIECES>() {
     constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
     rms_norm_kernel<T, TPR, PIECES>
@@ -451,15 +455,32 @@ template <class T> void run_norm(const NormArgs<T> &a) {
   NT_LAUNCH_CHECK();
 }
 
+template <class T> void run_norm(const NormArgs<T> &a) {
+  for (int64_t at = 0; at < a.rows; at += RN_MOST_ROWS) {
+    NormArgs<T> b = a;
+    b.rows = std::min(RN_MOST_ROWS, a.rows - at);
+    b.x += at * a.x_stride;
+    b.y += at * a.D;
+    if (a.res)
+      b.res += at * a.res_stride;
+    if (a.s)
+      b.s += at * a.D;
+    if (a.rstd)
+      b.rstd += at;
+    launch_norm(b);
+  }
+}
+
 template <class T> void run_norm_bwd(NormBackArgs<T> a, T *dw) {
   // Workgroups that walk rows: two waves to a SIMD, which fill the chip with loads
   // (8192 x 4096, both passes: 180 us, 184 with four and 191 with eight, whose parts
   // of dw are as many more).
   int64_t parts = 0;
   auto add_up = [&] {
-    if (dw) {
-      rms_norm_dw_kernel<T><<<dim3(uint32_t((a.D + 31) / 32)), 1024, 0, stream()>>>(
-          a.part, dw, int(parts), a.D);
+    for (int64_t at = 0; dw && at < a.D; at += RN_MOST_COLUMNS) {
+      const int64_t cols = std::min(RN_MOST_COLUMNS, a.D - at);
+      rms_norm_dw_kernel<T><<<dim3(uint32_t((cols + 31) / 32)), 1024, 0, stream()>>>(
+          a.part + at, dw + at, int(parts), a.D, cols);
       NT_LAUNCH_CHECK();
     }
   };
@@ -476,8 +497,17 @@ template <class T> void run_norm_bwd(NormBackArgs<T> a, T *dw) {
   });
   if (held)
     return;
-  if (a.ds) {
-    rms_norm_bwd_long_kernel<T><<<dim3(uint32_t(a.rows)), RN_MAX_THREADS, 0, stream()>>>(a);
+  for (int64_t at = 0; a.ds && at < a.rows; at += RN_MOST_ROWS) {
+    NormBackArgs<T> b = a;
+    b.s += at * a.s_stride;
+    b.rstd += at;
+    b.ds += at * a.D;
+    if (a.g)
+      b.g += at * a.g_stride;
+    if (a.gs)
+      b.gs += at * a.gs_stride;
+    rms_norm_bwd_long_kernel<T><<<dim3(uint32_t(std::min(RN_MOST_ROWS, a.rows - at))),
+                                  RN_MAX_THREADS, 0, stream()>>>(b);
     NT_LAUNCH_CHECK();
   }
   if (dw) {

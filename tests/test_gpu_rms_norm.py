@@ -219,6 +219,23 @@ def test_no_memory_is_kept_by_a_cycle(gpu):
         gc.enable()
 
 
+def test_more_rows_than_one_launch_counts(gpu):
+    """2^26 rows of one wave each are 2^32 work-items, one more than a launch has.
+    Rows of ones but for the last and one in the middle."""
+    rows, D = 2 ** 26 + 1, 4
+    x = nt.full(rows, D, value=2.0, device="cuda")
+    for at in (2 ** 25 + 3, rows - 1):
+        x[at] = nt.Tensor(np.array([1, 0, 0, 0], np.float32), device="cuda")
+    x.enable_grad()
+    y = nt.rms_norm(x, eps=0.0)
+    for at, want in ((0, [1, 1, 1, 1]), (2 ** 25 + 2, [1, 1, 1, 1]), (2 ** 25 + 3, [2, 0, 0, 0]),
+                     (rows - 2, [1, 1, 1, 1]), (rows - 1, [2, 0, 0, 0])):
+        assert host(y[at]).tolist() == want, at
+    # powers of two throughout: dx = r (g - n mean(g n)) without rounding
+    dx = y.grad_fn.backward(y)[0]
+    assert float(host(dx.max())) == 0.0 and float(host(dx.min())) == 0.0
+
+
 def test_module(gpu):
     norm = nn.RMSNorm(32)
     x = rng(1).standard_normal((4, 3, 32)).astype(np.float32)
