@@ -7,6 +7,8 @@ from typing import Sequence
 import math
 import struct
 
+import numpy as np
+
 from .. import _kernels as K
 from .. import autograd as ag
 from .._data_type import Dtype, is_float
@@ -62,6 +64,19 @@ class GradientDescent(Optimizer):
                         K.sgd_step(p, g, lr32)
                     else:
                         p -= g * self._lr
+
+
+def _memory(p: Tensor) -> np.ndarray:
+    """An array of p's extent, which is never read: for np.shares_memory."""
+    item = 4 if p._storage._dtype is Dtype.Float32 else 8
+
+    class Extent:
+        __array_interface__ = {
+            "version": 3, "typestr": f"<f{item}", "shape": p._shape,
+            "strides": tuple([s * item for s in p._strides]),
+            "data": (p._storage._ptr + p._offset * item, True)}
+
+    return np.asarray(Extent())
 
 
 class AdamW(Optimizer):
@@ -141,6 +156,15 @@ class AdamW(Optimizer):
         self._m, self._v = [t.to(Device.Cuda)._to_contiguous(force=True) for t in (m, v)]
         self._step = int(steps)
 
+    def _check_views(self, views: list[Tensor]) -> None:
+        """Refuses memory that is stepped twice; the library sees the views' copies."""
+        for p in views:
+            if any([n > 1 and s == 0 for n, s in zip(p._shape, p._strides)]) or any([
+                    q is not p and q._storage is p._storage
+                    and np.shares_memory(_memory(p), _memory(q)) for q, *_ in self._slots]):
+                raise RuntimeError("adamw: parameters that share memory with one another "
+                                   "cannot be updated together")
+
     def step(self) -> None:
         tensors: list[int] = []
         written = []
@@ -171,6 +195,8 @@ class AdamW(Optimizer):
             tensors += (to._storage._ptr + to._offset * item, g._storage._ptr + g._offset * item,
                         n, at)
             written.append(ps)
+        if copies:
+            self._check_views([p for _, p in copies])
         m, v = self.moments()
         K.adamw_step(tensors, m, v, self.lr, self._betas, self._eps, self._decay, self._step + 1)
         self._step += 1

@@ -182,3 +182,35 @@ def test_shared_memory_is_refused(gpu):
     with pytest.raises(RuntimeError, match="share memory"):
         nn.AdamW([one], 0.1).step()
     nn.AdamW([], 0.1).step()
+
+
+def test_views_that_share_memory_are_refused(gpu):
+    """Views are stepped as copies: of one memory, one would undo the other's step.
+    Views of one memory that only lie between each other are stepped."""
+    r = rng(6)
+    a, g = [r.standard_normal((8, 6)).astype(np.float32) for _ in range(2)]
+
+    def views(*each):
+        buf = dev(a)
+        out = [nt.Tensor._new_view(buf.storage, *v) for v in each]
+        for p in out:
+            p.enable_grad()
+            p._grad = dev(np.ascontiguousarray(g.reshape(-1)[:p.numel].reshape(p.shape)))
+        return buf, out
+
+    for each in ([((6, 8), (1, 6), 0), ((8, 6), (6, 1), 0)],
+                 [((8, 6), (6, 1), 0), ((6, 8), (1, 6), 0)],
+                 [((8, 3), (6, 2), 0), ((8, 2), (6, 2), 2)],
+                 [((8, 6), (0, 1), 0)]):
+        buf, ps = views(*each)
+        with pytest.raises(RuntimeError, match="share memory"):
+            nn.AdamW(ps, 0.1).step()
+        assert_bitexact(host(buf), a)
+    buf, ps = views(((8, 3), (6, 2), 0), ((8, 3), (6, 2), 1))
+    nn.AdamW(ps, 0.1).step()
+    gs = g.reshape(-1)[:24].reshape(8, 3)
+    for at, p in enumerate(ps):
+        x = np.ascontiguousarray(a[:, at::2])
+        want = step(x, gs, np.zeros_like(x), np.zeros_like(x), 1, 0.1, 1e-8, 0.01,
+                    U[np.float32])[0]
+        check(host(p), want, "p")
