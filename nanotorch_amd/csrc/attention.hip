@@ -1196,7 +1196,8 @@ void by_sequences(const nt_view *(&views)[N], size_t first_array, F &&f) {
   for (size_t i = 0; i < N && !whole; ++i) { // not of one batch: reported by the whole call
     const nt_view *v = views[i];
     if (v && (v->ndim < 1 || v->ndim > NT_MAX_DIMS ||
-              (i < first_array ? v->shape[0] != B : numel(v) % B != 0)))
+              (i < first_array ? v->shape[0] != B
+                               : numel(v) % B != 0 || !is_contiguous(v))))
       whole = true;
   }
   if (whole)

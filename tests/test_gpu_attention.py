@@ -3,7 +3,7 @@ long double where the operator itself works in 64 bits.
 
 Tolerances.  u is the unit roundoff (2^-24, 2^-53).  A dot product of D terms is
 off by at most (D + 8) u of the sum of its terms' magnitudes, the scale's
-roundings among them: with A_ij = scale sum |q| |k|, a score and the maximum that
+roundings among them: with A_ij = |scale| sum |q| |k|, a score and the maximum that
 it is compared with are off by (D + 8) u A each, and exp doubles neither, so a
 probability is off by
     r_i = 2 (D + 8) u (max_j A_ij + 1) + u (n / 4 + 64)
@@ -68,7 +68,7 @@ def reference(q, k, v, g, see, scale, u):
                 x, K, V = [t.astype(wide) for t in
                            (q[b, rows, h], k[b, on, h // G], v[b, on, h // G])]
                 z = np.where(s, x @ K.T * scale, -np.inf)
-                A = np.where(s, np.abs(x) @ np.abs(K).T * scale, 0).max(1, keepdims=True)
+                A = np.where(s, np.abs(x) @ np.abs(K).T * abs(scale), 0).max(1, keepdims=True)
                 top = z.max(1, keepdims=True)
                 p = np.exp(z - np.where(n > 0, top, 0))
                 p /= np.where(n > 0, p.sum(1, keepdims=True), 1)
@@ -356,6 +356,55 @@ def test_views(gpu, dtype):
     y2, _ = run(q, one, one)
     check(y2, reference(q, np.repeat(k[:1], B, 0), np.repeat(k[:1], B, 0), None,
                         visible(B, Tq, Tk, False), D ** -0.5, U[dtype])["y"], "expanded")
+
+
+def test_large_views(gpu):
+    """Queries, keys and values as parts of one projection's output, a gradient with
+    heads before tokens, and one head's keys for all: the half-precision planes'
+    kernels read them in place."""
+    B, T, H, D = 2, 1180, 3, 64
+    r = rng(seed_of("large views"))
+    x = (r.standard_normal((B, T, 3 * H, D)) * 1.5).astype(np.float32)
+    g = (r.standard_normal((B, T, H, D)) * 0.1).astype(np.float32)
+    q, k, v = [np.ascontiguousarray(x[:, :, i * H:(i + 1) * H]) for i in range(3)]
+    X = dev(x)
+    parts = [X[:, :, i * H:(i + 1) * H] for i in range(3)]
+    for p in parts:
+        p.enable_grad()
+    y = nt.attention(*parts, causal=True)
+    G = dev(np.ascontiguousarray(g.transpose(0, 2, 1, 3))).transpose(1, 2)
+    want = reference(q, k, v, g, visible(B, T, T, True), D ** -0.5, U[np.float32])
+    check(host(y), want["y"], "y")
+    for name, t in zip(("dq", "dk", "dv"), y.grad_fn.backward(G)[:3]):
+        check(host(t), want[name], name)
+    one = dev(k[:, :, :1]).expand(B, T, H, D)
+    same = np.repeat(k[:, :, :1], H, 2)
+    got, _ = run(q, one, one)
+    check(got, reference(q, same, same, None, visible(B, T, T, False), D ** -0.5,
+                         U[np.float32])["y"], "expanded")
+
+
+@pytest.mark.parametrize("scale", [-0.7, 1.0, 1e-20])
+def test_large_scales(gpu, scale):
+    r = rng(seed_of("large scale"))
+    q, k, v, g = inputs(r, 2, 1200, 1200, 2, 2, 64, np.float32, sharp=0.5)
+    check_all(q, k, v, g, visible(2, 1200, 1200, True), np.float32, scale=scale, causal=True)
+
+
+@pytest.mark.parametrize("T,H", [(33, 2), (1250, 2)])  # of either kind of kernels
+def test_one_tensor_as_queries_keys_and_values(gpu, T, H):
+    r = rng(seed_of("one tensor", T))
+    x = r.standard_normal((2, T, H, 64)).astype(np.float32)
+    g = (r.standard_normal(x.shape) * 0.1).astype(np.float32)
+    X = dev(x, True)
+    y = nt.attention(X, X, X, causal=True)
+    (y * dev(g)).sum().backward()
+    want = reference(x, x, x, g, visible(2, T, T, True), 64 ** -0.5, U[np.float32])
+    check(host(y), want["y"], "y")
+    value, tol = [sum(want[n][i] for n in ("dq", "dk", "dv")) for i in range(2)]
+    # three roundings of sums of them
+    tol = tol + 3 * U[np.float32] * sum(np.abs(want[n][0]) for n in ("dq", "dk", "dv"))
+    check(host(X.grad), (value, tol), "dx")
 
 
 def test_results_repeat(gpu):
