@@ -36,7 +36,7 @@
 // power that they draw: 8192 tokens, 16 heads over 4 of 128, causal, take 733 us
 // forward, 1237 for dq, 1290 and 783 for dk and dv, 41 and 82 for packing, 80 for
 // adding parts; 3 products for one make that 1.1, 1.0, 1.0 and 1.05 PFLOP/s, as many
-// as a large float16 product of the library's reaches here (1.07), at 1.9 to 2.1 GHz.
+// as a large float16 product of the library's reaches here (1.07), at 1.75 to 2.2 GHz.
 // With heads of 64 the exponentials and conversions weigh as much as the products: 4 x
 // 2048 tokens, 16 heads, 135, 195 and 272 us, 0.8 PFLOP/s.  Row statistics, rescaling and masks are
 // then a lane's own, and sums over own rows' columns need no exchange.
@@ -110,7 +110,6 @@ struct PackTensor {
 struct PackArgs {
   AttnShape s;
   PackTensor t[4];
-  int count;
   uint32_t *words;
   int per;
   // the gradient's: y, the forward statistics, and what becomes of them
@@ -1003,7 +1002,6 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     float *k_scale = reinterpret_cast<float *>(v + form), *v_scale = k_scale + bhs * size_t(tiles);
     PackArgs p{};
     p.s = s;
-    p.count = 2;
     p.words = words;
     p.per = a.gate.per;
     p.t[0] = {a.k, k, nullptr, k_scale, s.Tk, tiles, 1, bhs * uint32_t(tiles), 0};
@@ -1056,7 +1054,6 @@ void run_split_bwd(AttnBwd<float> &a, uint32_t *words) {
     float *v_scale = k_scale + size_t(bhs) * size_t(kt), *q_scale = v_scale + size_t(bhs) * size_t(kt);
     PackArgs p{};
     p.s = s;
-    p.count = 4;
     p.words = words;
     p.per = a.gate.per;
     p.y = a.y;
