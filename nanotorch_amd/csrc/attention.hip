@@ -39,9 +39,9 @@
 // of up to 8192 x 8 x 128: 80 us for 403 MB and 7 for joining the 16 parts, 5.0 TB/s;
 // of rows that four heads share, 12 of each instruction's 16 are empty, which costs
 // nothing here); small texts, latency (4 x 128 tokens, 4 heads of 64: 8 us forward,
-// 12 backward, of which an empty launch is 3); float64, loads that nothing hides (one
+// 12 backward, of which an empty launch is 3); float64, loads that little hides (one
 // or two waves to a SIMD): 1024 x 8 heads of 64 both passes 17 TFLOP/s of the 71 that
-// a large product reaches.
+// a large product reaches, 2000 x 4 heads of 128 19.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -119,73 +119,9 @@ __device__ __forceinline__ T times(const Frag<T, DP> &a, const Frag<T, DP> &b) {
   return sum;
 }
 
-// Own rows of up to 1 KB stay in registers (those over 512 bytes with one wave to a
-// SIMD).  Longer ones, float64 over 128 wide, are read again with every tile of
-// items, 256 bytes at a time.  A workgroup keeps at most so many bytes of its sums'
-// columns; where that is less than a row, several workgroups form the same
-// probabilities, each for columns of its own (in one, wide float64 rows would need a
-// thousand registers a lane).
-template <class T, int DP> constexpr bool IN_REGISTERS = DP * sizeof(T) <= 1024;
-template <class T, int DP> constexpr int COLUMNS_OF(int bytes) {
-  return std::min(DP, bytes / int(sizeof(T)));
-}
-// y and dq; dk and dv.
-template <class T, int DP>
-constexpr int COLUMNS = COLUMNS_OF<T, DP>(IN_REGISTERS<T, DP> ? 1024 : 512);
-template <class T, int DP> constexpr int KEY_COLUMNS = COLUMNS_OF<T, DP>(512);
-
-template <class T, int DP> struct Own {
-  Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> f;
-  const T *row;
-  __device__ __forceinline__ void load(const T *p, int W, int h) {
-    row = p;
-    if constexpr (IN_REGISTERS<T, DP>)
-      f.load(p, 0, W, h);
-  }
-  // With the lane's item row.
-  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, int W, int h) const {
-    if constexpr (IN_REGISTERS<T, DP>) {
-      Frag<T, DP> x;
-      x.load(item, 0, W, h);
-      return nt::dots<T, DP>(x, f);
-    } else {
-      constexpr int PART = 256 / sizeof(T);
-      typename Mma<T>::V4 s{};
-#pragma unroll 1
-      for (int d = 0; d < W; d += PART) {
-        Frag<T, PART> x, o;
-        x.load(item, d, W, h);
-        o.load(row, d, W, h);
-        s += nt::dots<T, PART>(x, o);
-      }
-      return s;
-    }
-  }
-  // As dots, and the lane's item row times `other`, elements of its own.
-  __device__ __forceinline__ typename Mma<T>::V4 dots(const T *item, const T *other, int W, int h,
-                                                      T &product) const {
-    constexpr int PART = IN_REGISTERS<T, DP> ? DP : int(256 / sizeof(T));
-    typename Mma<T>::V4 s{};
-    product = 0;
-#pragma unroll 1
-    for (int d = 0; d < W; d += PART) {
-      Frag<T, PART> x, y, o;
-      x.load(item, d, W, h);
-      y.load(other, d, W, h);
-      if constexpr (IN_REGISTERS<T, DP>) {
-        s = nt::dots<T, PART>(x, f);
-      } else {
-        o.load(row, d, W, h);
-        s += nt::dots<T, PART>(x, o);
-      }
-      product += times<T, PART>(x, y);
-      // (the loads of what follows wait, where the registers are full)
-      if constexpr (IN_REGISTERS<T, DP>)
-        break;
-    }
-    return s;
-  }
-};
+// Columns of dk and dv that a workgroup keeps, at most 512 bytes of each; of wider
+// rows, two workgroups form the same probabilities.
+template <class T, int DP> constexpr int KEY_COLUMNS = std::min(DP, 512 / int(sizeof(T)));
 
 // Items' rows as operand of sums: of the four items row(h, r), pieces at
 // 16 N c + N n of a workgroup's columns.  Where a result's columns are: see
@@ -330,9 +266,8 @@ constexpr int FWD_WAVES =
 // MAY_AHEAD: the next keys may be loaded under a block.
 template <class T, int DP, bool WHOLE, bool MAY_AHEAD>
 __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, uint32_t item,
-                                              uint32_t split, int col0) {
+                                              uint32_t split) {
   using M = Mma<T>;
-  constexpr int SC = COLUMNS<T, DP>;
   constexpr int TILES = FWD_TILES<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   __shared__ T stat[2][AT_WAVES][16];
@@ -356,34 +291,32 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
                 int64_t(qg) * a.q.sInner;
   const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
   const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
-  Own<T, DP> q;
-  q.load(qp, s.W, h);
-  Sums<T, SC> sums;
+  Frag<T, DP> q;
+  q.load(qp, 0, s.W, h);
+  Sums<T, DP> sums;
   sums.clear();
   T m = NEG_INF<T>, l = 0;
   // this workgroup's blocks of keys, dealt to its waves
   const int blocks = (end + 16 * TILES - 1) / (16 * TILES);
   const int per = (blocks + a.splits - 1) / a.splits;
   const int stop = std::min(blocks, int(split + 1) * per);
-  // A block's keys (of rows in registers) and its values.
   struct Keys {
-    Frag<T, IN_REGISTERS<T, DP> ? DP : 4 * RowVec<T>::N> k[TILES];
+    Frag<T, DP> k[TILES];
   };
   constexpr int STEP = 16 * TILES;
   // past the end the last key again, which no row sees there
   auto load_keys = [&](Keys &x, int j0) {
 #pragma unroll
-    for (int i = 0; i < TILES; ++i)
-      if constexpr (IN_REGISTERS<T, DP>) {
-        const int j = j0 + 16 * i + n;
-        const T *p = kp + int64_t(std::min(j, end - 1)) * a.k.sOuter;
-        if constexpr (WHOLE)
-          x.k[i].load_whole(p, h);
-        else
-          x.k[i].load(p, 0, s.W, h);
-      }
+    for (int i = 0; i < TILES; ++i) {
+      const int j = j0 + 16 * i + n;
+      const T *p = kp + int64_t(std::min(j, end - 1)) * a.k.sOuter;
+      if constexpr (WHOLE)
+        x.k[i].load_whole(p, h);
+      else
+        x.k[i].load(p, 0, s.W, h);
+    }
   };
-  Items<T, SC> v[TILES];
+  Items<T, DP> v[TILES];
   auto load_values = [&](int j0) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
@@ -392,9 +325,9 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
         const int j = j0 + 16 * i + M::row(h, r);
         const T *p = vp + int64_t(std::min(j, end - 1)) * a.v.sOuter;
         if constexpr (WHOLE)
-          v[i].load_whole(r, p + col0, n);
+          v[i].load_whole(r, p, n);
         else
-          v[i].load(r, p, col0, s.W, n);
+          v[i].load(r, p, 0, s.W, n);
       }
   };
   auto take = [&](const Keys &x, int j0) {
@@ -403,13 +336,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
     T top = NEG_INF<T>;
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
-      typename M::V4 d;
-      if constexpr (IN_REGISTERS<T, DP>) {
-        d = dots<T, DP>(x.k[i], q.f);
-      } else {
-        const int j = j0 + 16 * i + n;
-        d = q.dots(kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, s.W, h);
-      }
+      const auto d = dots<T, DP>(x.k[i], q);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         vis[i][r] = j0 + 16 * i + M::row(h, r) < limit;
@@ -439,9 +366,9 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i;
-      if (j + 16 > all && !all_finite<T, SC>(v[i]))
-        sums.add_visible(z[i], vis[i], s.D - col0, lane, [&](int item) {
-          return j + item < end ? vp + int64_t(j + item) * a.v.sOuter + col0 : nullptr;
+      if (j + 16 > all && !all_finite<T, DP>(v[i]))
+        sums.add_visible(z[i], vis[i], s.D, lane, [&](int item) {
+          return j + item < end ? vp + int64_t(j + item) * a.v.sOuter : nullptr;
         });
       else
         sums.add(z[i], v[i]);
@@ -496,23 +423,21 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
   const T mine = M::exp2(m - base);
   if (a.splits > 1) {
     const int64_t slot = (int64_t(bh) * tiles + item) * a.splits + split;
-    if (wave == 0 && h == 0 && col0 == 0) {
+    if (wave == 0 && h == 0) {
       a.part_stat[slot * 32 + n] = top;
       a.part_stat[slot * 32 + 16 + n] = total;
     }
-    join_waves<T, SC>(sums, mine, lds, [&](int r, int d, T v) {
-      d += col0;
+    join_waves<T, DP>(sums, mine, lds, [&](int r, int d, T v) {
       if (d < s.D && tile * 16 + r < s.rows)
         a.part_acc[(slot * 16 + r) * s.D + d] = v;
     });
     return;
   }
-  if (a.lse && wave == 0 && h == 0 && live && col0 == 0)
+  if (a.lse && wave == 0 && h == 0 && live)
     a.lse[int64_t(bh) * s.rows + row] = top == NEG_INF<T> ? T(0) : top + M::log2(total);
   const T factor = limit > 0 ? mine / total : T(0);
-  join_waves<T, SC>(sums, factor, lds, [&](int r, int d, T v) {
+  join_waves<T, DP>(sums, factor, lds, [&](int r, int d, T v) {
     const int w = tile * 16 + r;
-    d += col0;
     if (d >= s.D || w >= s.rows)
       return;
     const uint32_t i = s.by_group.div(uint32_t(w));
@@ -524,15 +449,11 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
 template <class T, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * AT_WAVES, (FWD_WAVES<T, DP>)) void attn_fwd_kernel(
     const AttnFwd<T> a) {
-  constexpr uint32_t GROUPS = DP / COLUMNS<T, DP>;
   const uint32_t splits = uint32_t(a.splits);
   uint32_t bh, item;
   head_item(blockIdx.x, uint32_t(a.s.B) * uint32_t(a.s.Hk),
-            uint32_t(a.s.rows + 15) / 16 * splits * GROUPS, bh, item);
-  const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
-  item /= GROUPS;
-  if (col0 < a.s.D)
-    attn_fwd_tile<T, DP, WHOLE, true>(a, bh, item / splits, item % splits, col0);
+            uint32_t(a.s.rows + 15) / 16 * splits, bh, item);
+  attn_fwd_tile<T, DP, WHOLE, true>(a, bh, item / splits, item % splits);
 }
 
 // What the kernels on half-precision planes left: the tiles of each (sequence,
@@ -546,7 +467,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_left_kernel(
   const uint32_t tiles = uint32_t(a.s.rows + 15) / 16;
   for (uint32_t t = blockIdx.x % groups; t < tiles; t += groups) {
     __syncthreads();
-    attn_fwd_tile<float, DP, false, false>(a, bh, t, 0, 0);
+    attn_fwd_tile<float, DP, false, false>(a, bh, t, 0);
   }
 }
 
@@ -617,10 +538,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnFwd<T> a) {
 // row read with each of g.
 
 template <class T, int DP>
-__device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
-                                             int col0) {
+__device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item) {
   using M = Mma<T>;
-  constexpr int SC = COLUMNS<T, DP>;
   __shared__ T lds[JOIN_ELEMENTS<T>];
   const AttnShape &s = a.s;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
@@ -639,13 +558,13 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
   const int all = seen(s, keys, first, int(s.by_group.div(uint32_t(tile * 16))));
   const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
   const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
-  Own<T, DP> q, g;
+  const T *gp = a.g.p + b * a.g.sB + hk * a.g.sHead + int64_t(qi) * a.g.sOuter +
+                int64_t(qg) * a.g.sInner;
+  Frag<T, DP> q, g;
   q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
              int64_t(qg) * a.q.sInner,
-         s.W, h);
-  g.load(a.g.p + b * a.g.sB + hk * a.g.sHead + int64_t(qi) * a.g.sOuter +
-             int64_t(qg) * a.g.sInner,
-         s.W, h);
+         0, s.W, h);
+  g.load(gp, 0, s.W, h);
   const T lse = a.lse[int64_t(bh) * s.rows + at];
   const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead + int64_t(qi) * a.y.sOuter +
                 int64_t(qg) * a.y.sInner;
@@ -653,24 +572,27 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
 #pragma unroll 1
   for (int d = 0; d < s.W; d += 4 * RowVec<T>::N * 4) {
     Frag<T, 16 * RowVec<T>::N> x, y;
-    x.load(g.row, d, s.W, h);
+    x.load(gp, d, s.W, h);
     y.load(yp, d, s.W, h);
     delta += times<T, 16 * RowVec<T>::N>(x, y);
   }
   delta += __shfl_xor(delta, 16);
   delta += __shfl_xor(delta, 32);
-  Sums<T, SC> sums;
+  Sums<T, DP> sums;
   sums.clear();
   for (int j0 = wave * 16; j0 < end; j0 += 16 * AT_WAVES) {
-    Items<T, SC> x;
+    Items<T, DP> x;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = j0 + M::row(h, r);
-      x.load(r, kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, col0, s.W, n);
+      x.load(r, kp + int64_t(std::min(j, end - 1)) * a.k.sOuter, 0, s.W, n);
     }
     const int64_t j = std::min(j0 + n, end - 1);
-    const auto z = q.dots(kp + j * a.k.sOuter, s.W, h);
-    const auto dp = g.dots(vp + j * a.v.sOuter, s.W, h);
+    Frag<T, DP> f;
+    f.load(kp + j * a.k.sOuter, 0, s.W, h);
+    const auto z = dots<T, DP>(f, q);
+    f.load(vp + j * a.v.sOuter, 0, s.W, h);
+    const auto dp = dots<T, DP>(f, g);
     T ds[4];
     bool vis[4];
 #pragma unroll
@@ -678,16 +600,15 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
       vis[r] = j0 + M::row(h, r) < limit;
       ds[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse) * (dp[r] - delta) : T(0);
     }
-    if (j0 + 16 > all && !all_finite<T, SC>(x))
-      sums.add_visible(ds, vis, s.D - col0, lane, [&](int item) {
-        return j0 + item < end ? kp + int64_t(j0 + item) * a.k.sOuter + col0 : nullptr;
+    if (j0 + 16 > all && !all_finite<T, DP>(x))
+      sums.add_visible(ds, vis, s.D, lane, [&](int item) {
+        return j0 + item < end ? kp + int64_t(j0 + item) * a.k.sOuter : nullptr;
       });
     else
       sums.add(ds, x);
   }
-  join_waves<T, SC>(sums, a.scale, lds, [&](int r, int d, T v) {
+  join_waves<T, DP>(sums, a.scale, lds, [&](int r, int d, T v) {
     const int w = tile * 16 + r;
-    d += col0;
     if (d >= s.D || w >= s.rows)
       return;
     const uint32_t i = s.by_group.div(uint32_t(w));
@@ -715,10 +636,10 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
     const uint32_t i = s.by_group.div(uint32_t(row));
     return p + int64_t(i) * x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * x.sInner;
   };
-  Own<T, DP> k, v;
+  Frag<T, DP> k, v;
   const int64_t own_key = std::min(key, s.Tk - 1);
-  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + own_key * a.k.sOuter, s.W, h);
-  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + own_key * a.v.sOuter, s.W, h);
+  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + own_key * a.k.sOuter, 0, s.W, h);
+  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + own_key * a.v.sOuter, 0, s.W, h);
   Sums<T, SC> dk, dv;
   dk.clear();
   dv.clear();
@@ -738,12 +659,8 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
         x.load(r, at(base, of, row < s.rows ? row : 0), col0, s.W, n);
       }
     };
-    // float64 rows of 1 KB leave no registers for them yet
-    constexpr bool LATE = sizeof(T) == 8 && DP * sizeof(T) == 1024;
-    if constexpr (!LATE) {
-      load(xq, qp, a.q);
-      load(xg, gp, a.g);
-    }
+    load(xq, qp, a.q);
+    load(xg, gp, a.g);
     T lse[4], delta[4];
     int limit[4];
 #pragma unroll
@@ -755,12 +672,15 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
     }
     const bool live = r0 + n < s.rows;
     const int own = live ? r0 + n : 0;
-    const auto z = k.dots(at(qp, a.q, own), s.W, h);
-    if constexpr (DP * sizeof(T) == 1024)
+    Frag<T, DP> x, y;
+    x.load(at(qp, a.q, own), 0, s.W, h);
+    const auto z = dots<T, DP>(x, k);
+    if constexpr (DP * sizeof(T) == 1024) // (the registers are full)
       __builtin_amdgcn_sched_barrier(0);
-    T product;
-    const auto dp =
-        v.dots(at(gp, a.g, own), at(yp, a.y, own), s.W, h, product);
+    x.load(at(gp, a.g, own), 0, s.W, h);
+    y.load(at(yp, a.y, own), 0, s.W, h);
+    const auto dp = dots<T, DP>(x, v);
+    T product = times<T, DP>(x, y);
     product += __shfl_xor(product, 16);
     product += __shfl_xor(product, 32);
 #pragma unroll
@@ -780,18 +700,10 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
         return r0 + item < s.rows ? at(base, x, r0 + item) + col0 : nullptr;
       };
     };
-    if constexpr (LATE) {
-      __builtin_amdgcn_sched_barrier(0);
-      load(xg, gp, a.g);
-    }
     if (__any(some) && !all_finite<T, SC>(xg))
       dv.add_visible(p, vis, s.D - col0, lane, row_of(gp, a.g));
     else
       dv.add(p, xg);
-    if constexpr (LATE) {
-      __builtin_amdgcn_sched_barrier(0);
-      load(xq, qp, a.q);
-    }
     if (__any(some) && !all_finite<T, SC>(xq))
       dk.add_visible(ds, vis, s.D - col0, lane, row_of(qp, a.q));
     else
@@ -814,7 +726,7 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
 template <class T, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_kernel(const AttnBwd<T> a,
                                                                  uint32_t key_blocks) {
-  constexpr uint32_t GROUPS = DP / COLUMNS<T, DP>, KEY_GROUPS = DP / KEY_COLUMNS<T, DP>;
+  constexpr uint32_t KEY_GROUPS = DP / KEY_COLUMNS<T, DP>;
   const AttnShape &s = a.s;
   const uint32_t heads = uint32_t(s.B) * uint32_t(s.Hk);
   uint32_t bh, item;
@@ -824,10 +736,8 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_kernel(const AttnBwd<T
     if (col0 < s.D)
       attn_dkv_tile<T, DP>(a, bh, item / KEY_GROUPS, col0);
   } else {
-    head_item(blockIdx.x - key_blocks, heads, uint32_t(s.rows + 15) / 16 * GROUPS, bh, item);
-    const int col0 = int(item % GROUPS) * COLUMNS<T, DP>;
-    if (col0 < s.D)
-      attn_dq_tile<T, DP>(a, bh, item / GROUPS, col0);
+    head_item(blockIdx.x - key_blocks, heads, uint32_t(s.rows + 15) / 16, bh, item);
+    attn_dq_tile<T, DP>(a, bh, item);
   }
 }
 
@@ -842,7 +752,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const Attn
   if (DQ && a.dq)
     for (uint32_t t = blockIdx.x % groups; t < rows; t += groups) {
       __syncthreads();
-      attn_dq_tile<float, DP>(a, bh, t, 0);
+      attn_dq_tile<float, DP>(a, bh, t);
     }
   if (DKV && (a.dk || a.dv))
     for (uint32_t t = blockIdx.x % groups; t < keys; t += groups) {
@@ -851,6 +761,357 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const Attn
         attn_dkv_tile<float, DP>(a, bh, t, col0);
       }
     }
+}
+
+// ------------------------------------------------------- wide float64 rows
+
+// float64 rows over 64 wide: a workgroup's four waves take the same items, each a
+// quarter of the elements of every row, so that a quarter of the own rows, of the items
+// and of the sums' columns lies in a wave's registers and no score is formed twice.  A
+// score is the sum of the waves' four parts, which they exchange through two buffers
+// of LDS, one barrier to a tile.  (Workgroups that formed all scores again for each 64
+// columns, one wave to a SIMD, took 1100 us for 740 of 2000 x 4 heads of 128 and 2040
+// for 930 of 900 x 6 over 3 of 256, both passes.)
+template <class T, int DP> constexpr bool SHARED_ITEMS = sizeof(T) == 8 && DP >= 128;
+
+// The waves' parts of a tile's result, summed in order; `turn` alternates.
+template <class T> struct Exchange {
+  using V4 = typename Mma<T>::V4;
+  T part[2][AT_WAVES][4][64];
+  __device__ __forceinline__ void put(int turn, int wave, int lane, V4 v) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      part[turn][wave][r][lane] = v[r];
+  }
+  __device__ __forceinline__ V4 get(int turn, int lane) const {
+    V4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v[r] = part[turn][0][r][lane];
+#pragma unroll
+      for (int w = 1; w < AT_WAVES; ++w)
+        v[r] += part[turn][w][r][lane];
+    }
+    return v;
+  }
+};
+
+// Calls out(column, value) for the own row n's sums, times a factor.
+template <class T, int DP, class F>
+__device__ __forceinline__ void each_sum(const Sums<T, DP> &s, T factor, int h, F out) {
+#pragma unroll
+  for (int c = 0; c < Sums<T, DP>::C; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < Sums<T, DP>::N; ++e)
+        out(Sums<T, DP>::column(c, e, h, r), s.acc[c][e][r] * factor);
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES, DP <= 128 ? 2 : 1) void attn_wide_fwd_kernel(const AttnFwd<T> a) {
+  using M = Mma<T>;
+  constexpr int PART = DP / AT_WAVES;
+  __shared__ Exchange<T> scores;
+  const AttnShape &s = a.s;
+  const uint32_t splits = uint32_t(a.splits), tiles = uint32_t(s.rows + 15) / 16;
+  uint32_t bh, item;
+  head_item(blockIdx.x, uint32_t(s.B) * uint32_t(s.Hk), tiles * splits, bh, item);
+  const uint32_t split = item % splits;
+  item /= splits;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const int col0 = wave * PART, tile = int(tiles - 1 - item);
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, threadIdx.x == 0, keys, first);
+  const int row = tile * 16 + n;
+  const bool live = row < s.rows;
+  const uint32_t at = uint32_t(std::min(row, s.rows - 1));
+  const uint32_t qi = s.by_group.div(at), qg = at - qi * uint32_t(s.G);
+  const int limit = live ? seen(s, keys, first, int(qi)) : 0;
+  const int last = std::min(tile * 16 + 15, s.rows - 1);
+  const int end = seen(s, keys, first, int(s.by_group.div(uint32_t(last)))); // of any row
+  const int all = seen(s, keys, first, int(s.by_group.div(uint32_t(tile * 16)))); // of every row
+  const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
+  const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
+  Frag<T, PART> q;
+  q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
+             int64_t(qg) * a.q.sInner,
+         col0, s.W, h);
+  Sums<T, PART> sums;
+  sums.clear();
+  T m = NEG_INF<T>, l = 0;
+  const int blocks = (end + 15) / 16, per = (blocks + int(splits) - 1) / int(splits);
+  const int stop = std::min(blocks, int(split + 1) * per);
+  Frag<T, PART> k;
+  auto load_keys = [&](int blk) { // past the end the last key again, which no row sees
+    k.load(kp + int64_t(std::min(blk * 16 + n, end - 1)) * a.k.sOuter, col0, s.W, h);
+  };
+  int turn = 0, blk = int(split) * per;
+  if (blk < stop)
+    load_keys(blk);
+  for (; blk < stop; ++blk, turn ^= 1) {
+    const int j0 = blk * 16;
+    Items<T, PART> v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      v.load(r, vp + int64_t(std::min(j0 + M::row(h, r), end - 1)) * a.v.sOuter, col0, s.W, n);
+    scores.put(turn, wave, lane, dots<T, PART>(k, q));
+    load_keys(std::min(blk + 1, stop - 1)); // on their way over the barrier
+    __syncthreads();
+    const auto d = scores.get(turn, lane);
+    T z[4], top = NEG_INF<T>;
+    bool vis[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vis[r] = j0 + M::row(h, r) < limit;
+      z[r] = vis[r] ? d[r] * a.scale2 : NEG_INF<T>;
+      top = fmax(top, z[r]);
+    }
+    top = fmax(top, __shfl_xor(top, 16));
+    top = fmax(top, __shfl_xor(top, 32));
+    const T next = fmax(m, top);
+    const T base = next == NEG_INF<T> ? T(0) : next;
+    const T shrink = M::exp2(m - base);
+    m = next;
+    l *= shrink;
+    sums.scale(shrink);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      z[r] = vis[r] ? M::exp2(z[r] - base) : T(0);
+      l += z[r];
+    }
+    if (j0 + 16 > all && !all_finite<T, PART>(v))
+      sums.add_visible(z, vis, s.D - col0, lane, [&](int i) {
+        return j0 + i < end ? vp + int64_t(j0 + i) * a.v.sOuter + col0 : nullptr;
+      });
+    else
+      sums.add(z, v);
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (splits > 1) {
+    const int64_t slot = (int64_t(bh) * tiles + item) * splits + split;
+    if (wave == 0 && h == 0) {
+      a.part_stat[slot * 32 + n] = m;
+      a.part_stat[slot * 32 + 16 + n] = l;
+    }
+    each_sum(sums, T(1), h, [&](int d, T x) {
+      if (col0 + d < s.D && live)
+        a.part_acc[(slot * 16 + n) * s.D + col0 + d] = x;
+    });
+    return;
+  }
+  if (!live)
+    return;
+  if (a.lse && wave == 0 && h == 0)
+    a.lse[int64_t(bh) * s.rows + row] = m == NEG_INF<T> ? T(0) : m + M::log2(l);
+  T *y = a.y + ((int64_t(b) * s.Tq + qi) * s.Hk * s.G + int64_t(hk) * s.G + qg) * s.D + col0;
+  each_sum(sums, limit > 0 ? T(1) / l : T(0), h, [&](int d, T x) {
+    if (col0 + d < s.D)
+      y[d] = x;
+  });
+}
+
+template <class T, int DP>
+__device__ __forceinline__ void attn_wide_dq_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
+                                                  Exchange<T> &scores, Exchange<T> &others) {
+  using M = Mma<T>;
+  constexpr int PART = DP / AT_WAVES;
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const int col0 = wave * PART, tile = int(uint32_t(s.rows + 15) / 16 - 1 - item);
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, false, keys, first);
+  const int row = tile * 16 + n;
+  const bool live = row < s.rows;
+  const uint32_t at = uint32_t(std::min(row, s.rows - 1));
+  const uint32_t qi = s.by_group.div(at), qg = at - qi * uint32_t(s.G);
+  const int limit = live ? seen(s, keys, first, int(qi)) : 0;
+  const int last = std::min(tile * 16 + 15, s.rows - 1);
+  const int end = seen(s, keys, first, int(s.by_group.div(uint32_t(last))));
+  const int all = seen(s, keys, first, int(s.by_group.div(uint32_t(tile * 16))));
+  const T *kp = a.k.p + b * a.k.sB + hk * a.k.sHead;
+  const T *vp = a.v.p + b * a.v.sB + hk * a.v.sHead;
+  const T *gp = a.g.p + b * a.g.sB + hk * a.g.sHead + int64_t(qi) * a.g.sOuter +
+                int64_t(qg) * a.g.sInner;
+  const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead + int64_t(qi) * a.y.sOuter +
+                int64_t(qg) * a.y.sInner;
+  Frag<T, PART> q, g;
+  q.load(a.q.p + b * a.q.sB + hk * a.q.sHead + int64_t(qi) * a.q.sOuter +
+             int64_t(qg) * a.q.sInner,
+         col0, s.W, h);
+  g.load(gp, col0, s.W, h);
+  const T lse = a.lse[int64_t(bh) * s.rows + at];
+  T delta = 0;
+#pragma unroll 1
+  for (int d = 0; d < s.W; d += 16 * RowVec<T>::N) {
+    Frag<T, 16 * RowVec<T>::N> x, y;
+    x.load(gp, d, s.W, h);
+    y.load(yp, d, s.W, h);
+    delta += times<T, 16 * RowVec<T>::N>(x, y);
+  }
+  delta += __shfl_xor(delta, 16);
+  delta += __shfl_xor(delta, 32);
+  Sums<T, PART> sums;
+  sums.clear();
+  int turn = 0;
+  for (int j0 = 0; j0 < end; j0 += 16, turn ^= 1) {
+    Frag<T, PART> k, v;
+    Items<T, PART> x;
+    const int64_t j = std::min(j0 + n, end - 1);
+    k.load(kp + j * a.k.sOuter, col0, s.W, h);
+    v.load(vp + j * a.v.sOuter, col0, s.W, h);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      x.load(r, kp + int64_t(std::min(j0 + M::row(h, r), end - 1)) * a.k.sOuter, col0, s.W, n);
+    scores.put(turn, wave, lane, dots<T, PART>(k, q));
+    others.put(turn, wave, lane, dots<T, PART>(v, g));
+    __syncthreads();
+    const auto z = scores.get(turn, lane), dp = others.get(turn, lane);
+    T ds[4];
+    bool vis[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vis[r] = j0 + M::row(h, r) < limit;
+      ds[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse) * (dp[r] - delta) : T(0);
+    }
+    if (j0 + 16 > all && !all_finite<T, PART>(x))
+      sums.add_visible(ds, vis, s.D - col0, lane, [&](int i) {
+        return j0 + i < end ? kp + int64_t(j0 + i) * a.k.sOuter + col0 : nullptr;
+      });
+    else
+      sums.add(ds, x);
+  }
+  if (!live)
+    return;
+  T *out = a.dq + ((int64_t(b) * s.Tq + qi) * s.Hk * s.G + int64_t(hk) * s.G + qg) * s.D + col0;
+  each_sum(sums, a.scale, h, [&](int d, T x) {
+    if (col0 + d < s.D)
+      out[d] = x;
+  });
+}
+
+template <class T, int DP>
+__device__ __forceinline__ void attn_wide_dkv_tile(const AttnBwd<T> &a, uint32_t bh, uint32_t item,
+                                                   Exchange<T> &scores, Exchange<T> &others,
+                                                   T (&deltas)[2][AT_WAVES][16]) {
+  using M = Mma<T>;
+  constexpr int PART = DP / AT_WAVES;
+  const AttnShape &s = a.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const int col0 = wave * PART, key0 = int(item) * 16, key = key0 + n;
+  const int b = int(bh) / s.Hk, hk = int(bh) % s.Hk;
+  int keys, first;
+  sequence(s, b, false, keys, first);
+  const T *qp = a.q.p + b * a.q.sB + hk * a.q.sHead;
+  const T *gp = a.g.p + b * a.g.sB + hk * a.g.sHead;
+  const T *yp = a.y.p + b * a.y.sB + hk * a.y.sHead;
+  auto at = [&](const T *p, const Rows<const T> &x, int row) {
+    const uint32_t i = s.by_group.div(uint32_t(row));
+    return p + int64_t(i) * x.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * x.sInner;
+  };
+  Frag<T, PART> k, v;
+  const int64_t own_key = std::min(key, s.Tk - 1);
+  k.load(a.k.p + b * a.k.sB + hk * a.k.sHead + own_key * a.k.sOuter, col0, s.W, h);
+  v.load(a.v.p + b * a.v.sB + hk * a.v.sHead + own_key * a.v.sOuter, col0, s.W, h);
+  Sums<T, PART> dk, dv;
+  dk.clear();
+  dv.clear();
+  // rows before the first query that sees any of these keys take no part
+  int row0 = 0;
+  if (key0 >= keys)
+    row0 = s.rows;
+  else if (s.causal && key0 > first)
+    row0 = int(std::min<int64_t>(int64_t(key0 - first) * s.G, s.rows)) & ~15;
+  const int clear = key0 + 16; // a row that sees so many sees all of this tile
+  int turn = 0;
+  for (int r0 = row0; r0 < s.rows; r0 += 16, turn ^= 1) {
+    const int own = r0 + n < s.rows ? r0 + n : 0;
+    Frag<T, PART> x, g, y;
+    x.load(at(qp, a.q, own), col0, s.W, h);
+    g.load(at(gp, a.g, own), col0, s.W, h);
+    y.load(at(yp, a.y, own), col0, s.W, h);
+    Items<T, PART> xq, xg;
+    T lse[4];
+    int limit[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = r0 + M::row(h, r);
+      const bool on = row < s.rows;
+      xg.load(r, at(gp, a.g, on ? row : 0), col0, s.W, n);
+      xq.load(r, at(qp, a.q, on ? row : 0), col0, s.W, n);
+      lse[r] = a.lse[int64_t(bh) * s.rows + (on ? row : 0)];
+      limit[r] = on ? seen(s, keys, first, int(s.by_group.div(uint32_t(row)))) : 0;
+    }
+    scores.put(turn, wave, lane, dots<T, PART>(x, k));
+    others.put(turn, wave, lane, dots<T, PART>(g, v));
+    T product = times<T, PART>(g, y);
+    product += __shfl_xor(product, 16);
+    product += __shfl_xor(product, 32);
+    if (h == 0)
+      deltas[turn][wave][n] = product;
+    __syncthreads();
+    const auto z = scores.get(turn, lane), dp = others.get(turn, lane);
+    T p[4], ds[4];
+    bool vis[4], some = false;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      T delta = 0;
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w)
+        delta += deltas[turn][w][M::row(h, r)];
+      vis[r] = key < limit[r];
+      some = some || limit[r] < clear;
+      p[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse[r]) : T(0);
+      ds[r] = vis[r] ? p[r] * (dp[r] - delta) : T(0);
+    }
+    auto row_of = [&](const T *base, const Rows<const T> &of) {
+      return [&, base](int i) {
+        return r0 + i < s.rows ? at(base, of, r0 + i) + col0 : nullptr;
+      };
+    };
+    if (__any(some) && !all_finite<T, PART>(xg))
+      dv.add_visible(p, vis, s.D - col0, lane, row_of(gp, a.g));
+    else
+      dv.add(p, xg);
+    if (__any(some) && !all_finite<T, PART>(xq))
+      dk.add_visible(ds, vis, s.D - col0, lane, row_of(qp, a.q));
+    else
+      dk.add(ds, xq);
+  }
+  if (key >= s.Tk)
+    return;
+  const int64_t out = ((int64_t(b) * s.Tk + key) * s.Hk + hk) * s.D + col0;
+  if (a.dv)
+    each_sum(dv, T(1), h, [&](int d, T x) {
+      if (col0 + d < s.D)
+        a.dv[out + d] = x;
+    });
+  if (a.dk)
+    each_sum(dk, a.scale, h, [&](int d, T x) {
+      if (col0 + d < s.D)
+        a.dk[out + d] = x;
+    });
+}
+
+// As attn_bwd_kernel.
+template <class T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES, DP <= 128 ? 2 : 1) void attn_wide_bwd_kernel(
+    const AttnBwd<T> a, uint32_t key_blocks) {
+  __shared__ Exchange<T> scores, others;
+  __shared__ T deltas[2][AT_WAVES][16];
+  const AttnShape &s = a.s;
+  const uint32_t heads = uint32_t(s.B) * uint32_t(s.Hk);
+  uint32_t bh, item;
+  if (blockIdx.x < key_blocks) {
+    head_item(blockIdx.x, heads, uint32_t(s.Tk + 15) / 16, bh, item);
+    attn_wide_dkv_tile<T, DP>(a, bh, item, scores, others, deltas);
+  } else {
+    head_item(blockIdx.x - key_blocks, heads, uint32_t(s.rows + 15) / 16, bh, item);
+    attn_wide_dq_tile<T, DP>(a, bh, item, scores, others);
+  }
 }
 
 // x [B, tokens, heads, D] -> contiguous rows of W elements, zeros past D.
@@ -1075,8 +1336,10 @@ template <class T> void run_attention(AttnFwd<T> &a) {
   a.part_acc = acc.template get<T>();
   a.part_stat = stat.template get<T>();
   dispatch_width<T>(s.D, [&]<int DP>() {
-    const dim3 grid(uint32_t(tiles * a.splits * (DP / COLUMNS<T, DP>)));
-    if (a.vec && s.D == DP)
+    const dim3 grid(uint32_t(tiles * a.splits));
+    if constexpr (SHARED_ITEMS<T, DP>)
+      attn_wide_fwd_kernel<T, DP><<<grid, 64 * AT_WAVES, 0, stream()>>>(a);
+    else if (a.vec && s.D == DP)
       attn_fwd_kernel<T, DP, true><<<grid, 64 * AT_WAVES, 0, stream()>>>(a);
     else
       attn_fwd_kernel<T, DP, false><<<grid, 64 * AT_WAVES, 0, stream()>>>(a);
@@ -1109,12 +1372,16 @@ template <class T> void run_attention_bwd(AttnBwd<T> &a) {
     }
   dispatch_width<T>(s.D, [&]<int DP>() {
     const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
-    const uint32_t keys =
-        a.dk || a.dv ? bhs * uint32_t((s.Tk + 15) / 16) * (DP / KEY_COLUMNS<T, DP>) : 0;
-    const uint32_t rows = a.dq ? bhs * uint32_t((s.rows + 15) / 16) * (DP / COLUMNS<T, DP>) : 0;
+    constexpr bool SHARED = SHARED_ITEMS<T, DP>;
+    constexpr uint32_t KEY_GROUPS = SHARED ? 1 : DP / KEY_COLUMNS<T, DP>;
+    const uint32_t keys = a.dk || a.dv ? bhs * uint32_t((s.Tk + 15) / 16) * KEY_GROUPS : 0;
+    const uint32_t rows = a.dq ? bhs * uint32_t((s.rows + 15) / 16) : 0;
     if (keys + rows == 0)
       return;
-    attn_bwd_kernel<T, DP><<<dim3(keys + rows), 64 * AT_WAVES, 0, stream()>>>(a, keys);
+    if constexpr (SHARED)
+      attn_wide_bwd_kernel<T, DP><<<dim3(keys + rows), 64 * AT_WAVES, 0, stream()>>>(a, keys);
+    else
+      attn_bwd_kernel<T, DP><<<dim3(keys + rows), 64 * AT_WAVES, 0, stream()>>>(a, keys);
     NT_LAUNCH_CHECK();
   });
 }
