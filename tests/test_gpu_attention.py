@@ -267,7 +267,8 @@ def test_lengths_and_starts(gpu, causal, starts, wide, dtype):
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("T,D,dtype", [(37, 24, np.float32), (37, 24, np.float64),
                                        (150, 64, np.float32), (150, 64, np.float64),
-                                       (1860, 64, np.float32)])
+                                       (1860, 64, np.float32), (90, 90, np.float64),
+                                       (70, 201, np.float64)])
 def test_what_is_not_seen_does_not_matter(gpu, dtype, bad, T, D):
     """A key, value, query or gradient that is no number reaches the rows that
     see it and no other."""
@@ -299,6 +300,23 @@ def test_long_rows_of_few_queries(gpu, causal):
     lengths = np.array([9001, 5003])
     see = visible(B, Tq, Tk, causal, lengths)
     check_all(q, k, v, None, see, np.float32, causal=causal, lengths=dev(lengths))
+
+
+@pytest.mark.parametrize("Tq,Tk,H,Hk,D", [(2, 2500, 6, 2, 100), (1, 3001, 4, 4, 256),
+                                          (5, 1111, 33, 1, 65), (300, 290, 4, 2, 128),
+                                          (150, 170, 3, 3, 250)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_wide_rows_in_64_bits(gpu, Tq, Tk, H, Hk, D, causal):
+    """Split keys, lengths that leave tiles of no row and of one, values that are
+    no numbers behind them."""
+    r = rng(seed_of("wide", Tq, Tk, D, causal))
+    q, k, v, g = inputs(r, 3, Tq, Tk, H, Hk, D, np.float64, sharp=2.0)
+    lengths = np.array([Tk, 0, Tk // 2 + 1])
+    for b, n in enumerate(lengths):
+        k[b, n:] = np.nan
+        v[b, n:] = np.inf
+    see = visible(3, Tq, Tk, causal, lengths)
+    check_all(q, k, v, g, see, np.float64, causal=causal, lengths=dev(lengths))
 
 
 def test_a_cache_longer_than_32_bits(gpu):
