@@ -224,7 +224,7 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, *, residual: Tensor | None
     return NormRowOp.apply(out, 0), NormRowOp.apply(out, 1)
 
 
-def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False,
+def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool | None = None,
               lengths: Tensor | None = None, starts: Tensor | int | None = None,
               scale: float | None = None) -> Tensor:
     """softmax(scale q . k) v: queries [B, Tq, H, D] over keys and values
@@ -239,6 +239,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False,
       their sequences: starts = lengths - Tq.  (A batch of texts padded at
       their ends has starts=0.)
 
+    With ``causal=False`` starts have no effect.  Starts without a word on causal,
+    which is then False, are refused: their caller meant it to be True.
+
     A query that sees no key gives zeros and has no gradient.  What a query does
     not see, behind a length or later than itself, does not reach its result,
     whatever it holds.  Lengths are checked on the device: one
@@ -249,14 +252,16 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = False,
     Every result comes out the same every time."""
     check_attention(q, k, v, lengths, starts)
     start, mode = 0, 0
-    if starts is not None and not causal:
-        raise ValueError("attention() takes starts only with causal=True.")
+    if starts is not None and causal is None:
+        raise ValueError("attention() takes starts only where causal is given.")
     if causal:
         mode = 1 if starts is None else 2
-        if starts is not None and not isinstance(starts, Tensor):
-            start, starts = operator.index(starts), None  # TypeError for a float or a list
-            if not -2**63 <= start < 2**63:  # the library's 64 bits would wrap round
-                raise ValueError(f"starts must fit 64 bits, got {start}.")
+    if starts is not None and not isinstance(starts, Tensor):
+        start, starts = operator.index(starts), None  # TypeError for a float or a list
+        if not -2**63 <= start < 2**63:  # the library's 64 bits would wrap round
+            raise ValueError(f"starts must fit 64 bits, got {start}.")
+    if not causal:
+        start, starts = 0, None
     scale = q._shape[-1] ** -0.5 if scale is None else float(scale)
     return autograd.AttentionOp.apply(q, k, v, mode, lengths, starts, start, scale)
 

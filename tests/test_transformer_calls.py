@@ -81,6 +81,19 @@ def test_attention_refuses_starts_that_are_no_whole_number(lib, bad):  # noqa: F
     assert [n for n, _ in lib.calls if n == "nt_attention"]
 
 
+def test_starts_without_a_causal_mask_have_no_effect(lib):  # noqa: F811
+    """A program that switches the mask off keeps its other arguments."""
+    q = heads(2, 4, 2, 8)
+    for starts in (0, 3, tensor(2, dtype=Dtype.Int32)):
+        nt.attention(q, q, q, causal=False, starts=starts)
+        a = lib.args("nt_attention")
+        assert a[4] is None and a[5:7] == (0, 0)
+    with pytest.raises(TypeError):
+        nt.attention(q, q, q, causal=False, starts=1.5)
+    with pytest.raises(ValueError):
+        nt.attention(q, q, q, causal=False, starts=tensor(3, dtype=Dtype.Int32))
+
+
 def test_host_tensors_are_refused():
     x = nt.Tensor(np.ones((1, 3, 2, 4), np.float32))
     with pytest.raises(RuntimeError, match="GPU"):
