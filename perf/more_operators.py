@@ -264,7 +264,7 @@ def _own_attn(s, case):
     import nanotorch_amd as nt
 
     y = nt.attention(s["q"], s["k"], s["v"], causal=case["causal"], lengths=s.get("lengths"),
-                     starts=_starts(case) if case["causal"] else None)
+                     starts=_starts(case))
     out = {"y": _torch(y)}
     if case["kind"] == "train":
         dq, dk, dv = y.grad_fn.backward(s["g"])[:3]
