@@ -107,6 +107,43 @@ def test_coefficients(gpu, t):
         assert_bitexact(host(opt.moments()[0])[500:], m[500:])
 
 
+@pytest.mark.parametrize("lr", [1e-5, 5e-6, 2e-6])
+def test_small_decay_adds_up(gpu, lr):
+    """A decay lr wd of 1e-7 to 2e-8 of p is less than p's own rounding, which an
+    update of like size carries to one side or the other: over many parameters the
+    mean change is update plus decay.
+
+    p's spacing s in [1/2, 1) is 2^-24, and p lies on it, so its rounding's error e is
+    that of the update u alone, with period s and mean zero over one.  For a density f
+    of u the mean of e is at most s^2 / 8, the largest of e's antiderivative, times
+    the total variation of f.  u = lr g / (|g| + 1) with g uniform in [-1, 1] has
+    f = 1 / (2 lr (1 - |u| / lr)^2) up to lr / 2, from 1 / (2 lr) to 2 / lr: a variation of
+    7 / lr with the jumps at both ends, and 7 s^2 / (8 lr) = 3.2e-15 / lr.  The mean of
+    n = 2^20 independent errors is off from that by less than six of
+    s / sqrt(12 n), 1.0e-10 in all.  The decay's mean is 0.75 lr wd, 1.5e-8 and more."""
+    n, wd = 1 << 20, 0.01
+    r = rng(seed_of("small decay", lr))
+    a = r.uniform(0.5 + 2.0 ** -8, 1 - 2.0 ** -8, n).astype(np.float32)
+    g = r.uniform(-1, 1, n).astype(np.float32)
+    p = leaf(a)
+    p._grad = dev(g)
+    nn.AdamW([p], lr, betas=(0.0, 0.9), eps=1.0, weight_decay=wd).step()
+    want = step(a, g, np.zeros_like(a), np.zeros_like(a), 1, lr, 1.0, wd, U[np.float32],
+                (0.0, 0.9))
+    check(host(p), want[0], "p")
+    off = (host(p).astype(np.float64) - want[0][0]).mean()
+    assert abs(off) < 1.0e-10 + 3.2e-15 / lr, (off, lr * wd * 0.75)
+
+
+def test_infinite_parameters_without_decay(gpu):
+    a = np.array([np.inf, -np.inf, 1.0], np.float32)
+    p = leaf(a)
+    p._grad = dev(np.ones(3, np.float32))
+    nn.AdamW([p], 0.1, weight_decay=0.0).step()
+    got = host(p)
+    assert got[0] == np.inf and got[1] == -np.inf and np.isfinite(got[2])
+
+
 def test_continues_bit_for_bit(gpu):
     r = rng(3)
     a = r.standard_normal((30, 40)).astype(np.float32)
