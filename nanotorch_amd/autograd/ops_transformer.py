@@ -73,8 +73,9 @@ class RmsNormOp(Function):
         return True
 
     def _backward_into(self, g: Tensor, needs, targets):
+        # of x and the residual; the weight, mostly a leaf, has a gradient of its own
         tensors = [t for t in self._inputs if isinstance(t, Tensor)]
-        leaf = any([t.is_leaf for t, need in zip(tensors, needs) if need])
+        leaf = any([tensors[i].is_leaf for i in (0, len(needs) - 1) if needs[i]])
         return self._grad(g, needs, targets, not leaf)
 
     def _grad(self, g: Tensor, needs, targets, share: bool) -> list:

@@ -136,6 +136,24 @@ def test_gradients_shared_by_inner_tensors(gpu):
     np.testing.assert_allclose(da - db, 15 * host(a) ** 2, rtol=1e-12, atol=1e-12)
 
 
+def test_gradients_shared_beside_a_trained_weight(gpu):
+    """As above, with a weight that is a leaf."""
+    r = rng(14)
+    a, b = [dev(r.standard_normal((5, 8)), True) for _ in range(2)]
+    w = dev(1 + 0.1 * r.standard_normal(8), True)
+    x, h = a * 1.0, b * 1.0
+    y, s = nt.rms_norm(x, w, residual=h)
+    ((y * y * y).sum() + (s * s).sum() + (x * x * x).sum() * 5.0).backward()
+    da, db = host(a.grad), host(b.grad)
+    np.testing.assert_allclose(da - db, 15 * host(a) ** 2, rtol=1e-12, atol=1e-12)
+    X, R = host(a), host(b)
+    y0 = reference(X, host(w), R, None, None, U[np.float64])["y"][0]
+    want = reference(X, host(w), R, 3 * y0 ** 2, 2 * (X + R), U[np.float64])
+    np.testing.assert_allclose(db, want["ds"][0].astype(np.float64), rtol=1e-11, atol=1e-12)
+    np.testing.assert_allclose(host(w.grad), want["dw"][0].astype(np.float64), rtol=1e-11,
+                               atol=1e-12)
+
+
 def test_same_tensor_twice(gpu):
     r = rng(6)
     x = r.standard_normal((3, 9))

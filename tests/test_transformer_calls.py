@@ -156,6 +156,32 @@ def test_rms_norm_calls(lib):  # noqa: F811
     assert a[1] is a[2] is a[5] is a[6] is None
 
 
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("leaf", ["none", "x", "residual"])
+def test_rms_norm_gradients_of_one_memory(lib, weighted, leaf):  # noqa: F811
+    """x and the residual share their gradient's memory unless one of them is a
+    leaf, which keeps it; whether the weight is trained does not matter."""
+    x, res = [tensor(4, 6, requires_grad=True) for _ in range(2)]
+    w = tensor(6, requires_grad=True) if weighted else None
+    if leaf != "x":
+        x = x * 2.0
+    if leaf != "residual":
+        res = res * 2.0
+    y, _ = nt.rms_norm(x, w, residual=res)
+    fn = y.grad_fn.inputs[0].grad_fn
+    n = 3 if weighted else 2
+    lib.calls.clear()
+    got = fn._backward_into(tensor(2, 4, 6), [True] * n, [None] * n)
+    assert (got[0]._storage is got[-1]._storage) == (leaf == "none")
+    if leaf == "none":
+        assert [name for name, _ in lib.calls] == ["nt_rms_norm_bwd"]
+        assert got[0]._shared and got[-1]._shared
+    # a weight that alone is wanted
+    if weighted:
+        got = fn._backward_into(tensor(2, 4, 6), [False, True, False], [None] * 3)
+        assert got[0] is got[2] is None and got[1]._shape == (6,)
+
+
 def test_adamw_refuses(lib):  # noqa: F811
     p = tensor(4, requires_grad=True)
     for kw in ({"lr": math.nan}, {"lr": math.inf}, {"betas": (1.0, 0.9)}, {"betas": (0.9, -0.1)},
