@@ -241,7 +241,12 @@ class Attention(Module):
                 raise RuntimeError("A cache is not differentiated: use no_grad().")
             starts = cache.tokens
             k, v = cache.append(k, v)
-        y = attention(q, k, v, causal=self._causal, lengths=lengths, starts=starts)
+        try:
+            y = attention(q, k, v, causal=self._causal, lengths=lengths, starts=starts)
+        except BaseException:
+            if cache is not None:
+                cache.tokens = starts  # a refused call adds nothing
+            raise
         return self._out(y.reshape(B * T, dim)).reshape(B, T, dim)
 
 

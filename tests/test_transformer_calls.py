@@ -222,6 +222,21 @@ def test_adamw_calls(lib):  # noqa: F811
     assert opt.steps == 1
 
 
+def test_a_refused_call_leaves_the_cache(lib):  # noqa: F811
+    for dtype, heads_, dim in ((Dtype.Float64, 2, 8), (Dtype.Float32, 1, 300)):
+        a = nn.Attention(dim, heads_)
+        cache = a.cache(2, 10)
+        with nt.no_grad():
+            if dtype is Dtype.Float32:
+                with pytest.raises(ValueError, match="1 to 256"):
+                    a(tensor(2, 4, dim), cache=cache)
+            else:
+                a(tensor(2, 3, dim), cache=cache)
+                with pytest.raises(ValueError, match="one dtype"):
+                    a(tensor(2, 4, dim, dtype=dtype), cache=cache)
+        assert cache.tokens == (0 if dtype is Dtype.Float32 else 3)
+
+
 def test_modules_refuse():
     for args in ((0, 1), (8, 3), (8, 4, 3), (8, 0), (8, 4, 0)):
         with pytest.raises(ValueError):
