@@ -32,14 +32,15 @@ struct AttnShape {
 // hold the tile's values.  words null: no packing took place.
 struct AttnGate {
   const uint32_t *words;
-  int per; // of each (sequence, key head)
+  int per;    // looked at of each (sequence, key head)
+  int stride; // from one to the next
 };
 
 // Whether any word is set; the same for all work-items of the workgroup.
 __device__ __forceinline__ bool gate_set(const AttnGate &g, uint32_t bh) {
   uint32_t any = 0;
   for (int i = threadIdx.x; i < g.per; i += blockDim.x)
-    any |= g.words[int64_t(bh) * g.per + i];
+    any |= g.words[int64_t(bh) * g.stride + i];
   return __syncthreads_or(int(any)) != 0;
 }
 

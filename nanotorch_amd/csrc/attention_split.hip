@@ -2,18 +2,27 @@
 // products large enough that arithmetic bounds them (attention.hip has the
 // mathematics, and the kernels for all others).
 //
-// A float32 x, scaled by a power of two to below 2^15, is hi + lo with hi the
-// nearest half and lo the nearest half of the rest: off by 2^-22 of x at most,
-// 2^-24 in the root mean square, where a float32 itself is off by 2^-24 at most.
-// Products of halves are exact in float32, so a . b is lo hi' + hi lo' + hi hi'
-// on v_mfma_f32_32x32x16_f16, which does sixteen times the work of the float32
-// instructions: 5.3 times their rate with three products for one.  What is left
-// out, lo lo', is 2^-22 of a b at most.
+// A float32 x, scaled by a power of two to below 2^15, is hi + 2^-12 lo with hi the
+// nearest half and lo the nearest half of 2^12 times the rest.  Products of halves
+// are exact in float32, so a . b is hi hi' + 2^-12 (lo hi' + hi lo') on
+// v_mfma_f32_32x32x16_f16, which does sixteen times the work of the float32
+// instructions: 5.3 times their rate with three products for one.
+//
+// What that loses.  A half is normal from 2^-14 on: a scaled x of at least that is off
+// by 2^-22 of itself at most, 2^-24 in the root mean square (a float32 is off by 2^-24
+// at most), and what is left out of a product, lo lo', is 2^-22 of it at most.  Below
+// 2^-14 both grow as 1 / x, and at 2^-17 they are 2^-20 and, with a factor from 2^-14
+// on, 2^-19.  (Without the 2^12, x of 2^-3 and less would lose bits.)  So a value may lie
+// 2^28 below the largest that shares its power of two; groups with one that is not
+// zero and lies below 2^-17, which for normally distributed numbers is one element in
+// 2^30, are not computed here (see the gate below).  ds, which the kernels form, is
+// scaled for each row (or key) and step of 32 items by the largest among these; of
+// smaller ones the same holds, and those 2^31 and more below it keep an error of 2^-50 of
+// the largest.  Probabilities have a power of two to a row.
 //
 // The matrix cores do not round their running sums to nearest, so no long sum
 // stays in them: the products of 32 or 64 rows are summed there, the small ones
-// apart from or before the large ones, and the vector unit adds that to the
-// running result.
+// apart from the large ones, and the vector unit adds that to the running result.
 //
 // A packing kernel writes the operands as planes of halves in the order in which
 // the other kernels' LDS and registers hold them, 32 rows to a unit:
@@ -24,11 +33,13 @@
 //             rows that a lane of a 32 by 32 result holds: probabilities go from
 //             one matrix instruction into the next without leaving their lane
 // A unit is a plane of hi pieces and one of lo pieces.  Keys, values and queries
-// have one power of two to a tile of 64 rows, gradients one to a row.  A tile with
-// a value that is not finite, or whose rows' largest values lie further apart than
-// 2^12 (the small ones would lose bits), is reported in a word, and the whole
-// (sequence, key head) is then left to attention.hip's kernels, queued behind.
-// So a masked key's value never coarsens the others.
+// have one power of two to a tile of 64 rows (the forward pass's queries, which are not
+// packed, one to a row), gradients one to a row.
+//
+// The gate: a tile with a value that is not finite, or that is not zero and lies below
+// 2^-17 once scaled, is reported in a word, and the whole (sequence, key head) is then
+// left to attention.hip's kernels, queued behind.
+// So a masked key's value coarsens no other, nor does a large column.
 //
 // Every kernel's own rows (queries forward and for dq, keys for dk and dv) are the
 // lanes of a result, l % 32, and the other operand's units stream through two
@@ -71,21 +82,26 @@ __device__ __forceinline__ int up_exponent(float most) {
   return min(14 - e, 126);
 }
 
-// Two values to an instruction where they are rounded; the rest x - hi, which is
-// exact, as a sum of mixed types: two instructions a value.
+constexpr float SA_LO = 4096.f;          // lo is so many times the rest
+constexpr float SA_LEAST = 0x1p-17f;     // of a scaled value that is not zero
+
+// hi, two values to an instruction; lo, rounded once, as a sum of mixed types:
+// 2^12 x - 2^12 hi is exact.
 __device__ __forceinline__ void split8(const float (&x)[8], half8 &hi, half8 &lo) {
   typedef float float2v __attribute__((ext_vector_type(2)));
   typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-  float minus = -1.f;
-  asm("" : "+s"(minus)); // a known -1 would make it a conversion and a difference
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     const half2v h = __builtin_convertvector(float2v{x[j], x[j + 1]}, half2v);
-    const float2v rest = {fmaf(float(h.x), minus, x[j]), fmaf(float(h.y), minus, x[j + 1])};
-    const half2v l = __builtin_convertvector(rest, half2v);
     hi[j] = h.x, hi[j + 1] = h.y;
-    lo[j] = l.x, lo[j + 1] = l.y;
+    lo[j] = _Float16(fmaf(float(h.x), -SA_LO, x[j] * SA_LO));
+    lo[j + 1] = _Float16(fmaf(float(h.y), -SA_LO, x[j + 1] * SA_LO));
   }
+}
+
+// Magnitudes as integers in their order, zero the largest.
+__device__ __forceinline__ uint32_t nonzero_bits(float x) {
+  return (__float_as_uint(x) & 0x7fffffffu) - 1;
 }
 
 __device__ __forceinline__ floatx16 mma(half8 a, half8 b, floatx16 c) {
@@ -111,7 +127,8 @@ struct PackArgs {
   AttnShape s;
   PackTensor t[4];
   uint32_t *words;
-  int per;
+  int stride;        // words of a (sequence, key head)
+  int zero;          // the one among them that later kernels set; -1: none
   // the gradient's: y, the forward statistics, and what becomes of them
   Rows<const float> y;
   const float *lse;
@@ -124,7 +141,7 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
   constexpr int DP = 32 * DB, PITCH = DP + 4, CH = SA_CHUNK<DB>;
   __shared__ float x[SA_TILE * PITCH];
   __shared__ float factor[SA_TILE];
-  __shared__ int wave_most[4], wave_least[4];
+  __shared__ uint32_t wave_most[4], wave_least[4];
   int which = 0;
   while (blockIdx.x >= a.t[which].blocks)
     ++which;
@@ -152,32 +169,38 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
       x[r * PITCH + d + j] = live ? v[j] : 0.f;
   }
   __syncthreads();
-  // four work-items to a row: its largest magnitude (NaN above infinity)
+  // four work-items to a row: its largest magnitude (NaN above infinity) and its
+  // smallest but zero
   const int r = threadIdx.x / 4, part = threadIdx.x % 4;
-  uint32_t top = 0;
-  for (int d = part; d < DP; d += 4)
-    top = max(top, __float_as_uint(x[r * PITCH + d]) & 0x7fffffffu);
-  top = max(top, uint32_t(__shfl_xor(int(top), 1)));
-  top = max(top, uint32_t(__shfl_xor(int(top), 2)));
-  // the tile's largest, and its smallest that is not 0
-  int hi = int(top), lo = top ? int(top) : 0x7fffffff;
+  uint32_t most = 0, least = ~0u;
+  for (int d = part; d < DP; d += 4) {
+    most = max(most, __float_as_uint(x[r * PITCH + d]) & 0x7fffffffu);
+    least = min(least, nonzero_bits(x[r * PITCH + d]));
+  }
+  // of the row where that has a power of two of its own, and of the tile
+  auto group = [&](int from, int to) {
 #pragma unroll
-  for (int o = 4; o < 64; o <<= 1) {
-    hi = max(hi, __shfl_xor(hi, o));
-    lo = min(lo, __shfl_xor(lo, o));
-  }
-  if ((threadIdx.x & 63) == 0) {
-    wave_most[threadIdx.x >> 6] = hi;
-    wave_least[threadIdx.x >> 6] = lo;
-  }
-  __syncthreads();
-  hi = max(max(wave_most[0], wave_most[1]), max(wave_most[2], wave_most[3]));
-  lo = min(min(wave_least[0], wave_least[1]), min(wave_least[2], wave_least[3]));
-  // a gradient's row of zeros counts least among the rows that it is summed with
-  const int up = !t.scale && top == 0 ? 126 : up_exponent(__int_as_float(t.scale ? hi : int(top)));
-  bool bad = hi >= 0x7f800000;
+    for (int o = from; o < to; o <<= 1) {
+      most = max(most, uint32_t(__shfl_xor(int(most), o)));
+      least = min(least, uint32_t(__shfl_xor(int(least), o)));
+    }
+  };
+  group(1, 4);
   if (t.scale) {
-    bad = bad || (hi > lo && (hi >> 23) - (lo >> 23) > 12);
+    group(4, 64);
+    if ((threadIdx.x & 63) == 0) {
+      wave_most[threadIdx.x >> 6] = most;
+      wave_least[threadIdx.x >> 6] = least;
+    }
+    __syncthreads();
+    most = max(max(wave_most[0], wave_most[1]), max(wave_most[2], wave_most[3]));
+    least = min(min(wave_least[0], wave_least[1]), min(wave_least[2], wave_least[3]));
+  }
+  // a gradient's row of zeros counts least among the rows that it is summed with
+  const int up = !t.scale && most == 0 ? 126 : up_exponent(__uint_as_float(most));
+  const bool bad = most >= __float_as_uint(SA_INF) ||
+                   (most != 0 && __uint_as_float(least + 1) * pow2(up) < SA_LEAST);
+  if (t.scale) {
     if (threadIdx.x == 0)
       t.scale[int64_t(bh) * t.tiles + tile] = pow2(-up);
   } else { // the gradient: its rows' statistics
@@ -210,9 +233,12 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
   }
   if (part == 0)
     factor[r] = pow2(up);
-  if (threadIdx.x == 0)
-    a.words[int64_t(bh) * a.per + t.word + tile] = bad;
-  __syncthreads();
+  const int any = __syncthreads_or(int(bad)); // (also: the factors are there)
+  if (threadIdx.x == 0) {
+    a.words[int64_t(bh) * a.stride + t.word + tile] = uint32_t(any != 0);
+    if (a.zero >= 0 && which == 0 && tile == 0)
+      a.words[int64_t(bh) * a.stride + a.zero] = 0;
+  }
   const int64_t unit0 = (int64_t(bh) * t.tiles + tile) * 2;
   // pieces of both units, a wave for each
   const int lane = threadIdx.x & 63, l = lane & 31, h = lane >> 5;
@@ -276,46 +302,70 @@ __device__ __forceinline__ void keep_order() {
   __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x10); // vector, scalar, global memory
 }
 
+// How the small products are kept from the large ones'.  APART: in a sum of their own.
+// In turn, where registers are short (two waves to a SIMD, heads of 65 to 128): first
+// the small ones, whose sum the large ones are added to; the hi pieces wait for their
+// turn in registers where those are two or four, else they are read again.
+template <int DB> constexpr bool SA_APART = DB <= 2 || DB > 4;
+
 // sum over NF pieces of (pieces . operand), pieces at at(0) ..; pre holds the first
-// two pairs and gets those at next(0) and next(1).  The small products come first,
-// so that their sum is not rounded as the large ones' is; the hi pieces wait for
-// their turn in registers (KEEP), or are read again where those are few.
-template <int NF, bool KEEP, int HALF, class At, class Next>
+// two pairs and gets those at next(0) and next(1).
+template <int NF, bool APART, int HALF, class At, class Next>
 __device__ __forceinline__ floatx16 stream_sum(At at, Next next, const half8 *hi, const half8 *lo,
                                                Pair (&pre)[2], int lane) {
-  floatx16 s{};
-  half8 xh[KEEP ? NF : 2];
   auto pair = [&](const char *p) { return Pair{frag(p, lane), frag(p + HALF, lane)}; };
+  floatx16 small{};
+  if constexpr (APART) {
+    floatx16 large{};
 #pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    const Pair x = pre[f & 1];
-    if constexpr (KEEP) {
-      xh[f] = x.h;
+    for (int f = 0; f < NF; ++f) {
+      const Pair x = pre[f & 1];
       pre[f & 1] = pair(f + 2 < NF ? at(f + 2) : next(f + 2 - NF));
-    } else if (f + 2 < NF) {
-      pre[f & 1] = pair(at(f + 2));
-    } else {
-      xh[f & 1] = frag(at(f & 1), lane);
-    }
-    keep_order();
-    s = mma(x.l, hi[f], s);
-    s = mma(x.h, lo[f], s);
-    keep_order();
-  }
-#pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    const half8 x = xh[KEEP ? f : f & 1];
-    if constexpr (!KEEP) {
-      if (f + 2 < NF)
-        xh[f & 1] = frag(at(f + 2), lane);
-      else
-        pre[f & 1] = pair(next(f & 1));
+      keep_order();
+      small = mma(x.l, hi[f], small);
+      large = mma(x.h, hi[f], large);
+      small = mma(x.h, lo[f], small);
       keep_order();
     }
-    s = mma(x, hi[f], s);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      large[r] = fmaf(small[r], 1.f / SA_LO, large[r]);
+    return large;
+  } else {
+    constexpr bool KEEP = NF <= 4;
+    half8 xh[KEEP ? NF : 2];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const Pair x = pre[f & 1];
+      if constexpr (KEEP) {
+        xh[f] = x.h;
+        pre[f & 1] = pair(f + 2 < NF ? at(f + 2) : next(f + 2 - NF));
+      } else if (f + 2 < NF) {
+        pre[f & 1] = pair(at(f + 2));
+      } else {
+        xh[f & 1] = frag(at(f & 1), lane);
+      }
+      keep_order();
+      small = mma(x.l, hi[f], small);
+      small = mma(x.h, lo[f], small);
+      keep_order();
+    }
+    small *= 1.f / SA_LO;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const half8 x = xh[KEEP ? f : f & 1];
+      if constexpr (!KEEP) {
+        if (f + 2 < NF)
+          xh[f & 1] = frag(at(f + 2), lane);
+        else
+          pre[f & 1] = pair(next(f & 1));
+        keep_order();
+      }
+      small = mma(x, hi[f], small);
+    }
+    keep_order();
+    return small;
   }
-  keep_order();
-  return s;
 }
 
 // items' row form (a unit) . own rows: result[item, own]; pre and next as above.
@@ -323,7 +373,7 @@ template <int DB, class Next>
 __device__ __forceinline__ floatx16 dots32(const char *unit, const half8 (&hi)[2 * DB],
                                            const half8 (&lo)[2 * DB], Pair (&pre)[2], Next next,
                                            int lane) {
-  return stream_sum<2 * DB, DB <= 3, SA_CHUNK<DB> / 2>(
+  return stream_sum<2 * DB, SA_APART<DB>, SA_CHUNK<DB> / 2>(
       [&](int f) { return unit + f * 1024; }, next, hi, lo, pre, lane);
 }
 
@@ -369,7 +419,7 @@ __device__ __forceinline__ void sums32(floatx16 (&acc)[DB], const char *unit, co
                                        const char *after, int lane) {
 #pragma unroll
   for (int db = 0; db < DB; ++db) {
-    const floatx16 t = stream_sum<2, true, SA_CHUNK<DB> / 2>(
+    const floatx16 t = stream_sum<2, SA_APART<DB>, SA_CHUNK<DB> / 2>(
         [&](int f) { return unit + (2 * db + f) * 1024; },
         [&](int f) { return (db + 1 < DB ? unit + (2 * db + 2) * 1024 : after) + f * 1024; }, hi,
         lo, pre, lane);
@@ -419,6 +469,7 @@ struct SplitFwd {
   float *y, *lse;
   float scale2;
   AttnGate gate;
+  uint32_t *q_word;              // of each (sequence, key head), gate.stride apart
   int parts;                     // of the keys; over one: sums [part][bh, row][D] and
   float *sums, *tops;            // maxima, sums of p [part][2][bh, row]
 };
@@ -474,6 +525,7 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
       qp += int64_t(i) * a.q.sOuter + int64_t(uint32_t(row) - i * uint32_t(s.G)) * a.q.sInner;
     float v[2 * DB][8];
     float most = 0.f;
+    uint32_t least = ~0u;
 #pragma unroll
     for (int f = 0; f < 2 * DB; ++f)
 #pragma unroll
@@ -483,12 +535,17 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
         for (int j = 0; j < 4; ++j) {
           v[f][4 * u + j] = x[j];
           most = fmaxf(most, fabsf(x[j]));
+          least = min(least, nonzero_bits(x[j]));
         }
       }
     most = fmaxf(most, __shfl_xor(most, 32));
     const int up = up_exponent(most < SA_INF ? most : 0.f);
     const float k = a.scale2 > 0.f ? pow2(up) : a.scale2 < 0.f ? -pow2(up) : 0.f;
     q_scale = pow2(-up);
+    // (a row that is no number, or infinite, gives what it gives here too)
+    if (most > 0.f && most < SA_INF &&
+        __uint_as_float(least + 1) * pow2(up) < SA_LEAST)
+      a.q_word[int64_t(bh) * a.gate.stride] = 1;
 #pragma unroll
     for (int f = 0; f < 2 * DB; ++f) {
 #pragma unroll
@@ -551,7 +608,7 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
       split16(z[u], ph + 2 * u, pl + 2 * u);
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
-      const floatx16 o = stream_sum<2 * UNITS, true, CH / 2>(
+      const floatx16 o = stream_sum<2 * UNITS, SA_APART<DB>, CH / 2>(
           [&](int f) { return st + (UNITS + f / 2) * CH + (2 * db + f % 2) * 1024; },
           [&](int f) { return st + UNITS * CH + (2 * (db + 1 < DB ? db + 1 : 0) + f) * 1024; }, ph, pl,
           pre, lane);
@@ -987,14 +1044,14 @@ bool split_takes(const AttnShape &s, bool backward) {
 
 size_t split_gate_words(const AttnShape &s, bool backward) {
   const size_t k = size_t(tiles_of(s.Tk)), q = size_t(tiles_of(s.rows));
-  return size_t(s.B) * size_t(s.Hk) * (2 * k + (backward ? 2 * q : 0));
+  return size_t(s.B) * size_t(s.Hk) * (2 * k + (backward ? 2 * q : 1));
 }
 
 void run_split(AttnFwd<float> &a, uint32_t *words) {
   const AttnShape &s = a.s;
   const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
   const int tiles = tiles_of(s.Tk);
-  a.gate = {words, 2 * tiles};
+  a.gate = {words, 2 * tiles + 1, 2 * tiles + 1}; // the keys', the values', the queries'
   dispatch_blocks(s.D, [&]<int DB>() {
     const size_t form = size_t(bhs) * size_t(tiles) * 2 * SA_CHUNK<DB>;
     DeviceScratch planes(2 * form + 2 * size_t(bhs) * size_t(tiles) * sizeof(float));
@@ -1003,7 +1060,8 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     PackArgs p{};
     p.s = s;
     p.words = words;
-    p.per = a.gate.per;
+    p.stride = a.gate.stride;
+    p.zero = 2 * tiles;
     p.t[0] = {a.k, k, nullptr, k_scale, s.Tk, tiles, 1, bhs * uint32_t(tiles), 0};
     p.t[1] = {a.v, nullptr, v, v_scale, s.Tk, tiles, 1, 2 * bhs * uint32_t(tiles), tiles};
     attn_pack_kernel<DB><<<dim3(p.t[1].blocks), 256, 0, stream()>>>(p);
@@ -1016,7 +1074,8 @@ void run_split(AttnFwd<float> &a, uint32_t *words) {
     f.tiles = tiles;
     f.y = a.y, f.lse = a.lse;
     f.scale2 = a.scale2;
-    f.gate = a.gate;
+    f.gate = {words, 2 * tiles, a.gate.stride}; // the queries' are set meanwhile
+    f.q_word = words + 2 * tiles;
     const uint32_t groups = bhs * uint32_t((s.rows + SF_ROWS<DB> - 1) / SF_ROWS<DB>);
     f.parts = parts_of(groups, tiles * 2 / SF_UNITS<DB>);
     const size_t rows = size_t(bhs) * size_t(s.rows), kept = f.parts > 1 ? size_t(f.parts) : 0;
@@ -1037,7 +1096,7 @@ void run_split_bwd(AttnBwd<float> &a, uint32_t *words) {
   const AttnShape &s = a.s;
   const uint32_t bhs = uint32_t(s.B) * uint32_t(s.Hk);
   const int kt = tiles_of(s.Tk), qt = tiles_of(s.rows);
-  a.gate = {words, 2 * kt + 2 * qt};
+  a.gate = {words, 2 * kt + 2 * qt, 2 * kt + 2 * qt};
   dispatch_blocks(s.D, [&]<int DB>() {
     const size_t kform = size_t(bhs) * size_t(kt) * 2 * SA_CHUNK<DB>;
     const size_t qform = size_t(bhs) * size_t(qt) * 2 * SA_CHUNK<DB>;
@@ -1055,7 +1114,8 @@ void run_split_bwd(AttnBwd<float> &a, uint32_t *words) {
     PackArgs p{};
     p.s = s;
     p.words = words;
-    p.per = a.gate.per;
+    p.stride = a.gate.stride;
+    p.zero = -1;
     p.y = a.y;
     p.lse = a.lse;
     p.stats = stats;

@@ -236,6 +236,48 @@ def test_large_with_an_outlier(gpu, what, D):
         check(dq[:, :at], [t[:, :at] for t in clean["dq"]], "dq")
 
 
+@pytest.mark.parametrize("T,D", [(1820, 64), (1300, 128), (1200, 160)])
+@pytest.mark.parametrize("power", [10, 17, 20, 24, 28, 32, 40])
+@pytest.mark.parametrize("what", ["v", "g", "q up", "k up"])
+def test_large_with_a_column_apart(gpu, what, power, T, D):
+    """One column far above the others, which keep their bits: the columns of a
+    result are no concern of one another's.  Queries and keys are scaled against
+    each other, so that scores stay as they are."""
+    r = rng(seed_of("column", what, power, D))
+    q, k, v, g = inputs(r, 1, T, T, 2, 1, D, np.float32)
+    by = np.float32(2.0 ** power)
+    if what == "v":
+        v[..., 5] *= by
+        g[..., 5] /= by
+    elif what == "g":
+        g[..., 5] *= by
+        v[..., 5] /= by
+    else:
+        q[..., 5] *= by if what == "q up" else 1 / by
+        k[..., 5] *= 1 / by if what == "q up" else by
+    check_all(q, k, v, g, visible(1, T, T, True), np.float32, causal=True)
+
+
+@pytest.mark.parametrize("power", [15, 25, 33])
+@pytest.mark.parametrize("what", ["v", "k", "q", "g"])
+def test_large_elements_in_every_row_and_column(gpu, what, power):
+    """Rows are alike and columns are alike, but no row has all the large values that
+    its columns have: rows that do not see a column's large ones keep their bits."""
+    r = rng(seed_of("diagonal", what, power))
+    T, D = 1820, 64
+    q, k, v, g = inputs(r, 1, T, T, 2, 1, D, np.float32, sharp=0.5)
+    x = {"q": q, "k": k, "v": v, "g": g}[what]
+    other = {"q": k, "k": q}.get(what)
+    at = np.arange(T)
+    if other is not None:  # no score is large: the other side has zeros there
+        some = r.integers(0, D // 2, T)
+        other[..., :D // 2] = 0
+        x[0, at, :, some] *= np.float32(2.0 ** power)
+    else:
+        x[0, at, :, at % D] *= np.float32(2.0 ** power)
+    check_all(q, k, v, g, visible(1, T, T, True), np.float32, causal=True)
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("wide", [np.int32, np.int64])
 @pytest.mark.parametrize("causal,starts", [(False, None), (True, None), (True, 0), (True, -3),
