@@ -36,9 +36,10 @@
 // have one power of two to a tile of 64 rows (the forward pass's queries, which are not
 // packed, one to a row), gradients one to a row.
 //
-// The gate: a tile with a value that is not finite, or that is not zero and lies below
-// 2^-17 once scaled, is reported in a word, and the whole (sequence, key head) is then
-// left to attention.hip's kernels, queued behind.
+// The gate: a tile with a value that is not finite, that is not zero and lies below
+// 2^-17 once scaled, or that is 2^18 or more (products of three such and sums of them
+// could pass float32's range before they are scaled back) is reported in a word, and
+// the whole (sequence, key head) is then left to attention.hip's kernels, queued behind.
 // So a masked key's value coarsens no other, nor does a large column.
 //
 // Every kernel's own rows (queries forward and for dq, keys for dk and dv) are the
@@ -84,6 +85,7 @@ __device__ __forceinline__ int up_exponent(float most) {
 
 constexpr float SA_LO = 4096.f;          // lo is so many times the rest
 constexpr float SA_LEAST = 0x1p-17f;     // of a scaled value that is not zero
+constexpr float SA_MOST = 0x1p18f;       // of a value
 
 // hi, two values to an instruction; lo, rounded once, as a sum of mixed types:
 // 2^12 x - 2^12 hi is exact.
@@ -198,7 +200,7 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
   }
   // a gradient's row of zeros counts least among the rows that it is summed with
   const int up = !t.scale && most == 0 ? 126 : up_exponent(__uint_as_float(most));
-  const bool bad = most >= __float_as_uint(SA_INF) ||
+  const bool bad = most >= __float_as_uint(SA_MOST) ||
                    (most != 0 && __uint_as_float(least + 1) * pow2(up) < SA_LEAST);
   if (t.scale) {
     if (threadIdx.x == 0)
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
     q_scale = pow2(-up);
     // (a row that is no number, or infinite, gives what it gives here too)
     if (most > 0.f && most < SA_INF &&
-        __uint_as_float(least + 1) * pow2(up) < SA_LEAST)
+        (most >= SA_MOST || __uint_as_float(least + 1) * pow2(up) < SA_LEAST))
       a.q_word[int64_t(bh) * a.gate.stride] = 1;
 #pragma unroll
     for (int f = 0; f < 2 * DB; ++f) {

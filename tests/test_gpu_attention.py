@@ -278,6 +278,17 @@ def test_large_elements_in_every_row_and_column(gpu, what, power):
     check_all(q, k, v, g, visible(1, T, T, True), np.float32, causal=True)
 
 
+def test_large_values_with_small_gradients(gpu):
+    """Values of 2^110 and their gradients of 2^-66: nothing passes float32's range that
+    the results do not pass."""
+    r = rng(seed_of("range"))
+    T, D = 1820, 64
+    q, k, v, g = inputs(r, 1, T, T, 2, 1, D, np.float32)
+    v *= np.float32(2.0 ** 110)
+    g *= np.float32(2.0 ** -66)
+    check_all(q, k, v, g, visible(1, T, T, True), np.float32, causal=True)
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("wide", [np.int32, np.int64])
 @pytest.mark.parametrize("causal,starts", [(False, None), (True, None), (True, 0), (True, -3),
