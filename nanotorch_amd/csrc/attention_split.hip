@@ -15,10 +15,10 @@
 // on, 2^-19.  (Without the 2^12, x of 2^-3 and less would lose bits.)  So a value may lie
 // 2^28 below the largest that shares its power of two; groups with one that is not
 // zero and lies below 2^-17, which for normally distributed numbers is one element in
-// 2^30, are not computed here (see the gate below).  ds, which the kernels form, is
-// scaled for each row (or key) and step of 32 items by the largest among these; of
-// smaller ones the same holds, and those 2^31 and more below it keep an error of 2^-50 of
-// the largest.  Probabilities have a power of two to a row.
+// 2^30, are not computed here (see the gate below).  Probabilities and ds, which the
+// kernels form, are scaled for each row (or key) and step of 32 or 64 items by the
+// largest among these; of smaller ones the same holds, and those 2^31 and more below it
+// keep an error of 2^-50 of the largest.
 //
 // The matrix cores do not round their running sums to nearest, so no long sum
 // stays in them: the products of 32 or 64 rows are summed there, the small ones
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
     // positive and finite, so that it takes -inf to -inf
     const float cz = fminf(fmaxf(c * q_scale * a.k_scale[int64_t(bh) * a.tiles + it * UNITS / 2], 1.2e-38f),
                            3.4e38f);
-    const float v_scale = a.v_scale[int64_t(bh) * a.tiles + it * UNITS / 2];
+    float v_scale = a.v_scale[int64_t(bh) * a.tiles + it * UNITS / 2];
     floatx16 z[UNITS];
     Pair pre[2];
     first_pairs<DB>(pre, st, lane);
@@ -591,8 +591,12 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
       for (int r = 0; r < 16; ++r)
         top = fmaxf(top, z[u][r]);
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float next = fmaxf(m, top * cz), base = next == -SA_INF ? 0.f : next;
-    const float shrink = __builtin_amdgcn_exp2f(m - base);
+    // Probabilities relative to this step's largest, so that none is too small for its
+    // halves beside a larger one of another step, whose values may be far smaller.
+    const float here = top * cz, base = here == -SA_INF ? 0.f : here;
+    const float next = fmaxf(m, here), whole = next == -SA_INF ? 0.f : next;
+    const float shrink = __builtin_amdgcn_exp2f(m - whole);
+    const float weight = __builtin_amdgcn_exp2f(here - whole);
     m = next;
     float sum = 0.f;
 #pragma unroll
@@ -603,11 +607,12 @@ __global__ __launch_bounds__(64 * SF_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
         z[u][r] = __builtin_amdgcn_exp2f(fmaf(z[u][r], cz, 14.f - base));
         sum += z[u][r];
       }
-    l = fmaf(l, shrink, sum);
+    l = fmaf(l, shrink, sum * weight);
     half8 ph[2 * UNITS], pl[2 * UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u)
       split16(z[u], ph + 2 * u, pl + 2 * u);
+    v_scale *= weight;
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
       const floatx16 o = stream_sum<2 * UNITS, SA_APART<DB>, CH / 2>(

@@ -278,6 +278,23 @@ def test_large_elements_in_every_row_and_column(gpu, what, power):
     check_all(q, k, v, g, visible(1, T, T, True), np.float32, causal=True)
 
 
+@pytest.mark.parametrize("small", [1.0])
+def test_large_with_small_probabilities(gpu, small):
+    """Keys that no query cares for, with columns of values of their own: what is e^-30
+    beside the rest is all that those columns have."""
+    r = rng(seed_of("tail"))
+    T, D = 1820, 64
+    q, k, v, g = inputs(r, 1, T, T, 2, 1, D, np.float32, sharp=0.2)
+    q[..., 0] = 10.0
+    k[..., 0] = 12.0
+    some = np.zeros(T, bool)
+    some[1728:1792] = True  # behind others
+    k[:, some, :, 0] = -12.0
+    v[:, ~some, :, :8] = 0
+    g *= np.float32(small)
+    check_all(q, k, v, g, visible(1, T, T, False), np.float32)
+
+
 def test_large_values_with_small_gradients(gpu):
     """Values of 2^110 and their gradients of 2^-66: nothing passes float32's range that
     the results do not pass."""
