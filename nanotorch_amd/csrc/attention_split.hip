@@ -86,6 +86,9 @@ __device__ __forceinline__ int up_exponent(float most) {
 constexpr float SA_LO = 4096.f;          // lo is so many times the rest
 constexpr float SA_LEAST = 0x1p-17f;     // of a scaled value that is not zero
 constexpr float SA_MOST = 0x1p18f;       // of a value
+// Gradients' powers of two reach dv's and dk's sums times this, so that a probability
+// times that of a small row is no subnormal number.
+constexpr int SA_LIFT = 40;
 
 // hi, two values to an instruction; lo, rounded once, as a sum of mixed types:
 // 2^12 x - 2^12 hi is exact.
@@ -229,7 +232,7 @@ template <int DB> __global__ __launch_bounds__(256) void attn_pack_kernel(const 
       // a row that sees nothing: exp2(z - inf) = 0
       st[0] = limit > 0 ? a.lse[int64_t(bh) * t.rows + row] : SA_INF;
       st[SA_UNIT] = dot * pow2(up);
-      st[2 * SA_UNIT] = pow2(-up);
+      st[2 * SA_UNIT] = pow2(min(SA_LIFT - up, 127));
       reinterpret_cast<int *>(st)[3 * SA_UNIT] = limit;
     }
   }
@@ -821,7 +824,7 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
   const int64_t head = int64_t(hk) * s.G + (uint32_t(row) - i * uint32_t(s.G));
   const int64_t size = int64_t(s.B) * s.Hk * s.rows * s.D;
   store_row<DB>(a.dq + part * size + ((int64_t(b) * s.Tq + i) * s.Hk * s.G + head) * s.D, acc,
-                a.scale * g_scale, s.D, h);
+                a.scale * (g_scale * pow2(-SA_LIFT)), s.D, h);
 }
 
 // DK, DV: which of the two.  Both in one kernel share the probabilities; of heads
@@ -927,7 +930,7 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * q + j;
-        // p times the row's scale: what multiplies its packed gradient
+        // p times the row's scale (and 2^SA_LIFT): what multiplies its packed gradient
         w[r] = __builtin_amdgcn_exp2f(fmaf(w[r], cz, -ls[j])) * gs[j];
         if constexpr (DK)
           ds[r] = w[r] * fmaf(ds[r], v_scale, -de[j]);
@@ -966,9 +969,9 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
   const int64_t size = int64_t(s.B) * s.Tk * s.Hk * s.D;
   const int64_t at = part * size + ((int64_t(b) * s.Tk + key) * s.Hk + hk) * s.D;
   if (DK && a.dk)
-    store_row<DB>(a.dk + at, dk, a.scale, s.D, h);
+    store_row<DB>(a.dk + at, dk, a.scale * pow2(-SA_LIFT), s.D, h);
   if (DV && a.dv)
-    store_row<DB>(a.dv + at, dv, 1.f, s.D, h);
+    store_row<DB>(a.dv + at, dv, pow2(-SA_LIFT), s.D, h);
 }
 
 // The parts of a gradient [B, T, Hk G, D] added up in order; what the gate left to

@@ -278,10 +278,11 @@ def test_large_elements_in_every_row_and_column(gpu, what, power):
     check_all(q, k, v, g, visible(1, T, T, True), np.float32, causal=True)
 
 
-@pytest.mark.parametrize("small", [1.0])
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -80])
 def test_large_with_small_probabilities(gpu, small):
     """Keys that no query cares for, with columns of values of their own: what is e^-30
-    beside the rest is all that those columns have."""
+    beside the rest is all that those columns have.  With gradients so small that
+    probability times gradient is next to float32's smallest number."""
     r = rng(seed_of("tail"))
     T, D = 1820, 64
     q, k, v, g = inputs(r, 1, T, T, 2, 1, D, np.float32, sharp=0.2)
