@@ -126,6 +126,14 @@ __device__ __forceinline__ typename RowVec<T>::V piece(const T *row, int d, int 
   return v;
 }
 
+// W, which the compiler does not know to be the same for every `by`: comparisons with
+// it are made again for each.  (Kept through a loop, a lane mask for each piece of a row
+// outgrew the scalar registers.)
+template <class B> __device__ __forceinline__ int afresh(int W, B by) {
+  asm("" : "+v"(W) : "v"(by));
+  return W;
+}
+
 // attention_split.hip: whether its kernels take a product of this shape, and
 // their launches.  The forward launch leaves a.gate for the kernels that follow
 // it; `words` is its memory, which must outlive them.

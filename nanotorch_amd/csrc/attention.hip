@@ -83,6 +83,7 @@ template <class T, int DP> struct Frag {
   typename RowVec<T>::V v[C];
   // From element d0 of a row of W on.
   __device__ __forceinline__ void load(const T *row, int d0, int W, int h) {
+    W = afresh(W, row);
 #pragma unroll
     for (int c = 0; c < C; ++c)
       v[c] = piece(row, d0 + 4 * N * c + N * h, W);
@@ -131,6 +132,7 @@ template <class T, int DP> struct Items {
   typename RowVec<T>::V v[4][C];
   // The columns from d0 on of a row of W.
   __device__ __forceinline__ void load(int r, const T *row, int d0, int W, int n) {
+    W = afresh(W, row);
 #pragma unroll
     for (int c = 0; c < C; ++c)
       v[r][c] = piece(row, d0 + N * (16 * c + n), W);
@@ -172,10 +174,12 @@ template <class T, int DP> struct Sums {
         for (int e = 0; e < N; ++e)
           acc[c][e] = Mma<T>::mma(x.v[r][c][e], a[r], acc[c][e]);
   }
-  // The same over visible pairs only, from memory: `row(item)` is the item's
-  // row, null past the end.
+  // The same over visible pairs only, from memory: `row(item)` is the item's row from
+  // the sums' first column on, null past the end, with W elements from there (none, or
+  // fewer than none, where the columns begin past its end).  In place of what lies past
+  // its end its last piece is read, for sums that no one stores: no branches of a lane.
   template <class F>
-  __device__ __forceinline__ void add_visible(const T (&a)[4], const bool (&vis)[4], int D,
+  __device__ __forceinline__ void add_visible(const T (&a)[4], const bool (&vis)[4], int W,
                                               int lane, F row) {
     const int n = lane & 15, h = lane >> 4;
 #pragma unroll 1
@@ -191,18 +195,18 @@ template <class T, int DP> struct Sums {
             w = __shfl(a[r], n + 16 * g);
             on = __shfl(int(vis[r]), n + 16 * g);
           }
-      if (p == nullptr || !on)
+      if (p == nullptr)
         continue;
+      const int last = afresh(W, item) - N;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < N; ++e)
+        for (int r = 0; r < 4; ++r) {
+          const auto x = RowVec<T>::load(p + std::min(column(c, 0, h, r), last));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int d = column(c, e, h, r);
-            if (d < D)
-              acc[c][e][r] = fma(w, p[d], acc[c][e][r]);
-          }
+          for (int e = 0; e < N; ++e)
+            acc[c][e][r] = on ? fma(w, x[e], acc[c][e][r]) : acc[c][e][r];
+        }
     }
   }
 };
@@ -367,7 +371,7 @@ __device__ __forceinline__ void attn_fwd_tile(const AttnFwd<T> &a, uint32_t bh, 
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i;
       if (j + 16 > all && !all_finite<T, DP>(v[i]))
-        sums.add_visible(z[i], vis[i], s.D, lane, [&](int item) {
+        sums.add_visible(z[i], vis[i], s.W, lane, [&](int item) {
           return j + item < end ? vp + int64_t(j + item) * a.v.sOuter : nullptr;
         });
       else
@@ -601,7 +605,7 @@ __device__ __forceinline__ void attn_dq_tile(const AttnBwd<T> &a, uint32_t bh, u
       ds[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse) * (dp[r] - delta) : T(0);
     }
     if (j0 + 16 > all && !all_finite<T, DP>(x))
-      sums.add_visible(ds, vis, s.D, lane, [&](int item) {
+      sums.add_visible(ds, vis, s.W, lane, [&](int item) {
         return j0 + item < end ? kp + int64_t(j0 + item) * a.k.sOuter : nullptr;
       });
     else
@@ -701,11 +705,11 @@ __device__ __forceinline__ void attn_dkv_tile(const AttnBwd<T> &a, uint32_t bh, 
       };
     };
     if (__any(some) && !all_finite<T, SC>(xg))
-      dv.add_visible(p, vis, s.D - col0, lane, row_of(gp, a.g));
+      dv.add_visible(p, vis, s.W - col0, lane, row_of(gp, a.g));
     else
       dv.add(p, xg);
     if (__any(some) && !all_finite<T, SC>(xq))
-      dk.add_visible(ds, vis, s.D - col0, lane, row_of(qp, a.q));
+      dk.add_visible(ds, vis, s.W - col0, lane, row_of(qp, a.q));
     else
       dk.add(ds, xq);
   }
@@ -882,7 +886,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, DP <= 128 ? 2 : 1) void attn_wide_fw
       l += z[r];
     }
     if (j0 + 16 > all && !all_finite<T, PART>(v))
-      sums.add_visible(z, vis, s.D - col0, lane, [&](int i) {
+      sums.add_visible(z, vis, s.W - col0, lane, [&](int i) {
         return j0 + i < end ? vp + int64_t(j0 + i) * a.v.sOuter + col0 : nullptr;
       });
     else
@@ -978,7 +982,7 @@ __device__ __forceinline__ void attn_wide_dq_tile(const AttnBwd<T> &a, uint32_t 
       ds[r] = vis[r] ? M::exp2(z[r] * a.scale2 - lse) * (dp[r] - delta) : T(0);
     }
     if (j0 + 16 > all && !all_finite<T, PART>(x))
-      sums.add_visible(ds, vis, s.D - col0, lane, [&](int i) {
+      sums.add_visible(ds, vis, s.W - col0, lane, [&](int i) {
         return j0 + i < end ? kp + int64_t(j0 + i) * a.k.sOuter + col0 : nullptr;
       });
     else
@@ -1073,11 +1077,11 @@ __device__ __forceinline__ void attn_wide_dkv_tile(const AttnBwd<T> &a, uint32_t
       };
     };
     if (__any(some) && !all_finite<T, PART>(xg))
-      dv.add_visible(p, vis, s.D - col0, lane, row_of(gp, a.g));
+      dv.add_visible(p, vis, s.W - col0, lane, row_of(gp, a.g));
     else
       dv.add(p, xg);
     if (__any(some) && !all_finite<T, PART>(xq))
-      dk.add_visible(ds, vis, s.D - col0, lane, row_of(qp, a.q));
+      dk.add_visible(ds, vis, s.W - col0, lane, row_of(qp, a.q));
     else
       dk.add(ds, xq);
   }
