@@ -437,7 +437,8 @@ int nt_rms_norm_bwd(const nt_view *sum, const nt_view *weight,
  * else that a query does not see, whatever it holds.  A length outside [0, Tk] is taken
  * as the nearer end, and the next nt_sync() or nt_memcpy_d2h() returns
  * NT_ERR_INDEX.  y is contiguous; lse, which nt_attention_bwd needs, receives
- * B H Tq statistics or is NULL.  Hk max(Tq H / Hk, Tk) is below 2^25. */
+ * B H Tq statistics or is NULL.  Hk max(Tq H / Hk, Tk) is below 2^25, |scale| below
+ * 2^127 (float32) or 2^1023 (NT_ERR_VALUE). */
 int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v,
                  const nt_view *lengths, const nt_view *starts, int64_t start,
                  int32_t causal, double scale, const nt_view *y,

@@ -1204,8 +1204,10 @@ int64_t sequences_at_once(const nt_view *q, const nt_view *k) {
 
 AttnShape attn_shape(const nt_view *q, const nt_view *k, const nt_view *v,
                      const nt_view *lengths, const nt_view *starts, int64_t start,
-                     int32_t causal) {
+                     int32_t causal, double scale) {
   check_heads(q, q, "q");
+  if (!(std::abs(scale) < (q->dtype == NT_FLOAT32 ? 0x1p127 : 0x1p1023)))
+    fail(NT_ERR_VALUE, "attention: the scale must be finite in the operands' type");
   check_heads(k, q, "k");
   check_heads(v, q, "v");
   require_same_shape(k, v, "attention");
@@ -1403,7 +1405,7 @@ namespace {
 void attention(const nt_view *q, const nt_view *k, const nt_view *v, const nt_view *lengths,
                const nt_view *starts, int64_t start, int32_t causal, double scale,
                const nt_view *y, const nt_view *lse) {
-  const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
+  const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal, scale);
   dispatch_float(q->dtype, [&]<class T>() {
     AttnFwd<T> a{};
     a.s = s;
@@ -1428,7 +1430,7 @@ void attention_bwd(const nt_view *q, const nt_view *k, const nt_view *v, const n
                    const nt_view *starts, int64_t start, int32_t causal, double scale,
                    const nt_view *y, const nt_view *lse, const nt_view *g, const nt_view *dq,
                    const nt_view *dk, const nt_view *dv) {
-  const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal);
+  const AttnShape s = attn_shape(q, k, v, lengths, starts, start, causal, scale);
   check_heads(g, q, "g");
   require_same_shape(g, q, "attention_bwd");
   dispatch_float(q->dtype, [&]<class T>() {

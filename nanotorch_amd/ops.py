@@ -263,6 +263,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool | None = None,
     if not causal:
         start, starts = 0, None
     scale = q._shape[-1] ** -0.5 if scale is None else float(scale)
+    # times log2 e in the operands' type, in which the kernels hold it
+    if not abs(scale) < (2.0**127 if q._storage._dtype is Dtype.Float32 else 2.0**1023):
+        raise ValueError(f"attention() needs a finite scale, got {scale}.")
     return autograd.AttentionOp.apply(q, k, v, mode, lengths, starts, start, scale)
 
 

@@ -26,6 +26,7 @@ import pytest
 from helpers import assert_bitexact, dev, host, rng, seed_of
 
 import nanotorch_amd as nt
+from nanotorch_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -521,6 +522,16 @@ def test_scale_and_no_batch(gpu):
             assert (grads[0] == 0).all() and (grads[1] == 0).all()
             assert np.abs(y - want["y"][0]).max() < 18 * 2.0 ** -24 * 4
     check_all(q, k, v, g, visible(1, 12, 18, False), np.float32, scale=0.9)
+
+
+@pytest.mark.parametrize("dtype,bad", [(nt.float32, 1e39), (nt.float32, np.nan),
+                                       (nt.float64, np.inf), (nt.float64, -2.0 ** 1023)])
+def test_an_abi_call_refuses_scales(gpu, dtype, bad):
+    view = _lib.pack_view(0, 0, dtype, (1, 0, 1, 4), (4, 4, 4, 1))
+    for name, args in (("nt_attention", (view, None)),
+                       ("nt_attention_bwd", (view, view, view, None, None, None))):
+        with pytest.raises(ValueError, match="scale must be finite"):
+            _lib.call_packed(name, view, view, view, None, None, 0, 0, bad, *args)
 
 
 @pytest.mark.parametrize("shape", [(0, 4, 4), (2, 0, 5), (2, 5, 0)])

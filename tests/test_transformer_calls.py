@@ -94,6 +94,17 @@ def test_starts_without_a_causal_mask_have_no_effect(lib):  # noqa: F811
         nt.attention(q, q, q, causal=False, starts=tensor(3, dtype=Dtype.Int32))
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 2.0**127, -1e39])
+def test_attention_refuses_scales_that_are_not_finite(lib, bad):  # noqa: F811
+    q = heads(2, 4, 2, 8)
+    with pytest.raises(ValueError, match="finite scale"):
+        nt.attention(q, q, q, scale=bad)
+    assert not [n for n, _ in lib.calls if n == "nt_attention"]
+    if math.isfinite(bad):
+        q = heads(2, 4, 2, 8, dtype=Dtype.Float64)
+        nt.attention(q, q, q, scale=bad)
+
+
 def test_host_tensors_are_refused():
     x = nt.Tensor(np.ones((1, 3, 2, 4), np.float32))
     with pytest.raises(RuntimeError, match="GPU"):
