@@ -433,10 +433,11 @@ int nt_rms_norm_bwd(const nt_view *sum, const nt_view *weight,
  *   1  j <= lengths[b] - Tq + i: the queries end with the sequence;
  *   2  j <= starts[b] + i, or start + i where starts is NULL.
  * lengths and starts are 1-D int32 or int64 [B].  A query that sees nothing
- * gives zeros.  What lies from lengths[b] on has no influence, nor has anything
- * else that a query does not see, whatever it holds.  A length outside [0, Tk] is taken
- * as the nearer end, and the next nt_sync() or nt_memcpy_d2h() returns
- * NT_ERR_INDEX.  y is contiguous; lse, which nt_attention_bwd needs, receives
+ * gives zeros.  What lies from lengths[b] on has no influence.  What else a query
+ * does not see has none but on the last bits of its result, whatever it holds: in
+ * float32 it can change which kernels compute the head, and how its neighbours' values
+ * are scaled.  A length outside [0, Tk] is taken as the nearer end, and the next
+ * nt_sync() or nt_memcpy_d2h() returns NT_ERR_INDEX.  y is contiguous; lse, which nt_attention_bwd needs, receives
  * B H Tq statistics or is NULL.  Hk max(Tq H / Hk, Tk) is below 2^25, |scale| below
  * 2^127 (float32) or 2^1023 (NT_ERR_VALUE). */
 int nt_attention(const nt_view *q, const nt_view *k, const nt_view *v,

@@ -36,12 +36,12 @@
 // infinity would be NaN).
 //
 // What bounds them: few rows over a long cache, HBM (8 tokens of 32 heads over caches
-// of up to 8192 x 8 x 128: 80 us for 403 MB and 7 for joining the 16 parts, 5.0 TB/s;
+// of up to 8192 x 8 x 128: 77 us for 403 MB and 7 for joining the 16 parts, 5.2 TB/s;
 // of rows that four heads share, 12 of each instruction's 16 are empty, which costs
 // nothing here); small texts, latency (4 x 128 tokens, 4 heads of 64: 8 us forward,
-// 12 backward, of which an empty launch is 3); float64, loads that little hides (one
-// or two waves to a SIMD): 1024 x 8 heads of 64 both passes 17 TFLOP/s of the 71 that
-// a large product reaches, 2000 x 4 heads of 128 19.
+// 11 backward, of which an empty launch is 3); float64, loads that little hides (one
+// or two waves to a SIMD): 2 x 1024 x 8 heads of 64 both passes 17 TFLOP/s of the 71 that
+// a large product reaches, 2000 x 4 heads of 128 18.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -120,8 +120,9 @@ __device__ __forceinline__ T times(const Frag<T, DP> &a, const Frag<T, DP> &b) {
   return sum;
 }
 
-// Columns of dk and dv that a workgroup keeps, at most 512 bytes of each; of wider
-// rows, two workgroups form the same probabilities.
+// Columns of dk and dv that a workgroup keeps, at most 512 bytes of each; of float32
+// rows over 128 wide, two workgroups form the same probabilities (float64 rows over 64
+// wide have kernels of their own below).
 template <class T, int DP> constexpr int KEY_COLUMNS = std::min(DP, 512 / int(sizeof(T)));
 
 // Items' rows as operand of sums: of the four items row(h, r), pieces at
@@ -774,8 +775,8 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_bwd_left_kernel(const Attn
 // and of the sums' columns lies in a wave's registers and no score is formed twice.  A
 // score is the sum of the waves' four parts, which they exchange through two buffers
 // of LDS, one barrier to a tile.  (Workgroups that formed all scores again for each 64
-// columns, one wave to a SIMD, took 1100 us for 740 of 2000 x 4 heads of 128 and 2040
-// for 930 of 900 x 6 over 3 of 256, both passes.)
+// columns, one wave to a SIMD, took 1100 us for 776 of 2000 x 4 heads of 128 and 2040
+// for 950 of 900 x 6 over 3 of 256, both passes.)
 template <class T, int DP> constexpr bool SHARED_ITEMS = sizeof(T) == 8 && DP >= 128;
 
 // The waves' parts of a tile's result, summed in order; `turn` alternates.
@@ -1164,7 +1165,7 @@ Tokens per_sequence(const nt_view *v, int64_t B, const char *what) {
   return t;
 }
 
-// Tiles of 16 rows of one launch: its work-items are counted in 32 bits, with four
+// Tiles of 16 rows of one launch: its work-items are counted in 32 bits, with three
 // workgroups of 256 at most for a tile of rows and one of keys.
 constexpr int64_t MOST_TILES = int64_t(1) << 21;
 
@@ -1309,7 +1310,8 @@ template <class T, class F> void dispatch_width(int D, F &&f) {
 }
 
 // Into how many parts each tile's keys are split: as many as fill the chip
-// (eight workgroups a CU), with at least two blocks to a wave.
+// (four workgroups a CU; three and six measured no faster), with at least two blocks
+// to a wave.
 int key_splits(const AttnShape &s) {
   const int64_t groups = int64_t(s.B) * s.Hk * ((s.rows + 15) / 16);
   const int64_t want = int64_t(device_cu_count()) * 4 / std::max<int64_t>(groups, 1);

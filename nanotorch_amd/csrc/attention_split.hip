@@ -45,12 +45,13 @@
 // Every kernel's own rows (queries forward and for dq, keys for dk and dv) are the
 // lanes of a result, l % 32, and the other operand's units stream through two
 // stages of LDS, loaded there directly.  The matrix cores are what bounds them, or the
-// power that they draw: 8192 tokens, 16 heads over 4 of 128, causal, take 733 us
-// forward, 1237 for dq, 1290 and 783 for dk and dv, 41 and 82 for packing, 80 for
-// adding parts; 3 products for one make that 1.1, 1.0, 1.0 and 1.05 PFLOP/s, as many
-// as a large float16 product of the library's reaches here (1.07), at 1.75 to 2.2 GHz.
+// power that they draw: 8192 tokens, 16 heads over 4 of 128, causal, take 781 us
+// forward, 1330 for dq, 1342 and 862 for dk and dv, 41 and 82 for packing, 79 for
+// adding parts; 3 products for one make that 1.06, 0.93, 0.92 and 0.96 PFLOP/s of the
+// 1.07 that a large float16 product of the library's reaches here, at 1.8 to 2.2 GHz.
 // With heads of 64 the exponentials and conversions weigh as much as the products: 4 x
-// 2048 tokens, 16 heads, 135, 195 and 272 us, 0.8 PFLOP/s.  Row statistics, rescaling and masks are
+// 2048 tokens, 16 heads, 126, 193 and 281 us, 0.73 to 0.82 PFLOP/s.  (lo without its
+// 2^12, in one sum with hi, was 4 to 5% faster.)  Row statistics, rescaling and masks are
 // then a lane's own, and sums over own rows' columns need no exchange.
 #include <algorithm>
 #include <cmath>
@@ -830,8 +831,8 @@ __global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_spl
 // DK, DV: which of the two.  Both in one kernel share the probabilities; of heads
 // over 64 wide both sums and both own operands do not fit the registers of two
 // waves to a SIMD, and one wave leaves the matrix cores idle while it forms
-// probabilities: 8192 tokens, 16 heads over 4 of 128, 2.53 ms in one kernel and 2.07
-// in two, which form them twice.
+// probabilities: 8192 tokens, 16 heads over 4 of 128, 2.53 ms in one kernel where two,
+// which form them twice, took 2.07 (2.20 with lo times 2^12).
 template <int DB, bool DK, bool DV>
 __global__ __launch_bounds__(64 * SB_WAVES<DB>, (DB <= 4 ? 2 : 1)) void attn_split_dkv_kernel(
     const SplitBwd a) {

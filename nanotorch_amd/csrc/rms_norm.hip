@@ -6,11 +6,12 @@
 //
 // (gs: the gradient of s itself, which the next residual hands back.)  Forward
 // and backward each read and write every array once: a row lives in the
-// registers of one to sixteen waves, as many as its length needs at four to
-// eight 16-byte pieces a lane, between the sum over it and its use.  The sums
+// registers of one to sixteen waves, as many as its length needs at up to four
+// 16-byte pieces a lane, between the sum over it and its use.  The sums
 // are held in the row's type.  Rows longer than that are read twice, the
-// second time mostly from the L2.  HBM bound: 8192 x 4096 with a residual takes
-// 92 us forward and 83 backward, 537 MB each (5.8 and 6.5 TB/s).
+// second time mostly from the L2, and three times backward, the third for dw.  HBM
+// bound: 8192 x 4096 with a residual takes 92 us forward and 82 backward, 537 MB each
+// (5.8 and 6.5 TB/s).
 //
 // dw: every workgroup takes rows w, w + groups, ... and keeps the sums of its
 // columns in registers; its partial sums are one row of a workspace, which a
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const T *part, T *dw,
 namespace {
 
 // The fewest work-items whose registers hold a row of D elements, at 4 pieces
-// each (8 in the largest workgroup); false: none do.
+// each; false: none do.
 template <class T, class F> bool norm_shape(int64_t D, F &&f) {
   const int64_t pieces = (D + RowVec<T>::N - 1) / RowVec<T>::N;
   if (pieces <= 64)
@@ -472,9 +473,9 @@ template <class T> void run_norm(const NormArgs<T> &a) {
 }
 
 template <class T> void run_norm_bwd(NormBackArgs<T> a, T *dw) {
-  // Workgroups that walk rows: two waves to a SIMD, which fill the chip with loads
-  // (8192 x 4096, both passes: 180 us, 184 with four and 191 with eight, whose parts
-  // of dw are as many more).
+  // Workgroups that walk rows: two waves to a SIMD (of 1024 work-items one workgroup to
+  // a CU, four), which fill the chip with loads (8192 x 4096, both passes: 180 us, 184
+  // with four and 191 with eight, whose parts of dw are as many more).
   int64_t parts = 0;
   auto add_up = [&] {
     for (int64_t at = 0; dw && at < a.D; at += RN_MOST_COLUMNS) {

@@ -242,9 +242,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool | None = None,
     With ``causal=False`` starts have no effect.  Starts without a word on causal,
     which is then False, are refused: their caller meant it to be True.
 
-    A query that sees no key gives zeros and has no gradient.  What a query does
-    not see, behind a length or later than itself, does not reach its result,
-    whatever it holds.  Lengths are checked on the device: one
+    A query that sees no key gives zeros and has no gradient.  What lies behind a length
+    does not reach a result.  What a query does not see within it, later than
+    itself, reaches no more than its result's rounding, whatever it holds.  Lengths are checked on the device: one
     outside [0, Tk] is taken as the nearer end, and the next synchronisation
     (``sync``, ``cpu``) raises IndexError.
 
